@@ -276,6 +276,45 @@ int vqb_bq_fit(float threshold, uint8_t low, uint8_t high);
 int vqb_bq_quantize(vqb_ctx *ctx, float threshold, uint8_t low, uint8_t high, const float *x,
                     size_t n_elems, uint8_t *out);
 
+/* ---- 8-bit codes with a scale for each row, and their products ---------------------------------------------
+ * The reference's ScalarQuantizer has one range for all values; here every row has a scale of its own, and the codes are signed whole
+ * numbers that are multiplied without being turned back.  No counterpart in the reference.
+ *
+ *   code   q[i][k] = x[i][k] / s[i] to the nearest whole number (halves to even), s[i] = max(max_k |x[i][k]| / 127, 2^-126);
+ *          s[i] = 0 for a row of zeros; s[i] = NaN for a row that holds an infinity or a NaN; the codes are 0 in both
+ *   y[i][j] = (sum_k q[i][k] w[j][k]) s[i] t[j] + bias[j]         w, t: codes and scales of the matrix's rows (channels)
+ *
+ * The sum is exact; the steps behind it are f32.  A matrix may be one of `groups`: group g then has the rows offsets[g] .. offsets[g + 1] - 1
+ * of the call, any number of them.  Rows of no group (in front of offsets[0], behind offsets[groups]) are not written, or become 0
+ * with VQB_ZERO_REST.  Offsets in device memory are not looked at by the host: where they are not ascending, or leave
+ * 0 .. n, nothing outside the n rows is touched, but which results are written is not defined.
+ *
+ * Values are f32, f16 or bf16 (the same bits in and out as the caller's); ld: values from row to row (>= the row's width).  Outputs may not
+ * overlap inputs.  No rows (n == 0) is no error.  Limits: width 131071 (VQB_ERR_UNSUPPORTED beyond: the sums are 32 bits), 1024 groups, 2^30 - 1 rows. */
+enum vqb_value_type { VQB_F32 = 0, VQB_F16 = 1, VQB_BF16 = 2 };
+#define VQB_ZERO_REST 1     /* flag of a product: rows of no group become 0 */
+#define VQB_QMAT_GRADIENT 1 /* flag of a matrix: its codes are kept transposed too, for vqb_qmat_input_gradient */
+/* n x dim codes and n scales. */
+int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim, size_t ld, int8_t *codes, float *scales);
+typedef struct vqb_qmat vqb_qmat;
+/* groups x outputs x inputs weights, each row quantized as above.  The matrix keeps a copy, laid out for the products. */
+int vqb_qmat_fit(vqb_ctx *ctx, const void *weights, int type, size_t groups, size_t outputs, size_t inputs, int flags, vqb_qmat **out);
+int vqb_qmat_from_parts(vqb_ctx *ctx, const int8_t *codes, const float *scales, size_t groups, size_t outputs, size_t inputs, int flags, vqb_qmat **out);
+int vqb_qmat_shape(const vqb_qmat *qm, size_t *groups, size_t *outputs, size_t *inputs);
+int vqb_qmat_parts(const vqb_qmat *qm, int8_t *codes_out /* groups x outputs x inputs */, float *scales_out /* groups x outputs */);
+/* Quantizes the rows and multiplies them: y is n x outputs of y_type.  offsets: groups + 1, or NULL with one group (all rows); bias: groups x
+ * outputs f32, or NULL. */
+int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim, size_t ld, const int64_t *offsets, const float *bias, void *y, int y_type,
+                     size_t y_ld, int flags);
+/* The same for rows that are quantized already (n x dim codes, n scales). */
+int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, const float *scales, size_t n, size_t dim, const int64_t *offsets, const float *bias, void *y,
+                           int y_type, size_t y_ld, int flags);
+/* dx[i][k] = sum_j dy[i][j] t[j] w[j][k]: the product's gradient with respect to the rows that were quantized (the rounding taken for the identity).
+ * dy[i][j] t[j] enters in 15 bits: as the nearest of 16256 steps up to the row's largest magnitude.  dy is n x outputs, dx n x inputs, both f16 or
+ * both bf16 (f32 is refused: it would promise more digits than that).  Needs VQB_QMAT_GRADIENT. */
+int vqb_qmat_input_gradient(vqb_qmat *qm, const void *dy, int type, size_t n, size_t dim, size_t ld, const int64_t *offsets, void *dx, size_t dx_ld, int flags);
+int vqb_qmat_destroy(vqb_qmat *qm);
+
 /* ---- stand-in row sampler ----------------------------------------------- */
 /* For hosts without the reference's StdRng: one SplitMix64 stream per LBG call, seeded `seed + stream` (src/pq.rs:119).
  * vqb_seeder_sample draws the initial rows of `streams` sub-spaces (streams x k indices); the other three are a

@@ -668,6 +668,283 @@ class BinaryQuantizer:
         return out
 
 
+# ---- 8-bit codes with a scale for each row, and their products ----------------------------------
+_VALUE_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+
+
+def _type_name(dtype) -> str:
+    """"float32" for torch.float32, numpy.float32 or its name."""
+    if isinstance(dtype, str):
+        return dtype
+    return str(dtype).removeprefix("torch.") if type(dtype).__module__.partition(".")[0] == "torch" else np.dtype(dtype).name
+
+
+class _Values:
+    """The caller's rows as they are: float32, float16 or bfloat16 (other types are turned into float32), any distance from row to row.
+    `integers`: int8 codes instead, contiguous."""
+
+    __slots__ = ("cuda", "keep", "shape", "ptr", "single", "n", "dim", "ld", "type", "stream")
+
+    def __init__(self, x, ctx, what="x", integers=False):
+        if isinstance(x, Vector):
+            x = x.data
+        self.cuda = _is_torch(x) and x.is_cuda
+        if self.cuda:
+            torch = sys.modules["torch"]
+            if x.get_device() != ctx.device:
+                raise ValueError(f"{what} is on cuda:{x.get_device()}, the context on cuda:{ctx.device}")
+            if x.requires_grad:
+                x = x.detach()
+            if integers:
+                if x.dtype is not torch.int8:
+                    raise ValueError(f"{what} must be int8")
+                x = x.contiguous()
+                self.type = None
+            else:
+                self.type = _VALUE_TYPES.get(str(x.dtype)[6:])
+                if self.type is None:
+                    x, self.type = x.to(torch.float32), 0
+            self.stream = torch._C._cuda_getCurrentRawStream(ctx.device)
+        else:
+            if _is_torch(x):
+                x = x.detach()
+                x = (x.float() if str(x.dtype) == "torch.bfloat16" else x).numpy()
+            x = np.asarray(x)
+            if integers:
+                if x.dtype != np.int8:
+                    raise ValueError(f"{what} must be int8")
+                self.type = None
+            else:
+                if x.dtype.name not in ("float32", "float16"):
+                    x = x.astype(np.float32)
+                self.type = _VALUE_TYPES[x.dtype.name]
+            x = np.ascontiguousarray(x)
+            self.stream = None
+        shape = x.shape
+        self.single = len(shape) == 1
+        if len(shape) not in (1, 2):
+            raise ValueError("expected a vector or a matrix of row vectors")
+        self.n, self.dim = (1, shape[0]) if self.single else shape
+        self.ld = self.dim
+        if self.cuda and not integers:
+            strides = x.stride()
+            step = strides[0] if not self.single and self.n > 1 else self.dim
+            if (self.dim > 1 and strides[-1] != 1) or step < self.dim:
+                x, step = x.contiguous(), self.dim
+            self.ld = step
+        self.keep, self.shape = x, shape
+        self.ptr = x.data_ptr() if self.cuda else x.ctypes.data
+
+
+def _result(x: _Values, width: int, dtype, out):
+    """(array, pointer, type, values from row to row) of a product's result: a fresh one, or the caller's `out`, whose rows may be further
+    apart than they are wide.  It lives where the rows live."""
+    shape = (width,) if x.single else (x.n, width)
+    if out is None:
+        name = _type_name(dtype)
+        if name not in _VALUE_TYPES or (name == "bfloat16" and not x.cuda):
+            raise ValueError(f"a result of {name} is not offered" + ("" if x.cuda else " for rows in host memory"))
+        if x.cuda:
+            a = x.keep.new_empty(shape, dtype=getattr(sys.modules["torch"], name))
+            return a, a.data_ptr(), _VALUE_TYPES[name], width
+        a = np.empty(shape, np.dtype(name))
+        return a, a.ctypes.data, _VALUE_TYPES[name], width
+    if dtype is not None and _type_name(dtype) != _type_name(out.dtype):
+        raise ValueError("out has another dtype than asked for")
+    kind = _VALUE_TYPES.get(_type_name(out.dtype))
+    if x.cuda:
+        ok = _is_torch(out) and out.is_cuda and out.get_device() == x.keep.get_device()
+        strides = out.stride() if ok else ()
+    else:
+        given, out = out, out.numpy() if _is_torch(out) and not out.is_cuda and out.dtype in (sys.modules["torch"].float32, sys.modules["torch"].float16) else out
+        ok = isinstance(out, np.ndarray) and out.flags.writeable
+        strides = tuple(s // out.itemsize for s in out.strides) if ok and all(s % out.itemsize == 0 for s in out.strides) else ()
+    ok = ok and kind is not None and tuple(out.shape) == shape and len(strides) == len(shape) and (width <= 1 or strides[-1] == 1)
+    ld = strides[0] if ok and not x.single and x.n > 1 else width
+    if not ok or ld < width:
+        raise ValueError(f"out must be a float32, float16 or bfloat16 array of shape {shape} on the input's side, its rows not overlapping")
+    return (out, out.data_ptr(), kind, ld) if x.cuda else (given, out.ctypes.data, kind, ld)
+
+
+def _beside(v, x: _Values, name: str, shape, what: str):
+    """A small array of one type that goes with the rows `x`: (to keep alive, pointer)."""
+    if x.cuda and _is_torch(v) and v.is_cuda:
+        if v.get_device() != x.keep.get_device():
+            raise ValueError(f"{what} is on another device than the rows")
+        v = v.detach().to(getattr(sys.modules["torch"], name)).contiguous()
+        found, ptr = tuple(v.shape), v.data_ptr()
+    else:
+        if _is_torch(v):
+            v = v.detach().cpu()
+            v = (v.float() if str(v.dtype) == "torch.bfloat16" else v).numpy()
+        v = np.ascontiguousarray(v, dtype=name).reshape(np.shape(v))  # (a single scale stays one)
+        found, ptr = v.shape, v.ctypes.data
+    if found not in shape:
+        raise ValueError(f"{what} must have shape {shape[0]}, not {found}")
+    return v, ptr
+
+
+class RowQuantizer:
+    """int8 codes with a scale for each row: ``codes[i] * scales[i]`` is next to row i, off by at most half a scale.
+
+    The scale is a 127th of the row's largest magnitude (0 for a row of zeros, NaN for one that holds an infinity or a NaN), the
+    code the whole number nearest to ``x / scale``, halves to even.  Unlike ScalarQuantizer there is no range to choose, and the codes can be
+    multiplied as they are (QuantizedMatrix)."""
+
+    def __init__(self, ctx):
+        self._ctx = ctx
+
+    @classmethod
+    def fit(cls, *, ctx: Context | None = None):
+        """Nothing is learned from data; here for the likeness of ScalarQuantizer.fit."""
+        return cls(ctx)
+
+    def quantize(self, rows):
+        """(codes, scales) of one vector or of a batch: int8 of the rows' shape, float32 with one value a row."""
+        ctx = self._ctx or default_context()
+        x = _Values(rows, ctx, "rows")
+        if x.cuda:
+            torch = sys.modules["torch"]
+            codes, scales = x.keep.new_empty(x.shape, dtype=torch.int8), x.keep.new_empty(x.shape[:-1], dtype=torch.float32)
+            cptr, sptr = codes.data_ptr(), scales.data_ptr()
+        else:
+            codes, scales = np.empty(x.shape, np.int8), np.empty(x.shape[:-1], np.float32)
+            cptr, sptr = codes.ctypes.data, scales.ctypes.data
+        with ctx._lock:
+            if x.stream != ctx._stream:
+                ctx._run_on(x.stream)
+            rc = ctx._L.vqb_row_quantize(ctx.handle, x.ptr, x.type, x.n, x.dim, x.ld, cptr, sptr)
+            if rc:
+                _raise(rc, ctx.handle)
+        return codes, scales
+
+
+class QuantizedMatrix:
+    """A matrix (outputs x inputs), or one for each of several groups of rows (groups x outputs x inputs), held as int8 codes with a
+    scale for each output channel, and its products with rows that are quantized too.
+
+    ``product`` takes rows of float32, float16 or bfloat16, quantizes each as RowQuantizer does and multiplies: the sums of products
+    of codes are exact.  With `offsets` (groups + 1 ascending row numbers, int64; best where the rows are) group g's matrix takes the rows
+    offsets[g] .. offsets[g + 1] - 1; rows of no group come out as 0 in a fresh result and stay as they are in the caller's `out`.  `gradient`:
+    keep the codes transposed too, for ``input_gradient``."""
+
+    def __init__(self, handle, ctx: Context, grouped: bool):
+        self._h, self._ctx, self._grouped = handle, ctx, grouped
+        g, o, i = C.c_size_t(), C.c_size_t(), C.c_size_t()
+        _lib.load().vqb_qmat_shape(handle, C.byref(g), C.byref(o), C.byref(i))
+        self._shape = int(g.value), int(o.value), int(i.value)
+
+    @classmethod
+    def fit(cls, weights, *, gradient: bool = False, ctx: Context | None = None):
+        """Quantizes every channel (row) of the weights by itself; float32, float16 or bfloat16 weights."""
+        ctx = ctx or default_context()
+        flat, (groups, outputs) = cls._flat(weights)
+        x = _Values(flat, ctx, "weights")
+        if x.ld != x.dim:
+            x = _Values(flat.contiguous(), ctx, "weights")
+        h = C.c_void_p()
+        ctx.call(x, _lib.load().vqb_qmat_fit, ctx.handle, x.ptr, x.type, groups, outputs, x.dim, 1 if gradient else 0, C.byref(h))
+        return cls(h, ctx, len(weights.shape) == 3)
+
+    @classmethod
+    def from_parts(cls, codes, scales, *, gradient: bool = False, ctx: Context | None = None):
+        """A matrix of given int8 codes and the scales of its channels."""
+        ctx = ctx or default_context()
+        flat, (groups, outputs) = cls._flat(codes)
+        x = _Values(flat, ctx, "codes", integers=True)
+        keep, sptr = _beside(scales, x, "float32", [tuple(codes.shape[:-1])], "scales")
+        h = C.c_void_p()
+        ctx.call(x, _lib.load().vqb_qmat_from_parts, ctx.handle, x.ptr, sptr, groups, outputs, x.dim, 1 if gradient else 0, C.byref(h))
+        return cls(h, ctx, len(codes.shape) == 3)
+
+    @staticmethod
+    def _flat(m):
+        if not hasattr(m, "shape") or len(m.shape) not in (2, 3):
+            raise ValueError("expected outputs x inputs or groups x outputs x inputs")
+        shape = tuple(int(v) for v in m.shape)
+        return m.reshape(-1 if 0 not in shape else shape[0] * shape[-2] if len(shape) == 3 else shape[0], shape[-1]), (shape[0] if len(shape) == 3 else 1, shape[-2])
+
+    def shape(self):
+        """(groups, outputs, inputs)"""
+        return self._shape
+
+    def _parts(self, which):
+        g, o, i = self._shape
+        lead = (g, o) if self._grouped else (o,)
+        out = np.empty(lead + (i,), np.int8) if which == 0 else np.empty(lead, np.float32)
+        self._ctx.call(None, _lib.load().vqb_qmat_parts, self._h, out.ctypes.data if which == 0 else None, out.ctypes.data if which else None)
+        return out
+
+    @property
+    def codes(self) -> np.ndarray:
+        return self._parts(0)
+
+    @property
+    def scales(self) -> np.ndarray:
+        return self._parts(1)
+
+    def _groups(self, x, offsets):
+        """(to keep alive, pointer) of the offsets."""
+        if offsets is None:
+            if self._grouped:
+                raise ValueError("a matrix of groups needs offsets")
+            return None, None
+        return _beside(offsets, x, "int64", [(self._shape[0] + 1,)], "offsets")
+
+    def _bias(self, x, bias):
+        g, o, _ = self._shape
+        return (None, None) if bias is None else _beside(bias, x, "float32", [(g, o) if self._grouped else (o,)], "bias")
+
+    def _call(self, x, fn, *args):
+        ctx = self._ctx
+        with ctx._lock:
+            if x.stream != ctx._stream:
+                ctx._run_on(x.stream)
+            rc = fn(self._h, *args)
+            if rc:
+                _raise(rc, ctx.handle)
+
+    def product(self, rows, bias=None, *, offsets=None, dtype=None, out=None):
+        """rows (n x inputs, or one vector) times the matrix: n x outputs of `dtype` (the rows' own by default), plus the bias (outputs, or
+        groups x outputs; added in float32)."""
+        x = _Values(rows, self._ctx, "rows")
+        ko, optr = self._groups(x, offsets)
+        kb, bptr = self._bias(x, bias)
+        y, yptr, kind, ld = _result(x, self._shape[1], dtype or (x.keep.dtype if out is None else None), out)
+        self._call(x, self._ctx._L.vqb_qmat_product, x.ptr, x.type, x.n, x.dim, x.ld, optr, bptr, yptr, kind, ld, 1 if out is None else 0)
+        return y
+
+    def product_of_codes(self, codes, scales, bias=None, *, offsets=None, dtype=None, out=None):
+        """The same for what RowQuantizer.quantize returned, so that several matrices can share it; `dtype` is float32 by default."""
+        x = _Values(codes, self._ctx, "codes", integers=True)
+        ks, sptr = _beside(scales, x, "float32", [() if x.single else (x.n,)], "scales")
+        ko, optr = self._groups(x, offsets)
+        kb, bptr = self._bias(x, bias)
+        y, yptr, kind, ld = _result(x, self._shape[1], dtype or (np.float32 if out is None else None), out)
+        self._call(x, self._ctx._L.vqb_qmat_product_codes, x.ptr, sptr, x.n, x.dim, optr, bptr, yptr, kind, ld, 1 if out is None else 0)
+        return y
+
+    def input_gradient(self, dy, *, offsets=None, out=None):
+        """The gradient of ``product`` with respect to its rows, given the one with respect to its result (n x outputs, float16 or bfloat16): n x inputs of
+        the same type.  The rounding to codes counts as the identity.  Each dy * channel scale enters as the nearest of 16256 steps up
+        to the largest of its row."""
+        x = _Values(dy, self._ctx, "dy")
+        ko, optr = self._groups(x, offsets)
+        y, yptr, kind, ld = _result(x, self._shape[2], x.keep.dtype if out is None else None, out)
+        if kind != x.type:
+            raise ValueError("out must have dy's dtype")
+        self._call(x, self._ctx._L.vqb_qmat_input_gradient, x.ptr, x.type, x.n, x.dim, x.ld, optr, yptr, ld, 1 if out is None else 0)
+        return y
+
+    def __del__(self):
+        try:
+            if self._h:
+                _lib.load().vqb_qmat_destroy(self._h)
+                self._h = None
+        except Exception:
+            pass
+
+
 class TSVQ:
     """TSVQ (src/tsvq.rs:189-250): ``TSVQ(training_data, max_depth, distance)`` builds the tree, ``quantize`` returns the
     leaf centroid as f16.  ``tree()`` gives (centroids, left, right) with nodes numbered breadth-first."""

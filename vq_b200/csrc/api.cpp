@@ -14,6 +14,7 @@
 #include "call_lock.hpp"
 #include "cuda_device.hpp"
 #include "opq_parts.hpp"
+#include "qmat.hpp"
 #include "tsvq.hpp"
 
 namespace vqb {
@@ -53,6 +54,11 @@ struct vqb_tsvq {
     int metric;
     double p;
     TsvqTree tree;
+};
+
+struct vqb_qmat {
+    vqb_ctx *ctx;
+    Qmat mat;
 };
 
 struct vqb_opq {
@@ -289,6 +295,125 @@ struct HostPipeline {
         cudaEventDestroy(start);
     }
 };
+
+// Memory of one call.
+struct Scratch {
+    CudaDevice &dev;
+    unsigned char *d;
+    Scratch(CudaDevice &dv, size_t bytes) : dev(dv), d(static_cast<unsigned char *>(dv.alloc(bytes))) {}
+    ~Scratch() { dev.release(d); }
+    Scratch(const Scratch &) = delete;
+    Scratch &operator=(const Scratch &) = delete;
+};
+
+void check_values(const char *what, const void *p, int type, size_t width, size_t ld)
+{
+    if (type != VALUE_F32 && type != VALUE_F16 && type != VALUE_BF16) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + ": unknown value type");
+    if (!p) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + " is NULL");
+    if (reinterpret_cast<uintptr_t>(p) % value_bytes(type)) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + " is not aligned to its values");
+    if (ld < width) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + ": rows overlap");
+}
+
+void check_words(const char *what, const void *p, size_t bytes)
+{
+    if (reinterpret_cast<uintptr_t>(p) % bytes) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + " is not aligned to its values");
+}
+
+void check_row_count(size_t n)
+{
+    if (n > QMAT_MOST_ROWS) throw Error(VQB_ERR_UNSUPPORTED, "more than 2^30 - 1 rows: split the batch");
+}
+
+// Bytes from the first value of the first row to the last one of the last.
+size_t span(size_t n, size_t width, size_t ld, size_t bytes) { return n ? ((n - 1) * ld + width) * bytes : 0; }
+
+// The groups' offsets: on the device as they are, from the host once they have been looked at.
+struct OffsetsIn {
+    std::unique_ptr<In> in;
+    OffsetsIn(CudaDevice &dev, const int64_t *offsets, size_t groups, size_t n)
+    {
+        if (!offsets) {
+            if (groups != 1) throw Error(VQB_ERR_BAD_ARGUMENT, "a matrix of several groups needs offsets");
+            return;
+        }
+        check_words("offsets", offsets, sizeof(int64_t));
+        if (!dev.is_device_pointer(offsets))
+            for (size_t g = 0; g <= groups; ++g)
+                if (offsets[g] < (g ? offsets[g - 1] : 0) || offsets[g] > (int64_t)n)
+                    throw Error(VQB_ERR_INVALID_PARAMETER, "Invalid parameter: offsets must ascend from 0 or more to at most the number of rows");
+        in.reset(new In(dev, offsets, sizeof(int64_t) * (groups + 1)));
+    }
+    const int64_t *get() const { return in ? in->as<int64_t>() : nullptr; }
+};
+
+// A product's result.  Host memory that the product does not write all of is brought in first.
+struct RowsOut {
+    Out out;
+    RowsOut(CudaDevice &dev, void *y, size_t n, size_t width, size_t ld, int type, bool all) : out(dev, y, span(n, width, ld, value_bytes(type)))
+    {
+        if (out.host && (!all || ld != width)) VQB_CUDA_CHECK(cudaMemcpyAsync(out.d, out.host, out.bytes, cudaMemcpyHostToDevice, dev.stream()));
+    }
+};
+
+void check_qmat_shape(size_t groups, size_t outputs, size_t inputs, int flags)
+{
+    if (groups == 0 || outputs == 0 || inputs == 0) throw Error(VQB_ERR_EMPTY_INPUT, "Empty input: at least one vector is required.");
+    if (flags & ~VQB_QMAT_GRADIENT) throw Error(VQB_ERR_BAD_ARGUMENT, "unknown flag");
+    if (inputs > QMAT_MOST_WIDTH) throw Error(VQB_ERR_UNSUPPORTED, "more than 131071 inputs: the sums would leave 32 bits");
+    if ((flags & VQB_QMAT_GRADIENT) && outputs > QMAT_MOST_WIDTH) throw Error(VQB_ERR_UNSUPPORTED, "a gradient over more than 131071 outputs: the sums would leave 32 bits");
+    if (groups > QMAT_MOST_GROUPS) throw Error(VQB_ERR_UNSUPPORTED, "more than 1024 groups");
+    if (outputs > QMAT_MOST_ROWS / groups || inputs > QMAT_MOST_ROWS / groups) throw Error(VQB_ERR_UNSUPPORTED, "more than 2^30 - 1 channels in all groups");
+}
+
+// A matrix with room for its codes; what is left of it when something fails is released.
+struct NewQmat {
+    CudaDevice &dev;
+    std::unique_ptr<vqb_qmat> qm;
+    NewQmat(vqb_ctx *ctx, size_t groups, size_t outputs, size_t inputs, int flags) : dev(*ctx->dev), qm(new vqb_qmat{ctx, Qmat{}})
+    {
+        Qmat &m = qm->mat;
+        m.groups = groups, m.outputs = outputs, m.inputs = inputs;
+        try {
+            m.codes = static_cast<int8_t *>(dev.alloc(groups * outputs * codes_ld(inputs)));
+            m.scales = static_cast<float *>(dev.alloc(groups * outputs * sizeof(float)));
+            if (flags & VQB_QMAT_GRADIENT) m.turned = static_cast<int8_t *>(dev.alloc(groups * inputs * codes_ld(outputs)));
+        } catch (...) {
+            drop();
+            throw;
+        }
+    }
+    void drop()
+    {
+        if (!qm) return;
+        dev.release(qm->mat.codes), dev.release(qm->mat.scales), dev.release(qm->mat.turned);
+        qm.reset();
+    }
+    vqb_qmat *done()
+    {
+        Qmat &m = qm->mat;
+        if (m.turned) launch_turn_codes(dev, m.codes, m.groups, m.outputs, m.inputs, m.turned);
+        return qm.release();
+    }
+    ~NewQmat() { drop(); }
+};
+
+Product product_of(const Qmat &m)
+{
+    Product p;
+    p.codes = m.codes, p.channel_scales = m.scales, p.groups = m.groups, p.channels = m.outputs, p.width = m.inputs;
+    return p;
+}
+
+std::string dim_mismatch(size_t expected, size_t found);
+
+void check_product(const Qmat &m, size_t n, size_t dim, const float *bias, void *y, int y_type, size_t y_ld, int flags)
+{
+    if (dim != m.inputs) throw Error(VQB_ERR_DIMENSION_MISMATCH, dim_mismatch(m.inputs, dim));
+    check_row_count(n);
+    if (flags & ~VQB_ZERO_REST) throw Error(VQB_ERR_BAD_ARGUMENT, "unknown flag");
+    if (n) check_values("y", y, y_type, m.outputs, y_ld);
+    check_words("bias", bias, sizeof(float));
+}
 
 void check_minkowski(int metric, double p)
 {
@@ -1133,6 +1258,185 @@ int vqb_bq_quantize(vqb_ctx *ctx, float threshold, uint8_t low, uint8_t high, co
         dev.bq_quantize(threshold, low, high, ix.as<float>(), n_elems, o.as<uint8_t>());
         o.finish();
     });
+}
+
+int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim, size_t ld, int8_t *codes, float *scales)
+{
+    if (!ctx) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "ctx is NULL");
+    return locked(ctx, [&] {
+        if (dim == 0) throw Error(VQB_ERR_EMPTY_INPUT, "Empty input: at least one vector is required.");
+        check_row_count(n);
+        if (n == 0) return;
+        check_values("x", x, type, dim, ld);
+        if (!codes || !scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
+        check_words("scales", scales, sizeof(float));
+        CudaDevice &dev = *ctx->dev;
+        In ix(dev, x, span(n, dim, ld, value_bytes(type)));
+        Out oc(dev, codes, n * dim), os(dev, scales, sizeof(float) * n);
+        launch_quantize_rows(dev, ix.d, type, n, dim, ld, oc.as<int8_t>(), dim, os.as<float>());
+        finish(oc, os);
+    });
+}
+
+int vqb_qmat_fit(vqb_ctx *ctx, const void *weights, int type, size_t groups, size_t outputs, size_t inputs, int flags, vqb_qmat **out)
+{
+    if (!ctx) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "ctx is NULL");
+    return locked(ctx, [&] {
+        if (!out) throw Error(VQB_ERR_BAD_ARGUMENT, "out is NULL");
+        *out = nullptr;
+        check_qmat_shape(groups, outputs, inputs, flags);
+        check_values("weights", weights, type, inputs, inputs);
+        CudaDevice &dev = *ctx->dev;
+        In iw(dev, weights, groups * outputs * inputs * value_bytes(type));
+        NewQmat made(ctx, groups, outputs, inputs, flags);
+        Qmat &m = made.qm->mat;
+        launch_quantize_rows(dev, iw.d, type, groups * outputs, inputs, inputs, m.codes, codes_ld(inputs), m.scales);
+        *out = made.done();
+    });
+}
+
+int vqb_qmat_from_parts(vqb_ctx *ctx, const int8_t *codes, const float *scales, size_t groups, size_t outputs, size_t inputs, int flags, vqb_qmat **out)
+{
+    if (!ctx) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "ctx is NULL");
+    return locked(ctx, [&] {
+        if (!out) throw Error(VQB_ERR_BAD_ARGUMENT, "out is NULL");
+        *out = nullptr;
+        check_qmat_shape(groups, outputs, inputs, flags);
+        if (!codes || !scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
+        check_words("scales", scales, sizeof(float));
+        CudaDevice &dev = *ctx->dev;
+        In ic(dev, codes, groups * outputs * inputs), is(dev, scales, sizeof(float) * groups * outputs);
+        NewQmat made(ctx, groups, outputs, inputs, flags);
+        Qmat &m = made.qm->mat;
+        launch_align_codes(dev, ic.as<int8_t>(), groups * outputs, inputs, inputs, m.codes);
+        dev.copy(m.scales, is.d, sizeof(float) * groups * outputs);
+        *out = made.done();
+    });
+}
+
+int vqb_qmat_shape(const vqb_qmat *qm, size_t *groups, size_t *outputs, size_t *inputs)
+{
+    if (!qm) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "matrix is NULL");
+    if (groups) *groups = qm->mat.groups;
+    if (outputs) *outputs = qm->mat.outputs;
+    if (inputs) *inputs = qm->mat.inputs;
+    return VQB_OK;
+}
+
+int vqb_qmat_parts(const vqb_qmat *qm, int8_t *codes_out, float *scales_out)
+{
+    if (!qm) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "matrix is NULL");
+    vqb_ctx *ctx = qm->ctx;
+    return locked(ctx, [&] {
+        CudaDevice &dev = *ctx->dev;
+        const Qmat &m = qm->mat;
+        const size_t rows = m.groups * m.outputs;
+        Out oc(dev, codes_out, rows * m.inputs), os(dev, scales_out, sizeof(float) * rows);
+        if (oc.d) VQB_CUDA_CHECK(cudaMemcpy2DAsync(oc.d, m.inputs, m.codes, codes_ld(m.inputs), m.inputs, rows, cudaMemcpyDeviceToDevice, dev.stream()));
+        if (os.d) dev.copy(os.d, m.scales, sizeof(float) * rows);
+        finish(oc, os);
+    });
+}
+
+int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim, size_t ld, const int64_t *offsets, const float *bias, void *y, int y_type,
+                     size_t y_ld, int flags)
+{
+    if (!qm) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "matrix is NULL");
+    vqb_ctx *ctx = qm->ctx;
+    return locked(ctx, [&] {
+        const Qmat &m = qm->mat;
+        check_product(m, n, dim, bias, y, y_type, y_ld, flags);
+        CudaDevice &dev = *ctx->dev;
+        OffsetsIn io(dev, offsets, m.groups, n);
+        if (n == 0) return;
+        check_values("x", x, type, dim, ld);
+        In ix(dev, x, span(n, dim, ld, value_bytes(type))), ib(dev, bias, bias ? sizeof(float) * m.groups * m.outputs : 0);
+        RowsOut oy(dev, y, n, m.outputs, y_ld, y_type, !offsets || (flags & VQB_ZERO_REST));
+        Product p = product_of(m);
+        p.n = n, p.rows_ld = codes_ld(dim), p.offsets = io.get(), p.bias = ib.as<float>();
+        p.y = oy.out.d, p.y_type = y_type, p.y_ld = y_ld, p.zero_rest = (flags & VQB_ZERO_REST) != 0;
+        Scratch codes(dev, n * p.rows_ld + n * sizeof(float));
+        float *scales = reinterpret_cast<float *>(codes.d + n * p.rows_ld);
+        launch_quantize_rows(dev, ix.d, type, n, dim, ld, reinterpret_cast<int8_t *>(codes.d), p.rows_ld, scales);
+        p.rows = reinterpret_cast<const int8_t *>(codes.d), p.row_scales = scales, p.rows_follow = true;
+        launch_product(dev, p);
+        oy.out.finish();
+    });
+}
+
+int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, const float *scales, size_t n, size_t dim, const int64_t *offsets, const float *bias, void *y,
+                           int y_type, size_t y_ld, int flags)
+{
+    if (!qm) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "matrix is NULL");
+    vqb_ctx *ctx = qm->ctx;
+    return locked(ctx, [&] {
+        const Qmat &m = qm->mat;
+        check_product(m, n, dim, bias, y, y_type, y_ld, flags);
+        CudaDevice &dev = *ctx->dev;
+        OffsetsIn io(dev, offsets, m.groups, n);
+        if (n == 0) return;
+        if (!codes || !scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
+        check_words("scales", scales, sizeof(float));
+        In ic(dev, codes, n * dim), is(dev, scales, sizeof(float) * n), ib(dev, bias, bias ? sizeof(float) * m.groups * m.outputs : 0);
+        RowsOut oy(dev, y, n, m.outputs, y_ld, y_type, !offsets || (flags & VQB_ZERO_REST));
+        Product p = product_of(m);
+        p.n = n, p.offsets = io.get(), p.bias = ib.as<float>(), p.row_scales = is.as<float>();
+        p.y = oy.out.d, p.y_type = y_type, p.y_ld = y_ld, p.zero_rest = (flags & VQB_ZERO_REST) != 0;
+        p.rows = ic.as<int8_t>(), p.rows_ld = dim;
+        std::unique_ptr<Scratch> aligned;
+        if (dim % 16 || reinterpret_cast<uintptr_t>(p.rows) % 16) {
+            p.rows_ld = codes_ld(dim);
+            aligned.reset(new Scratch(dev, n * p.rows_ld));
+            launch_align_codes(dev, p.rows, n, dim, dim, reinterpret_cast<int8_t *>(aligned->d));
+            p.rows = reinterpret_cast<const int8_t *>(aligned->d);
+        }
+        launch_product(dev, p);
+        oy.out.finish();
+    });
+}
+
+int vqb_qmat_input_gradient(vqb_qmat *qm, const void *dy, int type, size_t n, size_t dim, size_t ld, const int64_t *offsets, void *dx, size_t dx_ld, int flags)
+{
+    if (!qm) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "matrix is NULL");
+    vqb_ctx *ctx = qm->ctx;
+    return locked(ctx, [&] {
+        const Qmat &m = qm->mat;
+        if (!m.turned) throw Error(VQB_ERR_INVALID_PARAMETER, "Invalid parameter: the matrix was made without its gradient");
+        if (dim != m.outputs) throw Error(VQB_ERR_DIMENSION_MISMATCH, dim_mismatch(m.outputs, dim));
+        check_row_count(n);
+        if (flags & ~VQB_ZERO_REST) throw Error(VQB_ERR_BAD_ARGUMENT, "unknown flag");
+        if (type == VQB_F32) throw Error(VQB_ERR_UNSUPPORTED, "gradients are f16 or bf16: dy enters the product in 15 bits");
+        CudaDevice &dev = *ctx->dev;
+        OffsetsIn io(dev, offsets, m.groups, n);
+        if (n == 0) return;
+        check_values("dy", dy, type, dim, ld);
+        check_values("dx", dx, type, m.inputs, dx_ld);
+        In iy(dev, dy, span(n, dim, ld, value_bytes(type)));
+        RowsOut ox(dev, dx, n, m.inputs, dx_ld, type, !offsets || (flags & VQB_ZERO_REST));
+        Product p;
+        p.codes = m.turned, p.groups = m.groups, p.channels = m.inputs, p.width = m.outputs, p.digits = 2;
+        p.n = n, p.rows_ld = codes_ld(dim), p.offsets = io.get();
+        p.y = ox.out.d, p.y_type = type, p.y_ld = dx_ld, p.zero_rest = (flags & VQB_ZERO_REST) != 0;
+        Scratch codes(dev, 2 * n * p.rows_ld + n * sizeof(float));
+        float *scales = reinterpret_cast<float *>(codes.d + 2 * n * p.rows_ld);
+        launch_digit_rows(dev, iy.d, type, n, dim, ld, m.scales, m.groups, p.offsets, reinterpret_cast<int8_t *>(codes.d), p.rows_ld, scales);
+        p.rows = reinterpret_cast<const int8_t *>(codes.d), p.row_scales = scales, p.rows_follow = true;
+        launch_product(dev, p);
+        ox.out.finish();
+    });
+}
+
+int vqb_qmat_destroy(vqb_qmat *qm)
+{
+    if (!qm) return VQB_OK;
+    vqb_ctx *ctx = qm->ctx;
+    destroyed(ctx, [&] {
+        ctx->dev->release(qm->mat.codes);
+        ctx->dev->release(qm->mat.scales);
+        ctx->dev->release(qm->mat.turned);
+    });
+    delete qm;
+    return VQB_OK;
 }
 
 } // extern "C"

@@ -1,0 +1,98 @@
+// qmat.cuh -- what the kernels on 8-bit codes share: which rows a tile has, how a result leaves, when the rows are there.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "qmat.hpp"
+
+namespace vqb {
+
+// Kernels of a product may start before the kernel in front of them ends.  All earlier work of the stream is complete and visible
+// from here on; every thread calls it before it reads what that kernel may have written, or leaves.  (What is read before: a matrix, where
+// the kernel in front is this call's own quantizer, which has itself waited for everything earlier.)
+__device__ __forceinline__ void rows_are_there() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void product_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// A sum of products of codes to the value it stands for.  Sums above 2^24 round to f32 here, as each step behind does.
+__device__ __forceinline__ float finish_sum(float sum, float row_scale, float channel_scale, float bias)
+{
+    return __fmaf_rn(__fmul_rn(sum, row_scale), channel_scale, bias);
+}
+
+// Rows [first, end) of group g.  Offsets come from the device unchecked: whatever they are, the rows are some of the n that there are.
+struct GroupRows {
+    int first, end;
+};
+__device__ __forceinline__ GroupRows group_rows(const long long *offsets, int g, int n)
+{
+    if (!offsets) return {0, n};
+    const long long a = offsets[g], b = offsets[g + 1];
+    const int first = (int)(a < 0 ? 0 : a > n ? n : a);
+    return {first, (int)(b < first ? first : b > n ? n : b)};
+}
+
+// How the rows of all groups fall into tiles of at most `rows` rows: tile u belongs to the last group g with before[g] <= u, and starts at row
+// first[g] + (u - before[g]) * rows.  In shared memory: 2 (groups + 1) + groups words.
+struct RowTiles {
+    int *before; // groups + 1
+    int *first;  // groups
+    int *end;    // groups
+    static __host__ __device__ constexpr size_t bytes(size_t groups) { return (3 * groups + 1) * sizeof(int); }
+    __device__ __forceinline__ RowTiles(void *smem, int groups) : before(static_cast<int *>(smem)), first(before + groups + 1), end(first + groups) {}
+
+    // by all threads of the block; ends with a block barrier
+    __device__ __forceinline__ void build(const long long *offsets, int groups, int n, int rows)
+    {
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+            const GroupRows r = group_rows(offsets, g, n);
+            first[g] = r.first, end[g] = r.end;
+            before[g + 1] = (r.end - r.first + rows - 1) / rows;
+        }
+        if (threadIdx.x == 0) before[0] = 0;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            int carry = 0;
+            for (int g0 = 0; g0 < groups; g0 += 32) {
+                const int g = g0 + (int)threadIdx.x;
+                int v = g < groups ? before[g + 1] : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int up = __shfl_up_sync(~0u, v, d);
+                    if ((int)threadIdx.x >= d) v += up;
+                }
+                if (g < groups) before[g + 1] = carry + v;
+                carry += __shfl_sync(~0u, v, 31);
+            }
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ int group_of(int u, int groups) const
+    {
+        int lo = 0, hi = groups - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (before[mid] <= u) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    }
+};
+
+// Rows in front of the first group and behind the last one become 0, by `threads` threads of which this is number t.
+template <typename T> __device__ void zero_rest(T *y, size_t ld, int channels, int n, int head, int tail, size_t t, size_t threads)
+{
+    const size_t rest = (size_t)head + (size_t)(n - tail);
+    for (size_t i = t; i < rest * channels; i += threads) {
+        const size_t r = i / channels;
+        y[(r < (size_t)head ? r : r - head + tail) * ld + i % channels] = from_float<T>(0.0f);
+    }
+}
+
+} // namespace vqb

@@ -1,0 +1,65 @@
+// qmat.hpp -- products of 8-bit codes with a scale for each row (tokens) and for each channel (matrix rows).
+//
+//   y[i][j] = (sum_k q[i][k] w[j][k]) s[i] t[j] + b[j]        q, w: int8; the sum is a whole number, exact in 32 bits
+//
+// for one matrix, or for one matrix per group of consecutive rows (offsets); and the gradient of that with respect to what the rows
+// were quantized from.  rows.cu makes codes, product_plain.cu multiplies them.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+namespace vqb {
+
+class CudaDevice;
+
+enum ValueType : int { VALUE_F32 = 0, VALUE_F16 = 1, VALUE_BF16 = 2 };
+inline size_t value_bytes(int type) { return type == VALUE_F32 ? 4 : 2; }
+
+// 128 * 128 * QMAT_MOST_WIDTH < 2^31: no sum of products of codes leaves 32 bits
+constexpr size_t QMAT_MOST_WIDTH = 131071;
+constexpr size_t QMAT_MOST_GROUPS = 1024; // the products keep the groups' rows and tiles in shared memory
+constexpr size_t QMAT_MOST_ROWS = (size_t(1) << 30) - 1; // (two digit planes of them are numbered in 31 bits)
+
+// codes rows are 16-byte aligned: what TMA and 16-byte loads ask for
+inline size_t codes_ld(size_t width) { return (width + 15) / 16 * 16; }
+
+struct Qmat {
+    size_t groups = 0, outputs = 0, inputs = 0;
+    int8_t *codes = nullptr;  // groups x outputs x codes_ld(inputs)
+    float *scales = nullptr;  // groups x outputs
+    int8_t *turned = nullptr; // groups x inputs x codes_ld(outputs): the codes transposed, for gradients; null without
+};
+
+// One product: `channels` rows of codes for each group times n rows.
+struct Product {
+    const int8_t *codes = nullptr;        // groups x channels x codes_ld(width)
+    const float *channel_scales = nullptr; // groups x channels; null: 1
+    size_t groups = 1, channels = 0, width = 0;
+    const int8_t *rows = nullptr; // n x rows_ld; with two digits the low digits follow, another n x rows_ld
+    size_t rows_ld = 0, n = 0;
+    int digits = 1; // 2: a row's values are 128 high + low
+    const float *row_scales = nullptr; // n
+    const int64_t *offsets = nullptr;  // groups + 1: group g has rows offsets[g] .. offsets[g + 1] - 1; null: one group of all rows
+    const float *bias = nullptr;       // groups x channels, or null
+    void *y = nullptr;                 // n x y_ld values of y_type
+    int y_type = VALUE_F32;
+    size_t y_ld = 0;
+    bool zero_rest = false;   // rows of no group become 0 (otherwise they are left as they are)
+    bool rows_follow = false; // the kernel directly before wrote `rows` and `row_scales`, and nothing else of this
+};
+
+// codes[i][k] = x[i][k] / s[i] to the nearest whole number (halves to even, of the real quotient), s[i] = max_k |x[i][k]| / 127; s is 0 for
+// a row of zeros and NaN for one with an infinity or a NaN, with codes 0.  Bytes behind the row's width stay as they are.
+void launch_quantize_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, int8_t *codes, size_t ld_codes, float *scales);
+// u[i][j] = x[i][j] column_scales[g][j] of the row's group g as two digits: u / t = 128 high + low, t = max |u| / 16256.  digits: n x ld_codes high
+// ones and as many low ones.
+void launch_digit_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, const float *column_scales, size_t groups, const int64_t *offsets,
+                       int8_t *digits, size_t ld_codes, float *scales);
+// turned[g][k][j] = codes[g][j][k]
+void launch_turn_codes(CudaDevice &dev, const int8_t *codes, size_t groups, size_t rows, size_t width, int8_t *turned);
+// rows of any alignment to rows of codes_ld(width) bytes
+void launch_align_codes(CudaDevice &dev, const int8_t *codes, size_t n, size_t width, size_t ld, int8_t *aligned);
+
+void launch_product(CudaDevice &dev, const Product &p);
+
+} // namespace vqb

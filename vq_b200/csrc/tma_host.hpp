@@ -11,7 +11,7 @@
 
 namespace vqb {
 
-// T: float, or uint16_t for binary16 bits.  ld: elements from row to row (0: the rows follow each other)
+// T: float, uint16_t for binary16 bits, or int8_t.  ld: elements from row to row (0: the rows follow each other)
 template <typename T> inline CUtensorMap make_tensor_map_2d(const T *ptr, unsigned long long inner, unsigned long long rows, unsigned box_inner,
                                       unsigned box_rows, CUtensorMapSwizzle swizzle, unsigned long long ld = 0)
 {
@@ -32,7 +32,7 @@ template <typename T> inline CUtensorMap make_tensor_map_2d(const T *ptr, unsign
     cuuint64_t strides[1] = {(cuuint64_t)(ld ? ld : inner) * sizeof(T)};
     cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(&m, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<T *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    CUresult r = fn(&m, sizeof(T) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<T *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw Error(100, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
     return m;
