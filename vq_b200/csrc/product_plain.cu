@@ -1,4 +1,4 @@
-// product_plain.cu -- the products of codes on the CUDA cores.
+// product_plain.cu -- the products of codes on the CUDA cores: what VQB_NO_TENSOR=1 runs, and what product_tc.cu is compared with.
 //
 // A block takes 64 channels x 64 rows; 64 bytes of both at a time go through shared memory, a thread keeps 4 x 4 sums and adds four
 // products an instruction (dp4a).  What bounds it is that instruction: 64 of them an SM and cycle.
@@ -94,7 +94,7 @@ template <typename T> void product_plain_typed(CudaDevice &dev, const PlainParam
 
 } // namespace
 
-void launch_product(CudaDevice &dev, const Product &p)
+void launch_product_plain(CudaDevice &dev, const Product &p)
 {
     PlainParams P{p.codes, p.rows, p.rows + p.n * p.rows_ld, codes_ld(p.width), p.rows_ld, p.channel_scales, p.row_scales, p.bias, reinterpret_cast<const long long *>(p.offsets),
                   (int)p.groups, (int)p.channels, (int)p.width, (int)p.n, p.y, p.y_ld, p.zero_rest};

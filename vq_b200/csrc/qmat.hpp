@@ -3,7 +3,7 @@
 //   y[i][j] = (sum_k q[i][k] w[j][k]) s[i] t[j] + b[j]        q, w: int8; the sum is a whole number, exact in 32 bits
 //
 // for one matrix, or for one matrix per group of consecutive rows (offsets); and the gradient of that with respect to what the rows
-// were quantized from.  rows.cu makes codes, product_plain.cu multiplies them.
+// were quantized from.  rows.cu makes codes, product_tc.cu and product_plain.cu multiply them.
 #pragma once
 #include <cstddef>
 #include <cstdint>
@@ -61,5 +61,6 @@ void launch_turn_codes(CudaDevice &dev, const int8_t *codes, size_t groups, size
 void launch_align_codes(CudaDevice &dev, const int8_t *codes, size_t n, size_t width, size_t ld, int8_t *aligned);
 
 void launch_product(CudaDevice &dev, const Product &p);
+void launch_product_plain(CudaDevice &dev, const Product &p); // CUDA cores
 
 } // namespace vqb
