@@ -78,7 +78,12 @@ __device__ __forceinline__ Tile tile_at(const TcParams &P, const RowTiles &tiles
     return t;
 }
 
-__device__ __forceinline__ int columns_of(int rows) { return (rows + 31) / 32 * 32; }
+// Accumulator columns of one digit: rows in steps of 32.  The low digits' rows begin where the loads of the high ones end.
+template <int DIGITS> __device__ __forceinline__ int columns_of(const TcParams &P, int rows)
+{
+    const int step = DIGITS == 2 ? P.box_rows : 32;
+    return (rows + step - 1) / step * step;
+}
 
 template <typename T, int DIGITS>
 __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rows, const TcParams P)
@@ -131,7 +136,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             };
             for (long long id = blockIdx.x; ok && id < total; id += gridDim.x) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
-                const int columns = columns_of(t.rows);
+                const int columns = columns_of<DIGITS>(P, t.rows);
                 const uint32_t bytes = A_BYTES + (uint32_t)(DIGITS * ((columns + P.box_rows - 1) / P.box_rows) * P.box_rows * KB);
                 const int ahead = waited ? 0 : min(NST, chunks);
                 for (int c = 0; c < chunks; ++c, ++it) {
@@ -166,7 +171,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             bool ok = true;
             for (long long id = blockIdx.x; ok && id < total; id += gridDim.x, ++local) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
-                const uint32_t b = local & 1u, idesc = idesc_i8(DIGITS * columns_of(t.rows)), d_tmem = tmem_base + b * MOST_COLS;
+                const uint32_t b = local & 1u, idesc = idesc_i8(DIGITS * columns_of<DIGITS>(P, t.rows)), d_tmem = tmem_base + b * MOST_COLS;
                 if (!mbar_wait(&bars->tempty[b], ((local >> 1) & 1u) ^ 1u, abort_flag, P.error, 63)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int c = 0; c < chunks; ++c, ++it) {
@@ -197,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         for (long long id = blockIdx.x; id < total; id += gridDim.x, ++local) {
             const Tile t = tile_at(P, tiles, id, channel_tiles);
             const uint32_t b = local & 1u;
-            const int channel = t.channel0 + 32 * q + lane, columns = columns_of(t.rows);
+            const int channel = t.channel0 + 32 * q + lane, columns = columns_of<DIGITS>(P, t.rows);
             const bool there = channel < P.channels;
             const size_t at = (size_t)t.group * P.channels + channel;
             const float channel_scale = !there ? 0.0f : P.channel_scales ? P.channel_scales[at] : 1.0f, bias = there && P.bias ? P.bias[at] : 0.0f;
@@ -262,11 +267,11 @@ void launch_product(CudaDevice &dev, const Product &p)
     const size_t most = MOST_COLS / p.digits;
     if (p.offsets) {
         P.tile_rows = (int)most;
-        P.box_rows = 32;
+        P.box_rows = p.n / p.groups >= 64 ? 64 : 32;
     } else { // as few tiles as there can be, of the same size
         const size_t tiles = (p.n + most - 1) / most;
         P.tile_rows = (int)(((p.n + tiles - 1) / tiles + 31) / 32 * 32);
-        P.box_rows = p.digits == 1 ? P.tile_rows : 32; // (the low digits' rows begin where the tile's high ones end)
+        P.box_rows = P.tile_rows;
     }
     P.band = 8;
     const CUtensorMap map_codes = make_tensor_map_2d<int8_t>(p.codes, p.width, p.groups * p.channels, KB, BM, CU_TENSOR_MAP_SWIZZLE_128B, codes_ld(p.width));

@@ -4,12 +4,14 @@
 // it is memory: s + 1 bytes a value.
 //
 // The code is the nearest whole number to the REAL quotient x / s (halves to even), so that it depends on nothing but x and the
-// row's largest magnitude.  x (1 / s) in f32 is off by less than 128 2^-23 = 2^-16; only where its distance from a half is below that
-// does the quotient in f64 decide (two f32 numbers' quotient is either a half or further from it than f64 rounds by).
+// row's largest magnitude.  1 / s lies between two neighbouring f32 numbers; where x times either rounds to the same whole number, that is
+// the code, and elsewhere (the quotient is next to a half h) the sign of x - h s decides, which one fused multiply-add gives exactly.
 #include <algorithm>
+#include <type_traits>
 
 #include "cuda_device.hpp"
 #include "qmat.cuh"
+#include "umma.cuh"
 
 namespace vqb {
 
@@ -35,57 +37,120 @@ template <> struct Piece<__nv_bfloat16> {
     __device__ __forceinline__ float at(int i) const { return __uint_as_float((i & 1) ? ((&w.x)[i >> 1] & 0xFFFF0000u) : ((&w.x)[i >> 1] << 16)); }
 };
 
-// N values of a row from column k on, 0 behind its end
-template <typename T, bool ALIGNED> __device__ __forceinline__ Piece<T> load_values(const T *row, size_t k, size_t width)
+// Which columns a lane has.  Where rows and codes are aligned: N neighbouring ones a piece, 16 bytes loaded and N stored at once.  Elsewhere
+// every LANESth column: 4 or 2 bytes a lane, but a warp's are next to each other.
+template <int N, int LANES, bool ALIGNED> __device__ __forceinline__ size_t column(size_t piece, int lane, int i)
+{
+    return ALIGNED ? (piece * LANES + lane) * N + i : (piece * N + i) * LANES + lane;
+}
+
+// a piece of a row, 0 behind its end
+template <typename T, int LANES, bool ALIGNED> __device__ __forceinline__ Piece<T> load_values(const T *row, size_t piece, int lane, size_t width)
 {
     constexpr int N = Piece<T>::N;
     Piece<T> p;
     p.w = make_uint4(0, 0, 0, 0);
+    const size_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
     if (ALIGNED && k + N <= width) {
         p.w = *reinterpret_cast<const uint4 *>(row + k);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (k + i < width) {
-                if (sizeof(T) == 4) (&p.w.x)[i] = reinterpret_cast<const uint32_t *>(row)[k + i];
-                else (&p.w.x)[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(row)[k + i] << (16 * (i & 1));
+        for (int i = 0; i < N; ++i) {
+            const size_t at = column<N, LANES, ALIGNED>(piece, lane, i);
+            if (at < width) {
+                if (sizeof(T) == 4) (&p.w.x)[i] = reinterpret_cast<const uint32_t *>(row)[at];
+                else (&p.w.x)[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(row)[at] << (16 * (i & 1));
             }
+        }
     }
     return p;
 }
 
-// whole numbers of magnitudes up to 127 as bytes; `far`: no quotient was near a half
+// two f32 at a time
+__device__ __forceinline__ uint64_t pair_of(float a, float b)
+{
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void halves_of(uint64_t d, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// max(|a|, |b|) of two 16-bit floats each, with whatever sign; NaN wins
+template <typename T> __device__ __forceinline__ uint32_t larger_pair(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    if (std::is_same<T, __half>::value) asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// whole numbers of magnitudes up to 127 as bytes
 template <int N> struct Packed {
     uint32_t w[N / 4];
 };
-template <int N> __device__ __forceinline__ Packed<N> pack_codes(const float (&v)[N], float scale, float inverse)
-{
-    uint32_t m[N];
-    float off = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float t = __fmaf_rn(v[i], inverse, MAGIC);
-        m[i] = __float_as_uint(t);
-        off = fmaxf(off, fabsf(__fmaf_rn(v[i], inverse, __fsub_rn(MAGIC, t))));
+
+// What a row's values are multiplied by: the f32 numbers on both sides of 1 / scale.
+struct Inverse {
+    float scale;
+    uint64_t up, down;
+    __device__ __forceinline__ explicit Inverse(float s) : scale(s)
+    {
+        const uint32_t nearest = __float_as_uint(__frcp_rn(s));
+        const float u = __uint_as_float(nearest + 1), d = __uint_as_float(nearest - 1);
+        up = pair_of(u, u), down = pair_of(d, d);
     }
-    if (off > 0.5f - 0x1p-15f) { // some quotient may be nearer to the other neighbour
-#pragma unroll 1
-        for (int i = 0; i < N; ++i) m[i] = (uint32_t)__double2int_rn((double)v[i] / (double)scale);
+};
+
+template <int N> __device__ __forceinline__ Packed<N> pack_codes(const float (&v)[N], const Inverse &inverse)
+{
+    const uint64_t magic = pair_of(MAGIC, MAGIC), minus = pair_of(-1.0f, -1.0f);
+    float m[N];
+    uint64_t unlike = 0;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const uint64_t pair = pair_of(v[i], v[i + 1]), u = fma_pair(pair, inverse.up, magic), d = fma_pair(pair, inverse.down, magic);
+        const uint64_t off = fma_pair(d, minus, u);
+        unlike = fma_pair(off, off, unlike);
+        halves_of(u, m[i], m[i + 1]);
+    }
+    float ua, ub;
+    halves_of(unlike, ua, ub);
+    if (__builtin_expect(ua + ub > 0.0f, 0)) { // some quotient is next to a half
+        float down, unused;
+        halves_of(inverse.down, down, unused);
+        // twice the values where their difference could be below what f32 holds
+        const float scale = inverse.scale, twice = scale < 1.0f ? 2.0f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float a = m[i] - MAGIC, b = __fmaf_rn(v[i], down, MAGIC) - MAGIC;
+            if (a == b) continue;
+            const float lower = fminf(a, b), h = lower + 0.5f, beyond = __fmaf_rn(-(h * twice), scale, v[i] * twice); // which side of h: the sign is exact
+            m[i] = (beyond > 0.0f || (beyond == 0.0f && ((int)lower & 1)) ? lower + 1.0f : lower) + MAGIC;
+        }
     }
     Packed<N> out;
 #pragma unroll
     for (int i = 0; i < N / 4; ++i)
-        out.w[i] = __byte_perm(__byte_perm(m[4 * i], m[4 * i + 1], 0x0040), __byte_perm(m[4 * i + 2], m[4 * i + 3], 0x0040), 0x5410);
+        out.w[i] = __byte_perm(__byte_perm(__float_as_uint(m[4 * i]), __float_as_uint(m[4 * i + 1]), 0x0040),
+                               __byte_perm(__float_as_uint(m[4 * i + 2]), __float_as_uint(m[4 * i + 3]), 0x0040), 0x5410);
     return out;
 }
 
 // The two digits of u / t, |u / t| <= 16256: the high one is the whole number nearest to a 128th of it.
-template <int N> __device__ __forceinline__ void pack_digits(const float (&u)[N], float inverse, Packed<N> &high, Packed<N> &low)
+template <int N> __device__ __forceinline__ void pack_digits(const float (&u)[N], const Inverse &inverse, Packed<N> &high, Packed<N> &low)
 {
     uint32_t h[N], l[N];
+    float up, unused;
+    halves_of(inverse.up, up, unused);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int v = (int)__float_as_uint(__fmaf_rn(u[i], inverse, MAGIC)) - (int)__float_as_uint(MAGIC);
+        const int v = (int)__float_as_uint(__fmaf_rn(u[i], up, MAGIC)) - (int)__float_as_uint(MAGIC);
         const int top = (v + 64) >> 7; // -127 .. 127
         h[i] = (uint32_t)top, l[i] = (uint32_t)(v - (top << 7)); // -64 .. 63
     }
@@ -96,15 +161,18 @@ template <int N> __device__ __forceinline__ void pack_digits(const float (&u)[N]
     }
 }
 
-template <int N, bool ALIGNED> __device__ __forceinline__ void store_codes(int8_t *row, size_t k, size_t width, const Packed<N> &c)
+template <int N, int LANES, bool ALIGNED> __device__ __forceinline__ void store_codes(int8_t *row, size_t piece, int lane, size_t width, const Packed<N> &c)
 {
+    const size_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
     if (ALIGNED && k + N <= width) {
         if (N == 8) *reinterpret_cast<uint2 *>(row + k) = make_uint2(c.w[0], c.w[N / 4 - 1]);
         else *reinterpret_cast<uint32_t *>(row + k) = c.w[0];
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (k + i < width) row[k + i] = (int8_t)(c.w[i >> 2] >> (8 * (i & 3)));
+        for (int i = 0; i < N; ++i) {
+            const size_t at = column<N, LANES, ALIGNED>(piece, lane, i);
+            if (at < width) row[at] = (int8_t)(c.w[i >> 2] >> (8 * (i & 3)));
+        }
     }
 }
 
@@ -119,23 +187,100 @@ struct RowParams {
     int groups;
 };
 
-// Row r's column scales; null: the row belongs to no group.
+// Row r's column scales, by a whole warp; null: the row belongs to no group.
 __device__ __forceinline__ const float *columns_of(const RowParams &P, size_t r)
 {
     if (!P.offsets) return P.column_scales;
-    const long long row = (long long)r;
-    if (row < P.offsets[0] || row >= P.offsets[P.groups]) return nullptr;
-    int lo = 0, hi = P.groups - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (P.offsets[mid] <= row) lo = mid;
-        else hi = mid - 1;
+    int begun = 0; // offsets that are not behind the row
+    for (int g0 = 0; g0 <= P.groups; g0 += 32) {
+        const int g = g0 + (threadIdx.x & 31);
+        begun += __popc(__ballot_sync(~0u, g <= P.groups && P.offsets[g] <= (long long)r));
     }
-    return P.column_scales + (size_t)lo * P.width;
+    return begun == 0 || begun > P.groups ? nullptr : P.column_scales + (size_t)(begun - 1) * P.width;
 }
 
+// One row's arithmetic on pieces of it.
+template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
+    static constexpr int N = Piece<T>::N;
+    const RowParams &P;
+    size_t r;
+    int lane;
+    const float *columns;
+    bool columns4; // N neighbouring columns' scales are 16-byte aligned
+    uint32_t most = 0;
+
+    __device__ __forceinline__ RowOf(const RowParams &p, size_t row, int l, const float *c) : P(p), r(row), lane(l), columns(c), columns4(DIGITS == 2 && ALIGNED && p.width % 4 == 0) {}
+
+    __device__ __forceinline__ void values(const Piece<T> &p, size_t piece, float (&v)[N]) const
+    {
+        float c[N];
+        if (DIGITS == 2) {
+            const size_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
+            if (columns4 && k + N <= P.width) {
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(columns + k + i);
+                    c[i] = f.x, c[i + 1] = f.y, c[i + 2] = f.z, c[i + 3] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const size_t at = column<N, LANES, ALIGNED>(piece, lane, i);
+                    c[i] = at < P.width ? columns[at] : 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = DIGITS == 2 ? p.at(i) * c[i] : p.at(i);
+    }
+    // Magnitudes as whole numbers: their order is that of the bits, infinities and NaN on top.  (Two 16-bit ones at a time.)
+    __device__ __forceinline__ void look(const Piece<T> &p, size_t piece)
+    {
+        if (DIGITS == 1 && sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = larger_pair<T>(most, (&p.w.x)[i]);
+        } else {
+            float v[N];
+            values(p, piece, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) most = max(most, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        }
+    }
+    // the largest magnitude's bits, of the whole warp
+    __device__ __forceinline__ uint32_t largest() const
+    {
+        uint32_t m = most;
+        if (DIGITS == 1 && sizeof(T) == 2) {
+            Piece<T> one;
+            one.w = make_uint4(max(m & 0x7FFFu, (m >> 16) & 0x7FFFu), 0, 0, 0);
+            m = __float_as_uint(one.at(0)); // (a NaN stays one)
+        }
+        return __reduce_max_sync(~0u, m);
+    }
+    static __device__ __forceinline__ bool no_codes(uint32_t largest) { return largest == 0 || largest >= 0x7F800000u; }
+    static __device__ __forceinline__ float scale_of(uint32_t largest)
+    {
+        if (largest >= 0x7F800000u) return __int_as_float(0x7FC00000);
+        return largest == 0 ? 0.0f : fmaxf(__fdiv_rn(__uint_as_float(largest), DIGITS == 1 ? LARGEST_8 : LARGEST_15), 0x1p-126f);
+    }
+    __device__ __forceinline__ void pack(const Piece<T> &p, size_t piece, const Inverse &inverse, Packed<N> &high, Packed<N> &low) const
+    {
+        float v[N];
+        values(p, piece, v);
+        if (DIGITS == 1) high = pack_codes<N>(v, inverse);
+        else pack_digits<N>(v, inverse, high, low);
+    }
+    __device__ __forceinline__ void write(const Piece<T> &p, size_t piece, bool none, const Inverse &inverse) const
+    {
+        Packed<N> high = {}, low = {};
+        if (!none) pack(p, piece, inverse, high, low);
+        store_codes<N, LANES, ALIGNED>(P.codes + r * P.ld_codes, piece, lane, P.width, high);
+        if (DIGITS == 2) store_codes<N, LANES, ALIGNED>(P.low + r * P.ld_codes, piece, lane, P.width, low);
+    }
+};
+
 // LANES threads a row, HELD pieces a thread in registers; what is behind them is read a second time.
-template <typename T, int DIGITS, int LANES, int HELD, bool ALIGNED_X, bool ALIGNED_CODES>
+template <typename T, int DIGITS, int LANES, int HELD, bool ALIGNED>
 __global__ void __launch_bounds__(LANES < 128 ? 128 : LANES) quantize_rows_kernel(const RowParams P)
 {
     constexpr int N = Piece<T>::N, THREADS = LANES < 128 ? 128 : LANES, WARPS = LANES / 32;
@@ -148,89 +293,147 @@ __global__ void __launch_bounds__(LANES < 128 ? 128 : LANES) quantize_rows_kerne
     const T *row = static_cast<const T *>(P.x) + r * P.ld;
     const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr;
     if (DIGITS == 2 && !columns) return;
-
-    auto values = [&](const Piece<T> &p, size_t k, float(&v)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            v[i] = p.at(i);
-            if (DIGITS == 2) v[i] = k + i < P.width ? v[i] * columns[k + i] : 0.0f;
-        }
-    };
-    // magnitudes as whole numbers: their order is that of the bits, infinities and NaN on top
-    uint32_t most = 0;
-    auto look = [&](const Piece<T> &p, size_t k) {
-        float v[N];
-        values(p, k, v);
-#pragma unroll
-        for (int i = 0; i < N; ++i) most = max(most, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    };
+    const size_t pieces = (P.width + (size_t)LANES * N - 1) / ((size_t)LANES * N);
+    RowOf<T, DIGITS, LANES, ALIGNED> it(P, r, lane, columns);
     Piece<T> held[HELD];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) held[h] = load_values<T, ALIGNED_X>(row, (size_t)(h * LANES + lane) * N, P.width);
+    for (int h = 0; h < HELD; ++h) held[h] = load_values<T, LANES, ALIGNED>(row, h, lane, P.width);
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) look(held[h], (size_t)(h * LANES + lane) * N);
-    for (size_t k = (size_t)(HELD * LANES + lane) * N; k < P.width; k += (size_t)LANES * N) look(load_values<T, ALIGNED_X>(row, k, P.width), k);
-    most = __reduce_max_sync(~0u, most);
+    for (int h = 0; h < HELD; ++h) it.look(held[h], h);
+    for (size_t h = HELD; h < pieces; ++h) it.look(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h);
+    uint32_t most = it.largest();
     if (WARPS > 1) {
         if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = most;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) most = max(most, parts[w]);
     }
-    const bool finite = most < 0x7F800000u;
-    const float a = __uint_as_float(most);
-    const float scale = !finite ? __int_as_float(0x7FC00000) : most == 0 ? 0.0f : fmaxf(__fdiv_rn(a, DIGITS == 1 ? LARGEST_8 : LARGEST_15), 0x1p-126f);
+    const float scale = it.scale_of(most);
+    const bool none = it.no_codes(most);
     if (lane == 0) P.scales[r] = scale;
-    const bool none = !finite || most == 0; // all codes 0
-    const float inverse = none ? 0.0f : __frcp_rn(scale);
-    int8_t *codes = P.codes + r * P.ld_codes;
-    auto write = [&](const Piece<T> &p, size_t k) {
-        float v[N];
-        values(p, k, v);
+    const Inverse inverse(none ? 1.0f : scale);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = none ? 0.0f : v[i];
-        if (DIGITS == 1) {
-            store_codes<N, ALIGNED_CODES>(codes, k, P.width, pack_codes<N>(v, none ? 1.0f : scale, inverse));
-        } else {
-            Packed<N> high, low;
-            pack_digits<N>(v, inverse, high, low);
-            store_codes<N, ALIGNED_CODES>(codes, k, P.width, high);
-            store_codes<N, ALIGNED_CODES>(P.low + r * P.ld_codes, k, P.width, low);
-        }
-    };
-#pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        const size_t k = (size_t)(h * LANES + lane) * N;
-        if (k < P.width) write(held[h], k);
-    }
-    for (size_t k = (size_t)(HELD * LANES + lane) * N; k < P.width; k += (size_t)LANES * N) write(load_values<T, ALIGNED_X>(row, k, P.width), k);
+    for (int h = 0; h < HELD; ++h)
+        if (column<N, LANES, ALIGNED>(h, lane, 0) < P.width) it.write(held[h], h, none, inverse);
+    for (size_t h = HELD; h < pieces; ++h) it.write(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h, none, inverse);
 }
 
-template <typename T, int DIGITS, int LANES, int HELD> void quantize_rows_with(CudaDevice &dev, const RowParams &P, bool aligned_x, bool aligned_codes)
+// Many aligned rows: a block stays on its SM, every warp has `slots` rows in shared memory on their way (bulk copies) while it works on the one
+// before them, reading it twice from there.
+constexpr int STREAM_WARPS = 24, STREAM_SLOTS = 4; // at most
+constexpr size_t STREAM_BYTES = 192 << 10;
+
+template <typename T, int DIGITS> __global__ void __launch_bounds__(32 * STREAM_WARPS) stream_rows_kernel(const RowParams P, int slots, int *error)
+{
+    constexpr int N = Piece<T>::N;
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ unsigned long long full[STREAM_WARPS * STREAM_SLOTS];
+    __shared__ int abort_word;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const uint32_t bytes = (uint32_t)(P.width * sizeof(T));
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < warps * slots; ++i) mbar_init(&full[i], 1);
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    rows_are_there();
+    product_may_start();
+    const size_t first = (size_t)blockIdx.x * warps + warp, step = (size_t)gridDim.x * warps;
+    unsigned char *mine = ring + (size_t)warp * slots * bytes;
+    unsigned long long *bars = full + warp * slots;
+    auto fetch = [&](size_t r, int slot) {
+        mbar_expect_tx(&bars[slot], bytes);
+        bulk_load_1d(mine + (size_t)slot * bytes, static_cast<const T *>(P.x) + r * P.ld, bytes, &bars[slot]);
+    };
+    if (lane == 0)
+        for (int i = 0; i < slots && first + i * step < P.n; ++i) fetch(first + i * step, i);
+    const int last = (int)(bytes / 16); // 16-byte pieces of the row
+    int slot = 0;
+    uint32_t parity = 0;
+    for (size_t r = first; r < P.n; r += step) {
+        if (!__all_sync(~0u, mbar_wait(&bars[slot], parity, &abort_word, error, 71))) { // nothing is on its way to a block that has left
+            for (int i = 0; i < slots; ++i) {
+                if (r + i * step < P.n) mbar_wait(&bars[slot], parity, &abort_word, error, 72);
+                if (++slot == slots) slot = 0, parity ^= 1u;
+            }
+            break;
+        }
+        const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr;
+        if (DIGITS == 1 || columns) {
+            RowOf<T, DIGITS, 32, true> it(P, r, lane, columns);
+            const uint4 *row = reinterpret_cast<const uint4 *>(mine + (size_t)slot * bytes);
+#pragma unroll 4
+            for (int i = lane; i < last; i += 32) it.look(Piece<T>{row[i]}, i >> 5);
+            const uint32_t most = it.largest();
+            const float scale = it.scale_of(most);
+            if (lane == 0) P.scales[r] = scale;
+            int8_t *codes = P.codes + r * P.ld_codes, *lows = DIGITS == 2 ? P.low + r * P.ld_codes : nullptr;
+            auto put = [&](int8_t *to, int i, const Packed<N> &c) {
+                if (N == 8) reinterpret_cast<uint2 *>(to)[i] = make_uint2(c.w[0], c.w[N / 4 - 1]);
+                else reinterpret_cast<uint32_t *>(to)[i] = c.w[0];
+            };
+            if (it.no_codes(most)) {
+                for (int i = lane; i < last; i += 32) {
+                    put(codes, i, Packed<N>{});
+                    if (DIGITS == 2) put(lows, i, Packed<N>{});
+                }
+            } else {
+                const Inverse inverse(scale);
+#pragma unroll 4
+                for (int i = lane; i < last; i += 32) {
+                    Packed<N> high, low;
+                    it.pack(Piece<T>{row[i]}, i >> 5, inverse, high, low);
+                    put(codes, i, high);
+                    if (DIGITS == 2) put(lows, i, low);
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0 && r + slots * step < P.n) fetch(r + slots * step, slot);
+        if (++slot == slots) slot = 0, parity ^= 1u;
+    }
+}
+
+template <typename T, int DIGITS, int LANES, int HELD> void quantize_rows_with(CudaDevice &dev, const RowParams &P, bool aligned)
 {
     constexpr int THREADS = LANES < 128 ? 128 : LANES, ROWS = THREADS / LANES;
     const dim3 grid((unsigned)((P.n + ROWS - 1) / ROWS));
-    if (aligned_x && aligned_codes) launch_following(quantize_rows_kernel<T, DIGITS, LANES, HELD, true, true>, grid, dim3(THREADS), 0, dev.stream(), P);
-    else if (aligned_codes) launch_following(quantize_rows_kernel<T, DIGITS, LANES, HELD, false, true>, grid, dim3(THREADS), 0, dev.stream(), P);
-    else launch_following(quantize_rows_kernel<T, DIGITS, LANES, HELD, false, false>, grid, dim3(THREADS), 0, dev.stream(), P);
+    if (aligned) launch_following(quantize_rows_kernel<T, DIGITS, LANES, HELD, true>, grid, dim3(THREADS), 0, dev.stream(), P);
+    else launch_following(quantize_rows_kernel<T, DIGITS, LANES, HELD, false>, grid, dim3(THREADS), 0, dev.stream(), P);
 }
 
+// A warp a row where there are rows enough for eight warps an SM (no block barrier, all of a row's loads under way at once), otherwise, or
+// where a row does not fit a warp's registers, 256 threads.
 template <typename T, int DIGITS> void quantize_rows_typed(CudaDevice &dev, const RowParams &P)
 {
-    const bool aligned_x = (reinterpret_cast<uintptr_t>(P.x) | (P.ld * sizeof(T))) % 16 == 0;
-    const bool aligned_codes = (reinterpret_cast<uintptr_t>(P.codes) | P.ld_codes | reinterpret_cast<uintptr_t>(P.low)) % 8 == 0;
+    const bool aligned = (reinterpret_cast<uintptr_t>(P.x) | (P.ld * sizeof(T))) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.codes) | P.ld_codes | reinterpret_cast<uintptr_t>(P.low)) % 8 == 0;
     const size_t pieces = (P.width + Piece<T>::N - 1) / Piece<T>::N;
-    if (pieces <= 32 * 4) quantize_rows_with<T, DIGITS, 32, 4>(dev, P, aligned_x, aligned_codes);
-    else quantize_rows_with<T, DIGITS, 256, 4>(dev, P, aligned_x, aligned_codes);
+    const bool warps = P.n >= (size_t)dev.sm_count() * 8;
+    const size_t bytes = P.width * sizeof(T);
+    if (aligned && bytes % 16 == 0 && bytes >= 1024 && bytes * 12 <= STREAM_BYTES && P.n >= (size_t)dev.sm_count() * 12 && dev.error_word()) {
+        const int stream_warps = (int)std::min<size_t>(STREAM_WARPS, STREAM_BYTES / bytes), slots = (int)std::min<size_t>(STREAM_SLOTS, STREAM_BYTES / (bytes * stream_warps));
+        allow_shared_memory(dev, stream_rows_kernel<T, DIGITS>);
+        launch_following(stream_rows_kernel<T, DIGITS>, dim3((unsigned)dev.sm_count()), dim3(32 * stream_warps), slots * bytes * stream_warps, dev.stream(), P, slots, dev.error_word());
+        return;
+    }
+    if (pieces <= 32 * 2) quantize_rows_with<T, DIGITS, 32, 2>(dev, P, aligned);
+    else if (warps && pieces <= 32 * 4) quantize_rows_with<T, DIGITS, 32, 4>(dev, P, aligned);
+    else if (warps && pieces <= 32 * 8) quantize_rows_with<T, DIGITS, 32, 8>(dev, P, aligned);
+    else if (warps && pieces <= 32 * 16) quantize_rows_with<T, DIGITS, 32, 16>(dev, P, aligned);
+    else if (pieces <= 256 * 2) quantize_rows_with<T, DIGITS, 256, 2>(dev, P, aligned);
+    else if (pieces <= 256 * 4) quantize_rows_with<T, DIGITS, 256, 4>(dev, P, aligned);
+    else quantize_rows_with<T, DIGITS, 256, 8>(dev, P, aligned);
 }
 
 template <int DIGITS> void quantize_rows_any(CudaDevice &dev, const char *name, const RowParams &P, int type)
 {
     if (P.n == 0) return;
     KernelScope ks(dev, name);
-    if (type == VALUE_F32) quantize_rows_typed<float, DIGITS>(dev, P);
-    else if (type == VALUE_F16) quantize_rows_typed<__half, DIGITS>(dev, P);
-    else quantize_rows_typed<__nv_bfloat16, DIGITS>(dev, P);
+    if (type == VALUE_F16) quantize_rows_typed<__half, DIGITS>(dev, P);
+    else if (type == VALUE_BF16) quantize_rows_typed<__nv_bfloat16, DIGITS>(dev, P);
+    else if (DIGITS == 1) quantize_rows_typed<float, 1>(dev, P); // (two digits are 16-bit rows')
     dev.count_launch();
 }
 
