@@ -1,15 +1,17 @@
 // product_tc.cu -- the products of codes on the tensor cores (tcgen05, kind::i8, whole-number sums in tensor memory).
 //
 // Channels are the accumulator's lanes and rows of codes its columns, so that a tile can have any number of rows (a group's last
-// ones, a few tokens) at the cost of 32 each, and the result of one row leaves in pieces of 32 neighbouring channels.  A CTA keeps
-// taking tiles of 128 channels x up to 256 rows:
+// ones, a few tokens) at the cost of 32 each, and the result of one row leaves in pieces of 32 neighbouring channels.  Two CTAs of a
+// cluster (one pair of SMs, cta_group::2) keep taking tiles of 256 channels x up to 256 rows: each fetches its 128 channels and one half of
+// the rows, both halves are multiplied with both CTAs' channels, and each has its channels' sums in its own tensor memory.
 //
-//   warp 0      TMA: 128 bytes of 128 channels and of the tile's rows a stage, four stages
-//   warp 1      one thread issues tcgen05.mma, 4 x 32 bytes a stage; two accumulators of 256 columns, so that the next tile's sums
-//               begin while the last one's leave
+//   warp 0      TMA: 128 bytes of 128 channels and of half the tile's rows a stage, six stages
+//   warp 1      in the first CTA one thread issues tcgen05.mma for both, 4 x 32 bytes a stage; two accumulators of 256 columns,
+//               so that the next tile's sums begin while the last one's leave
 //   warps 2-5   epilogue: scales, bias, rounding, stores
 //
-// Two digits (gradients): the columns' first half are the rows' high digits, the second half the low ones; the epilogue joins them.
+// Two digits (gradients): the first CTA fetches the rows' high digits and the second one their low digits, so that the columns' first
+// half are the high sums and the second half the low ones; the epilogue joins them.
 #include <algorithm>
 
 #include "cuda_device.hpp"
@@ -21,15 +23,15 @@ namespace vqb {
 
 namespace {
 
-constexpr int BM = 128;        // channels a tile
+constexpr int BM = 128;        // channels a CTA and tile
 constexpr int MOST_COLS = 256; // accumulator columns a tile
 constexpr int KB = 128;        // bytes of K a stage: one swizzled row
-constexpr int NST = 4;
+constexpr int NST = 6;
 constexpr int THREADS = 192;
-constexpr uint32_t A_BYTES = BM * KB, B_BYTES = MOST_COLS * KB;
+constexpr uint32_t A_BYTES = BM * KB, B_BYTES = MOST_COLS / 2 * KB;
 
 struct alignas(8) Barriers {
-    unsigned long long full[NST], empty[NST], tfull[2], tempty[2], drained;
+    unsigned long long full[NST], empty[NST], tfull[2], tempty[2], drained; // full, tempty, drained: the first CTA's count for both
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -41,21 +43,52 @@ struct TcParams {
     void *y;
     size_t y_ld;
     int tile_rows; // rows a tile, a multiple of 32; times DIGITS at most 256
-    int box_rows;  // rows a token load brings
+    int box_rows;  // rows a token load brings: tile_rows x DIGITS / 2
     int band;      // tiles of rows that are taken together for one tile of channels
     int zero_rest, rows_follow;
     int *error;
 };
 
-// kind::i8: signed operands, 32-bit sums, both K-major, M = 128, N = n
-__device__ __forceinline__ uint32_t idesc_i8(int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24); }
+// kind::i8: signed operands, 32-bit sums, both K-major, M = 256 (two CTAs), N = n
+__device__ __forceinline__ uint32_t idesc_i8(int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(2 * BM >> 4) << 24); }
 
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(tmem_d),
-                 "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
+                 "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+                 "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
                  : "memory");
+}
+
+// Arrives at the same barrier of both CTAs once all that this thread has issued is done.
+__device__ __forceinline__ void commit_both(void *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void commit_here(void *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// The address of the first CTA's copy of a shared-memory object.
+__device__ __forceinline__ uint32_t in_first(const void *p)
+{
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+    return a;
+}
+// A load into this CTA that counts at a barrier of the first one (no multicast).
+__device__ __forceinline__ void tma_load_counted(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)), "l"(map),
+                 "r"(bar), "r"(c0), "r"(c1)
+                 : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 struct Tile {
@@ -72,18 +105,14 @@ __device__ __forceinline__ Tile tile_at(const TcParams &P, const RowTiles &tiles
     const int u = b * P.band + in % here;
     Tile t;
     t.group = tiles.group_of(u, P.groups);
-    t.channel0 = in / here * BM;
+    t.channel0 = in / here * (2 * BM);
     t.row0 = tiles.first[t.group] + (u - tiles.before[t.group]) * P.tile_rows;
     t.rows = min(P.tile_rows, tiles.end[t.group] - t.row0);
     return t;
 }
 
-// Accumulator columns of one digit: rows in steps of 32.  The low digits' rows begin where the loads of the high ones end.
-template <int DIGITS> __device__ __forceinline__ int columns_of(const TcParams &P, int rows)
-{
-    const int step = DIGITS == 2 ? P.box_rows : 32;
-    return (rows + step - 1) / step * step;
-}
+// Accumulator columns of one digit: rows in steps of 32 (16 for each CTA to fetch; with two digits each fetches them all).
+__device__ __forceinline__ int columns_of(int rows) { return (rows + 31) / 32 * 32; }
 
 template <typename T, int DIGITS>
 __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rows, const TcParams P)
@@ -96,6 +125,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     RowTiles tiles(bars + 1, P.groups);
     volatile int *abort_flag = &bars->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int half = blockIdx.x & 1; // this CTA's place in its cluster
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NST; ++s) {
@@ -104,7 +134,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bars->tfull[b], 1);
-            mbar_init(&bars->tempty[b], 4);
+            mbar_init(&bars->tempty[b], 8);
         }
         mbar_init(&bars->drained, 1);
         bars->abort_flag = 0;
@@ -112,84 +142,98 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     // Codes of the matrix may be fetched before the rows' are there, where only those are new.
     const bool codes_first = P.rows_follow && !P.offsets;
     if (!codes_first) rows_are_there();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     tiles.build(P.offsets, P.groups, P.n, P.tile_rows); // (block barriers)
+    cluster_sync();                                     // both CTAs' barriers are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = bars->tmem_base;
-    const int channel_tiles = (P.channels + BM - 1) / BM, chunks = (P.width + KB - 1) / KB;
+    const int channel_tiles = (P.channels + 2 * BM - 1) / (2 * BM), chunks = (P.width + KB - 1) / KB;
     const long long total = (long long)tiles.before[P.groups] * channel_tiles;
+    const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t it = 0;
+            int st = 0;
+            uint32_t parity = 0; // of the stages' current round
             bool ok = true, waited = !codes_first;
-            auto load_rows = [&](const Tile &t, int columns, int c, int st) {
-                unsigned char *to = b_smem + st * B_BYTES;
-                for (int d = 0; d < DIGITS; ++d, to += columns * KB)
-                    for (int i = 0; i < columns; i += P.box_rows) tma_load_2d(to + i * KB, &map_rows, c * KB, d * P.n + t.row0 + i, &bars->full[st]);
-            };
-            for (long long id = blockIdx.x; ok && id < total; id += gridDim.x) {
+            const uint32_t bytes = 2 * (A_BYTES + (uint32_t)P.box_rows * KB), full0 = in_first(&bars->full[0]);
+            unsigned long long loads = 0;
+            for (long long id = first; ok && id < total; id += step) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
-                const int columns = columns_of<DIGITS>(P, t.rows);
-                const uint32_t bytes = A_BYTES + (uint32_t)(DIGITS * ((columns + P.box_rows - 1) / P.box_rows) * P.box_rows * KB);
+                // this CTA's rows: one half of the columns, or one digit of all
+                const int row = DIGITS == 2 ? half * P.n + t.row0 : t.row0 + half * (columns_of(t.rows) / 2);
+                const int channel = t.group * P.channels + t.channel0 + half * BM;
                 const int ahead = waited ? 0 : min(NST, chunks);
-                for (int c = 0; c < chunks; ++c, ++it) {
-                    const int st = it % NST;
-                    if (!mbar_wait(&bars->empty[st], ((it / NST) & 1u) ^ 1u, abort_flag, P.error, 61)) {
+                for (int c = 0; c < chunks; ++c) {
+                    if (!mbar_wait(&bars->empty[st], parity ^ 1u, abort_flag, P.error, 61)) {
                         ok = false;
                         break;
                     }
-                    mbar_expect_tx(&bars->full[st], bytes);
-                    tma_load_2d(a_smem + st * A_BYTES, &map_codes, c * KB, t.group * P.channels + t.channel0, &bars->full[st]);
-                    if (c + 1 < ahead) continue;
-                    if (!waited) {
-                        rows_are_there();
-                        waited = true;
-                        for (int e = 0; e < ahead; ++e) load_rows(t, columns, e, e);
-                    } else {
-                        load_rows(t, columns, c, st);
+                    if (half == 0) mbar_expect_tx(&bars->full[st], bytes);
+                    tma_load_counted(a_smem + st * A_BYTES, &map_codes, c * KB, channel, full0 + 8u * st);
+                    ++loads;
+                    if (c + 1 >= ahead) {
+                        if (!waited) {
+                            rows_are_there();
+                            waited = true;
+                            for (int e = 0; e < ahead; ++e) tma_load_counted(b_smem + e * B_BYTES, &map_rows, e * KB, row, full0 + 8u * e);
+                        } else {
+                            tma_load_counted(b_smem + st * B_BYTES, &map_rows, c * KB, row, full0 + 8u * st);
+                        }
                     }
+                    if (++st == NST) st = 0, parity ^= 1u;
                 }
             }
             if (!waited) rows_are_there();
-            // what has been asked for has landed before the block leaves (a tile that is finished has been waited for)
-            if (!ok)
-                for (uint32_t i = it > NST ? it - NST : 0; i < it; ++i) mbar_wait(&bars->full[i % NST], (i / NST) & 1u, abort_flag, P.error, 62);
+            if (ok) { // the tensor core's arrivals here have come before the block leaves
+                for (int i = 0; i < NST; ++i) {
+                    if (loads + i >= NST) mbar_wait(&bars->empty[st], parity ^ 1u, abort_flag, P.error, 62);
+                    if (++st == NST) st = 0, parity ^= 1u;
+                }
+            } else { // what has been asked for lands
+                for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+            }
         } else if (codes_first) {
             rows_are_there();
         }
     } else if (warp == 1) {
         if (codes_first) rows_are_there();
-        if (lane == 0) {
-            uint32_t it = 0, local = 0;
+        if (half == 0 && elect_one()) {
+            int st = 0;
+            uint32_t parity = 0, local = 0;
             bool ok = true;
-            for (long long id = blockIdx.x; ok && id < total; id += gridDim.x, ++local) {
+            const uint64_t a0 = smem_desc_sw128(smem_u32(a_smem)), r0 = smem_desc_sw128(smem_u32(b_smem));
+            for (long long id = first; ok && id < total; id += step, ++local) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
-                const uint32_t b = local & 1u, idesc = idesc_i8(DIGITS * columns_of<DIGITS>(P, t.rows)), d_tmem = tmem_base + b * MOST_COLS;
+                const uint32_t b = local & 1u, idesc = idesc_i8(DIGITS * columns_of(t.rows)), d_tmem = tmem_base + b * MOST_COLS;
                 if (!mbar_wait(&bars->tempty[b], ((local >> 1) & 1u) ^ 1u, abort_flag, P.error, 63)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int c = 0; c < chunks; ++c, ++it) {
-                    const int st = it % NST;
-                    if (!mbar_wait(&bars->full[st], (it / NST) & 1u, abort_flag, P.error, 64)) {
+                for (int c = 0; c < chunks; ++c) {
+                    if (!mbar_wait(&bars->full[st], parity, abort_flag, P.error, 64)) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t a = smem_desc_sw128(smem_u32(a_smem + st * A_BYTES)), r = smem_desc_sw128(smem_u32(b_smem + st * B_BYTES));
-                    const int steps = min(KB / 32, (P.width - c * KB + 31) / 32);
-                    for (int s = 0; s < steps; ++s) umma_i8(d_tmem, a + (uint64_t)(2 * s), r + (uint64_t)(2 * s), idesc, (c | s) ? 1u : 0u);
-                    umma_commit(&bars->empty[st]);
+                    const uint64_t a = a0 + (uint32_t)(st * (int)(A_BYTES >> 4)), r = r0 + (uint32_t)(st * (int)(B_BYTES >> 4));
+                    // Always four: behind the width there are zeros.  (Rolled up, with a count, one such instruction took 54 ns to issue, as long
+                    // as the tensor core needs for 200 columns; a stage 0.42 instead of 0.27 us.)
+                    umma_i8(d_tmem, a, r, idesc, (uint32_t)c);
+                    umma_i8(d_tmem, a + 2, r + 2, idesc, 1u);
+                    umma_i8(d_tmem, a + 4, r + 4, idesc, 1u);
+                    umma_i8(d_tmem, a + 6, r + 6, idesc, 1u);
+                    commit_both(&bars->empty[st]);
+                    if (++st == NST) st = 0, parity ^= 1u;
                 }
-                if (ok) umma_commit(&bars->tfull[b]);
+                if (ok) commit_both(&bars->tfull[b]);
             }
-            if (*abort_flag) { // nothing of the tensor core's is under way when the block leaves
-                umma_commit(&bars->drained);
+            if (*abort_flag) { // nothing of the tensor core's is under way when the blocks leave
+                commit_here(&bars->drained);
                 mbar_wait(&bars->drained, 0, abort_flag, P.error, 65);
             }
         }
@@ -199,10 +243,10 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         float *mine = scales_smem + q * MOST_COLS;
         T *y = static_cast<T *>(P.y);
         uint32_t local = 0;
-        for (long long id = blockIdx.x; id < total; id += gridDim.x, ++local) {
+        for (long long id = first; id < total; id += step, ++local) {
             const Tile t = tile_at(P, tiles, id, channel_tiles);
             const uint32_t b = local & 1u;
-            const int channel = t.channel0 + 32 * q + lane, columns = columns_of<DIGITS>(P, t.rows);
+            const int channel = t.channel0 + half * BM + 32 * q + lane, columns = columns_of(t.rows);
             const bool there = channel < P.channels;
             const size_t at = (size_t)t.group * P.channels + channel;
             const float channel_scale = !there ? 0.0f : P.channel_scales ? P.channel_scales[at] : 1.0f, bias = there && P.bias ? P.bias[at] : 0.0f;
@@ -227,17 +271,18 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->tempty[b]);
+            if (lane == 0) arrive_at(in_first(&bars->tempty[b]));
         }
         if (P.zero_rest)
             zero_rest<T>(y, P.y_ld, P.channels, P.n, tiles.first[0], tiles.end[P.groups - 1], (size_t)blockIdx.x * 128 + (threadIdx.x - 64), (size_t)gridDim.x * 128);
     }
 
+    __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    cluster_sync(); // neither CTA's shared memory and barriers are needed any more
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     }
 }
 
@@ -245,7 +290,7 @@ template <typename T, int DIGITS> void product_tc_typed(CudaDevice &dev, const P
 {
     const size_t smem = 1024 + NST * (A_BYTES + B_BYTES) + 4 * MOST_COLS * sizeof(float) + sizeof(Barriers) + RowTiles::bytes(p.groups);
     allow_shared_memory(dev, product_tc_kernel<T, DIGITS>);
-    launch_following(product_tc_kernel<T, DIGITS>, dim3(grid), dim3(THREADS), smem, dev.stream(), map_codes, map_rows, P);
+    launch_following_clusters(product_tc_kernel<T, DIGITS>, dim3(grid), dim3(THREADS), smem, 2, dev.stream(), map_codes, map_rows, P);
 }
 
 template <typename T> void product_tc_digits(CudaDevice &dev, const Product &p, TcParams &P, const CUtensorMap &mc, const CUtensorMap &mr, unsigned grid)
@@ -264,20 +309,23 @@ void launch_product(CudaDevice &dev, const Product &p)
     P.offsets = reinterpret_cast<const long long *>(p.offsets);
     P.channel_scales = p.channel_scales, P.row_scales = p.row_scales, P.bias = p.bias;
     P.y = p.y, P.y_ld = p.y_ld, P.zero_rest = p.zero_rest, P.rows_follow = p.rows_follow, P.error = dev.error_word();
-    const size_t most = MOST_COLS / p.digits;
-    if (p.offsets) {
-        P.tile_rows = (int)most;
-        P.box_rows = p.n / p.groups >= 64 ? 64 : 32;
-    } else { // as few tiles as there can be, of the same size
-        const size_t tiles = (p.n + most - 1) / most;
-        P.tile_rows = (int)(((p.n + tiles - 1) / tiles + 31) / 32 * 32);
-        P.box_rows = P.tile_rows;
+    const size_t pairs = (size_t)dev.sm_count() / 2, channel_tiles = (p.channels + 2 * BM - 1) / (2 * BM);
+    const size_t a_group = (p.n + p.groups - 1) / p.groups; // rows
+    // The tile's rows: whatever makes the fewest rounds of all SM pairs last the shortest.  A stage's time is its rows', but not below that
+    // of some 64: the channels' bytes have to come in.
+    size_t best = 32, least = ~size_t(0);
+    for (size_t rows = 32; rows * p.digits <= MOST_COLS; rows += 32) {
+        const size_t tiles = p.groups * ((a_group + rows - 1) / rows) * channel_tiles, cost = (tiles + pairs - 1) / pairs * (std::max<size_t>(rows * p.digits, 64) + 16);
+        if (cost <= least) best = rows, least = cost;
     }
+    if (const char *e = getenv("VQB_TILE")) best = atoi(e);
+    P.tile_rows = (int)best;
+    P.box_rows = P.tile_rows * p.digits / 2;
     P.band = 8;
     const CUtensorMap map_codes = make_tensor_map_2d<int8_t>(p.codes, p.width, p.groups * p.channels, KB, BM, CU_TENSOR_MAP_SWIZZLE_128B, codes_ld(p.width));
     const CUtensorMap map_rows = make_tensor_map_2d<int8_t>(p.rows, p.width, p.digits * p.n, KB, (unsigned)P.box_rows, CU_TENSOR_MAP_SWIZZLE_128B, p.rows_ld);
     const size_t row_tiles = p.offsets ? p.n / P.tile_rows + p.groups : (p.n + P.tile_rows - 1) / P.tile_rows;
-    const unsigned grid = (unsigned)std::min<size_t>((size_t)dev.sm_count(), row_tiles * ((p.channels + BM - 1) / BM));
+    const unsigned grid = 2 * (unsigned)std::min<size_t>(pairs, row_tiles * channel_tiles);
     KernelScope ks(dev, "product_tc");
     if (p.y_type == VALUE_F32) product_tc_digits<float>(dev, p, P, map_codes, map_rows, grid);
     else if (p.y_type == VALUE_F16) product_tc_digits<__half>(dev, p, P, map_codes, map_rows, grid);
