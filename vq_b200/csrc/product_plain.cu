@@ -48,11 +48,11 @@ template <typename T, int DIGITS> __global__ void __launch_bounds__(256) product
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     T *y = static_cast<T *>(P.y);
     if (P.zero_rest)
-        zero_rest<T>(y, P.y_ld, P.channels, P.n, tiles.first[0], tiles.end[P.groups - 1], (size_t)blockIdx.x * blockDim.x + threadIdx.x, (size_t)gridDim.x * blockDim.x);
+        zero_rest<T>(y, P.y_ld, P.channels, P.n, tiles.first[0], tiles.end(P.groups - 1), (size_t)blockIdx.x * blockDim.x + threadIdx.x, (size_t)gridDim.x * blockDim.x);
     for (long long tile = blockIdx.x; tile < total; tile += gridDim.x) {
         const int u = (int)(tile / per_row_tile), j0 = (int)(tile % per_row_tile) * TILE;
         const int g = tiles.group_of(u, P.groups);
-        const int r0 = tiles.first[g] + (u - tiles.before[g]) * TILE, rows = min(TILE, tiles.end[g] - r0), channels = min(TILE, P.channels - j0);
+        const int r0 = tiles.first[g] + (u - tiles.before[g]) * TILE, rows = min(TILE, tiles.end(g) - r0), channels = min(TILE, P.channels - j0);
         int sum[DIGITS][4][4] = {};
         for (int k0 = 0; k0 < P.width; k0 += BYTES) {
             __syncthreads();

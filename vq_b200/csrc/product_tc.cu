@@ -8,7 +8,8 @@
 //   warp 0      TMA: 128 bytes of 128 channels and of half the tile's rows a stage, six stages
 //   warp 1      in the first CTA one thread issues tcgen05.mma for both, 4 x 32 bytes a stage; two accumulators of 256 columns,
 //               so that the next tile's sums begin while the last one's leave
-//   warps 2-5   epilogue: scales, bias, rounding, stores
+//   warps 2-9   epilogue: scales, bias, rounding, stores; two warps share the lanes that either may read and take turns at 32 columns each.
+//               16-bit results go through shared memory, two rows' values of a channel in a word, and leave 16 bytes at a time
 //
 // Two digits (gradients): the first CTA fetches the rows' high digits and the second one their low digits, so that the columns' first
 // half are the high sums and the second half the low ones; the epilogue joins them.
@@ -27,7 +28,8 @@ constexpr int BM = 128;        // channels a CTA and tile
 constexpr int MOST_COLS = 256; // accumulator columns a tile
 constexpr int KB = 128;        // bytes of K a stage: one swizzled row
 constexpr int NST = 6;
-constexpr int THREADS = 192;
+constexpr int EPILOGUE_WARPS = 8, THREADS = 64 + 32 * EPILOGUE_WARPS;
+constexpr int STAGE_WORDS = 36; // 32 channels' words and 16 bytes, so that rows start in different banks
 constexpr uint32_t A_BYTES = BM * KB, B_BYTES = MOST_COLS / 2 * KB;
 
 struct alignas(8) Barriers {
@@ -46,6 +48,7 @@ struct TcParams {
     int box_rows;  // rows a token load brings: tile_rows x DIGITS / 2
     int band;      // tiles of rows that are taken together for one tile of channels
     int zero_rest, rows_follow;
+    int wide; // results can be stored 16 bytes at a time
     int *error;
 };
 
@@ -91,23 +94,35 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// two results of one channel, of the rows 2 i (low half) and 2 i + 1
+template <typename T> __device__ __forceinline__ uint32_t two_values(float a, float b);
+template <> __device__ __forceinline__ uint32_t two_values<__half>(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t two_values<__nv_bfloat16>(float a, float b)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t two_values<float>(float, float) { return 0; } // (f32 leaves as it is)
+
 struct Tile {
     int group, channel0, row0, rows;
 };
 
 // Tile number id: `band` tiles of rows for one tile of channels, then the next channels, then the next band.  What a wave of CTAs reads is
 // then some channels and some rows, instead of all channels for each tile of rows.
-__device__ __forceinline__ Tile tile_at(const TcParams &P, const RowTiles &tiles, long long id, int channel_tiles)
+__device__ __forceinline__ Tile tile_at(const TcParams &P, const RowTiles &tiles, int id, int channel_tiles)
 {
-    const int all = tiles.before[P.groups];
-    const long long per_band = (long long)P.band * channel_tiles;
-    const int b = (int)(id / per_band), in = (int)(id % per_band), here = min(P.band, all - b * P.band);
-    const int u = b * P.band + in % here;
+    const int per_band = P.band * channel_tiles, b = id / per_band, in = id - b * per_band, here = min(P.band, tiles.before[P.groups] - b * P.band);
+    const int c = in / here, u = b * P.band + in - c * here;
     Tile t;
     t.group = tiles.group_of(u, P.groups);
-    t.channel0 = in / here * (2 * BM);
+    t.channel0 = c * (2 * BM);
     t.row0 = tiles.first[t.group] + (u - tiles.before[t.group]) * P.tile_rows;
-    t.rows = min(P.tile_rows, tiles.end[t.group] - t.row0);
+    t.rows = min(P.tile_rows, tiles.end(t.group) - t.row0);
     return t;
 }
 
@@ -120,8 +135,9 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     extern __shared__ unsigned char smem_raw[];
     unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *a_smem = base, *b_smem = base + NST * A_BYTES;
-    float *scales_smem = reinterpret_cast<float *>(b_smem + NST * B_BYTES); // 4 warps x 256
-    Barriers *bars = reinterpret_cast<Barriers *>(scales_smem + 4 * MOST_COLS);
+    float *scales_smem = reinterpret_cast<float *>(b_smem + NST * B_BYTES);                                 // 8 warps x 128
+    uint32_t *out_smem = reinterpret_cast<uint32_t *>(scales_smem + EPILOGUE_WARPS * MOST_COLS / 2);        // 8 warps x 16 x STAGE_WORDS
+    Barriers *bars = reinterpret_cast<Barriers *>(out_smem + EPILOGUE_WARPS * 16 * STAGE_WORDS);
     RowTiles tiles(bars + 1, P.groups);
     volatile int *abort_flag = &bars->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -134,7 +150,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bars->tfull[b], 1);
-            mbar_init(&bars->tempty[b], 8);
+            mbar_init(&bars->tempty[b], 2 * EPILOGUE_WARPS);
         }
         mbar_init(&bars->drained, 1);
         bars->abort_flag = 0;
@@ -154,8 +170,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = bars->tmem_base;
     const int channel_tiles = (P.channels + 2 * BM - 1) / (2 * BM), chunks = (P.width + KB - 1) / KB;
-    const long long total = (long long)tiles.before[P.groups] * channel_tiles;
-    const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int total = tiles.before[P.groups] * channel_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -164,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             bool ok = true, waited = !codes_first;
             const uint32_t bytes = 2 * (A_BYTES + (uint32_t)P.box_rows * KB), full0 = in_first(&bars->full[0]);
             unsigned long long loads = 0;
-            for (long long id = first; ok && id < total; id += step) {
+            for (int id = first; ok && id < total; id += step) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
                 // this CTA's rows: one half of the columns, or one digit of all
                 const int row = DIGITS == 2 ? half * P.n + t.row0 : t.row0 + half * (columns_of(t.rows) / 2);
@@ -209,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             uint32_t parity = 0, local = 0;
             bool ok = true;
             const uint64_t a0 = smem_desc_sw128(smem_u32(a_smem)), r0 = smem_desc_sw128(smem_u32(b_smem));
-            for (long long id = first; ok && id < total; id += step, ++local) {
+            for (int id = first; ok && id < total; id += step, ++local) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
                 const uint32_t b = local & 1u, idesc = idesc_i8(DIGITS * columns_of(t.rows)), d_tmem = tmem_base + b * MOST_COLS;
                 if (!mbar_wait(&bars->tempty[b], ((local >> 1) & 1u) ^ 1u, abort_flag, P.error, 63)) break;
@@ -239,34 +254,65 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         }
     } else {
         if (codes_first) rows_are_there();
-        const int q = warp & 3; // the quarter of the lanes that this warp may read
-        float *mine = scales_smem + q * MOST_COLS;
+        const int q = warp & 3, turn = (warp - 2) >> 2; // the quarter of the lanes that this warp may read, and which of its two warps it is
+        float *mine = scales_smem + (warp - 2) * (MOST_COLS / 2);
+        uint32_t *stage = out_smem + (warp - 2) * 16 * STAGE_WORDS;
         T *y = static_cast<T *>(P.y);
         uint32_t local = 0;
-        for (long long id = first; id < total; id += step, ++local) {
+        for (int id = first; id < total; id += step, ++local) {
             const Tile t = tile_at(P, tiles, id, channel_tiles);
             const uint32_t b = local & 1u;
-            const int channel = t.channel0 + half * BM + 32 * q + lane, columns = columns_of(t.rows);
+            const int channel0 = t.channel0 + half * BM + 32 * q, channel = channel0 + lane, columns = columns_of(t.rows);
             const bool there = channel < P.channels;
             const size_t at = (size_t)t.group * P.channels + channel;
             const float channel_scale = !there ? 0.0f : P.channel_scales ? P.channel_scales[at] : 1.0f, bias = there && P.bias ? P.bias[at] : 0.0f;
             __syncwarp();
-            for (int i = lane; i < columns; i += 32) mine[i] = i < t.rows ? P.row_scales[t.row0 + i] : 0.0f;
+            for (int c0 = 32 * turn; c0 < columns; c0 += 64) mine[c0 / 2 - 16 * turn + lane] = c0 + lane < t.rows ? P.row_scales[t.row0 + c0 + lane] : 0.0f;
             __syncwarp();
             if (!__all_sync(~0u, mbar_wait(&bars->tfull[b], (local >> 1) & 1u, abort_flag, P.error, 66))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(32 * q) << 16) + b * MOST_COLS;
-            for (int c0 = 0; c0 < columns; c0 += 32) {
+            for (int c0 = 32 * turn; c0 < columns; c0 += 64) {
+                const float *row_scales = mine + c0 / 2 - 16 * turn;
                 uint32_t acc[32], low[32];
                 tmem_ld32_issue(taddr + c0, acc);
                 if (DIGITS == 2) tmem_ld32_issue(taddr + columns + c0, low);
                 tmem_wait();
-                T *to = y + (size_t)(t.row0 + c0) * P.y_ld + channel;
-                const int left = there ? t.rows - c0 : 0;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
+                const int left = t.rows - c0;
+                auto value = [&](int i) {
                     const float sum = DIGITS == 2 ? __fmaf_rn(128.0f, (float)(int)acc[i], (float)(int)low[i]) : (float)(int)acc[i];
-                    if (i < left) to[(size_t)i * P.y_ld] = from_float<T>(finish_sum(sum, mine[c0 + i], channel_scale, bias));
+                    return finish_sum(sum, row_scales[i], channel_scale, bias);
+                };
+                if (sizeof(T) == 2 && P.wide) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) stage[i * STAGE_WORDS + lane] = two_values<T>(value(2 * i), value(2 * i + 1));
+                    __syncwarp();
+                    const int piece = lane & 3, here = P.channels - channel0 - 8 * piece; // 8 channels a lane
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int pair = 8 * i + (lane >> 2);
+                        const uint4 u = *reinterpret_cast<const uint4 *>(stage + pair * STAGE_WORDS + 8 * piece), v = *reinterpret_cast<const uint4 *>(stage + pair * STAGE_WORDS + 8 * piece + 4);
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            const uint32_t pick = d ? 0x7632u : 0x5410u;
+                            const uint4 w = make_uint4(__byte_perm(u.x, u.y, pick), __byte_perm(u.z, u.w, pick), __byte_perm(v.x, v.y, pick), __byte_perm(v.z, v.w, pick));
+                            if (2 * pair + d >= left) continue;
+                            T *to = y + (size_t)(t.row0 + c0 + 2 * pair + d) * P.y_ld + channel0 + 8 * piece;
+                            if (here >= 8) {
+                                *reinterpret_cast<uint4 *>(to) = w;
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 7; ++k)
+                                    if (k < here) reinterpret_cast<unsigned short *>(to)[k] = (unsigned short)((&w.x)[k >> 1] >> (16 * (k & 1)));
+                            }
+                        }
+                    }
+                    __syncwarp();
+                } else {
+                    T *to = y + (size_t)(t.row0 + c0) * P.y_ld + channel;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (there && i < left) to[(size_t)i * P.y_ld] = from_float<T>(value(i));
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -274,7 +320,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             if (lane == 0) arrive_at(in_first(&bars->tempty[b]));
         }
         if (P.zero_rest)
-            zero_rest<T>(y, P.y_ld, P.channels, P.n, tiles.first[0], tiles.end[P.groups - 1], (size_t)blockIdx.x * 128 + (threadIdx.x - 64), (size_t)gridDim.x * 128);
+            zero_rest<T>(y, P.y_ld, P.channels, P.n, tiles.first[0], tiles.end(P.groups - 1), (size_t)blockIdx.x * (THREADS - 64) + (threadIdx.x - 64),
+                         (size_t)gridDim.x * (THREADS - 64));
     }
 
     __syncwarp();
@@ -288,7 +335,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
 
 template <typename T, int DIGITS> void product_tc_typed(CudaDevice &dev, const Product &p, TcParams &P, const CUtensorMap &map_codes, const CUtensorMap &map_rows, unsigned grid)
 {
-    const size_t smem = 1024 + NST * (A_BYTES + B_BYTES) + 4 * MOST_COLS * sizeof(float) + sizeof(Barriers) + RowTiles::bytes(p.groups);
+    const size_t smem = 1024 + NST * (A_BYTES + B_BYTES) + EPILOGUE_WARPS * (MOST_COLS / 2 + 16 * STAGE_WORDS) * 4 + sizeof(Barriers) + RowTiles::bytes(p.groups);
     allow_shared_memory(dev, product_tc_kernel<T, DIGITS>);
     launch_following_clusters(product_tc_kernel<T, DIGITS>, dim3(grid), dim3(THREADS), smem, 2, dev.stream(), map_codes, map_rows, P);
 }
@@ -321,6 +368,7 @@ void launch_product(CudaDevice &dev, const Product &p)
     if (const char *e = getenv("VQB_TILE")) best = atoi(e);
     P.tile_rows = (int)best;
     P.box_rows = P.tile_rows * p.digits / 2;
+    P.wide = (reinterpret_cast<uintptr_t>(p.y) | (p.y_ld * 2)) % 16 == 0;
     P.band = 8;
     const CUtensorMap map_codes = make_tensor_map_2d<int8_t>(p.codes, p.width, p.groups * p.channels, KB, BM, CU_TENSOR_MAP_SWIZZLE_128B, codes_ld(p.width));
     const CUtensorMap map_rows = make_tensor_map_2d<int8_t>(p.rows, p.width, p.digits * p.n, KB, (unsigned)P.box_rows, CU_TENSOR_MAP_SWIZZLE_128B, p.rows_ld);

@@ -39,20 +39,21 @@ __device__ __forceinline__ GroupRows group_rows(const long long *offsets, int g,
 }
 
 // How the rows of all groups fall into tiles of at most `rows` rows: tile u belongs to the last group g with before[g] <= u, and starts at row
-// first[g] + (u - before[g]) * rows.  In shared memory: 2 (groups + 1) + groups words.
+// first[g] + (u - before[g]) * rows.  In shared memory.
 struct RowTiles {
     int *before; // groups + 1
-    int *first;  // groups
-    int *end;    // groups
-    static __host__ __device__ constexpr size_t bytes(size_t groups) { return (3 * groups + 1) * sizeof(int); }
-    __device__ __forceinline__ RowTiles(void *smem, int groups) : before(static_cast<int *>(smem)), first(before + groups + 1), end(first + groups) {}
+    int *first;  // groups + 1
+    static __host__ __device__ constexpr size_t bytes(size_t groups) { return 2 * (groups + 1) * sizeof(int); }
+    __device__ __forceinline__ RowTiles(void *smem, int groups) : before(static_cast<int *>(smem)), first(before + groups + 1) {}
+    __device__ __forceinline__ int end(int g) const { return max(first[g], first[g + 1]); }
 
     // by all threads of the block; ends with a block barrier
     __device__ __forceinline__ void build(const long long *offsets, int groups, int n, int rows)
     {
         for (int g = threadIdx.x; g < groups; g += blockDim.x) {
             const GroupRows r = group_rows(offsets, g, n);
-            first[g] = r.first, end[g] = r.end;
+            first[g] = r.first;
+            if (g == groups - 1) first[groups] = r.end;
             before[g + 1] = (r.end - r.first + rows - 1) / rows;
         }
         if (threadIdx.x == 0) before[0] = 0;
