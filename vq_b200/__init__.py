@@ -670,6 +670,12 @@ class BinaryQuantizer:
 
 # ---- 8-bit codes with a scale for each row, and their products ----------------------------------
 _VALUE_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_TORCH_VALUES = {}  # torch dtype -> value type, filled when the first CUDA tensor comes
+
+
+def _torch_values(torch):
+    _TORCH_VALUES.update({getattr(torch, name): kind for name, kind in _VALUE_TYPES.items()})
+    return _TORCH_VALUES
 
 
 def _type_name(dtype) -> str:
@@ -693,6 +699,7 @@ class _Values:
             torch = sys.modules["torch"]
             if x.get_device() != ctx.device:
                 raise ValueError(f"{what} is on cuda:{x.get_device()}, the context on cuda:{ctx.device}")
+            values = _TORCH_VALUES or _torch_values(torch)
             if x.requires_grad:
                 x = x.detach()
             if integers:
@@ -701,7 +708,7 @@ class _Values:
                 x = x.contiguous()
                 self.type = None
             else:
-                self.type = _VALUE_TYPES.get(str(x.dtype)[6:])
+                self.type = values.get(x.dtype)
                 if self.type is None:
                     x, self.type = x.to(torch.float32), 0
             self.stream = torch._C._cuda_getCurrentRawStream(ctx.device)
@@ -741,12 +748,16 @@ def _result(x: _Values, width: int, dtype, out):
     apart than they are wide.  It lives where the rows live."""
     shape = (width,) if x.single else (x.n, width)
     if out is None:
+        if x.cuda:
+            kind = _TORCH_VALUES.get(dtype)
+            if kind is not None:
+                a = sys.modules["torch"].empty_strided(shape, (1,) if x.single else (width, 1), dtype=dtype, device=x.keep.device)
+                return a, a.data_ptr(), kind, width
         name = _type_name(dtype)
         if name not in _VALUE_TYPES or (name == "bfloat16" and not x.cuda):
             raise ValueError(f"a result of {name} is not offered" + ("" if x.cuda else " for rows in host memory"))
         if x.cuda:
-            a = x.keep.new_empty(shape, dtype=getattr(sys.modules["torch"], name))
-            return a, a.data_ptr(), _VALUE_TYPES[name], width
+            return _result(x, width, getattr(sys.modules["torch"], name), None)
         a = np.empty(shape, np.dtype(name))
         return a, a.ctypes.data, _VALUE_TYPES[name], width
     if dtype is not None and _type_name(dtype) != _type_name(out.dtype):
@@ -804,8 +815,9 @@ class RowQuantizer:
         ctx = self._ctx or default_context()
         x = _Values(rows, ctx, "rows")
         if x.cuda:
-            torch = sys.modules["torch"]
-            codes, scales = x.keep.new_empty(x.shape, dtype=torch.int8), x.keep.new_empty(x.shape[:-1], dtype=torch.float32)
+            torch, device = sys.modules["torch"], x.keep.device
+            codes = torch.empty_strided(x.shape, (1,) if x.single else (x.dim, 1), dtype=torch.int8, device=device)
+            scales = torch.empty_strided(() if x.single else (x.n,), () if x.single else (1,), dtype=torch.float32, device=device)
             cptr, sptr = codes.data_ptr(), scales.data_ptr()
         else:
             codes, scales = np.empty(x.shape, np.int8), np.empty(x.shape[:-1], np.float32)
@@ -908,8 +920,8 @@ class QuantizedMatrix:
         """rows (n x inputs, or one vector) times the matrix: n x outputs of `dtype` (the rows' own by default), plus the bias (outputs, or
         groups x outputs; added in float32)."""
         x = _Values(rows, self._ctx, "rows")
-        ko, optr = self._groups(x, offsets)
-        kb, bptr = self._bias(x, bias)
+        ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
+        kb, bptr = self._bias(x, bias) if bias is not None else (None, None)
         y, yptr, kind, ld = _result(x, self._shape[1], dtype or (x.keep.dtype if out is None else None), out)
         self._call(x, self._ctx._L.vqb_qmat_product, x.ptr, x.type, x.n, x.dim, x.ld, optr, bptr, yptr, kind, ld, 1 if out is None else 0)
         return y

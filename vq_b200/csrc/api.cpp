@@ -375,6 +375,7 @@ struct NewQmat {
         m.groups = groups, m.outputs = outputs, m.inputs = inputs;
         try {
             m.codes = static_cast<int8_t *>(dev.alloc(groups * outputs * codes_ld(inputs)));
+            if (inputs % 16) dev.zero(m.codes, groups * outputs * codes_ld(inputs));
             m.scales = static_cast<float *>(dev.alloc(groups * outputs * sizeof(float)));
             if (flags & VQB_QMAT_GRADIENT) m.turned = static_cast<int8_t *>(dev.alloc(groups * inputs * codes_ld(outputs)));
         } catch (...) {
@@ -392,6 +393,7 @@ struct NewQmat {
     {
         Qmat &m = qm->mat;
         if (m.turned) launch_turn_codes(dev, m.codes, m.groups, m.outputs, m.inputs, m.turned);
+        dev.synchronize(); // products fetch a matrix without waiting for what is before them in the stream
         return qm.release();
     }
     ~NewQmat() { drop(); }
@@ -1355,6 +1357,7 @@ int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim
         Product p = product_of(m);
         p.n = n, p.rows_ld = codes_ld(dim), p.offsets = io.get(), p.bias = ib.as<float>();
         p.y = oy.out.d, p.y_type = y_type, p.y_ld = y_ld, p.zero_rest = (flags & VQB_ZERO_REST) != 0;
+        if (launch_product_few(dev, p, ix.d, type, ld)) return oy.out.finish();
         Scratch codes(dev, n * p.rows_ld + n * sizeof(float));
         float *scales = reinterpret_cast<float *>(codes.d + n * p.rows_ld);
         launch_quantize_rows(dev, ix.d, type, n, dim, ld, reinterpret_cast<int8_t *>(codes.d), p.rows_ld, scales);
@@ -1390,7 +1393,7 @@ int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, const float *scale
             launch_align_codes(dev, p.rows, n, dim, dim, reinterpret_cast<int8_t *>(aligned->d));
             p.rows = reinterpret_cast<const int8_t *>(aligned->d);
         }
-        launch_product(dev, p);
+        if (!launch_product_few(dev, p, nullptr, 0, 0)) launch_product(dev, p);
         oy.out.finish();
     });
 }

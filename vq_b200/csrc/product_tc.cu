@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
-    // Codes of the matrix may be fetched before the rows' are there, where only those are new.
-    const bool codes_first = P.rows_follow && !P.offsets;
+    // Codes of the matrix may be fetched before the rows' are there; which of them, offsets say, where there are some.
+    const bool codes_first = !P.offsets || P.rows_follow;
     if (!codes_first) rows_are_there();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     tiles.build(P.offsets, P.groups, P.n, P.tile_rows); // (block barriers)
@@ -358,12 +358,16 @@ void launch_product(CudaDevice &dev, const Product &p)
     P.y = p.y, P.y_ld = p.y_ld, P.zero_rest = p.zero_rest, P.rows_follow = p.rows_follow, P.error = dev.error_word();
     const size_t pairs = (size_t)dev.sm_count() / 2, channel_tiles = (p.channels + 2 * BM - 1) / (2 * BM);
     const size_t a_group = (p.n + p.groups - 1) / p.groups; // rows
-    // The tile's rows: whatever makes the fewest rounds of all SM pairs last the shortest.  A stage's time is its rows', but not below that
-    // of some 64: the channels' bytes have to come in.
+    // The tile's rows: whatever makes the rounds of all SM pairs last the shortest.  Measured, in units of one column's time in one stage
+    // (1.15 ns): a stage takes as long as its columns, but 160 and an eighth of them at least (0.20 us at 64 or 128 columns, 0.22 at 160, 0.30 at 256); a
+    // tile's change 400; its results leave at 10 a column, behind the next tile's stages or, at the end, behind nothing.
+    const size_t chunks = (p.width + KB - 1) / KB;
     size_t best = 32, least = ~size_t(0);
     for (size_t rows = 32; rows * p.digits <= MOST_COLS; rows += 32) {
-        const size_t tiles = p.groups * ((a_group + rows - 1) / rows) * channel_tiles, cost = (tiles + pairs - 1) / pairs * (std::max<size_t>(rows * p.digits, 64) + 16);
-        if (cost <= least) best = rows, least = cost;
+        const size_t columns = rows * p.digits, tiles = p.groups * ((a_group + rows - 1) / rows) * channel_tiles;
+        const size_t stages = chunks * std::max(columns, 160 + columns / 8) + 400, leaves = 10 * rows;
+        const size_t cost = (tiles + pairs - 1) / pairs * std::max(stages, leaves) + leaves;
+        if (cost < least) best = rows, least = cost;
     }
     if (const char *e = getenv("VQB_TILE")) best = atoi(e);
     P.tile_rows = (int)best;

@@ -10,8 +10,8 @@
 namespace vqb {
 
 // Kernels of a product may start before the kernel in front of them ends.  All earlier work of the stream is complete and visible
-// from here on; every thread calls it before it reads what that kernel may have written, or leaves.  (What is read before: a matrix, where
-// the kernel in front is this call's own quantizer, which has itself waited for everything earlier.)
+// from here on; every thread calls it before it reads what that kernel may have written, or leaves.  (What is read before: codes of a matrix,
+// which is complete when the call that made it returns.)
 __device__ __forceinline__ void rows_are_there() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void product_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

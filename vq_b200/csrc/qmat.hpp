@@ -3,7 +3,7 @@
 //   y[i][j] = (sum_k q[i][k] w[j][k]) s[i] t[j] + b[j]        q, w: int8; the sum is a whole number, exact in 32 bits
 //
 // for one matrix, or for one matrix per group of consecutive rows (offsets); and the gradient of that with respect to what the rows
-// were quantized from.  rows.cu makes codes, product_tc.cu and product_plain.cu multiply them.
+// were quantized from.  rows.cu makes codes, product_tc.cu, product_few.cu and product_plain.cu multiply them.
 #pragma once
 #include <cstddef>
 #include <cstdint>
@@ -25,12 +25,13 @@ inline size_t codes_ld(size_t width) { return (width + 15) / 16 * 16; }
 
 struct Qmat {
     size_t groups = 0, outputs = 0, inputs = 0;
-    int8_t *codes = nullptr;  // groups x outputs x codes_ld(inputs)
+    int8_t *codes = nullptr;  // groups x outputs x codes_ld(inputs), zeros behind the inputs
     float *scales = nullptr;  // groups x outputs
     int8_t *turned = nullptr; // groups x inputs x codes_ld(outputs): the codes transposed, for gradients; null without
 };
 
-// One product: `channels` rows of codes for each group times n rows.
+// One product: `channels` rows of codes for each group times n rows.  Nothing that may still be running has written the codes and scales of channels
+// (whoever makes a matrix waits for it); the rest is read once the kernels before this one have ended.
 struct Product {
     const int8_t *codes = nullptr;        // groups x channels x codes_ld(width)
     const float *channel_scales = nullptr; // groups x channels; null: 1
@@ -45,7 +46,7 @@ struct Product {
     int y_type = VALUE_F32;
     size_t y_ld = 0;
     bool zero_rest = false;   // rows of no group become 0 (otherwise they are left as they are)
-    bool rows_follow = false; // the kernel directly before wrote `rows` and `row_scales`, and nothing else of this
+    bool rows_follow = false; // the kernel directly before wrote `rows` and `row_scales`, and had itself waited for all that was before it
 };
 
 // codes[i][k] = x[i][k] / s[i] to the nearest whole number (halves to even, of the real quotient), s[i] = max_k |x[i][k]| / 127; s is 0 for
@@ -61,6 +62,9 @@ void launch_turn_codes(CudaDevice &dev, const int8_t *codes, size_t groups, size
 void launch_align_codes(CudaDevice &dev, const int8_t *codes, size_t n, size_t width, size_t ld, int8_t *aligned);
 
 void launch_product(CudaDevice &dev, const Product &p);
+// Up to eight rows with one matrix: takes the rows as values (p.rows and p.row_scales unused) or, where x is null, as codes.  False, having done nothing,
+// when it does not take them.  The matrix may not be written by what is still running.
+bool launch_product_few(CudaDevice &dev, const Product &p, const void *x, int type, size_t ld);
 void launch_product_plain(CudaDevice &dev, const Product &p); // CUDA cores
 
 } // namespace vqb
