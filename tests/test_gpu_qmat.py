@@ -375,3 +375,16 @@ def test_gradient_of_rows_of_zeros_and_rows_that_are_not_finite():
     want, size, extra, _ = gradient_limits(dy[3:], wq, ws)
     assert not dx[0].any() and bool(torch.isnan(dx[1:3]).all())
     check(dx[3:], want, size, extra)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("n,dim", [(14_300, 4096), (7_300, 8192), (14_209, 4104), (7_111, 6160)])
+def test_many_wide_rows_are_the_definitions(n, dim, dtype):
+    """Enough of them that they stream through shared memory; their number does not divide among the blocks."""
+    torch = torch_()
+    x = normal(n, n, dim, dtype=dtype)
+    x[5], x[n - 1, 3], x[n // 2, 0] = 0, float("nan"), float("inf")
+    q, s = vq.RowQuantizer.fit().quantize(x)
+    for part in torch.arange(n, device="cuda").split(2048):
+        want_q, want_s = codes64(x[part])
+        assert torch.equal(q[part].double(), want_q) and torch.equal(torch.nan_to_num(s[part], nan=-1.0).double(), torch.nan_to_num(want_s, nan=-1.0))
