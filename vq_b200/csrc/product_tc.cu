@@ -87,7 +87,8 @@ __device__ __forceinline__ void tma_load_counted(void *dst, const CUtensorMap *m
                  "r"(bar), "r"(c0), "r"(c1)
                  : "memory");
 }
-__device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Without release ordering: what is handed back has been read, and a release would wait for the results' stores (1 us a tile).
+__device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -258,30 +259,59 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         float *mine = scales_smem + (warp - 2) * (MOST_COLS / 2);
         uint32_t *stage = out_smem + (warp - 2) * 16 * STAGE_WORDS;
         T *y = static_cast<T *>(P.y);
+        // what the next tile's results are multiplied by, on its way while this one's leave
+        struct Scales {
+            Tile t;
+            float rows[MOST_COLS / 64], channel, bias; // of this lane's rows (one in each of the warp's turns) and channel
+        };
+        auto scales_of = [&](int id) {
+            Scales n;
+            n.t = tile_at(P, tiles, id, channel_tiles);
+#pragma unroll
+            for (int i = 0; i < MOST_COLS / 64; ++i) {
+                const int r = 64 * i + 32 * turn + lane;
+                n.rows[i] = r < n.t.rows ? P.row_scales[n.t.row0 + r] : 0.0f;
+            }
+            const int channel = n.t.channel0 + half * BM + 32 * q + lane;
+            const size_t at = (size_t)n.t.group * P.channels + channel;
+            n.channel = channel >= P.channels ? 0.0f : P.channel_scales ? P.channel_scales[at] : 1.0f;
+            n.bias = channel < P.channels && P.bias ? P.bias[at] : 0.0f;
+            return n;
+        };
         uint32_t local = 0;
+        Scales next;
+        if (first < total) next = scales_of(first);
         for (int id = first; id < total; id += step, ++local) {
-            const Tile t = tile_at(P, tiles, id, channel_tiles);
+            const Tile t = next.t;
             const uint32_t b = local & 1u;
             const int channel0 = t.channel0 + half * BM + 32 * q, channel = channel0 + lane, columns = columns_of(t.rows);
             const bool there = channel < P.channels;
-            const size_t at = (size_t)t.group * P.channels + channel;
-            const float channel_scale = !there ? 0.0f : P.channel_scales ? P.channel_scales[at] : 1.0f, bias = there && P.bias ? P.bias[at] : 0.0f;
+            const float channel_scale = next.channel, bias = next.bias;
             __syncwarp();
-            for (int c0 = 32 * turn; c0 < columns; c0 += 64) mine[c0 / 2 - 16 * turn + lane] = c0 + lane < t.rows ? P.row_scales[t.row0 + c0 + lane] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < MOST_COLS / 64; ++i) mine[32 * i + lane] = next.rows[i];
             __syncwarp();
+            if (id + step < total) next = scales_of(id + step);
             if (!__all_sync(~0u, mbar_wait(&bars->tfull[b], (local >> 1) & 1u, abort_flag, P.error, 66))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(32 * q) << 16) + b * MOST_COLS;
             for (int c0 = 32 * turn; c0 < columns; c0 += 64) {
-                const float *row_scales = mine + c0 / 2 - 16 * turn;
+                const float4 *row_scales = reinterpret_cast<const float4 *>(mine + c0 / 2 - 16 * turn);
                 uint32_t acc[32], low[32];
                 tmem_ld32_issue(taddr + c0, acc);
                 if (DIGITS == 2) tmem_ld32_issue(taddr + columns + c0, low);
                 tmem_wait();
+                if (c0 + 64 >= columns) { // the accumulator has been read
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive_at(in_first(&bars->tempty[b]));
+                }
                 const int left = t.rows - c0;
                 auto value = [&](int i) {
+                    const float4 s4 = row_scales[i >> 2];
+                    const float row_scale = (i & 3) == 0 ? s4.x : (i & 3) == 1 ? s4.y : (i & 3) == 2 ? s4.z : s4.w;
                     const float sum = DIGITS == 2 ? __fmaf_rn(128.0f, (float)(int)acc[i], (float)(int)low[i]) : (float)(int)acc[i];
-                    return finish_sum(sum, row_scales[i], channel_scale, bias);
+                    return finish_sum(sum, row_scale, channel_scale, bias);
                 };
                 if (sizeof(T) == 2 && P.wide) {
 #pragma unroll
@@ -315,9 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                         if (there && i < left) to[(size_t)i * P.y_ld] = from_float<T>(value(i));
                 }
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) arrive_at(in_first(&bars->tempty[b]));
+            if (32 * turn >= columns && lane == 0) arrive_at(in_first(&bars->tempty[b])); // (nothing of it was this warp's)
         }
         if (P.zero_rest)
             zero_rest<T>(y, P.y_ld, P.channels, P.n, tiles.first[0], tiles.end(P.groups - 1), (size_t)blockIdx.x * (THREADS - 64) + (threadIdx.x - 64),
