@@ -176,6 +176,17 @@ def test_products(n, inputs, outputs, dtype):
     assert np.array_equal(m.codes, wq[0].cpu().numpy()) and np.array_equal(m.scales, ws[0].float().cpu().numpy())
 
 
+@pytest.mark.parametrize("n,inputs,outputs", [(1, 4096, 14336), (2, 8200, 9001), (3, 16400, 5000), (8, 1030, 20_011), (16, 4096, 14336), (16, 9000, 3000), (5, 520, 40_000), (4, 64, 150_000)])
+def test_products_of_few_rows_with_large_matrices(n, inputs, outputs):
+    """Every block has many pieces of the matrix: more than it has room for at a time."""
+    torch = torch_()
+    x = normal(n, n, inputs, dtype="bfloat16")
+    m, wq, ws = matrix64(normal(inputs, outputs, inputs, scale=inputs**-0.5))
+    want, size, _ = product64(*codes64(x), wq, ws)
+    for _ in range(3):
+        check(m.product(x), want, size)
+
+
 @pytest.mark.parametrize("out", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("n,inputs,outputs", [(1, 160, 96), (12, 1000, 300), (40, 97, 64), (700, 513, 200)])
 def test_products_of_codes_up_to_the_largest(n, inputs, outputs, out):

@@ -1362,7 +1362,7 @@ int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim
         float *scales = reinterpret_cast<float *>(codes.d + n * p.rows_ld);
         launch_quantize_rows(dev, ix.d, type, n, dim, ld, reinterpret_cast<int8_t *>(codes.d), p.rows_ld, scales);
         p.rows = reinterpret_cast<const int8_t *>(codes.d), p.row_scales = scales, p.rows_follow = true;
-        launch_product(dev, p);
+        if (!launch_product_few(dev, p, nullptr, 0, 0)) launch_product(dev, p);
         oy.out.finish();
     });
 }

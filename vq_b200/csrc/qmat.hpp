@@ -62,7 +62,7 @@ void launch_turn_codes(CudaDevice &dev, const int8_t *codes, size_t groups, size
 void launch_align_codes(CudaDevice &dev, const int8_t *codes, size_t n, size_t width, size_t ld, int8_t *aligned);
 
 void launch_product(CudaDevice &dev, const Product &p);
-// Up to eight rows with one matrix: takes the rows as values (p.rows and p.row_scales unused) or, where x is null, as codes.  False, having done nothing,
+// Up to sixteen rows with one matrix: takes one or two as values (p.rows and p.row_scales unused) or, where x is null, codes (16-byte aligned rows).  False, having done nothing,
 // when it does not take them.  The matrix may not be written by what is still running.
 bool launch_product_few(CudaDevice &dev, const Product &p, const void *x, int type, size_t ld);
 void launch_product_plain(CudaDevice &dev, const Product &p); // CUDA cores
