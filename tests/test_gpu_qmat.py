@@ -187,6 +187,21 @@ def test_products_of_few_rows_with_large_matrices(n, inputs, outputs):
         check(m.product(x), want, size)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("n,inputs,outputs", [(64, 4096, 4096), (33, 5000, 700), (100, 8190, 1030), (300, 8192, 256), (17, 130, 257), (250, 1000, 100), (20, 40_000, 130)])
+def test_products_of_few_tiles_with_wide_matrices(n, inputs, outputs, dtype):
+    """Too few tiles for the SMs: several of them take a part of the width each.  The gradient's way too: outputs and inputs change places."""
+    x = normal(n, n, inputs, dtype=dtype)
+    m, wq, ws = matrix64(normal(inputs, outputs, inputs, scale=inputs**-0.5))
+    bias = normal(1, outputs)
+    want, size, _ = product64(*codes64(x), wq, ws, bias)
+    check(m.product(x, bias), want, size)
+    if dtype == "float16":
+        m, wq, ws = matrix64(normal(inputs, inputs, outputs, scale=0.02), gradient=True)
+        want, size, extra, _ = gradient_limits(x, wq, ws)
+        check(m.input_gradient(x), want, size, extra)
+
+
 @pytest.mark.parametrize("out", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("n,inputs,outputs", [(1, 160, 96), (12, 1000, 300), (40, 97, 64), (700, 513, 200)])
 def test_products_of_codes_up_to_the_largest(n, inputs, outputs, out):

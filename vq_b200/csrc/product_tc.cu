@@ -11,9 +11,15 @@
 //   warps 2-9   epilogue: scales, bias, rounding, stores; two warps share the lanes that either may read and take turns at 32 columns each.
 //               16-bit results go through shared memory, two rows' values of a channel in a word, and leave 16 bytes at a time
 //
+// Where there are too few tiles for the SMs, two or four pairs of a larger cluster take a part of the width each, one tile a cluster.  Their sums stay in
+// their shared memory (the ring is free by then), and every pair finishes some of the rows, adding up what the others have there: whole
+// numbers, so that nothing depends on their order, and no memory outside the SMs that would have to be zero.
+//
 // Two digits (gradients): the first CTA fetches the rows' high digits and the second one their low digits, so that the columns' first
 // half are the high sums and the second half the low ones; the epilogue joins them.
 #include <algorithm>
+#include <map>
+#include <mutex>
 
 #include "cuda_device.hpp"
 #include "qmat.cuh"
@@ -48,6 +54,7 @@ struct TcParams {
     int box_rows;  // rows a token load brings: tile_rows x DIGITS / 2
     int band;      // tiles of rows that are taken together for one tile of channels
     int zero_rest, rows_follow;
+    int parts; // of the width, a pair each
     int wide; // results can be stored 16 bytes at a time
     int *error;
 };
@@ -64,21 +71,27 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_
 }
 
 // Arrives at the same barrier of both CTAs once all that this thread has issued is done.
-__device__ __forceinline__ void commit_both(void *bar)
+__device__ __forceinline__ void commit_both(void *bar, uint32_t leader)
 {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)(3u << leader)) : "memory");
 }
 __device__ __forceinline__ void commit_here(void *bar)
 {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// The address of the first CTA's copy of a shared-memory object.
-__device__ __forceinline__ uint32_t in_first(const void *p)
+// The address of another CTA's copy of a shared-memory object.
+__device__ __forceinline__ uint32_t in_cta(const void *p, uint32_t rank)
 {
     uint32_t a;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
+}
+__device__ __forceinline__ int4 load_cluster(uint32_t addr)
+{
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 // A load into this CTA that counts at a barrier of the first one (no multicast).
 __device__ __forceinline__ void tma_load_counted(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar)
@@ -130,7 +143,7 @@ __device__ __forceinline__ Tile tile_at(const TcParams &P, const RowTiles &tiles
 // Accumulator columns of one digit: rows in steps of 32 (16 for each CTA to fetch; with two digits each fetches them all).
 __device__ __forceinline__ int columns_of(int rows) { return (rows + 31) / 32 * 32; }
 
-template <typename T, int DIGITS>
+template <typename T, int DIGITS, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rows, const TcParams P)
 {
     extern __shared__ unsigned char smem_raw[];
@@ -142,7 +155,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     RowTiles tiles(bars + 1, P.groups);
     volatile int *abort_flag = &bars->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int half = blockIdx.x & 1; // this CTA's place in its cluster
+    const int parts = SPLIT ? P.parts : 1, rank = blockIdx.x % (2 * parts), half = rank & 1, part = rank >> 1; // this CTA's place in its cluster
+    const uint32_t leader = rank & ~1;                                                                          // the first one of its pair
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NST; ++s) {
@@ -171,22 +185,23 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = bars->tmem_base;
     const int channel_tiles = (P.channels + 2 * BM - 1) / (2 * BM), chunks = (P.width + KB - 1) / KB;
-    const int total = tiles.before[P.groups] * channel_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int c_begin = chunks * part / parts, c_end = chunks * (part + 1) / parts;
+    const int total = tiles.before[P.groups] * channel_tiles, first = blockIdx.x / (2 * parts), step = gridDim.x / (2 * parts);
 
     if (warp == 0) {
         if (lane == 0) {
             int st = 0;
             uint32_t parity = 0; // of the stages' current round
             bool ok = true, waited = !codes_first;
-            const uint32_t bytes = 2 * (A_BYTES + (uint32_t)P.box_rows * KB), full0 = in_first(&bars->full[0]);
+            const uint32_t bytes = 2 * (A_BYTES + (uint32_t)P.box_rows * KB), full0 = in_cta(&bars->full[0], leader);
             unsigned long long loads = 0;
             for (int id = first; ok && id < total; id += step) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
                 // this CTA's rows: one half of the columns, or one digit of all
                 const int row = DIGITS == 2 ? half * P.n + t.row0 : t.row0 + half * (columns_of(t.rows) / 2);
                 const int channel = t.group * P.channels + t.channel0 + half * BM;
-                const int ahead = waited ? 0 : min(NST, chunks);
-                for (int c = 0; c < chunks; ++c) {
+                const int ahead = waited ? 0 : min(NST, c_end - c_begin);
+                for (int c = c_begin; c < c_end; ++c) {
                     if (!mbar_wait(&bars->empty[st], parity ^ 1u, abort_flag, P.error, 61)) {
                         ok = false;
                         break;
@@ -194,11 +209,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     if (half == 0) mbar_expect_tx(&bars->full[st], bytes);
                     tma_load_counted(a_smem + st * A_BYTES, &map_codes, c * KB, channel, full0 + 8u * st);
                     ++loads;
-                    if (c + 1 >= ahead) {
+                    if (c - c_begin + 1 >= ahead) {
                         if (!waited) {
                             rows_are_there();
                             waited = true;
-                            for (int e = 0; e < ahead; ++e) tma_load_counted(b_smem + e * B_BYTES, &map_rows, e * KB, row, full0 + 8u * e);
+                            for (int e = 0; e < ahead; ++e) tma_load_counted(b_smem + e * B_BYTES, &map_rows, (c_begin + e) * KB, row, full0 + 8u * e);
                         } else {
                             tma_load_counted(b_smem + st * B_BYTES, &map_rows, c * KB, row, full0 + 8u * st);
                         }
@@ -230,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 const uint32_t b = local & 1u, idesc = idesc_i8(DIGITS * columns_of(t.rows)), d_tmem = tmem_base + b * MOST_COLS;
                 if (!mbar_wait(&bars->tempty[b], ((local >> 1) & 1u) ^ 1u, abort_flag, P.error, 63)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int c = 0; c < chunks; ++c) {
+                for (int c = c_begin; c < c_end; ++c) {
                     if (!mbar_wait(&bars->full[st], parity, abort_flag, P.error, 64)) {
                         ok = false;
                         break;
@@ -239,14 +254,14 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     const uint64_t a = a0 + (uint32_t)(st * (int)(A_BYTES >> 4)), r = r0 + (uint32_t)(st * (int)(B_BYTES >> 4));
                     // Always four: behind the width there are zeros.  (Rolled up, with a count, one such instruction took 54 ns to issue, as long
                     // as the tensor core needs for 200 columns; a stage 0.42 instead of 0.27 us.)
-                    umma_i8(d_tmem, a, r, idesc, (uint32_t)c);
+                    umma_i8(d_tmem, a, r, idesc, (uint32_t)(c - c_begin));
                     umma_i8(d_tmem, a + 2, r + 2, idesc, 1u);
                     umma_i8(d_tmem, a + 4, r + 4, idesc, 1u);
                     umma_i8(d_tmem, a + 6, r + 6, idesc, 1u);
-                    commit_both(&bars->empty[st]);
+                    commit_both(&bars->empty[st], leader);
                     if (++st == NST) st = 0, parity ^= 1u;
                 }
-                if (ok) commit_both(&bars->tfull[b]);
+                if (ok) commit_both(&bars->tfull[b], leader);
             }
             if (*abort_flag) { // nothing of the tensor core's is under way when the blocks leave
                 commit_here(&bars->drained);
@@ -296,6 +311,18 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(32 * q) << 16) + b * MOST_COLS;
             for (int c0 = 32 * turn; c0 < columns; c0 += 64) {
+                if (SPLIT) { // this part's sums to the ring, a channel's next to each other
+                    uint32_t *dump = reinterpret_cast<uint32_t *>(base);
+#pragma unroll
+                    for (int d = 0; d < DIGITS; ++d) {
+                        uint32_t acc[32];
+                        tmem_ld32_issue(taddr + d * columns + c0, acc);
+                        tmem_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) dump[(d * columns + c0 + i) * BM + 32 * q + lane] = acc[i];
+                    }
+                    continue;
+                }
                 const float4 *row_scales = reinterpret_cast<const float4 *>(mine + c0 / 2 - 16 * turn);
                 uint32_t acc[32], low[32];
                 tmem_ld32_issue(taddr + c0, acc);
@@ -304,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 if (c0 + 64 >= columns) { // the accumulator has been read
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) arrive_at(in_first(&bars->tempty[b]));
+                    if (lane == 0) arrive_at(in_cta(&bars->tempty[b], leader));
                 }
                 const int left = t.rows - c0;
                 auto value = [&](int i) {
@@ -345,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                         if (there && i < left) to[(size_t)i * P.y_ld] = from_float<T>(value(i));
                 }
             }
-            if (32 * turn >= columns && lane == 0) arrive_at(in_first(&bars->tempty[b])); // (nothing of it was this warp's)
+            if (32 * turn >= columns && lane == 0) arrive_at(in_cta(&bars->tempty[b], leader)); // (nothing of it was this warp's)
         }
         if (P.zero_rest)
             zero_rest<T>(y, P.y_ld, P.channels, P.n, tiles.first[0], tiles.end(P.groups - 1), (size_t)blockIdx.x * (THREADS - 64) + (threadIdx.x - 64),
@@ -353,6 +380,50 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     }
 
     __syncwarp();
+    if (SPLIT) {
+        cluster_sync(); // all parts' sums are there
+        const Tile t = tile_at(P, tiles, first, channel_tiles);
+        const int columns = columns_of(t.rows), channel = t.channel0 + half * BM + 4 * lane; // a warp a row, four channels a lane
+        if (warp >= 2 && channel < P.channels) {
+            const size_t at = (size_t)t.group * P.channels + channel;
+            const int here = min(4, P.channels - channel);
+            float channel_scale[4], bias[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                channel_scale[k] = k < here && P.channel_scales ? P.channel_scales[at + k] : 1.0f;
+                bias[k] = k < here && P.bias ? P.bias[at + k] : 0.0f;
+            }
+            const uint32_t *mine = reinterpret_cast<const uint32_t *>(base) + 4 * lane;
+            T *y = static_cast<T *>(P.y) + (size_t)t.row0 * P.y_ld + channel;
+#pragma unroll 4
+            for (int r = EPILOGUE_WARPS * part + warp - 2; r < t.rows; r += EPILOGUE_WARPS * parts) {
+                int4 sums[DIGITS] = {};
+                for (int s = 0; s < parts; ++s)
+#pragma unroll
+                    for (int d = 0; d < DIGITS; ++d) {
+                        const int4 v = load_cluster(in_cta(mine + (d * columns + r) * BM, 2 * s + half));
+                        sums[d].x += v.x, sums[d].y += v.y, sums[d].z += v.z, sums[d].w += v.w;
+                    }
+                const float row_scale = P.row_scales[t.row0 + r];
+                alignas(16) T out[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float whole = (float)(&sums[0].x)[k], sum = DIGITS == 2 ? __fmaf_rn(128.0f, whole, (float)(&sums[DIGITS - 1].x)[k]) : whole;
+                    out[k] = from_float<T>(finish_sum(sum, row_scale, channel_scale[k], bias[k]));
+                }
+                T *to = y + (size_t)r * P.y_ld;
+                if (P.wide && here == 4) {
+                    if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(out);
+                    else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(out);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (k < here) to[k] = out[k];
+                }
+            }
+        }
+        __syncwarp();
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync(); // neither CTA's shared memory and barriers are needed any more
     if (warp == 1) {
@@ -361,17 +432,45 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     }
 }
 
-template <typename T, int DIGITS> void product_tc_typed(CudaDevice &dev, const Product &p, TcParams &P, const CUtensorMap &map_codes, const CUtensorMap &map_rows, unsigned grid)
+size_t smem_bytes(size_t groups) { return 1024 + NST * (A_BYTES + B_BYTES) + EPILOGUE_WARPS * (MOST_COLS / 2 + 16 * STAGE_WORDS) * 4 + sizeof(Barriers) + RowTiles::bytes(groups); }
+
+template <typename T, int DIGITS> void product_tc_typed(CudaDevice &dev, const Product &p, const TcParams &P, const CUtensorMap &map_codes, const CUtensorMap &map_rows, unsigned clusters)
 {
-    const size_t smem = 1024 + NST * (A_BYTES + B_BYTES) + EPILOGUE_WARPS * (MOST_COLS / 2 + 16 * STAGE_WORDS) * 4 + sizeof(Barriers) + RowTiles::bytes(p.groups);
-    allow_shared_memory(dev, product_tc_kernel<T, DIGITS>);
-    launch_following_clusters(product_tc_kernel<T, DIGITS>, dim3(grid), dim3(THREADS), smem, 2, dev.stream(), map_codes, map_rows, P);
+    if (P.parts == 1) {
+        allow_shared_memory(dev, product_tc_kernel<T, DIGITS, false>);
+        launch_following_clusters(product_tc_kernel<T, DIGITS, false>, dim3(2 * clusters), dim3(THREADS), smem_bytes(p.groups), 2, dev.stream(), map_codes, map_rows, P);
+    } else {
+        allow_shared_memory(dev, product_tc_kernel<T, DIGITS, true>);
+        launch_following_clusters(product_tc_kernel<T, DIGITS, true>, dim3(2 * P.parts * clusters), dim3(THREADS), smem_bytes(p.groups), 2 * P.parts, dev.stream(), map_codes,
+                                  map_rows, P);
+    }
 }
 
-template <typename T> void product_tc_digits(CudaDevice &dev, const Product &p, TcParams &P, const CUtensorMap &mc, const CUtensorMap &mr, unsigned grid)
+template <typename T> void product_tc_digits(CudaDevice &dev, const Product &p, const TcParams &P, const CUtensorMap &mc, const CUtensorMap &mr, unsigned clusters)
 {
-    if (p.digits == 2) product_tc_typed<T, 2>(dev, p, P, mc, mr, grid);
-    else product_tc_typed<T, 1>(dev, p, P, mc, mr, grid);
+    if (p.digits == 2) product_tc_typed<T, 2>(dev, p, P, mc, mr, clusters);
+    else product_tc_typed<T, 1>(dev, p, P, mc, mr, clusters);
+}
+
+// How many clusters of so many CTAs there is room for at a time (a cluster stays within a part of the GPU whose SMs need not be a multiple of it).
+size_t room_for_clusters(CudaDevice &dev, int ctas)
+{
+    static std::mutex mu;
+    static std::map<std::pair<int, int>, int> known;
+    std::lock_guard<std::mutex> lk(mu);
+    int &room = known[{dev.device(), ctas}];
+    if (room == 0) {
+        auto kernel = product_tc_kernel<float, 1, true>;
+        allow_shared_memory(dev, kernel);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem_bytes(1);
+        cudaLaunchAttribute attr = {};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr, cfg.numAttrs = 1;
+        VQB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&room, kernel, &cfg));
+    }
+    return (size_t)room;
 }
 
 } // namespace
@@ -386,30 +485,35 @@ void launch_product(CudaDevice &dev, const Product &p)
     P.y = p.y, P.y_ld = p.y_ld, P.zero_rest = p.zero_rest, P.rows_follow = p.rows_follow, P.error = dev.error_word();
     const size_t pairs = (size_t)dev.sm_count() / 2, channel_tiles = (p.channels + 2 * BM - 1) / (2 * BM);
     const size_t a_group = (p.n + p.groups - 1) / p.groups; // rows
-    // The tile's rows: whatever makes the rounds of all SM pairs last the shortest.  Measured, in units of one column's time in one stage
-    // (1.15 ns): a stage takes as long as its columns, but 160 and an eighth of them at least (0.20 us at 64 or 128 columns, 0.22 at 160, 0.30 at 256); a
-    // tile's change 400; its results leave at 10 a column, behind the next tile's stages or, at the end, behind nothing.
+    // The tile's rows, and among how many pairs its width is parted: whatever makes the rounds of all SM pairs last the shortest.  Measured, in units of one
+    // column's time in one stage (1.15 ns): a stage takes as long as its columns, but 160 and an eighth of them at least (0.20 us at 64 or 128 columns,
+    // 0.22 at 160, 0.30 at 256); a tile's change 400; its results leave at 10 a column, behind the next tile's stages or, at the end, behind
+    // nothing.  Joining parts takes 700 and 52 a column, shared by the pairs (us for 1, 2 and 4 parts: 128 rows of 8192 with 2048 channels 17.4, 13.4, 11.7; 100 of
+    // 1024 with 1024 6.3, 7.2, 7.1).
     const size_t chunks = (p.width + KB - 1) / KB;
-    size_t best = 32, least = ~size_t(0);
+    size_t least = ~size_t(0);
+    P.parts = 1;
     for (size_t rows = 32; rows * p.digits <= MOST_COLS; rows += 32) {
-        const size_t columns = rows * p.digits, tiles = p.groups * ((a_group + rows - 1) / rows) * channel_tiles;
-        const size_t stages = chunks * std::max(columns, 160 + columns / 8) + 400, leaves = 10 * rows;
+        const size_t columns = rows * p.digits, a_stage = std::max(columns, 160 + columns / 8), tiles = p.groups * ((a_group + rows - 1) / rows) * channel_tiles;
+        const size_t stages = chunks * a_stage + 400, leaves = 10 * rows;
         const size_t cost = (tiles + pairs - 1) / pairs * std::max(stages, leaves) + leaves;
-        if (cost < least) best = rows, least = cost;
+        if (cost < least) P.tile_rows = (int)rows, P.parts = 1, least = cost;
+        for (size_t parts = 2; parts <= 4 && !p.offsets && parts <= chunks && tiles * parts <= pairs; parts *= 2) {
+            const size_t split = (chunks + parts - 1) / parts * a_stage + 400 + 700 + 52 * columns / parts;
+            if (split < least && tiles <= room_for_clusters(dev, (int)(2 * parts))) P.tile_rows = (int)rows, P.parts = (int)parts, least = split;
+        }
     }
-    if (const char *e = getenv("VQB_TILE")) best = atoi(e);
-    P.tile_rows = (int)best;
     P.box_rows = P.tile_rows * p.digits / 2;
     P.wide = (reinterpret_cast<uintptr_t>(p.y) | (p.y_ld * 2)) % 16 == 0;
     P.band = 8;
     const CUtensorMap map_codes = make_tensor_map_2d<int8_t>(p.codes, p.width, p.groups * p.channels, KB, BM, CU_TENSOR_MAP_SWIZZLE_128B, codes_ld(p.width));
     const CUtensorMap map_rows = make_tensor_map_2d<int8_t>(p.rows, p.width, p.digits * p.n, KB, (unsigned)P.box_rows, CU_TENSOR_MAP_SWIZZLE_128B, p.rows_ld);
     const size_t row_tiles = p.offsets ? p.n / P.tile_rows + p.groups : (p.n + P.tile_rows - 1) / P.tile_rows;
-    const unsigned grid = 2 * (unsigned)std::min<size_t>(pairs, row_tiles * channel_tiles);
+    const unsigned clusters = (unsigned)(P.parts > 1 ? row_tiles * channel_tiles : std::min<size_t>(pairs, row_tiles * channel_tiles));
     KernelScope ks(dev, "product_tc");
-    if (p.y_type == VALUE_F32) product_tc_digits<float>(dev, p, P, map_codes, map_rows, grid);
-    else if (p.y_type == VALUE_F16) product_tc_digits<__half>(dev, p, P, map_codes, map_rows, grid);
-    else product_tc_digits<__nv_bfloat16>(dev, p, P, map_codes, map_rows, grid);
+    if (p.y_type == VALUE_F32) product_tc_digits<float>(dev, p, P, map_codes, map_rows, clusters);
+    else if (p.y_type == VALUE_F16) product_tc_digits<__half>(dev, p, P, map_codes, map_rows, clusters);
+    else product_tc_digits<__nv_bfloat16>(dev, p, P, map_codes, map_rows, clusters);
     dev.count_launch();
 }
 
