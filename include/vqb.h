@@ -294,8 +294,8 @@ int vqb_bq_quantize(vqb_ctx *ctx, float threshold, uint8_t low, uint8_t high, co
 enum vqb_value_type { VQB_F32 = 0, VQB_F16 = 1, VQB_BF16 = 2 };
 #define VQB_ZERO_REST 1     /* flag of a product: rows of no group become 0 */
 #define VQB_QMAT_GRADIENT 1 /* flag of a matrix: its codes are kept transposed too, for vqb_qmat_input_gradient */
-/* n x dim codes and n scales. */
-int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim, size_t ld, int8_t *codes, float *scales);
+/* n x dim codes (ld_codes from row to row: what is between the rows stays as it is) and n scales. */
+int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim, size_t ld, int8_t *codes, size_t ld_codes, float *scales);
 typedef struct vqb_qmat vqb_qmat;
 /* groups x outputs x inputs weights, each row quantized as above.  The matrix keeps a copy, laid out for the products. */
 int vqb_qmat_fit(vqb_ctx *ctx, const void *weights, int type, size_t groups, size_t outputs, size_t inputs, int flags, vqb_qmat **out);
@@ -306,9 +306,9 @@ int vqb_qmat_parts(const vqb_qmat *qm, int8_t *codes_out /* groups x outputs x i
  * outputs f32, or NULL. */
 int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim, size_t ld, const int64_t *offsets, const float *bias, void *y, int y_type,
                      size_t y_ld, int flags);
-/* The same for rows that are quantized already (n x dim codes, n scales). */
-int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, const float *scales, size_t n, size_t dim, const int64_t *offsets, const float *bias, void *y,
-                           int y_type, size_t y_ld, int flags);
+/* The same for rows that are quantized already (n x dim codes, n scales).  Where codes or ld_codes are not multiples of 16 the codes are copied first. */
+int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, size_t ld_codes, const float *scales, size_t n, size_t dim, const int64_t *offsets,
+                           const float *bias, void *y, int y_type, size_t y_ld, int flags);
 /* dx[i][k] = sum_j dy[i][j] t[j] w[j][k]: the product's gradient with respect to the rows that were quantized (the rounding taken for the identity).
  * dy[i][j] t[j] enters in 15 bits: as the nearest of 16256 steps up to the row's largest magnitude.  dy is n x outputs, dx n x inputs, both f16 or
  * both bf16 (f32 is refused: it would promise more digits than that).  Needs VQB_QMAT_GRADIENT. */

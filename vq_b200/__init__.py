@@ -687,7 +687,7 @@ def _type_name(dtype) -> str:
 
 class _Values:
     """The caller's rows as they are: float32, float16 or bfloat16 (other types are turned into float32), any distance from row to row.
-    `integers`: int8 codes instead, contiguous."""
+    `integers`: int8 codes instead."""
 
     __slots__ = ("cuda", "keep", "shape", "ptr", "single", "n", "dim", "ld", "type", "stream")
 
@@ -705,7 +705,6 @@ class _Values:
             if integers:
                 if x.dtype is not torch.int8:
                     raise ValueError(f"{what} must be int8")
-                x = x.contiguous()
                 self.type = None
             else:
                 self.type = values.get(x.dtype)
@@ -733,7 +732,7 @@ class _Values:
             raise ValueError("expected a vector or a matrix of row vectors")
         self.n, self.dim = (1, shape[0]) if self.single else shape
         self.ld = self.dim
-        if self.cuda and not integers:
+        if self.cuda:
             strides = x.stride()
             step = strides[0] if not self.single and self.n > 1 else self.dim
             if (self.dim > 1 and strides[-1] != 1) or step < self.dim:
@@ -811,21 +810,23 @@ class RowQuantizer:
         return cls(ctx)
 
     def quantize(self, rows):
-        """(codes, scales) of one vector or of a batch: int8 of the rows' shape, float32 with one value a row."""
+        """(codes, scales) of one vector or of a batch: int8 of the rows' shape, float32 with one value a row.  On the GPU the codes' rows begin at
+        multiples of 16 bytes (their stride), for the products' sake."""
         ctx = self._ctx or default_context()
         x = _Values(rows, ctx, "rows")
         if x.cuda:
             torch, device = sys.modules["torch"], x.keep.device
-            codes = torch.empty_strided(x.shape, (1,) if x.single else (x.dim, 1), dtype=torch.int8, device=device)
+            ld = x.dim + -x.dim % 16  # rows that begin at multiples of 16 bytes are multiplied as they are
+            codes = torch.empty_strided(x.shape, (1,) if x.single else (ld, 1), dtype=torch.int8, device=device)
             scales = torch.empty_strided(() if x.single else (x.n,), () if x.single else (1,), dtype=torch.float32, device=device)
             cptr, sptr = codes.data_ptr(), scales.data_ptr()
         else:
-            codes, scales = np.empty(x.shape, np.int8), np.empty(x.shape[:-1], np.float32)
+            ld, codes, scales = x.dim, np.empty(x.shape, np.int8), np.empty(x.shape[:-1], np.float32)
             cptr, sptr = codes.ctypes.data, scales.ctypes.data
         with ctx._lock:
             if x.stream != ctx._stream:
                 ctx._run_on(x.stream)
-            rc = ctx._L.vqb_row_quantize(ctx.handle, x.ptr, x.type, x.n, x.dim, x.ld, cptr, sptr)
+            rc = ctx._L.vqb_row_quantize(ctx.handle, x.ptr, x.type, x.n, x.dim, x.ld, cptr, ld, sptr)
             if rc:
                 _raise(rc, ctx.handle)
         return codes, scales
@@ -864,6 +865,8 @@ class QuantizedMatrix:
         ctx = ctx or default_context()
         flat, (groups, outputs) = cls._flat(codes)
         x = _Values(flat, ctx, "codes", integers=True)
+        if x.ld != x.dim:
+            x = _Values(flat.contiguous(), ctx, "codes", integers=True)
         keep, sptr = _beside(scales, x, "float32", [tuple(codes.shape[:-1])], "scales")
         h = C.c_void_p()
         ctx.call(x, _lib.load().vqb_qmat_from_parts, ctx.handle, x.ptr, sptr, groups, outputs, x.dim, 1 if gradient else 0, C.byref(h))
@@ -933,7 +936,7 @@ class QuantizedMatrix:
         ko, optr = self._groups(x, offsets)
         kb, bptr = self._bias(x, bias)
         y, yptr, kind, ld = _result(x, self._shape[1], dtype or (np.float32 if out is None else None), out)
-        self._call(x, self._ctx._L.vqb_qmat_product_codes, x.ptr, sptr, x.n, x.dim, optr, bptr, yptr, kind, ld, 1 if out is None else 0)
+        self._call(x, self._ctx._L.vqb_qmat_product_codes, x.ptr, x.ld, sptr, x.n, x.dim, optr, bptr, yptr, kind, ld, 1 if out is None else 0)
         return y
 
     def input_gradient(self, dy, *, offsets=None, out=None):

@@ -79,13 +79,13 @@ SIGNATURES = {
     "vqb_sq_quantize": (C.c_int, [_P, C.c_float, C.c_float, _SZ, C.c_float, _P, _SZ, _P]),
     "vqb_bq_fit": (C.c_int, [C.c_float, C.c_uint8, C.c_uint8]),
     "vqb_bq_quantize": (C.c_int, [_P, C.c_float, C.c_uint8, C.c_uint8, _P, _SZ, _P]),
-    "vqb_row_quantize": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, _P, _P]),
+    "vqb_row_quantize": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, _P, _SZ, _P]),
     "vqb_qmat_fit": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, C.c_int, C.POINTER(_P)]),
     "vqb_qmat_from_parts": (C.c_int, [_P, _P, _P, _SZ, _SZ, _SZ, C.c_int, C.POINTER(_P)]),
     "vqb_qmat_shape": (C.c_int, [_P, C.POINTER(_SZ), C.POINTER(_SZ), C.POINTER(_SZ)]),
     "vqb_qmat_parts": (C.c_int, [_P, _P, _P]),
     "vqb_qmat_product": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, _P, _P, _P, C.c_int, _SZ, C.c_int]),
-    "vqb_qmat_product_codes": (C.c_int, [_P, _P, _P, _SZ, _SZ, _P, _P, _P, C.c_int, _SZ, C.c_int]),
+    "vqb_qmat_product_codes": (C.c_int, [_P, _P, _SZ, _P, _SZ, _SZ, _P, _P, _P, C.c_int, _SZ, C.c_int]),
     "vqb_qmat_input_gradient": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, _P, _P, _SZ, C.c_int]),
     "vqb_qmat_destroy": (C.c_int, [_P]),
     "vqb_seeder_create": (C.c_int, [C.c_uint64, C.POINTER(_P)]),

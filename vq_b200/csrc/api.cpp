@@ -373,6 +373,9 @@ struct NewQmat {
     {
         Qmat &m = qm->mat;
         m.groups = groups, m.outputs = outputs, m.inputs = inputs;
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(dev.stream(), &capture) != cudaSuccess) cudaGetLastError(); // (the default stream while another one is being captured)
+        if (capture != cudaStreamCaptureStatusNone) throw Error(VQB_ERR_UNSUPPORTED, "a matrix cannot be made while its stream is being captured");
         try {
             m.codes = static_cast<int8_t *>(dev.alloc(groups * outputs * codes_ld(inputs)));
             if (inputs % 16) dev.zero(m.codes, groups * outputs * codes_ld(inputs));
@@ -1262,7 +1265,7 @@ int vqb_bq_quantize(vqb_ctx *ctx, float threshold, uint8_t low, uint8_t high, co
     });
 }
 
-int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim, size_t ld, int8_t *codes, float *scales)
+int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim, size_t ld, int8_t *codes, size_t ld_codes, float *scales)
 {
     if (!ctx) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "ctx is NULL");
     return locked(ctx, [&] {
@@ -1271,11 +1274,13 @@ int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim
         if (n == 0) return;
         check_values("x", x, type, dim, ld);
         if (!codes || !scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
+        if (ld_codes < dim) throw Error(VQB_ERR_BAD_ARGUMENT, "codes: rows overlap");
         check_words("scales", scales, sizeof(float));
         CudaDevice &dev = *ctx->dev;
         In ix(dev, x, span(n, dim, ld, value_bytes(type)));
-        Out oc(dev, codes, n * dim), os(dev, scales, sizeof(float) * n);
-        launch_quantize_rows(dev, ix.d, type, n, dim, ld, oc.as<int8_t>(), dim, os.as<float>());
+        Out oc(dev, codes, span(n, dim, ld_codes, 1)), os(dev, scales, sizeof(float) * n);
+        if (oc.host && ld_codes != dim) VQB_CUDA_CHECK(cudaMemcpyAsync(oc.d, oc.host, oc.bytes, cudaMemcpyHostToDevice, dev.stream()));
+        launch_quantize_rows(dev, ix.d, type, n, dim, ld, oc.as<int8_t>(), ld_codes, os.as<float>());
         finish(oc, os);
     });
 }
@@ -1367,8 +1372,8 @@ int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim
     });
 }
 
-int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, const float *scales, size_t n, size_t dim, const int64_t *offsets, const float *bias, void *y,
-                           int y_type, size_t y_ld, int flags)
+int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, size_t ld_codes, const float *scales, size_t n, size_t dim, const int64_t *offsets,
+                           const float *bias, void *y, int y_type, size_t y_ld, int flags)
 {
     if (!qm) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "matrix is NULL");
     vqb_ctx *ctx = qm->ctx;
@@ -1380,17 +1385,18 @@ int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, const float *scale
         if (n == 0) return;
         if (!codes || !scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
         check_words("scales", scales, sizeof(float));
-        In ic(dev, codes, n * dim), is(dev, scales, sizeof(float) * n), ib(dev, bias, bias ? sizeof(float) * m.groups * m.outputs : 0);
+        if (ld_codes < dim) throw Error(VQB_ERR_BAD_ARGUMENT, "codes: rows overlap");
+        In ic(dev, codes, span(n, dim, ld_codes, 1)), is(dev, scales, sizeof(float) * n), ib(dev, bias, bias ? sizeof(float) * m.groups * m.outputs : 0);
         RowsOut oy(dev, y, n, m.outputs, y_ld, y_type, !offsets || (flags & VQB_ZERO_REST));
         Product p = product_of(m);
         p.n = n, p.offsets = io.get(), p.bias = ib.as<float>(), p.row_scales = is.as<float>();
         p.y = oy.out.d, p.y_type = y_type, p.y_ld = y_ld, p.zero_rest = (flags & VQB_ZERO_REST) != 0;
-        p.rows = ic.as<int8_t>(), p.rows_ld = dim;
+        p.rows = ic.as<int8_t>(), p.rows_ld = n == 1 ? codes_ld(dim) : ld_codes; // (one row has no next one)
         std::unique_ptr<Scratch> aligned;
-        if (dim % 16 || reinterpret_cast<uintptr_t>(p.rows) % 16) {
+        if (p.rows_ld % 16 || reinterpret_cast<uintptr_t>(p.rows) % 16) {
             p.rows_ld = codes_ld(dim);
             aligned.reset(new Scratch(dev, n * p.rows_ld));
-            launch_align_codes(dev, p.rows, n, dim, dim, reinterpret_cast<int8_t *>(aligned->d));
+            launch_align_codes(dev, p.rows, n, dim, ld_codes, reinterpret_cast<int8_t *>(aligned->d));
             p.rows = reinterpret_cast<const int8_t *>(aligned->d);
         }
         if (!launch_product_few(dev, p, nullptr, 0, 0)) launch_product(dev, p);

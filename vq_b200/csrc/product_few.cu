@@ -118,10 +118,24 @@ template <typename T, int EIGHTS, int PAIRS> __global__ void __launch_bounds__(T
     const int n = (int)P.rows.n;
     rows_are_there();
     if constexpr (std::is_same<T, int8_t>::value) {
-        const int pieces = P.pitch / 16, last = P.ld / 16;
-        for (int i = threadIdx.x; i < NT * pieces; i += 32 * WARPS) {
-            const int t = i / pieces, k = i - t * pieces;
-            reinterpret_cast<uint4 *>(rows)[i] = t < n && k < last ? *reinterpret_cast<const uint4 *>(P.given + t * P.given_ld + 16 * k) : make_uint4(0, 0, 0, 0);
+        const int pieces = P.pitch / 16, width = (int)P.rows.width;
+        for (int i = threadIdx.x; i < NT * pieces; i += 32 * WARPS) { // (zeros behind the width)
+            const int t = i / pieces, k = 16 * (i - t * pieces);
+            const int8_t *from = P.given + t * P.given_ld + k;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (t < n && k + 16 <= width) {
+                v = *reinterpret_cast<const uint4 *>(from);
+            } else if (t < n && k < width) {
+#pragma unroll 1
+                for (int b = 0; k + b < width; ++b) {
+                    const uint32_t byte = (uint32_t)(uint8_t)from[b] << (8 * (b & 3));
+                    if (b < 4) v.x |= byte;
+                    else if (b < 8) v.y |= byte;
+                    else if (b < 12) v.z |= byte;
+                    else v.w |= byte;
+                }
+            }
+            reinterpret_cast<uint4 *>(rows)[i] = v;
         }
         if (threadIdx.x < NT) row_scales[threadIdx.x] = threadIdx.x < n ? P.given_scales[threadIdx.x] : 0.0f;
     } else {
@@ -226,7 +240,7 @@ bool launch_product_few(CudaDevice &dev, const Product &p, const void *x, int ty
 {
     if (!dev.error_word() || p.offsets || p.digits != 1 || p.n > 16) return false;
     // every block quantizes the rows: with more than 32 values a thread that takes longer than a kernel before this one
-    if (x && (p.n > 2 || p.n * p.width > 16384 || (reinterpret_cast<uintptr_t>(x) | (ld * value_bytes(type))) % 16)) return false;
+    if (x && (p.n > 2 || p.n * p.width > 16384 || (reinterpret_cast<uintptr_t>(x) | (p.n == 1 ? 0 : ld * value_bytes(type))) % 16)) return false;
     const size_t eights = (p.n + 7) / 8;
     FewParams P{};
     P.rows.x = x, P.rows.n = p.n, P.rows.width = p.width, P.rows.ld = ld;

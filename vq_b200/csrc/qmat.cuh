@@ -26,50 +26,50 @@ __device__ __forceinline__ float finish_sum(float sum, float row_scale, float ch
     return __fmaf_rn(__fmul_rn(sum, row_scale), channel_scale, bias);
 }
 
-// Rows [first, end) of group g.  Offsets come from the device unchecked: whatever they are, the rows are some of the n that there are.
-struct GroupRows {
-    int first, end;
-};
-__device__ __forceinline__ GroupRows group_rows(const long long *offsets, int g, int n)
-{
-    if (!offsets) return {0, n};
-    const long long a = offsets[g], b = offsets[g + 1];
-    const int first = (int)(a < 0 ? 0 : a > n ? n : a);
-    return {first, (int)(b < first ? first : b > n ? n : b)};
-}
-
 // How the rows of all groups fall into tiles of at most `rows` rows: tile u belongs to the last group g with before[g] <= u, and starts at row
-// first[g] + (u - before[g]) * rows.  In shared memory.
+// first[g] + (u - before[g]) * rows.  In shared memory.  Offsets come from the device unchecked: whatever they are, every group has some of the n
+// rows that there are, and no row has two groups.
 struct RowTiles {
     int *before; // groups + 1
-    int *first;  // groups + 1
+    int *first;  // groups + 1: group g has rows first[g] .. first[g + 1] - 1
     static __host__ __device__ constexpr size_t bytes(size_t groups) { return 2 * (groups + 1) * sizeof(int); }
     __device__ __forceinline__ RowTiles(void *smem, int groups) : before(static_cast<int *>(smem)), first(before + groups + 1) {}
-    __device__ __forceinline__ int end(int g) const { return max(first[g], first[g + 1]); }
+    __device__ __forceinline__ int end(int g) const { return first[g + 1]; }
 
     // by all threads of the block; ends with a block barrier
     __device__ __forceinline__ void build(const long long *offsets, int groups, int n, int rows)
     {
-        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-            const GroupRows r = group_rows(offsets, g, n);
-            first[g] = r.first;
-            if (g == groups - 1) first[groups] = r.end;
-            before[g + 1] = (r.end - r.first + rows - 1) / rows;
+        for (int g = threadIdx.x; g <= groups; g += blockDim.x) {
+            const long long a = offsets ? offsets[g] : g ? n : 0;
+            first[g] = (int)(a < 0 ? 0 : a > n ? n : a);
         }
-        if (threadIdx.x == 0) before[0] = 0;
         __syncthreads();
         if (threadIdx.x < 32) {
-            int carry = 0;
-            for (int g0 = 0; g0 < groups; g0 += 32) {
-                const int g = g0 + (int)threadIdx.x;
-                int v = g < groups ? before[g + 1] : 0;
+            const int lane = threadIdx.x;
+            int most = 0, tiles = 0;
+            for (int g0 = 0; g0 <= groups; g0 += 32) { // ascending
+                int v = g0 + lane <= groups ? first[g0 + lane] : 0;
 #pragma unroll
                 for (int d = 1; d < 32; d *= 2) {
                     const int up = __shfl_up_sync(~0u, v, d);
-                    if ((int)threadIdx.x >= d) v += up;
+                    if (lane >= d) v = max(v, up);
                 }
-                if (g < groups) before[g + 1] = carry + v;
-                carry += __shfl_sync(~0u, v, 31);
+                v = max(v, most);
+                if (g0 + lane <= groups) first[g0 + lane] = v;
+                most = __shfl_sync(~0u, v, 31);
+            }
+            __syncwarp();
+            if (lane == 0) before[0] = 0;
+            for (int g0 = 0; g0 < groups; g0 += 32) {
+                const int g = g0 + lane;
+                int v = g < groups ? (first[g + 1] - first[g] + rows - 1) / rows : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int up = __shfl_up_sync(~0u, v, d);
+                    if (lane >= d) v += up;
+                }
+                if (g < groups) before[g + 1] = tiles + v;
+                tiles += __shfl_sync(~0u, v, 31);
             }
         }
         __syncthreads();

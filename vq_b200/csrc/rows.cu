@@ -164,7 +164,8 @@ template <typename T, int DIGITS, int LANES, int HELD> void quantize_rows_with(C
 // As many threads a row as have two pieces of it each; many wide rows are streamed.
 template <typename T, int DIGITS> void quantize_rows_typed(CudaDevice &dev, const RowParams &P)
 {
-    const bool aligned = (reinterpret_cast<uintptr_t>(P.x) | (P.ld * sizeof(T))) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.codes) | P.ld_codes | reinterpret_cast<uintptr_t>(P.low)) % 8 == 0;
+    const size_t apart = P.n == 1 ? 0 : P.ld * sizeof(T), codes_apart = P.n == 1 ? 0 : P.ld_codes; // (one row has no next one)
+    const bool aligned = (reinterpret_cast<uintptr_t>(P.x) | apart) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.codes) | codes_apart | reinterpret_cast<uintptr_t>(P.low)) % 8 == 0;
     const size_t pieces = (P.width + Piece<T>::N - 1) / Piece<T>::N, bytes = P.width * sizeof(T);
     // Measured (us, streamed and not): 16384 x 4096 bf16 34 and 41, 8192 x 8192 44 and 52; but 8192 x 4096 26 and 25, 16384 x 2048 25 and 23.
     if (aligned && bytes % 16 == 0 && bytes >= 8192 && bytes <= STREAM_BYTES / 4 && dev.error_word()) {
