@@ -404,9 +404,9 @@ def test_gradient_of_rows_of_zeros_and_rows_that_are_not_finite():
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("n,dim", [(14_300, 4096), (7_300, 8192), (14_209, 4104), (7_111, 6160)])
+@pytest.mark.parametrize("n,dim", [(14_300, 4096), (7_300, 8192), (14_209, 4104), (7_111, 6160), (70_000, 128), (33_001, 515), (20_000, 1000), (9_000, 2048), (1_100, 16400)])
 def test_many_wide_rows_are_the_definitions(n, dim, dtype):
-    """Enough of them that they stream through shared memory; their number does not divide among the blocks."""
+    """Enough of them that bytes under way count: fewer threads a row, with more of it each."""
     torch = torch_()
     x = normal(n, n, dim, dtype=dtype)
     x[5], x[n - 1, 3], x[n // 2, 0] = 0, float("nan"), float("inf")

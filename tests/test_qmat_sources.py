@@ -9,7 +9,7 @@ def test_rows_are_not_taken_for_invariant():
         if "rows_are_there();" in body:
             seen.add(name)
             assert not _taken_for_invariant(params, body), name
-    assert seen == {"quantize_rows_kernel", "stream_rows_kernel", "product_tc_kernel", "product_few_kernel"}
+    assert seen == {"quantize_rows_kernel", "product_tc_kernel", "product_few_kernel"}
 
 
 def test_every_way_out_of_such_a_kernel_is_behind_the_wait():

@@ -6,7 +6,6 @@
 
 #include "cuda_device.hpp"
 #include "rows.cuh"
-#include "umma.cuh"
 
 namespace vqb {
 
@@ -66,93 +65,6 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>) quantize_rows_kernel(const 
     for (size_t h = HELD; h < pieces; ++h) it.write(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h, none, inverse);
 }
 
-// Many aligned rows: a block stays on its SM and has `ring` rows in shared memory, on their way (bulk copies) or worked on; a team of warps takes every
-// `teams`th of them and reads it twice from there.
-constexpr int STREAM_WARPS = 24;
-constexpr size_t STREAM_BYTES = 192 << 10;
-constexpr int STREAM_ROWS = STREAM_WARPS; // in the ring, at most
-
-template <typename T, int DIGITS> __global__ void __launch_bounds__(32 * STREAM_WARPS) stream_rows_kernel(const RowParams P, int teams, int slots, int *error)
-{
-    constexpr int N = Piece<T>::N;
-    extern __shared__ __align__(128) unsigned char ring[];
-    __shared__ unsigned long long full[STREAM_ROWS];
-    __shared__ uint32_t parts[2][STREAM_WARPS];
-    __shared__ int abort_word;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = STREAM_WARPS / teams, team = warp / size, threads = 32 * size, t = threadIdx.x - team * threads;
-    const uint32_t bytes = (uint32_t)(P.width * sizeof(T));
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < teams * slots; ++i) mbar_init(&full[i], 1);
-        abort_word = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    __syncthreads();
-    rows_are_there();
-    product_may_start();
-    auto together = [&] { // the team's warps
-        if (size == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(threads) : "memory");
-    };
-    const size_t first = (size_t)blockIdx.x * teams + team, step = (size_t)gridDim.x * teams;
-    unsigned char *mine = ring + (size_t)team * slots * bytes;
-    unsigned long long *bars = full + team * slots;
-    auto fetch = [&](size_t r, int slot) {
-        mbar_expect_tx(&bars[slot], bytes);
-        bulk_load_1d(mine + (size_t)slot * bytes, static_cast<const T *>(P.x) + r * P.ld, bytes, &bars[slot]);
-    };
-    if (t == 0)
-        for (int i = 0; i < slots && first + i * step < P.n; ++i) fetch(first + i * step, i);
-    const int last = (int)(bytes / 16); // 16-byte pieces of the row
-    int slot = 0, turn = 0;
-    uint32_t parity = 0;
-    for (size_t r = first; r < P.n; r += step, turn ^= 1) {
-        // A wait that is given up ends the row, not the loop: the team's other warps count on this one at their barriers, and every later wait ends at
-        // once.
-        const bool there = __all_sync(~0u, *(volatile int *)&abort_word == 0 && mbar_wait(&bars[slot], parity, &abort_word, error, 71));
-        const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr;
-        if (DIGITS == 1 || columns) { // (the same for the whole team)
-            RowOf<T, DIGITS, 1, true> it(P, r, 0, columns); // (piece i: 16 bytes at 16 i)
-            const uint4 *row = reinterpret_cast<const uint4 *>(mine + (size_t)slot * bytes);
-#pragma unroll 4
-            for (int i = t; i < last; i += threads) it.look(Piece<T>{row[i]}, i);
-            uint32_t most = it.largest();
-            if (size > 1) {
-                if (lane == 0) parts[turn][warp] = most;
-                together();
-                for (int w = 0; w < size; ++w) most = max(most, parts[turn][team * size + w]);
-            }
-            const float scale = it.scale_of(most);
-            if (t == 0 && there) P.scales[r] = scale;
-            int8_t *codes = P.codes + r * P.ld_codes, *lows = DIGITS == 2 ? P.low + r * P.ld_codes : nullptr;
-            auto put = [&](int8_t *to, int i, const Packed<N> &c) {
-                if (N == 8) reinterpret_cast<uint2 *>(to)[i] = make_uint2(c.w[0], c.w[N / 4 - 1]);
-                else reinterpret_cast<uint32_t *>(to)[i] = c.w[0];
-            };
-            if (it.no_codes(most)) {
-                for (int i = t; i < last; i += threads) {
-                    put(codes, i, Packed<N>{});
-                    if (DIGITS == 2) put(lows, i, Packed<N>{});
-                }
-            } else {
-                const Inverse inverse(scale);
-#pragma unroll 4
-                for (int i = t; i < last; i += threads) {
-                    Packed<N> high, low;
-                    it.pack(Piece<T>{row[i]}, i, inverse, high, low);
-                    put(codes, i, high);
-                    if (DIGITS == 2) put(lows, i, low);
-                }
-            }
-        }
-        together();
-        if (t == 0 && r + slots * step < P.n && there) fetch(r + slots * step, slot);
-        if (++slot == slots) slot = 0, parity ^= 1u;
-    }
-    if (*(volatile int *)&abort_word) // what has been asked for lands before the block leaves
-        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-}
-
 template <typename T, int DIGITS, int LANES, int HELD> void quantize_rows_with(CudaDevice &dev, const RowParams &P, bool aligned)
 {
     constexpr int THREADS = THREADS_OF<LANES>, ROWS = THREADS / LANES;
@@ -161,22 +73,20 @@ template <typename T, int DIGITS, int LANES, int HELD> void quantize_rows_with(C
     else launch_following(quantize_rows_kernel<T, DIGITS, LANES, HELD, false>, grid, dim3(THREADS), 0, dev.stream(), P);
 }
 
-// As many threads a row as have two pieces of it each; many wide rows are streamed.
+// As many threads a row as have two pieces of it each, or four where there are values enough that bytes under way count and not the time of one row
+// (us with two and four: 1024 x 1024 bf16 3.1 and 4.2, 8192 x 1024 9.5 and 8.3, 16384 x 1024 18.0 and 12.5, 4096 x 4096 13.4 and 12.4, 8192 x 4096 24.9 and 21.1).
 template <typename T, int DIGITS> void quantize_rows_typed(CudaDevice &dev, const RowParams &P)
 {
     const size_t apart = P.n == 1 ? 0 : P.ld * sizeof(T), codes_apart = P.n == 1 ? 0 : P.ld_codes; // (one row has no next one)
     const bool aligned = (reinterpret_cast<uintptr_t>(P.x) | apart) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.codes) | codes_apart | reinterpret_cast<uintptr_t>(P.low)) % 8 == 0;
-    const size_t pieces = (P.width + Piece<T>::N - 1) / Piece<T>::N, bytes = P.width * sizeof(T);
-    // Measured (us, streamed and not): 16384 x 4096 bf16 34 and 41, 8192 x 8192 44 and 52; but 8192 x 4096 26 and 25, 16384 x 2048 25 and 23.
-    if (aligned && bytes % 16 == 0 && bytes >= 8192 && bytes <= STREAM_BYTES / 4 && dev.error_word()) {
-        size_t teams = STREAM_WARPS; // two rows for each in the ring
-        while (2 * teams * bytes > STREAM_BYTES) teams /= 2;
-        if (P.n >= 8 * teams * (size_t)dev.sm_count()) {
-            const size_t slots = std::min<size_t>(STREAM_BYTES / (teams * bytes), STREAM_ROWS / teams);
-            allow_shared_memory(dev, stream_rows_kernel<T, DIGITS>);
-            launch_following(stream_rows_kernel<T, DIGITS>, dim3((unsigned)dev.sm_count()), dim3(32 * STREAM_WARPS), slots * bytes * teams, dev.stream(), P, (int)teams, (int)slots, dev.error_word());
-            return;
-        }
+    const size_t pieces = (P.width + Piece<T>::N - 1) / Piece<T>::N;
+    if (P.n >= (size_t(1) << 23) / P.width) {
+        if (pieces <= 128) quantize_rows_with<T, DIGITS, 32, 4>(dev, P, aligned);
+        else if (pieces <= 256) quantize_rows_with<T, DIGITS, 64, 4>(dev, P, aligned);
+        else if (pieces <= 512) quantize_rows_with<T, DIGITS, 128, 4>(dev, P, aligned);
+        else if (pieces <= 1024) quantize_rows_with<T, DIGITS, 256, 4>(dev, P, aligned);
+        else quantize_rows_with<T, DIGITS, 512, 4>(dev, P, aligned);
+        return;
     }
     if (pieces <= 64) quantize_rows_with<T, DIGITS, 32, 2>(dev, P, aligned);
     else if (pieces <= 128) quantize_rows_with<T, DIGITS, 64, 2>(dev, P, aligned);
