@@ -67,10 +67,10 @@ def test_results():
 def test_what_goes_with_the_rows():
     x = rows(3, 5)
     with pytest.raises(ValueError, match="offsets must have shape"):
-        vq._beside(np.zeros(4), x, "int64", [(3,)], "offsets")
+        vq._beside(np.zeros(4), x, "int64", (3,), "offsets")
     with pytest.raises(ValueError, match="bias must have shape"):
-        vq._beside(np.zeros((2, 5)), x, "float32", [(5,)], "bias")
-    v, _ = vq._beside([1, 2, 3], x, "int64", [(3,)], "offsets")
+        vq._beside(np.zeros((2, 5)), x, "float32", (5,), "bias")
+    v, _ = vq._beside([1, 2, 3], x, "int64", (3,), "offsets")
     assert v.dtype == np.int64
 
 

@@ -781,16 +781,20 @@ def _beside(v, x: _Values, name: str, shape, what: str):
     if x.cuda and _is_torch(v) and v.is_cuda:
         if v.get_device() != x.keep.get_device():
             raise ValueError(f"{what} is on another device than the rows")
-        v = v.detach().to(getattr(sys.modules["torch"], name)).contiguous()
-        found, ptr = tuple(v.shape), v.data_ptr()
+        want = getattr(sys.modules["torch"], name)
+        if v.dtype is not want:
+            v = v.detach().to(want)
+        if not v.is_contiguous():
+            v = v.contiguous()
+        found, ptr = v.shape, v.data_ptr()
     else:
         if _is_torch(v):
             v = v.detach().cpu()
             v = (v.float() if str(v.dtype) == "torch.bfloat16" else v).numpy()
         v = np.ascontiguousarray(v, dtype=name).reshape(np.shape(v))  # (a single scale stays one)
         found, ptr = v.shape, v.ctypes.data
-    if found not in shape:
-        raise ValueError(f"{what} must have shape {shape[0]}, not {found}")
+    if found != shape:
+        raise ValueError(f"{what} must have shape {shape}, not {tuple(found)}")
     return v, ptr
 
 
@@ -867,7 +871,7 @@ class QuantizedMatrix:
         x = _Values(flat, ctx, "codes", integers=True)
         if x.ld != x.dim:
             x = _Values(flat.contiguous(), ctx, "codes", integers=True)
-        keep, sptr = _beside(scales, x, "float32", [tuple(codes.shape[:-1])], "scales")
+        keep, sptr = _beside(scales, x, "float32", tuple(codes.shape[:-1]), "scales")
         h = C.c_void_p()
         ctx.call(x, _lib.load().vqb_qmat_from_parts, ctx.handle, x.ptr, sptr, groups, outputs, x.dim, 1 if gradient else 0, C.byref(h))
         return cls(h, ctx, len(codes.shape) == 3)
@@ -904,11 +908,11 @@ class QuantizedMatrix:
             if self._grouped:
                 raise ValueError("a matrix of groups needs offsets")
             return None, None
-        return _beside(offsets, x, "int64", [(self._shape[0] + 1,)], "offsets")
+        return _beside(offsets, x, "int64", (self._shape[0] + 1,), "offsets")
 
     def _bias(self, x, bias):
         g, o, _ = self._shape
-        return (None, None) if bias is None else _beside(bias, x, "float32", [(g, o) if self._grouped else (o,)], "bias")
+        return _beside(bias, x, "float32", (g, o) if self._grouped else (o,), "bias")
 
     def _call(self, x, fn, *args):
         ctx = self._ctx
@@ -932,9 +936,9 @@ class QuantizedMatrix:
     def product_of_codes(self, codes, scales, bias=None, *, offsets=None, dtype=None, out=None):
         """The same for what RowQuantizer.quantize returned, so that several matrices can share it; `dtype` is float32 by default."""
         x = _Values(codes, self._ctx, "codes", integers=True)
-        ks, sptr = _beside(scales, x, "float32", [() if x.single else (x.n,)], "scales")
-        ko, optr = self._groups(x, offsets)
-        kb, bptr = self._bias(x, bias)
+        ks, sptr = _beside(scales, x, "float32", () if x.single else (x.n,), "scales")
+        ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
+        kb, bptr = self._bias(x, bias) if bias is not None else (None, None)
         y, yptr, kind, ld = _result(x, self._shape[1], dtype or (np.float32 if out is None else None), out)
         self._call(x, self._ctx._L.vqb_qmat_product_codes, x.ptr, x.ld, sptr, x.n, x.dim, optr, bptr, yptr, kind, ld, 1 if out is None else 0)
         return y
@@ -944,7 +948,7 @@ class QuantizedMatrix:
         the same type.  The rounding to codes counts as the identity.  Each dy * channel scale enters as the nearest of 16256 steps up
         to the largest of its row."""
         x = _Values(dy, self._ctx, "dy")
-        ko, optr = self._groups(x, offsets)
+        ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
         y, yptr, kind, ld = _result(x, self._shape[2], x.keep.dtype if out is None else None, out)
         if kind != x.type:
             raise ValueError("out must have dy's dtype")

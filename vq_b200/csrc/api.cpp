@@ -1271,6 +1271,7 @@ int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim
     return locked(ctx, [&] {
         if (dim == 0) throw Error(VQB_ERR_EMPTY_INPUT, "Empty input: at least one vector is required.");
         check_row_count(n);
+        if (dim > QMAT_MOST_ROWS) throw Error(VQB_ERR_UNSUPPORTED, "rows of more than 2^30 - 1 values");
         if (n == 0) return;
         check_values("x", x, type, dim, ld);
         if (!codes || !scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");

@@ -243,7 +243,7 @@ bool launch_product_few(CudaDevice &dev, const Product &p, const void *x, int ty
     if (x && (p.n > 2 || p.n * p.width > 16384 || (reinterpret_cast<uintptr_t>(x) | (p.n == 1 ? 0 : ld * value_bytes(type))) % 16)) return false;
     const size_t eights = (p.n + 7) / 8;
     FewParams P{};
-    P.rows.x = x, P.rows.n = p.n, P.rows.width = p.width, P.rows.ld = ld;
+    P.rows.x = x, P.rows.n = p.n, P.rows.width = (uint32_t)p.width, P.rows.ld = ld;
     P.given = p.rows, P.given_ld = p.rows_ld, P.given_scales = p.row_scales;
     P.ld = (int)codes_ld(p.width), P.pitch = (P.ld + 127) / 128 * 128 + 64, P.channels = (int)p.channels;
     P.channel_scales = p.channel_scales, P.bias = p.bias, P.y = p.y, P.y_type = p.y_type, P.y_ld = p.y_ld, P.error = dev.error_word();

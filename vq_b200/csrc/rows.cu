@@ -40,14 +40,14 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>) quantize_rows_kernel(const 
     const T *row = static_cast<const T *>(P.x) + r * P.ld;
     const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr;
     if (DIGITS == 2 && !columns) return;
-    const size_t pieces = (P.width + (size_t)LANES * N - 1) / ((size_t)LANES * N);
+    const uint32_t pieces = (P.width + LANES * N - 1) / (LANES * N);
     RowOf<T, DIGITS, LANES, ALIGNED> it(P, r, lane, columns);
     Piece<T> held[HELD];
 #pragma unroll
     for (int h = 0; h < HELD; ++h) held[h] = load_values<T, LANES, ALIGNED>(row, h, lane, P.width);
 #pragma unroll
     for (int h = 0; h < HELD; ++h) it.look(held[h], h);
-    for (size_t h = HELD; h < pieces; ++h) it.look(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h);
+    for (uint32_t h = HELD; h < pieces; ++h) it.look(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h);
     uint32_t most = it.largest();
     if (WARPS > 1) {
         if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = most;
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>) quantize_rows_kernel(const 
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
         if (column<N, LANES, ALIGNED>(h, lane, 0) < P.width) it.write(held[h], h, none, inverse);
-    for (size_t h = HELD; h < pieces; ++h) it.write(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h, none, inverse);
+    for (uint32_t h = HELD; h < pieces; ++h) it.write(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h, none, inverse);
 }
 
 template <typename T, int DIGITS, int LANES, int HELD> void quantize_rows_with(CudaDevice &dev, const RowParams &P, bool aligned)
@@ -80,7 +80,7 @@ template <typename T, int DIGITS> void quantize_rows_typed(CudaDevice &dev, cons
     const size_t apart = P.n == 1 ? 0 : P.ld * sizeof(T), codes_apart = P.n == 1 ? 0 : P.ld_codes; // (one row has no next one)
     const bool aligned = (reinterpret_cast<uintptr_t>(P.x) | apart) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.codes) | codes_apart | reinterpret_cast<uintptr_t>(P.low)) % 8 == 0;
     const size_t pieces = (P.width + Piece<T>::N - 1) / Piece<T>::N;
-    if (P.n >= (size_t(1) << 23) / P.width) {
+    if (pieces > 64 && P.n >= (size_t(1) << 23) / P.width) {
         if (pieces <= 128) quantize_rows_with<T, DIGITS, 32, 4>(dev, P, aligned);
         else if (pieces <= 256) quantize_rows_with<T, DIGITS, 64, 4>(dev, P, aligned);
         else if (pieces <= 512) quantize_rows_with<T, DIGITS, 128, 4>(dev, P, aligned);
@@ -137,14 +137,14 @@ __global__ void align_codes_kernel(const int8_t *codes, size_t n, size_t width, 
 
 void launch_quantize_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, int8_t *codes, size_t ld_codes, float *scales)
 {
-    RowParams P{x, n, width, ld, codes, nullptr, ld_codes, scales, nullptr, nullptr, 0};
+    RowParams P{x, n, ld, (uint32_t)width, codes, nullptr, ld_codes, scales, nullptr, nullptr, 0};
     quantize_rows_any<1>(dev, "quantize_rows", P, type);
 }
 
 void launch_digit_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, const float *column_scales, size_t groups, const int64_t *offsets,
                        int8_t *digits, size_t ld_codes, float *scales)
 {
-    RowParams P{x, n, width, ld, digits, digits + n * ld_codes, ld_codes, scales, column_scales, reinterpret_cast<const long long *>(offsets), (int)groups};
+    RowParams P{x, n, ld, (uint32_t)width, digits, digits + n * ld_codes, ld_codes, scales, column_scales, reinterpret_cast<const long long *>(offsets), (int)groups};
     quantize_rows_any<2>(dev, "digit_rows", P, type);
 }
 

@@ -32,24 +32,24 @@ template <> struct Piece<__nv_bfloat16> {
 
 // Which columns a lane has.  Where rows and codes are aligned: N neighbouring ones a piece, 16 bytes loaded and N stored at once.  Elsewhere
 // every LANESth column: 4 or 2 bytes a lane, but a warp's are next to each other.
-template <int N, int LANES, bool ALIGNED> __device__ __forceinline__ size_t column(size_t piece, int lane, int i)
+template <int N, int LANES, bool ALIGNED> __device__ __forceinline__ uint32_t column(uint32_t piece, int lane, int i)
 {
     return ALIGNED ? (piece * LANES + lane) * N + i : (piece * N + i) * LANES + lane;
 }
 
 // a piece of a row, 0 behind its end
-template <typename T, int LANES, bool ALIGNED> __device__ __forceinline__ Piece<T> load_values(const T *row, size_t piece, int lane, size_t width)
+template <typename T, int LANES, bool ALIGNED> __device__ __forceinline__ Piece<T> load_values(const T *row, uint32_t piece, int lane, uint32_t width)
 {
     constexpr int N = Piece<T>::N;
     Piece<T> p;
     p.w = make_uint4(0, 0, 0, 0);
-    const size_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
+    const uint32_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
     if (ALIGNED && k + N <= width) {
         p.w = *reinterpret_cast<const uint4 *>(row + k);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const size_t at = column<N, LANES, ALIGNED>(piece, lane, i);
+            const uint32_t at = column<N, LANES, ALIGNED>(piece, lane, i);
             if (at < width) {
                 if (sizeof(T) == 4) (&p.w.x)[i] = reinterpret_cast<const uint32_t *>(row)[at];
                 else (&p.w.x)[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(row)[at] << (16 * (i & 1));
@@ -161,16 +161,16 @@ template <int N> __device__ __forceinline__ void pack_digits(const float (&u)[N]
     }
 }
 
-template <int N, int LANES, bool ALIGNED> __device__ __forceinline__ void store_codes(int8_t *row, size_t piece, int lane, size_t width, const Packed<N> &c)
+template <int N, int LANES, bool ALIGNED> __device__ __forceinline__ void store_codes(int8_t *row, uint32_t piece, int lane, uint32_t width, const Packed<N> &c)
 {
-    const size_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
+    const uint32_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
     if (ALIGNED && k + N <= width) {
         if (N == 8) *reinterpret_cast<uint2 *>(row + k) = make_uint2(c.w[0], c.w[N / 4 - 1]);
         else *reinterpret_cast<uint32_t *>(row + k) = c.w[0];
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const size_t at = column<N, LANES, ALIGNED>(piece, lane, i);
+            const uint32_t at = column<N, LANES, ALIGNED>(piece, lane, i);
             if (at < width) row[at] = (int8_t)(c.w[i >> 2] >> (8 * (i & 3)));
         }
     }
@@ -178,7 +178,8 @@ template <int N, int LANES, bool ALIGNED> __device__ __forceinline__ void store_
 
 struct RowParams {
     const void *x;
-    size_t n, width, ld;
+    size_t n, ld;
+    uint32_t width;
     int8_t *codes, *low; // low: the low digits' plane (two digits)
     size_t ld_codes;
     float *scales;
@@ -199,11 +200,11 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
 
     __device__ __forceinline__ RowOf(const RowParams &p, size_t row, int l, const float *c) : P(p), r(row), lane(l), columns(c), columns4(DIGITS == 2 && ALIGNED && p.width % 4 == 0) {}
 
-    __device__ __forceinline__ void values(const Piece<T> &p, size_t piece, float (&v)[N]) const
+    __device__ __forceinline__ void values(const Piece<T> &p, uint32_t piece, float (&v)[N]) const
     {
         float c[N];
         if (DIGITS == 2) {
-            const size_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
+            const uint32_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
             if (columns4 && k + N <= P.width) {
 #pragma unroll
                 for (int i = 0; i < N; i += 4) {
@@ -213,7 +214,7 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const size_t at = column<N, LANES, ALIGNED>(piece, lane, i);
+                    const uint32_t at = column<N, LANES, ALIGNED>(piece, lane, i);
                     c[i] = at < P.width ? columns[at] : 0.0f;
                 }
             }
@@ -222,7 +223,7 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
         for (int i = 0; i < N; ++i) v[i] = DIGITS == 2 ? p.at(i) * c[i] : p.at(i);
     }
     // the largest magnitude so far (two 16-bit ones at a time); its sign means nothing, NaN wins
-    __device__ __forceinline__ void look(const Piece<T> &p, size_t piece)
+    __device__ __forceinline__ void look(const Piece<T> &p, uint32_t piece)
     {
         if (DIGITS == 1 && sizeof(T) == 2) {
 #pragma unroll
@@ -251,14 +252,14 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
         if (largest >= 0x7F800000u) return __int_as_float(0x7FC00000);
         return largest == 0 ? 0.0f : fmaxf(__fdiv_rn(__uint_as_float(largest), DIGITS == 1 ? LARGEST_8 : LARGEST_15), 0x1p-126f);
     }
-    __device__ __forceinline__ void pack(const Piece<T> &p, size_t piece, const Inverse &inverse, Packed<N> &high, Packed<N> &low) const
+    __device__ __forceinline__ void pack(const Piece<T> &p, uint32_t piece, const Inverse &inverse, Packed<N> &high, Packed<N> &low) const
     {
         float v[N];
         values(p, piece, v);
         if (DIGITS == 1) high = pack_codes<N>(v, inverse);
         else pack_digits<N>(v, inverse, high, low);
     }
-    __device__ __forceinline__ void write(const Piece<T> &p, size_t piece, bool none, const Inverse &inverse) const
+    __device__ __forceinline__ void write(const Piece<T> &p, uint32_t piece, bool none, const Inverse &inverse) const
     {
         Packed<N> high = {}, low = {};
         if (!none) pack(p, piece, inverse, high, low);
