@@ -8,6 +8,7 @@
 //   vq::OptimizedProductQuantizer      <- opq::OptimizedProductQuantizer    (src/opq.rs:90-264)
 //   vq::ScalarQuantizer, BinaryQuantizer <- sq::, bq::                      (src/sq.rs, src/bq.rs)
 //   vq::VqError                        <- exceptions::VqError               (src/exceptions.rs:9-25)
+// vq::RowQuantizer and vq::QuantizedMatrix (8-bit codes with a scale for each row, and their products) have no counterpart there.
 // Where the reference panics, these functions throw vq::VqError whose what() is the reference's Display text.
 // Seeded sampling uses the documented SplitMix64 stand-in (see seeding.py): the reference's StdRng draws cannot be
 // reproduced without the `rand` crate, and the library takes row indices from its host for exactly that reason.
@@ -366,6 +367,59 @@ struct BinaryQuantizer {
         detail::check(vqb_bq_quantize(c, threshold, low, high, vector.data.data(), vector.len(), out.data.data()), c);
         return out;
     }
+};
+
+// int8 codes with a scale for each row (vqb_row_quantize; no counterpart in the reference).
+struct RowQuantizer {
+    struct Codes {
+        Vector<int8_t> codes;
+        float scale; // codes[k] * scale is next to the row's value, off by at most half a scale
+    };
+    static RowQuantizer fit() { return RowQuantizer{}; }
+    Codes quantize(const Vector<float> &vector) const
+    {
+        Codes out;
+        out.codes.data.resize(vector.len());
+        vqb_ctx *c = detail::context();
+        detail::check(vqb_row_quantize(c, vector.data.data(), VQB_F32, 1, vector.len(), vector.len(), out.codes.data.data(), vector.len(), &out.scale), c);
+        return out;
+    }
+};
+
+// A matrix held as int8 codes with a scale for each row (channel), and its products with rows that are quantized too (vqb_qmat_*).
+class QuantizedMatrix {
+  public:
+    static QuantizedMatrix fit(const std::vector<Vector<float>> &channels)
+    {
+        vqb_ctx *c = detail::context();
+        size_t dim = 0;
+        std::vector<float> flat = detail::pack_rows(channels, &dim);
+        vqb_qmat *h = nullptr;
+        detail::check(vqb_qmat_fit(c, flat.data(), VQB_F32, 1, channels.size(), dim, 0, &h), c);
+        return QuantizedMatrix(h, channels.size());
+    }
+    Vector<float> product(const Vector<float> &row) const
+    {
+        Vector<float> out;
+        out.data.resize(outputs_);
+        detail::check(vqb_qmat_product(h_.get(), row.data.data(), VQB_F32, 1, row.len(), row.len(), nullptr, nullptr, out.data.data(), VQB_F32, outputs_, 0),
+                      detail::context());
+        return out;
+    }
+    Vector<float> product(const RowQuantizer::Codes &row) const
+    {
+        Vector<float> out;
+        out.data.resize(outputs_);
+        detail::check(vqb_qmat_product_codes(h_.get(), row.codes.data.data(), row.codes.len(), &row.scale, 1, row.codes.len(), nullptr, nullptr, out.data.data(),
+                                             VQB_F32, outputs_, 0),
+                      detail::context());
+        return out;
+    }
+
+  private:
+    QuantizedMatrix(vqb_qmat *h, size_t outputs) : h_(h, vqb_qmat_destroy), outputs_(outputs) {}
+    std::shared_ptr<vqb_qmat> h_;
+    size_t outputs_;
 };
 
 // lbg_quantize (src/utils.rs:32-109); crate-private in the reference, exposed here because its unit tests are part
