@@ -289,6 +289,9 @@ int vqb_bq_quantize(vqb_ctx *ctx, float threshold, uint8_t low, uint8_t high, co
  * with VQB_ZERO_REST.  Offsets in device memory are not looked at by the host: where they are not ascending, or leave
  * 0 .. n, nothing outside the n rows is touched, but which results are written is not defined.
  *
+ * A matrix is complete when the call that makes it returns (which therefore cannot be captured into a graph); a graph of a product reads the matrix
+ * whenever it is replayed.  Products may be captured; but for one or two rows with one matrix they take memory of the call, which then is the graph's.
+ *
  * Values are f32, f16 or bf16 (the same bits in and out as the caller's); ld: values from row to row (>= the row's width).  Outputs may not
  * overlap inputs.  No rows (n == 0) is no error.  Limits: width 131071 (VQB_ERR_UNSUPPORTED beyond: the sums are 32 bits), 1024 groups, 2^30 - 1 rows. */
 enum vqb_value_type { VQB_F32 = 0, VQB_F16 = 1, VQB_BF16 = 2 };

@@ -414,3 +414,30 @@ def test_many_wide_rows_are_the_definitions(n, dim, dtype):
     for part in torch.arange(n, device="cuda").split(2048):
         want_q, want_s = codes64(x[part])
         assert torch.equal(q[part].double(), want_q) and torch.equal(torch.nan_to_num(s[part], nan=-1.0).double(), torch.nan_to_num(want_s, nan=-1.0))
+
+
+def test_as_many_groups_as_there_may_be():
+    torch = torch_()
+    counts = [(7 * g) % 5 for g in range(1024)]
+    n = sum(counts) + 9
+    off = offsets_of(counts, 4)
+    x, w = normal(1, n, 48, dtype="bfloat16"), normal(2, 1024, 40, 48, scale=0.1)
+    m, wq, ws = matrix64(w, gradient=True)
+    y = m.product(x, offsets=torch.from_numpy(off).cuda())
+    want, size, within = product64(*codes64(x), wq, ws, None, off)
+    check(y[within], want[within], size[within])
+    assert not y[~within].any()
+    dy = normal(3, n, 40, dtype="bfloat16")
+    want, size, extra, within = gradient_limits(dy, wq, ws, off)
+    check(m.input_gradient(dy, offsets=off)[within], want[within], size[within], extra[within])
+
+
+def test_one_group_with_offsets_takes_some_of_the_rows():
+    torch = torch_()
+    x = normal(1, 50, 64, dtype="float16")
+    m, wq, ws = matrix64(normal(2, 30, 64))
+    off = np.array([7, 33])
+    want, size, within = product64(*codes64(x), wq, ws, None, off)
+    y = m.product(x, offsets=off)
+    check(y[within], want[within], size[within])
+    assert not y[~within].any()

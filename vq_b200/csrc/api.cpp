@@ -374,7 +374,10 @@ struct NewQmat {
         Qmat &m = qm->mat;
         m.groups = groups, m.outputs = outputs, m.inputs = inputs;
         cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(dev.stream(), &capture) != cudaSuccess) cudaGetLastError(); // (the default stream while another one is being captured)
+        if (cudaStreamIsCapturing(dev.stream(), &capture) != cudaSuccess) { // (the default stream while another one is being captured)
+            cudaGetLastError();
+            capture = cudaStreamCaptureStatusActive;
+        }
         if (capture != cudaStreamCaptureStatusNone) throw Error(VQB_ERR_UNSUPPORTED, "a matrix cannot be made while its stream is being captured");
         try {
             m.codes = static_cast<int8_t *>(dev.alloc(groups * outputs * codes_ld(inputs)));

@@ -458,8 +458,8 @@ size_t room_for_clusters(CudaDevice &dev, int ctas)
     static std::mutex mu;
     static std::map<std::pair<int, int>, int> known;
     std::lock_guard<std::mutex> lk(mu);
-    int &room = known[{dev.device(), ctas}];
-    if (room == 0) {
+    auto found = known.find({dev.device(), ctas});
+    if (found == known.end()) {
         auto kernel = product_tc_kernel<float, 1, true>;
         allow_shared_memory(dev, kernel);
         cudaLaunchConfig_t cfg = {};
@@ -468,9 +468,14 @@ size_t room_for_clusters(CudaDevice &dev, int ctas)
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cfg.attrs = &attr, cfg.numAttrs = 1;
-        VQB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&room, kernel, &cfg));
+        int room = 0;
+        if (cudaOccupancyMaxActiveClusters(&room, kernel, &cfg) != cudaSuccess) { // none, then
+            cudaGetLastError();
+            room = 0;
+        }
+        found = known.insert({{dev.device(), ctas}, room}).first;
     }
-    return (size_t)room;
+    return (size_t)found->second;
 }
 
 } // namespace

@@ -38,13 +38,13 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>) quantize_rows_kernel(const 
     const int lane = threadIdx.x % LANES;
     if (r >= P.n) return; // (whole warps; where a block barrier follows, a block is one row)
     const T *row = static_cast<const T *>(P.x) + r * P.ld;
-    const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr;
-    if (DIGITS == 2 && !columns) return;
     const uint32_t pieces = (P.width + LANES * N - 1) / (LANES * N);
-    RowOf<T, DIGITS, LANES, ALIGNED> it(P, r, lane, columns);
     Piece<T> held[HELD];
 #pragma unroll
     for (int h = 0; h < HELD; ++h) held[h] = load_values<T, LANES, ALIGNED>(row, h, lane, P.width);
+    const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr; // (its loads beside the row's)
+    if (DIGITS == 2 && !columns) return;
+    RowOf<T, DIGITS, LANES, ALIGNED> it(P, r, lane, columns);
 #pragma unroll
     for (int h = 0; h < HELD; ++h) it.look(held[h], h);
     for (uint32_t h = HELD; h < pieces; ++h) it.look(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h);
