@@ -45,8 +45,12 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>) quantize_rows_kernel(const 
     const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr; // (its loads beside the row's)
     if (DIGITS == 2 && !columns) return;
     RowOf<T, DIGITS, LANES, ALIGNED> it(P, r, lane, columns);
+    float u[DIGITS == 2 ? HELD : 1][N]; // two digits: what the columns' scales make of the row is kept instead
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) it.look(held[h], h);
+    for (int h = 0; h < HELD; ++h) {
+        if (DIGITS == 2) it.values(held[h], h, u[DIGITS == 2 ? h : 0]), it.look(u[DIGITS == 2 ? h : 0]);
+        else it.look(held[h], h);
+    }
     for (uint32_t h = HELD; h < pieces; ++h) it.look(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h);
     uint32_t most = it.largest();
     if (WARPS > 1) {
@@ -61,7 +65,10 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>) quantize_rows_kernel(const 
     const Inverse inverse(none ? 1.0f : scale);
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-        if (column<N, LANES, ALIGNED>(h, lane, 0) < P.width) it.write(held[h], h, none, inverse);
+        if (column<N, LANES, ALIGNED>(h, lane, 0) < P.width) {
+            if (DIGITS == 2) it.write(u[DIGITS == 2 ? h : 0], h, none, inverse);
+            else it.write(held[h], h, none, inverse);
+        }
     for (uint32_t h = HELD; h < pieces; ++h) it.write(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h, none, inverse);
 }
 

@@ -231,9 +231,13 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
         } else {
             float v[N];
             values(p, piece, v);
-#pragma unroll
-            for (int i = 0; i < N; ++i) most = __float_as_uint(larger(__uint_as_float(most), v[i]));
+            look(v);
         }
+    }
+    __device__ __forceinline__ void look(const float (&v)[N])
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) most = __float_as_uint(larger(__uint_as_float(most), v[i]));
     }
     // the largest magnitude's bits, of the whole warp (their order is that of the magnitudes, infinities and NaN on top)
     __device__ __forceinline__ uint32_t largest() const
@@ -256,6 +260,10 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
     {
         float v[N];
         values(p, piece, v);
+        pack(v, inverse, high, low);
+    }
+    __device__ __forceinline__ void pack(const float (&v)[N], const Inverse &inverse, Packed<N> &high, Packed<N> &low) const
+    {
         if (DIGITS == 1) high = pack_codes<N>(v, inverse);
         else pack_digits<N>(v, inverse, high, low);
     }
@@ -263,6 +271,16 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
     {
         Packed<N> high = {}, low = {};
         if (!none) pack(p, piece, inverse, high, low);
+        store(piece, high, low);
+    }
+    __device__ __forceinline__ void write(const float (&v)[N], uint32_t piece, bool none, const Inverse &inverse) const
+    {
+        Packed<N> high = {}, low = {};
+        if (!none) pack(v, inverse, high, low);
+        store(piece, high, low);
+    }
+    __device__ __forceinline__ void store(uint32_t piece, const Packed<N> &high, const Packed<N> &low) const
+    {
         store_codes<N, LANES, ALIGNED>(P.codes + r * P.ld_codes, piece, lane, P.width, high);
         if (DIGITS == 2) store_codes<N, LANES, ALIGNED>(P.low + r * P.ld_codes, piece, lane, P.width, low);
     }
