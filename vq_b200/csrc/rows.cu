@@ -39,9 +39,13 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>) quantize_rows_kernel(const 
     if (r >= P.n) return; // (whole warps; where a block barrier follows, a block is one row)
     const T *row = static_cast<const T *>(P.x) + r * P.ld;
     const uint32_t pieces = (P.width + LANES * N - 1) / (LANES * N);
+    const bool full = ALIGNED && HELD * LANES * N <= P.width; // all of the held pieces are whole
     Piece<T> held[HELD];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) held[h] = load_values<T, LANES, ALIGNED>(row, h, lane, P.width);
+    for (int h = 0; h < HELD; ++h) {
+        if (full) held[h].w = *reinterpret_cast<const uint4 *>(row + column<N, LANES, true>(h, lane, 0));
+        else held[h] = load_values<T, LANES, ALIGNED>(row, h, lane, P.width);
+    }
     const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr; // (its loads beside the row's)
     if (DIGITS == 2 && !columns) return;
     RowOf<T, DIGITS, LANES, ALIGNED> it(P, r, lane, columns);
@@ -63,12 +67,34 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>) quantize_rows_kernel(const 
     const bool none = it.no_codes(most);
     if (lane == 0) P.scales[r] = scale;
     const Inverse inverse(none ? 1.0f : scale);
+    Packed<N> high[HELD] = {}, low[DIGITS == 2 ? HELD : 1] = {};
+    if (!none) {
+        uint64_t unlike[HELD] = {};
+        bool some = false;
 #pragma unroll
-    for (int h = 0; h < HELD; ++h)
-        if (column<N, LANES, ALIGNED>(h, lane, 0) < P.width) {
-            if (DIGITS == 2) it.write(u[DIGITS == 2 ? h : 0], h, none, inverse);
-            else it.write(held[h], h, none, inverse);
+        for (int h = 0; h < HELD; ++h) {
+            if (DIGITS == 2) {
+                pack_digits<N>(u[DIGITS == 2 ? h : 0], inverse, high[h], low[DIGITS == 2 ? h : 0]);
+            } else {
+                it.values(held[h], h, u[0]);
+                high[h] = pack_most<N>(u[0], inverse, unlike[h]);
+                some |= any_unlike(unlike[h]);
+            }
         }
+        if (DIGITS == 1 && some) {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h) {
+                if (!any_unlike(unlike[h])) continue;
+                it.values(held[h], h, u[0]);
+                high[h] = pack_all<N>(u[0], inverse);
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        if (full) it.put(h, high[h], low[DIGITS == 2 ? h : 0]);
+        else if (column<N, LANES, ALIGNED>(h, lane, 0) < P.width) it.store(h, high[h], low[DIGITS == 2 ? h : 0]);
+    }
     for (uint32_t h = HELD; h < pieces; ++h) it.write(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h, none, inverse);
 }
 

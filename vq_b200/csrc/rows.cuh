@@ -107,11 +107,21 @@ struct Inverse {
     }
 };
 
-template <int N> __device__ __forceinline__ Packed<N> pack_codes(const float (&v)[N], const Inverse &inverse)
+template <int N> __device__ __forceinline__ Packed<N> low_bytes(const float (&m)[N])
+{
+    Packed<N> out;
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+        out.w[i] = __byte_perm(__byte_perm(__float_as_uint(m[4 * i]), __float_as_uint(m[4 * i + 1]), 0x0040),
+                               __byte_perm(__float_as_uint(m[4 * i + 2]), __float_as_uint(m[4 * i + 3]), 0x0040), 0x5410);
+    return out;
+}
+
+// The codes, unless some quotient is next to a half: then a half of `unlike` becomes positive.
+template <int N> __device__ __forceinline__ Packed<N> pack_most(const float (&v)[N], const Inverse &inverse, uint64_t &unlike)
 {
     const uint64_t magic = pair_of(MAGIC, MAGIC), minus = pair_of(-1.0f, -1.0f);
     float m[N];
-    uint64_t unlike = 0;
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
         const uint64_t pair = pair_of(v[i], v[i + 1]), u = fma_pair(pair, inverse.up, magic), d = fma_pair(pair, inverse.down, magic);
@@ -119,27 +129,43 @@ template <int N> __device__ __forceinline__ Packed<N> pack_codes(const float (&v
         unlike = fma_pair(off, off, unlike);
         halves_of(u, m[i], m[i + 1]);
     }
-    float ua, ub;
-    halves_of(unlike, ua, ub);
-    if (__builtin_expect(ua + ub > 0.0f, 0)) { // some quotient is next to a half
-        float down, unused;
-        halves_of(inverse.down, down, unused);
-        // twice the values where their difference could be below what f32 holds
-        const float scale = inverse.scale, twice = scale < 1.0f ? 2.0f : 1.0f;
+    return low_bytes<N>(m);
+}
+__device__ __forceinline__ bool any_unlike(uint64_t unlike)
+{
+    float a, b;
+    halves_of(unlike, a, b);
+    return a + b > 0.0f;
+}
+
+// The codes, whatever the quotients.  r = v times a neighbour of 1 / s, to a whole number, is right or one off; e = v - r s is exact (a multiple of half the last place
+// of s, and not above 1.5 s) and says which: beyond s / 2, or s / 2 itself with r odd, r moves towards v.  In 16-bit rows halves are not rare (v and the row's largest are
+// eight-bit numbers): this is taken for one piece in some ten.
+template <int N> __device__ __forceinline__ Packed<N> pack_all(const float (&v)[N], const Inverse &inverse)
+{
+    float up, unused;
+    halves_of(inverse.up, up, unused);
+    // twice the values where e could be below what f32 holds
+    const float twice = inverse.scale < 1.0f ? 2.0f : 1.0f, s = inverse.scale * twice;
+    const uint32_t half = __float_as_uint(0.5f * s);
+    float m[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float a = m[i] - MAGIC, b = __fmaf_rn(v[i], down, MAGIC) - MAGIC;
-            if (a == b) continue;
-            const float lower = fminf(a, b), h = lower + 0.5f, beyond = __fmaf_rn(-(h * twice), scale, v[i] * twice); // which side of h: the sign is exact
-            m[i] = (beyond > 0.0f || (beyond == 0.0f && ((int)lower & 1)) ? lower + 1.0f : lower) + MAGIC;
-        }
+    for (int i = 0; i < N; ++i) {
+        const float t = __fmaf_rn(v[i], up, MAGIC), e = __fmaf_rn(-__fsub_rn(t, MAGIC), s, v[i] * twice);
+        const float border = __uint_as_float(half - (__float_as_uint(t) & 1u)); // (odd: the next number below)
+        uint32_t bits = __float_as_uint(t);
+        if (e > border) ++bits;
+        if (e < -border) --bits;
+        m[i] = __uint_as_float(bits);
     }
-    Packed<N> out;
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i)
-        out.w[i] = __byte_perm(__byte_perm(__float_as_uint(m[4 * i]), __float_as_uint(m[4 * i + 1]), 0x0040),
-                               __byte_perm(__float_as_uint(m[4 * i + 2]), __float_as_uint(m[4 * i + 3]), 0x0040), 0x5410);
-    return out;
+    return low_bytes<N>(m);
+}
+
+template <int N> __device__ __forceinline__ Packed<N> pack_codes(const float (&v)[N], const Inverse &inverse)
+{
+    uint64_t unlike = 0;
+    const Packed<N> out = pack_most<N>(v, inverse, unlike);
+    return __builtin_expect(any_unlike(unlike), 0) ? pack_all<N>(v, inverse) : out;
 }
 
 // The two digits of v = u / t, |v| <= 16256: the high one is the whole number nearest to v / 128.  With w = v + 64 in 16 bits they are w >> 7 and
@@ -273,11 +299,15 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
         if (!none) pack(p, piece, inverse, high, low);
         store(piece, high, low);
     }
-    __device__ __forceinline__ void write(const float (&v)[N], uint32_t piece, bool none, const Inverse &inverse) const
+    // a whole piece, aligned
+    __device__ __forceinline__ void put(uint32_t piece, const Packed<N> &high, const Packed<N> &low) const
     {
-        Packed<N> high = {}, low = {};
-        if (!none) pack(v, inverse, high, low);
-        store(piece, high, low);
+        const size_t at = r * P.ld_codes + column<N, LANES, true>(piece, lane, 0);
+        if (N == 8) *reinterpret_cast<uint2 *>(P.codes + at) = make_uint2(high.w[0], high.w[N / 4 - 1]);
+        else *reinterpret_cast<uint32_t *>(P.codes + at) = high.w[0];
+        if (DIGITS == 1) return;
+        if (N == 8) *reinterpret_cast<uint2 *>(P.low + at) = make_uint2(low.w[0], low.w[N / 4 - 1]);
+        else *reinterpret_cast<uint32_t *>(P.low + at) = low.w[0];
     }
     __device__ __forceinline__ void store(uint32_t piece, const Packed<N> &high, const Packed<N> &low) const
     {
