@@ -29,7 +29,7 @@ template <int LANES> constexpr int THREADS_OF = LANES < 64 ? 128 : LANES;
 // LANES threads a row, HELD pieces a thread in registers; what is behind them is read a second time.  (256 threads: five blocks an SM, 8192 x 8192 bf16 in 39 us; 44 with
 // the registers that four leave.  Blocks of 128 take 35 instead of 32 for 16384 x 4096 when they are held to fewer.)
 template <typename T, int DIGITS, int LANES, int HELD, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS_OF<LANES>, DIGITS == 1 && LANES == 256 ? 5 : 1) quantize_rows_kernel(const RowParams P)
+__global__ void __launch_bounds__(THREADS_OF<LANES>, DIGITS == 1 && LANES == 256 ? 5 : 0) quantize_rows_kernel(const RowParams P)
 {
     constexpr int N = Piece<T>::N, THREADS = THREADS_OF<LANES>, WARPS = LANES / 32;
     __shared__ uint32_t parts[WARPS > 1 ? WARPS : 1];
