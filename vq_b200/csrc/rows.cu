@@ -107,26 +107,18 @@ template <typename T, int DIGITS, int LANES, int HELD> void quantize_rows_with(C
     else launch_following(quantize_rows_kernel<T, DIGITS, LANES, HELD, false>, grid, dim3(THREADS), 0, dev.stream(), P);
 }
 
-// As many threads a row as have two pieces of it each, or four where there are values enough that bytes under way count and not the time of one row
-// (us with two and four: 1024 x 1024 bf16 3.1 and 4.2, 8192 x 1024 9.5 and 8.3, 16384 x 1024 18.0 and 12.5, 4096 x 4096 13.4 and 12.4, 8192 x 4096 24.9 and 21.1).
+// As many threads a row as have four pieces of it each: bytes under way and not threads are what it takes (us with two and four pieces: 1024 x 1024 bf16 2.6 and
+// 2.5, 16384 x 1024 18.0 and 10.6, 4096 x 4096 12.9 and 10.8, 8192 x 4096 24.6 and 19.5); two where a warp has them all.
 template <typename T, int DIGITS> void quantize_rows_typed(CudaDevice &dev, const RowParams &P)
 {
     const size_t apart = P.n == 1 ? 0 : P.ld * sizeof(T), codes_apart = P.n == 1 ? 0 : P.ld_codes; // (one row has no next one)
     const bool aligned = (reinterpret_cast<uintptr_t>(P.x) | apart) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.codes) | codes_apart | reinterpret_cast<uintptr_t>(P.low)) % 8 == 0;
     const size_t pieces = (P.width + Piece<T>::N - 1) / Piece<T>::N;
-    if (pieces > 64 && P.n >= (size_t(1) << 23) / P.width) {
-        if (pieces <= 128) quantize_rows_with<T, DIGITS, 32, 4>(dev, P, aligned);
-        else if (pieces <= 256) quantize_rows_with<T, DIGITS, 64, 4>(dev, P, aligned);
-        else if (pieces <= 512) quantize_rows_with<T, DIGITS, 128, 4>(dev, P, aligned);
-        else if (pieces <= 1024) quantize_rows_with<T, DIGITS, 256, 4>(dev, P, aligned);
-        else quantize_rows_with<T, DIGITS, 512, 4>(dev, P, aligned);
-        return;
-    }
     if (pieces <= 64) quantize_rows_with<T, DIGITS, 32, 2>(dev, P, aligned);
-    else if (pieces <= 128) quantize_rows_with<T, DIGITS, 64, 2>(dev, P, aligned);
-    else if (pieces <= 256) quantize_rows_with<T, DIGITS, 128, 2>(dev, P, aligned);
-    else if (pieces <= 512) quantize_rows_with<T, DIGITS, 256, 2>(dev, P, aligned);
-    else if (pieces <= 1024) quantize_rows_with<T, DIGITS, 512, 2>(dev, P, aligned);
+    else if (pieces <= 128) quantize_rows_with<T, DIGITS, 32, 4>(dev, P, aligned);
+    else if (pieces <= 256) quantize_rows_with<T, DIGITS, 64, 4>(dev, P, aligned);
+    else if (pieces <= 512) quantize_rows_with<T, DIGITS, 128, 4>(dev, P, aligned);
+    else if (pieces <= 1024) quantize_rows_with<T, DIGITS, 256, 4>(dev, P, aligned);
     else quantize_rows_with<T, DIGITS, 512, 4>(dev, P, aligned);
 }
 
