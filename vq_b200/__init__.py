@@ -692,26 +692,25 @@ class _Values:
     __slots__ = ("cuda", "keep", "shape", "ptr", "single", "n", "dim", "ld", "type", "stream")
 
     def __init__(self, x, ctx, what="x", integers=False):
-        if isinstance(x, Vector):
-            x = x.data
-        self.cuda = _is_torch(x) and x.is_cuda
+        torch = sys.modules.get("torch")
+        self.cuda = torch is not None and isinstance(x, torch.Tensor) and x.is_cuda
         if self.cuda:
-            torch = sys.modules["torch"]
-            if x.get_device() != ctx.device:
-                raise ValueError(f"{what} is on cuda:{x.get_device()}, the context on cuda:{ctx.device}")
-            values = _TORCH_VALUES or _torch_values(torch)
-            if x.requires_grad:
-                x = x.detach()
+            device = ctx.device
+            if x.get_device() != device:
+                raise ValueError(f"{what} is on cuda:{x.get_device()}, the context on cuda:{device}")
+            values, dtype = _TORCH_VALUES or _torch_values(torch), x.dtype
             if integers:
-                if x.dtype is not torch.int8:
+                if dtype is not torch.int8:
                     raise ValueError(f"{what} must be int8")
                 self.type = None
             else:
-                self.type = values.get(x.dtype)
+                self.type = values.get(dtype)
                 if self.type is None:
-                    x, self.type = x.to(torch.float32), 0
-            self.stream = torch._C._cuda_getCurrentRawStream(ctx.device)
+                    x, self.type = x.detach().to(torch.float32), 0
+            self.stream = torch._C._cuda_getCurrentRawStream(device)
         else:
+            if isinstance(x, Vector):
+                x = x.data
             if _is_torch(x):
                 x = x.detach()
                 x = (x.float() if str(x.dtype) == "torch.bfloat16" else x).numpy()
@@ -727,19 +726,26 @@ class _Values:
             x = np.ascontiguousarray(x)
             self.stream = None
         shape = x.shape
-        self.single = len(shape) == 1
-        if len(shape) not in (1, 2):
+        axes = len(shape)
+        if axes == 2:
+            self.single = False
+            self.n, self.dim = n, dim = shape
+        elif axes == 1:
+            self.single, self.n, self.dim = True, 1, shape[0]
+            n, dim = 1, shape[0]
+        else:
             raise ValueError("expected a vector or a matrix of row vectors")
-        self.n, self.dim = (1, shape[0]) if self.single else shape
-        self.ld = self.dim
+        self.ld = dim
         if self.cuda:
             strides = x.stride()
-            step = strides[0] if not self.single and self.n > 1 else self.dim
-            if (self.dim > 1 and strides[-1] != 1) or step < self.dim:
-                x, step = x.contiguous(), self.dim
+            step = strides[0] if n > 1 else dim
+            if (dim > 1 and strides[-1] != 1) or step < dim:
+                x, step = x.detach().contiguous(), dim
             self.ld = step
+            self.ptr = x.data_ptr()
+        else:
+            self.ptr = x.ctypes.data
         self.keep, self.shape = x, shape
-        self.ptr = x.data_ptr() if self.cuda else x.ctypes.data
 
 
 def _result(x: _Values, width: int, dtype, out):
@@ -798,6 +804,14 @@ def _beside(v, x: _Values, name: str, shape, what: str):
     return v, ptr
 
 
+def _context_of(rows) -> Context:
+    """The context of the device that the rows are on."""
+    if _is_torch(rows) and rows.is_cuda:
+        device = rows.get_device()
+        return _default.get(device) or default_context(device)
+    return default_context()
+
+
 class RowQuantizer:
     """int8 codes with a scale for each row: ``codes[i] * scales[i]`` is next to row i, off by at most half a scale.
 
@@ -816,13 +830,13 @@ class RowQuantizer:
     def quantize(self, rows):
         """(codes, scales) of one vector or of a batch: int8 of the rows' shape, float32 with one value a row.  On the GPU the codes' rows begin at
         multiples of 16 bytes (their stride), for the products' sake."""
-        ctx = self._ctx or default_context()
+        ctx = self._ctx or _context_of(rows)
         x = _Values(rows, ctx, "rows")
         if x.cuda:
             torch, device = sys.modules["torch"], x.keep.device
             ld = x.dim + -x.dim % 16  # rows that begin at multiples of 16 bytes are multiplied as they are
             codes = torch.empty_strided(x.shape, (1,) if x.single else (ld, 1), dtype=torch.int8, device=device)
-            scales = torch.empty_strided(() if x.single else (x.n,), () if x.single else (1,), dtype=torch.float32, device=device)
+            scales = torch.empty_strided(x.shape[:-1], () if x.single else (1,), dtype=torch.float32, device=device)
             cptr, sptr = codes.data_ptr(), scales.data_ptr()
         else:
             ld, codes, scales = x.dim, np.empty(x.shape, np.int8), np.empty(x.shape[:-1], np.float32)
@@ -854,7 +868,7 @@ class QuantizedMatrix:
     @classmethod
     def fit(cls, weights, *, gradient: bool = False, ctx: Context | None = None):
         """Quantizes every channel (row) of the weights by itself; float32, float16 or bfloat16 weights."""
-        ctx = ctx or default_context()
+        ctx = ctx or _context_of(weights)
         flat, (groups, outputs) = cls._flat(weights)
         x = _Values(flat, ctx, "weights")
         if x.ld != x.dim:
@@ -866,7 +880,7 @@ class QuantizedMatrix:
     @classmethod
     def from_parts(cls, codes, scales, *, gradient: bool = False, ctx: Context | None = None):
         """A matrix of given int8 codes and the scales of its channels."""
-        ctx = ctx or default_context()
+        ctx = ctx or _context_of(codes)
         flat, (groups, outputs) = cls._flat(codes)
         x = _Values(flat, ctx, "codes", integers=True)
         if x.ld != x.dim:
