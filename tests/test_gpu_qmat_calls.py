@@ -341,3 +341,33 @@ def test_rows_beyond_32_bits(lowest):
     for at in (0, n // 2 - 1, n - 300):
         want_q, want_s = codes64(x[at:at + 300])
         assert torch.equal(q[at:at + 300].double(), want_q) and torch.equal(torch.nan_to_num(s[at:at + 300].double(), -1.0), torch.nan_to_num(want_s, -1.0))
+
+
+def test_work_from_before_a_captured_call_is_waited_for_after_it():
+    """A long call on one stream, a captured one, and a call on a third stream, which uses the first one's scratch."""
+    torch = torch_()
+    from vq_b200 import synth
+    books = [synth.uniform01(16 * 256, 8, 3 + i).reshape(16, 256, 8) for i in range(2)]
+    a, b = (vq.ProductQuantizer.from_codebooks(c, vq.Distance.Euclidean) for c in books)
+    x = torch.from_numpy(synth.uniform01(300_000, 128, 9)).cuda()
+    small = x[:5_000].contiguous()
+    m, rows = vq.QuantizedMatrix.fit(normal(1, 64, 128)), normal(2, 40, 128)
+    want_a, want_b, want_y = a.quantize(x, return_codes=True)[1].clone(), b.quantize(small, return_codes=True)[1].clone(), m.product(rows).clone()
+    first, third = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(10):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        got = []
+        with torch.cuda.stream(first):
+            got.append(a.quantize(x, return_codes=True)[1])
+            got.append(a.quantize(x, return_codes=True)[1])
+        capture = torch.cuda.Stream()
+        with torch.cuda.stream(capture):
+            graph.capture_begin()
+            y = m.product(rows)
+            graph.capture_end()
+        with torch.cuda.stream(third):
+            got.append(b.quantize(small, return_codes=True)[1])
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want_a) and torch.equal(got[1], want_a) and torch.equal(got[2], want_b) and torch.equal(y, want_y)

@@ -203,12 +203,12 @@ void CudaDevice::set_stream(cudaStream_t s)
     const cudaStream_t old = stream_;
     if (s == old) return;
     stream_ = s;
-    if (!unfinished_ || captured(s)) return;
+    if (!unfinished_) return;
     if (lasting(old)) {
         if (captured(old)) return;
         VQB_CUDA_CHECK(cudaEventRecord(order_event_, old));
     }
-    VQB_CUDA_CHECK(cudaStreamWaitEvent(s, order_event_, 0));
+    if (!captured(s)) VQB_CUDA_CHECK(cudaStreamWaitEvent(s, order_event_, 0)); // (otherwise the first call after the capture does)
 }
 
 bool CudaDevice::lasting(cudaStream_t s) const { return s == own_stream_ || s == nullptr || s == cudaStreamLegacy; }
@@ -219,8 +219,8 @@ void CudaDevice::end_call()
     bop_fresh_ = dense_fresh_ = nullptr; // the next call's centroids may have the same address
     if (upload_at_) upload_at_ = UPLOAD_BYTES; // and its stream another one: its first upload waits for the last of this call
     if (!unfinished_ || lasting(stream_)) return;
-    if (captured(stream_)) unfinished_ = false;
-    else if (cudaEventRecord(order_event_, stream_) != cudaSuccess) cudaGetLastError(); // (not the next launch's error)
+    // (What was unfinished before a captured call still is, and has its event.)
+    if (!captured(stream_) && cudaEventRecord(order_event_, stream_) != cudaSuccess) cudaGetLastError(); // (not the next launch's error)
 }
 
 cudaStream_t CudaDevice::aux_stream(int i)
