@@ -371,3 +371,22 @@ def test_work_from_before_a_captured_call_is_waited_for_after_it():
             graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want_a) and torch.equal(got[1], want_a) and torch.equal(got[2], want_b) and torch.equal(y, want_y)
+
+
+def test_a_matrix_dropped_inside_a_capture_leaves_the_capture_alone():
+    """As a garbage collector may do it: its memory goes back after the capture."""
+    torch = torch_()
+    w, x = normal(1, 4096, 4096), normal(2, 20, 4096)
+    keep = vq.QuantizedMatrix.fit(normal(3, 40, 4096))
+    want = keep.product(x)
+    for _ in range(20):
+        drop = vq.QuantizedMatrix.fit(w, gradient=True)
+        drop.product(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = keep.product(x)
+            del drop
+            z = keep.product(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(z, want) and torch.equal(keep.product(x), want)

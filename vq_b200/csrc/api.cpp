@@ -1444,9 +1444,9 @@ int vqb_qmat_destroy(vqb_qmat *qm)
     if (!qm) return VQB_OK;
     vqb_ctx *ctx = qm->ctx;
     destroyed(ctx, [&] {
-        ctx->dev->release(qm->mat.codes);
-        ctx->dev->release(qm->mat.scales);
-        ctx->dev->release(qm->mat.turned);
+        ctx->dev->release_later(qm->mat.codes);
+        ctx->dev->release_later(qm->mat.scales);
+        ctx->dev->release_later(qm->mat.turned);
     });
     delete qm;
     return VQB_OK;

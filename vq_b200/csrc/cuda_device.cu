@@ -84,6 +84,7 @@ CudaDevice::~CudaDevice()
     if (own_stream_) {
         cudaSetDevice(device_);
         cudaStreamSynchronize(own_stream_);
+        for (void *p : later_) cudaFree(p);
         for (int i = 0; i < 2; ++i)
             if (aux_[i]) cudaStreamDestroy(aux_[i]);
         if (stage_event_) cudaEventDestroy(stage_event_);
@@ -218,6 +219,11 @@ void CudaDevice::end_call()
     release_dense();
     bop_fresh_ = dense_fresh_ = nullptr; // the next call's centroids may have the same address
     if (upload_at_) upload_at_ = UPLOAD_BYTES; // and its stream another one: its first upload waits for the last of this call
+    if (!later_.empty() && !captured(stream_)) {
+        for (void *p : later_) release(p);
+        later_.clear();
+        unfinished_ = true;
+    }
     if (!unfinished_ || lasting(stream_)) return;
     // (What was unfinished before a captured call still is, and has its event.)
     if (!captured(stream_) && cudaEventRecord(order_event_, stream_) != cudaSuccess) cudaGetLastError(); // (not the next launch's error)
@@ -263,6 +269,13 @@ void *CudaDevice::alloc(size_t bytes)
 void CudaDevice::release(void *p)
 {
     if (p) cudaFreeAsync(p, stream_);
+}
+
+void CudaDevice::release_later(void *p)
+{
+    if (!p) return;
+    if (captured(stream_)) later_.push_back(p);
+    else release(p);
 }
 
 // Reads mapped host memory over the link; used for small uploads while a large copy occupies the copy engine.

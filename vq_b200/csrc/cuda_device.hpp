@@ -34,6 +34,9 @@ class CudaDevice : public Device {
     static constexpr size_t PQ_KEPT_CODES = size_t(32) << 20;
     uint8_t *pq_kept_codes() const { return pq_codes_; }
     void release(void *p) override;
+    // The same at any time: while the stream is being captured, where a free would become part of the graph, the memory is kept until the end of the first call
+    // after that.
+    void release_later(void *p);
     void upload(void *dst, const void *src, size_t bytes) override;
     void upload_queued(void *dst, const void *src, size_t bytes) override;
     void download(void *dst, const void *src, size_t bytes) override;
@@ -134,6 +137,7 @@ class CudaDevice : public Device {
     // puts that one behind order_event_.
     bool unfinished_ = false; // nothing has waited for stream_ since the last launch or copy
     cudaEvent_t order_event_ = nullptr;
+    std::vector<void *> later_; // release_later
     bool lasting(cudaStream_t s) const;
     static constexpr size_t STAGE_BYTES = 1u << 20; // pinned staging for small downloads
     static constexpr size_t UPLOAD_BYTES = 1u << 20; // behind it, a ring for small uploads
