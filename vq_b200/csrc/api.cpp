@@ -1284,7 +1284,7 @@ int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim
         In ix(dev, x, span(n, dim, ld, value_bytes(type)));
         Out oc(dev, codes, span(n, dim, ld_codes, 1)), os(dev, scales, sizeof(float) * n);
         if (oc.host && ld_codes != dim) VQB_CUDA_CHECK(cudaMemcpyAsync(oc.d, oc.host, oc.bytes, cudaMemcpyHostToDevice, dev.stream()));
-        launch_quantize_rows(dev, ix.d, type, n, dim, ld, oc.as<int8_t>(), ld_codes, os.as<float>());
+        launch_quantize_rows(dev, ix.d, type, n, dim, ld, oc.as<int8_t>(), ld_codes, os.as<float>(), false);
         finish(oc, os);
     });
 }
@@ -1301,7 +1301,7 @@ int vqb_qmat_fit(vqb_ctx *ctx, const void *weights, int type, size_t groups, siz
         In iw(dev, weights, groups * outputs * inputs * value_bytes(type));
         NewQmat made(ctx, groups, outputs, inputs, flags);
         Qmat &m = made.qm->mat;
-        launch_quantize_rows(dev, iw.d, type, groups * outputs, inputs, inputs, m.codes, codes_ld(inputs), m.scales);
+        launch_quantize_rows(dev, iw.d, type, groups * outputs, inputs, inputs, m.codes, codes_ld(inputs), m.scales, false);
         *out = made.done();
     });
 }
@@ -1369,7 +1369,7 @@ int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim
         if (launch_product_few(dev, p, ix.d, type, ld)) return oy.out.finish();
         Scratch codes(dev, n * p.rows_ld + n * sizeof(float));
         float *scales = reinterpret_cast<float *>(codes.d + n * p.rows_ld);
-        launch_quantize_rows(dev, ix.d, type, n, dim, ld, reinterpret_cast<int8_t *>(codes.d), p.rows_ld, scales);
+        launch_quantize_rows(dev, ix.d, type, n, dim, ld, reinterpret_cast<int8_t *>(codes.d), p.rows_ld, scales, true);
         p.rows = reinterpret_cast<const int8_t *>(codes.d), p.row_scales = scales, p.rows_follow = true;
         if (!launch_product_few(dev, p, nullptr, 0, 0)) launch_product(dev, p);
         oy.out.finish();

@@ -117,7 +117,6 @@ template <typename T, int EIGHTS, int PAIRS> __global__ void __launch_bounds__(T
     for (int i = threadIdx.x; i < NT * count; i += 32 * WARPS) sums[i] = 0;
     const int n = (int)P.rows.n;
     rows_are_there();
-    product_may_start(); // (the next product's launch and first fetches beside this one's end)
     if constexpr (std::is_same<T, int8_t>::value) {
         const int pieces = P.pitch / 16, width = (int)P.rows.width;
         for (int i = threadIdx.x; i < NT * pieces; i += 32 * WARPS) { // (zeros behind the width)

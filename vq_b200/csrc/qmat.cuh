@@ -13,6 +13,7 @@ namespace vqb {
 // from here on; every thread calls it before it reads what that kernel may have written, or leaves.  (What is read before: codes of a matrix,
 // which is complete when the call that made it returns.)
 __device__ __forceinline__ void rows_are_there() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Only where a product of the same call comes next: a kernel of another call may take this one's results for memory that stays the same.
 __device__ __forceinline__ void product_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename T> __device__ __forceinline__ T from_float(float v);

@@ -51,7 +51,9 @@ struct Product {
 
 // codes[i][k] = x[i][k] / s[i] to the nearest whole number (halves to even, of the real quotient), s[i] = max_k |x[i][k]| / 127; s is 0 for
 // a row of zeros and NaN for one with an infinity or a NaN, with codes 0.  Bytes behind the row's width stay as they are.
-void launch_quantize_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, int8_t *codes, size_t ld_codes, float *scales);
+// product_follows: the caller's next launch is launch_product or launch_product_few (which waits for these codes itself; other kernels that may start early take
+// what was written for invariant).
+void launch_quantize_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, int8_t *codes, size_t ld_codes, float *scales, bool product_follows);
 // u[i][j] = x[i][j] column_scales[g][j] of the row's group g as two digits: u / t = 128 high + low, t = max |u| / 16256.  digits: n x ld_codes high
 // ones and as many low ones.
 void launch_digit_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, const float *column_scales, size_t groups, const int64_t *offsets,

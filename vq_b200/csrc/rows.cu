@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>, DIGITS == 1 && LANES == 256
     constexpr int N = Piece<T>::N, THREADS = THREADS_OF<LANES>, WARPS = LANES / 32;
     __shared__ uint32_t parts[WARPS > 1 ? WARPS : 1];
     rows_are_there();
-    product_may_start();
+    if (P.product_follows) product_may_start();
     const size_t r = (size_t)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES;
     if (r >= P.n) return; // (whole warps; where a block barrier follows, a block is one row)
@@ -161,16 +161,17 @@ __global__ void align_codes_kernel(const int8_t *codes, size_t n, size_t width, 
 
 } // namespace
 
-void launch_quantize_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, int8_t *codes, size_t ld_codes, float *scales)
+void launch_quantize_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, int8_t *codes, size_t ld_codes, float *scales,
+                          bool product_follows)
 {
-    RowParams P{x, n, ld, (uint32_t)width, codes, nullptr, ld_codes, scales, nullptr, nullptr, 0};
+    RowParams P{x, n, ld, (uint32_t)width, codes, nullptr, ld_codes, scales, nullptr, nullptr, 0, product_follows};
     quantize_rows_any<1>(dev, "quantize_rows", P, type);
 }
 
 void launch_digit_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, const float *column_scales, size_t groups, const int64_t *offsets,
                        int8_t *digits, size_t ld_codes, float *scales)
 {
-    RowParams P{x, n, ld, (uint32_t)width, digits, digits + n * ld_codes, ld_codes, scales, column_scales, reinterpret_cast<const long long *>(offsets), (int)groups};
+    RowParams P{x, n, ld, (uint32_t)width, digits, digits + n * ld_codes, ld_codes, scales, column_scales, reinterpret_cast<const long long *>(offsets), (int)groups, true};
     quantize_rows_any<2>(dev, "digit_rows", P, type);
 }
 

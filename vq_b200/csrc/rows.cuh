@@ -212,6 +212,7 @@ struct RowParams {
     const float *column_scales; // groups x width (two digits)
     const long long *offsets;
     int groups;
+    bool product_follows; // the next kernel of the stream is a product of this call
 };
 
 // One row's arithmetic on pieces of it.
