@@ -959,8 +959,8 @@ class QuantizedMatrix:
 
     def input_gradient(self, dy, *, offsets=None, out=None):
         """The gradient of ``product`` with respect to its rows, given the one with respect to its result (n x outputs, float16 or bfloat16): n x inputs of
-        the same type.  The rounding to codes counts as the identity.  Each dy * channel scale enters as the nearest of 16256 steps up
-        to the largest of its row."""
+        the same type.  The rounding to codes counts as the identity.  Each dy * channel scale enters with 24 bits of the largest of its
+        row, as a sum of them in float32 would hold it."""
         x = _Values(dy, self._ctx, "dy")
         ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
         y, yptr, kind, ld = _result(x, self._shape[2], x.keep.dtype if out is None else None, out)

@@ -1418,7 +1418,7 @@ int vqb_qmat_input_gradient(vqb_qmat *qm, const void *dy, int type, size_t n, si
         if (dim != m.outputs) throw Error(VQB_ERR_DIMENSION_MISMATCH, dim_mismatch(m.outputs, dim));
         check_row_count(n);
         if (flags & ~VQB_ZERO_REST) throw Error(VQB_ERR_BAD_ARGUMENT, "unknown flag");
-        if (type == VQB_F32) throw Error(VQB_ERR_UNSUPPORTED, "gradients are f16 or bf16: dy enters the product in 15 bits");
+        if (type == VQB_F32) throw Error(VQB_ERR_UNSUPPORTED, "gradients are f16 or bf16");
         CudaDevice &dev = *ctx->dev;
         OffsetsIn io(dev, offsets, m.groups, n);
         if (n == 0) return;
@@ -1427,11 +1427,11 @@ int vqb_qmat_input_gradient(vqb_qmat *qm, const void *dy, int type, size_t n, si
         In iy(dev, dy, span(n, dim, ld, value_bytes(type)));
         RowsOut ox(dev, dx, n, m.inputs, dx_ld, type, !offsets || (flags & VQB_ZERO_REST));
         Product p;
-        p.codes = m.turned, p.groups = m.groups, p.channels = m.inputs, p.width = m.outputs, p.digits = 2;
+        p.codes = m.turned, p.groups = m.groups, p.channels = m.inputs, p.width = m.outputs, p.digits = 3;
         p.n = n, p.rows_ld = codes_ld(dim), p.offsets = io.get();
         p.y = ox.out.d, p.y_type = type, p.y_ld = dx_ld, p.zero_rest = (flags & VQB_ZERO_REST) != 0;
-        Scratch codes(dev, 2 * n * p.rows_ld + n * sizeof(float));
-        float *scales = reinterpret_cast<float *>(codes.d + 2 * n * p.rows_ld);
+        Scratch codes(dev, p.digits * n * p.rows_ld + n * sizeof(float));
+        float *scales = reinterpret_cast<float *>(codes.d + p.digits * n * p.rows_ld);
         launch_digit_rows(dev, iy.d, type, n, dim, ld, m.scales, m.groups, p.offsets, reinterpret_cast<int8_t *>(codes.d), p.rows_ld, scales);
         p.rows = reinterpret_cast<const int8_t *>(codes.d), p.row_scales = scales, p.rows_follow = true;
         launch_product(dev, p);

@@ -162,9 +162,9 @@ template <typename T, int EIGHTS, int PAIRS> __global__ void __launch_bounds__(T
         };
 #pragma unroll 2
         for (int i = l; i < pieces; i += step) { // (zeros behind the width)
-            Packed<N> c = {}, unused;
-            if (!none && i < last) it.pack(i == l ? held : load_values<T, 1, true>(row, i, 0, P.rows.width), i, inverse, c, unused);
-            put(t, i, c);
+            Packed<N> c[1] = {};
+            if (!none && i < last) it.pack(i == l ? held : load_values<T, 1, true>(row, i, 0, P.rows.width), i, inverse, c);
+            put(t, i, c[0]);
         }
         for (int i = threadIdx.x; i < (NT - n) * pieces; i += 32 * WARPS) put(n + i / pieces, i % pieces, Packed<N>{});
     }

@@ -14,8 +14,8 @@ namespace {
 constexpr int TILE = 64, BYTES = 64, PITCH = BYTES / 4 + 1;
 
 struct PlainParams {
-    const int8_t *codes, *rows, *low;
-    size_t ld, rows_ld;
+    const int8_t *codes, *rows;
+    size_t ld, rows_ld, plane; // plane: bytes from digit to digit
     const float *channel_scales, *row_scales, *bias;
     const long long *offsets;
     int groups, channels, width, n;
@@ -57,8 +57,8 @@ template <typename T, int DIGITS> __global__ void __launch_bounds__(256) product
         for (int k0 = 0; k0 < P.width; k0 += BYTES) {
             __syncthreads();
             stage(P.codes + ((size_t)g * P.channels + j0) * P.ld, P.ld, channels, k0, P.width, cs);
-            stage(P.rows + (size_t)r0 * P.rows_ld, P.rows_ld, rows, k0, P.width, rs[0]);
-            if (DIGITS == 2) stage(P.low + (size_t)r0 * P.rows_ld, P.rows_ld, rows, k0, P.width, rs[DIGITS - 1]);
+#pragma unroll
+            for (int d = 0; d < DIGITS; ++d) stage(P.rows + d * P.plane + (size_t)r0 * P.rows_ld, P.rows_ld, rows, k0, P.width, rs[d]);
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < BYTES / 4; ++k)
@@ -76,7 +76,7 @@ template <typename T, int DIGITS> __global__ void __launch_bounds__(256) product
                 const int r = ty + 16 * a, j = tx + 16 * b;
                 if (r >= rows || j >= channels) continue;
                 const size_t channel = (size_t)g * P.channels + j0 + j;
-                const float s = DIGITS == 2 ? __fmaf_rn(128.0f, (float)sum[0][a][b], (float)sum[DIGITS - 1][a][b]) : (float)sum[0][a][b];
+                const float s = DIGITS == 3 ? join_digits(sum[0][a][b], sum[DIGITS / 2][a][b], sum[DIGITS - 1][a][b]) : (float)sum[0][a][b];
                 y[(size_t)(r0 + r) * P.y_ld + j0 + j] = from_float<T>(finish_sum(s, P.row_scales[r0 + r], P.channel_scales ? P.channel_scales[channel] : 1.0f, P.bias ? P.bias[channel] : 0.0f));
             }
     }
@@ -87,7 +87,7 @@ template <typename T> void product_plain_typed(CudaDevice &dev, const PlainParam
     const size_t tiles = ((size_t)P.n / TILE + P.groups) * ((P.channels + TILE - 1) / TILE);
     const dim3 grid((unsigned)std::min<size_t>(tiles, (size_t)dev.sm_count() * 8));
     const size_t smem = RowTiles::bytes(P.groups);
-    if (digits == 2) product_plain_kernel<T, 2><<<grid, 256, smem, dev.stream()>>>(P);
+    if (digits == 3) product_plain_kernel<T, 3><<<grid, 256, smem, dev.stream()>>>(P);
     else product_plain_kernel<T, 1><<<grid, 256, smem, dev.stream()>>>(P);
     VQB_CUDA_CHECK(cudaGetLastError());
 }
@@ -96,7 +96,7 @@ template <typename T> void product_plain_typed(CudaDevice &dev, const PlainParam
 
 void launch_product_plain(CudaDevice &dev, const Product &p)
 {
-    PlainParams P{p.codes, p.rows, p.rows + p.n * p.rows_ld, codes_ld(p.width), p.rows_ld, p.channel_scales, p.row_scales, p.bias, reinterpret_cast<const long long *>(p.offsets),
+    PlainParams P{p.codes, p.rows, codes_ld(p.width), p.rows_ld, p.n * p.rows_ld, p.channel_scales, p.row_scales, p.bias, reinterpret_cast<const long long *>(p.offsets),
                   (int)p.groups, (int)p.channels, (int)p.width, (int)p.n, p.y, p.y_ld, p.zero_rest};
     KernelScope ks(dev, "product_plain");
     if (p.y_type == VALUE_F32) product_plain_typed<float>(dev, P, p.digits);

@@ -15,8 +15,9 @@
 // their shared memory (the ring is free by then), and every pair finishes some of the rows, adding up what the others have there: whole
 // numbers, so that nothing depends on their order, and no memory outside the SMs that would have to be zero.
 //
-// Two digits (gradients): the first CTA fetches the rows' high digits and the second one their low digits, so that the columns' first
-// half are the high sums and the second half the low ones; the epilogue joins them.
+// Three digits (gradients): the first CTA fetches the rows' first digits and the second one their middle digits, each half of the last ones; two instructions a step, the
+// first one's columns' halves are the first and the middle sums, the second one's the last sums.  A tile of 128 rows has 384 columns, for which there is room once: its sums
+// are joined in registers, and the next tile's begin, before they leave.  (Tiles of 64 rows, two at a time, read 1.9 GB of L2 for 4096 x 4096 x 4096 and take 170 us for that, not 81.)
 #include <algorithm>
 #include <map>
 #include <mutex>
@@ -33,13 +34,14 @@ namespace {
 constexpr int BM = 128;        // channels a CTA and tile
 constexpr int MOST_COLS = 256; // accumulator columns a tile
 constexpr int KB = 128;        // bytes of K a stage: one swizzled row
-constexpr int NST = 6;
+constexpr int MOST_STAGES = 6;
 constexpr int EPILOGUE_WARPS = 8, THREADS = 64 + 32 * EPILOGUE_WARPS;
 constexpr int STAGE_WORDS = 36; // 32 channels' words and 16 bytes, so that rows start in different banks
-constexpr uint32_t A_BYTES = BM * KB, B_BYTES = MOST_COLS / 2 * KB;
+constexpr uint32_t A_BYTES = BM * KB, B_BYTES = MOST_COLS / 2 * KB; // with three digits another half of B_BYTES follows
+template <int DIGITS> constexpr uint32_t STAGE_BYTES = A_BYTES + (DIGITS == 3 ? B_BYTES * 3 / 2 : B_BYTES);
 
 struct alignas(8) Barriers {
-    unsigned long long full[NST], empty[NST], tfull[2], tempty[2], drained; // full, tempty, drained: the first CTA's count for both
+    unsigned long long full[MOST_STAGES], empty[MOST_STAGES], tfull[2], tempty[2], drained; // full, tempty, drained: the first CTA's count for both
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -50,8 +52,8 @@ struct TcParams {
     const float *channel_scales, *row_scales, *bias;
     void *y;
     size_t y_ld;
-    int tile_rows; // rows a tile, a multiple of 32; times DIGITS at most 256
-    int box_rows;  // rows a token load brings: tile_rows x DIGITS / 2
+    int tile_rows; // rows a tile, a multiple of 32, at most 256; 128 with three digits
+    int stages;    // 6; with three digits 5, or 4 beside many groups' offsets
     int band;      // tiles of rows that are taken together for one tile of channels
     int zero_rest, rows_follow;
     int parts; // of the width, a pair each
@@ -100,6 +102,13 @@ __device__ __forceinline__ void tma_load_counted(void *dst, const CUtensorMap *m
                  "r"(bar), "r"(c0), "r"(c1)
                  : "memory");
 }
+// The same of a map with planes.
+__device__ __forceinline__ void tma_load_plane_counted(void *dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)), "l"(map),
+                 "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
 // Without release ordering: what is handed back has been read, and a release would wait for the results' stores (1 us a tile).
 __device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void cluster_sync()
@@ -140,16 +149,19 @@ __device__ __forceinline__ Tile tile_at(const TcParams &P, const RowTiles &tiles
     return t;
 }
 
-// Accumulator columns of one digit: rows in steps of 32 (16 for each CTA to fetch; with two digits each fetches them all).
+// Accumulator columns of one digit: rows in steps of 32 (16 for each box).
 __device__ __forceinline__ int columns_of(int rows) { return (rows + 31) / 32 * 32; }
 
 template <typename T, int DIGITS, bool SPLIT>
-__global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rows, const TcParams P)
+__global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rows,
+                                                                const __grid_constant__ CUtensorMap map_half, const TcParams P)
 {
     extern __shared__ unsigned char smem_raw[];
     unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *a_smem = base, *b_smem = base + NST * A_BYTES;
-    float *scales_smem = reinterpret_cast<float *>(b_smem + NST * B_BYTES);                                 // 8 warps x 128
+    const int nst = DIGITS == 3 ? P.stages : MOST_STAGES;
+    constexpr uint32_t B_STAGE = STAGE_BYTES<DIGITS> - A_BYTES;
+    unsigned char *a_smem = base, *b_smem = base + nst * A_BYTES;
+    float *scales_smem = reinterpret_cast<float *>(b_smem + nst * B_STAGE);                                 // 8 warps x 128
     uint32_t *out_smem = reinterpret_cast<uint32_t *>(scales_smem + EPILOGUE_WARPS * MOST_COLS / 2);        // 8 warps x 16 x STAGE_WORDS
     Barriers *bars = reinterpret_cast<Barriers *>(out_smem + EPILOGUE_WARPS * 16 * STAGE_WORDS);
     RowTiles tiles(bars + 1, P.groups);
@@ -159,7 +171,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     const uint32_t leader = rank & ~1;                                                                          // the first one of its pair
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < NST; ++s) {
+        for (int s = 0; s < nst; ++s) {
             mbar_init(&bars->full[s], 1);
             mbar_init(&bars->empty[s], 1);
         }
@@ -184,6 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     cluster_sync();                                     // both CTAs' barriers are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = bars->tmem_base;
+    const int twice = DIGITS == 1 || 3 * P.tile_rows <= MOST_COLS; // room for two tiles' sums
     const int channel_tiles = (P.channels + 2 * BM - 1) / (2 * BM), chunks = (P.width + KB - 1) / KB;
     const int c_begin = chunks * part / parts, c_end = chunks * (part + 1) / parts;
     const int total = tiles.before[P.groups] * channel_tiles, first = blockIdx.x / (2 * parts), step = gridDim.x / (2 * parts);
@@ -193,14 +206,24 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             int st = 0;
             uint32_t parity = 0; // of the stages' current round
             bool ok = true, waited = !codes_first;
-            const uint32_t bytes = 2 * (A_BYTES + (uint32_t)P.box_rows * KB), full0 = in_cta(&bars->full[0], leader);
+            const uint32_t bytes = 2 * (A_BYTES + (uint32_t)(DIGITS == 3 ? 3 : 1) * P.tile_rows / 2 * KB), full0 = in_cta(&bars->full[0], leader);
             unsigned long long loads = 0;
             for (int id = first; ok && id < total; id += step) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
-                // this CTA's rows: one half of the columns, or one digit of all
-                const int row = DIGITS == 2 ? half * P.n + t.row0 : t.row0 + half * (columns_of(t.rows) / 2);
+                // This CTA's rows: one half of the columns, or one digit of all and half of the last one's.  Boxes are those of a whole tile: what is behind the tile's rows is
+                // not multiplied.
+                const int mid = t.row0 + half * (columns_of(t.rows) / 2);
                 const int channel = t.group * P.channels + t.channel0 + half * BM;
-                const int ahead = waited ? 0 : min(NST, c_end - c_begin);
+                auto load_rows = [&](int stage, int c) {
+                    unsigned char *to = b_smem + stage * B_STAGE;
+                    if (DIGITS == 1) {
+                        tma_load_counted(to, &map_rows, c * KB, mid, full0 + 8u * stage);
+                    } else {
+                        tma_load_plane_counted(to, &map_rows, c * KB, t.row0, half, full0 + 8u * stage);
+                        tma_load_plane_counted(to + B_BYTES, &map_half, c * KB, mid, 2, full0 + 8u * stage);
+                    }
+                };
+                const int ahead = waited ? 0 : min(nst, c_end - c_begin);
                 for (int c = c_begin; c < c_end; ++c) {
                     if (!mbar_wait(&bars->empty[st], parity ^ 1u, abort_flag, P.error, 61)) {
                         ok = false;
@@ -213,19 +236,19 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                         if (!waited) {
                             rows_are_there();
                             waited = true;
-                            for (int e = 0; e < ahead; ++e) tma_load_counted(b_smem + e * B_BYTES, &map_rows, (c_begin + e) * KB, row, full0 + 8u * e);
+                            for (int e = 0; e < ahead; ++e) load_rows(e, c_begin + e);
                         } else {
-                            tma_load_counted(b_smem + st * B_BYTES, &map_rows, c * KB, row, full0 + 8u * st);
+                            load_rows(st, c);
                         }
                     }
-                    if (++st == NST) st = 0, parity ^= 1u;
+                    if (++st == nst) st = 0, parity ^= 1u;
                 }
             }
             if (!waited) rows_are_there();
             if (ok) { // the tensor core's arrivals here have come before the block leaves
-                for (int i = 0; i < NST; ++i) {
-                    if (loads + i >= NST) mbar_wait(&bars->empty[st], parity ^ 1u, abort_flag, P.error, 62);
-                    if (++st == NST) st = 0, parity ^= 1u;
+                for (int i = 0; i < nst; ++i) {
+                    if (loads + i >= nst) mbar_wait(&bars->empty[st], parity ^ 1u, abort_flag, P.error, 62);
+                    if (++st == nst) st = 0, parity ^= 1u;
                 }
             } else { // what has been asked for lands
                 for (int i = 0; i < 1000; ++i) __nanosleep(1000);
@@ -242,8 +265,10 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
             const uint64_t a0 = smem_desc_sw128(smem_u32(a_smem)), r0 = smem_desc_sw128(smem_u32(b_smem));
             for (int id = first; ok && id < total; id += step, ++local) {
                 const Tile t = tile_at(P, tiles, id, channel_tiles);
-                const uint32_t b = local & 1u, idesc = idesc_i8(DIGITS * columns_of(t.rows)), d_tmem = tmem_base + b * MOST_COLS;
-                if (!mbar_wait(&bars->tempty[b], ((local >> 1) & 1u) ^ 1u, abort_flag, P.error, 63)) break;
+                const int columns = columns_of(t.rows);
+                const uint32_t b = twice ? local & 1u : 0u, idesc = idesc_i8(DIGITS == 3 ? 2 * columns : columns), d_tmem = tmem_base + b * MOST_COLS;
+                const uint32_t idesc_last = idesc_i8(columns), last_tmem = d_tmem + 2 * columns; // (three digits)
+                if (!mbar_wait(&bars->tempty[b], ((twice ? local >> 1 : local) & 1u) ^ 1u, abort_flag, P.error, 63)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int c = c_begin; c < c_end; ++c) {
                     if (!mbar_wait(&bars->full[st], parity, abort_flag, P.error, 64)) {
@@ -251,15 +276,19 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t a = a0 + (uint32_t)(st * (int)(A_BYTES >> 4)), r = r0 + (uint32_t)(st * (int)(B_BYTES >> 4));
+                    const uint64_t a = a0 + (uint32_t)(st * (int)(A_BYTES >> 4)), r = r0 + (uint32_t)(st * (int)(B_STAGE >> 4));
                     // Always four: behind the width there are zeros.  (Rolled up, with a count, one such instruction took 54 ns to issue, as long
                     // as the tensor core needs for 200 columns; a stage 0.42 instead of 0.27 us.)
                     umma_i8(d_tmem, a, r, idesc, (uint32_t)(c - c_begin));
+                    if (DIGITS == 3) umma_i8(last_tmem, a, r + (B_BYTES >> 4), idesc_last, (uint32_t)(c - c_begin));
                     umma_i8(d_tmem, a + 2, r + 2, idesc, 1u);
+                    if (DIGITS == 3) umma_i8(last_tmem, a + 2, r + (B_BYTES >> 4) + 2, idesc_last, 1u);
                     umma_i8(d_tmem, a + 4, r + 4, idesc, 1u);
+                    if (DIGITS == 3) umma_i8(last_tmem, a + 4, r + (B_BYTES >> 4) + 4, idesc_last, 1u);
                     umma_i8(d_tmem, a + 6, r + 6, idesc, 1u);
+                    if (DIGITS == 3) umma_i8(last_tmem, a + 6, r + (B_BYTES >> 4) + 6, idesc_last, 1u);
                     commit_both(&bars->empty[st], leader);
-                    if (++st == NST) st = 0, parity ^= 1u;
+                    if (++st == nst) st = 0, parity ^= 1u;
                 }
                 if (ok) commit_both(&bars->tfull[b], leader);
             }
@@ -275,15 +304,16 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         uint32_t *stage = out_smem + (warp - 2) * 16 * STAGE_WORDS;
         T *y = static_cast<T *>(P.y);
         // what the next tile's results are multiplied by, on its way while this one's leave
+        constexpr int TURNS = DIGITS == 3 ? 2 : MOST_COLS / 64;
         struct Scales {
             Tile t;
-            float rows[MOST_COLS / 64], channel, bias; // of this lane's rows (one in each of the warp's turns) and channel
+            float rows[TURNS], channel, bias; // of this lane's rows (one in each of the warp's turns) and channel
         };
         auto scales_of = [&](int id) {
             Scales n;
             n.t = tile_at(P, tiles, id, channel_tiles);
 #pragma unroll
-            for (int i = 0; i < MOST_COLS / 64; ++i) {
+            for (int i = 0; i < TURNS; ++i) {
                 const int r = 64 * i + 32 * turn + lane;
                 n.rows[i] = r < n.t.rows ? P.row_scales[n.t.row0 + r] : 0.0f;
             }
@@ -298,47 +328,37 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
         if (first < total) next = scales_of(first);
         for (int id = first; id < total; id += step, ++local) {
             const Tile t = next.t;
-            const uint32_t b = local & 1u;
+            const uint32_t b = twice ? local & 1u : 0u;
             const int channel0 = t.channel0 + half * BM + 32 * q, channel = channel0 + lane, columns = columns_of(t.rows);
             const bool there = channel < P.channels;
             const float channel_scale = next.channel, bias = next.bias;
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < MOST_COLS / 64; ++i) mine[32 * i + lane] = next.rows[i];
+            for (int i = 0; i < TURNS; ++i) mine[32 * i + lane] = next.rows[i];
             __syncwarp();
             if (id + step < total) next = scales_of(id + step);
-            if (!__all_sync(~0u, mbar_wait(&bars->tfull[b], (local >> 1) & 1u, abort_flag, P.error, 66))) break;
+            if (!__all_sync(~0u, mbar_wait(&bars->tfull[b], (twice ? local >> 1 : local) & 1u, abort_flag, P.error, 66))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(32 * q) << 16) + b * MOST_COLS;
-            for (int c0 = 32 * turn; c0 < columns; c0 += 64) {
-                if (SPLIT) { // this part's sums to the ring, a channel's next to each other
-                    uint32_t *dump = reinterpret_cast<uint32_t *>(base);
+            if (SPLIT) { // this part's sums to the ring, a channel's next to each other
+                uint32_t *dump = reinterpret_cast<uint32_t *>(base);
+                for (int c0 = 32 * turn; c0 < DIGITS * columns; c0 += 64) {
+                    uint32_t acc[32];
+                    tmem_ld32_issue(taddr + c0, acc);
+                    tmem_wait();
 #pragma unroll
-                    for (int d = 0; d < DIGITS; ++d) {
-                        uint32_t acc[32];
-                        tmem_ld32_issue(taddr + d * columns + c0, acc);
-                        tmem_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) dump[(d * columns + c0 + i) * BM + 32 * q + lane] = acc[i];
-                    }
-                    continue;
+                    for (int i = 0; i < 32; ++i) dump[(c0 + i) * BM + 32 * q + lane] = acc[i];
                 }
+                continue;
+            }
+            // 32 rows' results, from column c0 on, of their sums
+            auto leave = [&](int c0, auto sum_of) {
                 const float4 *row_scales = reinterpret_cast<const float4 *>(mine + c0 / 2 - 16 * turn);
-                uint32_t acc[32], low[32];
-                tmem_ld32_issue(taddr + c0, acc);
-                if (DIGITS == 2) tmem_ld32_issue(taddr + columns + c0, low);
-                tmem_wait();
-                if (c0 + 64 >= columns) { // the accumulator has been read
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) arrive_at(in_cta(&bars->tempty[b], leader));
-                }
                 const int left = t.rows - c0;
                 auto value = [&](int i) {
                     const float4 s4 = row_scales[i >> 2];
                     const float row_scale = (i & 3) == 0 ? s4.x : (i & 3) == 1 ? s4.y : (i & 3) == 2 ? s4.z : s4.w;
-                    const float sum = DIGITS == 2 ? __fmaf_rn(128.0f, (float)(int)acc[i], (float)(int)low[i]) : (float)(int)acc[i];
-                    return finish_sum(sum, row_scale, channel_scale, bias);
+                    return finish_sum(sum_of(i), row_scale, channel_scale, bias);
                 };
                 if (sizeof(T) == 2 && P.wide) {
 #pragma unroll
@@ -371,8 +391,43 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                     for (int i = 0; i < 32; ++i)
                         if (there && i < left) to[(size_t)i * P.y_ld] = from_float<T>(value(i));
                 }
+            };
+            auto has_been_read = [&] {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive_at(in_cta(&bars->tempty[b], leader));
+            };
+            if (DIGITS == 3) {
+                float held[2][32]; // both of the warp's turns, so that the accumulator is free before either leaves
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int c0 = 32 * turn + 64 * k;
+                    if (c0 >= columns) break;
+                    uint32_t acc[32], last[32];
+                    tmem_ld32_issue(taddr + columns + c0, acc);
+                    tmem_ld32_issue(taddr + 2 * columns + c0, last);
+                    tmem_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) held[k][i] = __fmaf_rn(256.0f, (float)(int)acc[i], (float)(int)last[i]); // (join_digits, in two steps)
+                    tmem_ld32_issue(taddr + c0, acc);
+                    tmem_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) held[k][i] = __fmaf_rn(65536.0f, (float)(int)acc[i], held[k][i]);
+                }
+                has_been_read();
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (32 * turn + 64 * k < columns) leave(32 * turn + 64 * k, [&](int i) { return held[k][i]; });
+            } else {
+                if (32 * turn >= columns) has_been_read(); // (nothing of it is this warp's)
+                for (int c0 = 32 * turn; c0 < columns; c0 += 64) {
+                    uint32_t acc[32];
+                    tmem_ld32_issue(taddr + c0, acc);
+                    tmem_wait();
+                    if (c0 + 64 >= columns) has_been_read();
+                    leave(c0, [&](int i) { return (float)(int)acc[i]; });
+                }
             }
-            if (32 * turn >= columns && lane == 0) arrive_at(in_cta(&bars->tempty[b], leader)); // (nothing of it was this warp's)
         }
         if (P.zero_rest)
             zero_rest<T>(y, P.y_ld, P.channels, P.n, tiles.first[0], tiles.end(P.groups - 1), (size_t)blockIdx.x * (THREADS - 64) + (threadIdx.x - 64),
@@ -408,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
                 alignas(16) T out[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float whole = (float)(&sums[0].x)[k], sum = DIGITS == 2 ? __fmaf_rn(128.0f, whole, (float)(&sums[DIGITS - 1].x)[k]) : whole;
+                    const float sum = DIGITS == 3 ? join_digits((&sums[0].x)[k], (&sums[DIGITS / 2].x)[k], (&sums[DIGITS - 1].x)[k]) : (float)(&sums[0].x)[k];
                     out[k] = from_float<T>(finish_sum(sum, row_scale, channel_scale[k], bias[k]));
                 }
                 T *to = y + (size_t)r * P.y_ld;
@@ -432,24 +487,22 @@ __global__ void __launch_bounds__(THREADS, 1) product_tc_kernel(const __grid_con
     }
 }
 
-size_t smem_bytes(size_t groups) { return 1024 + NST * (A_BYTES + B_BYTES) + EPILOGUE_WARPS * (MOST_COLS / 2 + 16 * STAGE_WORDS) * 4 + sizeof(Barriers) + RowTiles::bytes(groups); }
+static_assert(3 * MOST_COLS / 2 * BM * sizeof(int) <= 5 * STAGE_BYTES<3>, "three digits' sums, where the width is parted, lie in the ring");
+size_t smem_bytes(size_t groups, size_t ring) { return 1024 + ring + EPILOGUE_WARPS * (MOST_COLS / 2 + 16 * STAGE_WORDS) * 4 + sizeof(Barriers) + RowTiles::bytes(groups); }
 
-template <typename T, int DIGITS> void product_tc_typed(CudaDevice &dev, const Product &p, const TcParams &P, const CUtensorMap &map_codes, const CUtensorMap &map_rows, unsigned clusters)
+template <typename T, int DIGITS>
+void product_tc_typed(CudaDevice &dev, const Product &p, const TcParams &P, const CUtensorMap &map_codes, const CUtensorMap &map_rows, const CUtensorMap &map_half, unsigned clusters)
 {
+    const size_t smem = smem_bytes(p.groups, P.stages * STAGE_BYTES<DIGITS>);
     if (P.parts == 1) {
         allow_shared_memory(dev, product_tc_kernel<T, DIGITS, false>);
-        launch_following_clusters(product_tc_kernel<T, DIGITS, false>, dim3(2 * clusters), dim3(THREADS), smem_bytes(p.groups), 2, dev.stream(), map_codes, map_rows, P);
+        launch_following_clusters(product_tc_kernel<T, DIGITS, false>, dim3(2 * clusters), dim3(THREADS), smem, 2, dev.stream(), map_codes, map_rows, map_half,
+                                  P);
     } else {
         allow_shared_memory(dev, product_tc_kernel<T, DIGITS, true>);
-        launch_following_clusters(product_tc_kernel<T, DIGITS, true>, dim3(2 * P.parts * clusters), dim3(THREADS), smem_bytes(p.groups), 2 * P.parts, dev.stream(), map_codes,
-                                  map_rows, P);
+        launch_following_clusters(product_tc_kernel<T, DIGITS, true>, dim3(2 * P.parts * clusters), dim3(THREADS), smem, 2 * P.parts, dev.stream(), map_codes,
+                                  map_rows, map_half, P);
     }
-}
-
-template <typename T> void product_tc_digits(CudaDevice &dev, const Product &p, const TcParams &P, const CUtensorMap &mc, const CUtensorMap &mr, unsigned clusters)
-{
-    if (p.digits == 2) product_tc_typed<T, 2>(dev, p, P, mc, mr, clusters);
-    else product_tc_typed<T, 1>(dev, p, P, mc, mr, clusters);
 }
 
 // How many clusters of so many CTAs there is room for at a time (a cluster stays within a part of the GPU whose SMs need not be a multiple of it).
@@ -463,7 +516,7 @@ size_t room_for_clusters(CudaDevice &dev, int ctas)
         auto kernel = product_tc_kernel<float, 1, true>;
         allow_shared_memory(dev, kernel);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem_bytes(1);
+        cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem_bytes(1, MOST_STAGES * STAGE_BYTES<1>);
         cudaLaunchAttribute attr = {};
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
@@ -498,7 +551,8 @@ void launch_product(CudaDevice &dev, const Product &p)
     const size_t chunks = (p.width + KB - 1) / KB;
     size_t least = ~size_t(0);
     P.parts = 1;
-    for (size_t rows = 32; rows * p.digits <= MOST_COLS; rows += 32) {
+    const size_t most_rows = p.digits == 3 ? MOST_COLS / 2 : MOST_COLS;
+    for (size_t rows = 32; rows <= most_rows; rows += 32) {
         const size_t columns = rows * p.digits, a_stage = std::max(columns, 160 + columns / 8), tiles = p.groups * ((a_group + rows - 1) / rows) * channel_tiles;
         const size_t stages = chunks * a_stage + 400, leaves = 10 * rows;
         const size_t cost = (tiles + pairs - 1) / pairs * std::max(stages, leaves) + leaves;
@@ -508,17 +562,24 @@ void launch_product(CudaDevice &dev, const Product &p)
             if (split < least && tiles <= room_for_clusters(dev, (int)(2 * parts))) P.tile_rows = (int)rows, P.parts = (int)parts, least = split;
         }
     }
-    P.box_rows = P.tile_rows * p.digits / 2;
     P.wide = (reinterpret_cast<uintptr_t>(p.y) | (p.y_ld * 2)) % 16 == 0;
     P.band = 8;
     const CUtensorMap map_codes = make_tensor_map_2d<int8_t>(p.codes, p.width, p.groups * p.channels, KB, BM, CU_TENSOR_MAP_SWIZZLE_128B, codes_ld(p.width));
-    const CUtensorMap map_rows = make_tensor_map_2d<int8_t>(p.rows, p.width, p.digits * p.n, KB, (unsigned)P.box_rows, CU_TENSOR_MAP_SWIZZLE_128B, p.rows_ld);
+    // a box: half a tile of one digit's rows; with three digits a whole one of each CTA's and half of the last one's
+    auto rows_map = [&](int rows) {
+        return make_tensor_map<int8_t>(p.rows, p.width, p.n, KB, (unsigned)rows, CU_TENSOR_MAP_SWIZZLE_128B, p.rows_ld, (unsigned)p.digits, p.n * p.rows_ld);
+    };
+    const CUtensorMap map_half = rows_map(P.tile_rows / 2), map_rows = p.digits == 3 ? rows_map(P.tile_rows) : map_half;
+    P.stages = p.digits == 1 ? MOST_STAGES : smem_bytes(p.groups, 5 * STAGE_BYTES<3>) <= dev.smem_limit() ? 5 : 4;
     const size_t row_tiles = p.offsets ? p.n / P.tile_rows + p.groups : (p.n + P.tile_rows - 1) / P.tile_rows;
     const unsigned clusters = (unsigned)(P.parts > 1 ? row_tiles * channel_tiles : std::min<size_t>(pairs, row_tiles * channel_tiles));
     KernelScope ks(dev, "product_tc");
-    if (p.y_type == VALUE_F32) product_tc_digits<float>(dev, p, P, map_codes, map_rows, clusters);
-    else if (p.y_type == VALUE_F16) product_tc_digits<__half>(dev, p, P, map_codes, map_rows, clusters);
-    else product_tc_digits<__nv_bfloat16>(dev, p, P, map_codes, map_rows, clusters);
+    if (p.digits == 3) { // (gradients are 16-bit)
+        if (p.y_type == VALUE_F16) product_tc_typed<__half, 3>(dev, p, P, map_codes, map_rows, map_half, clusters);
+        else product_tc_typed<__nv_bfloat16, 3>(dev, p, P, map_codes, map_rows, map_half, clusters);
+    } else if (p.y_type == VALUE_F32) product_tc_typed<float, 1>(dev, p, P, map_codes, map_rows, map_half, clusters);
+    else if (p.y_type == VALUE_F16) product_tc_typed<__half, 1>(dev, p, P, map_codes, map_rows, map_half, clusters);
+    else product_tc_typed<__nv_bfloat16, 1>(dev, p, P, map_codes, map_rows, map_half, clusters);
     dev.count_launch();
 }
 

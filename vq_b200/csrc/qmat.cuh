@@ -27,6 +27,9 @@ __device__ __forceinline__ float finish_sum(float sum, float row_scale, float ch
     return __fmaf_rn(__fmul_rn(sum, row_scale), channel_scale, bias);
 }
 
+// What the sums of three digits stand for.
+__device__ __forceinline__ float join_digits(int first, int middle, int last) { return __fmaf_rn(65536.0f, (float)first, __fmaf_rn(256.0f, (float)middle, (float)last)); }
+
 // How the rows of all groups fall into tiles of at most `rows` rows: tile u belongs to the last group g with before[g] <= u, and starts at row
 // first[g] + (u - before[g]) * rows.  In shared memory.  Offsets come from the device unchecked: whatever they are, every group has some of the n
 // rows that there are, and no row has two groups.

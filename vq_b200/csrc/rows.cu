@@ -47,13 +47,13 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>, DIGITS == 1 && LANES == 256
         if (full) held[h].w = *reinterpret_cast<const uint4 *>(row + column<N, LANES, true>(h, lane, 0));
         else held[h] = load_values<T, LANES, ALIGNED>(row, h, lane, P.width);
     }
-    const float *columns = DIGITS == 2 ? columns_of(P, r) : nullptr; // (its loads beside the row's)
-    if (DIGITS == 2 && !columns) return;
+    const float *columns = DIGITS == 3 ? columns_of(P, r) : nullptr; // (its loads beside the row's)
+    if (DIGITS == 3 && !columns) return;
     RowOf<T, DIGITS, LANES, ALIGNED> it(P, r, lane, columns);
-    float u[DIGITS == 2 ? HELD : 1][N]; // two digits: what the columns' scales make of the row is kept instead
+    float u[DIGITS == 3 ? HELD : 1][N]; // three digits: what the columns' scales make of the row is kept instead
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
-        if (DIGITS == 2) it.values(held[h], h, u[DIGITS == 2 ? h : 0]), it.look(u[DIGITS == 2 ? h : 0]);
+        if (DIGITS == 3) it.values(held[h], h, u[DIGITS == 3 ? h : 0]), it.look(u[DIGITS == 3 ? h : 0]);
         else it.look(held[h], h);
     }
     for (uint32_t h = HELD; h < pieces; ++h) it.look(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h);
@@ -68,17 +68,17 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>, DIGITS == 1 && LANES == 256
     const bool none = it.no_codes(most);
     if (lane == 0) P.scales[r] = scale;
     const Inverse inverse(none ? 1.0f : scale);
-    Packed<N> high[HELD] = {}, low[DIGITS == 2 ? HELD : 1] = {};
+    Packed<N> packed[HELD][DIGITS] = {};
     if (!none) {
         uint64_t unlike[HELD] = {};
         bool some = false;
 #pragma unroll
         for (int h = 0; h < HELD; ++h) {
-            if (DIGITS == 2) {
-                pack_digits<N>(u[DIGITS == 2 ? h : 0], inverse, high[h], low[DIGITS == 2 ? h : 0]);
+            if constexpr (DIGITS == 3) {
+                pack_digits<N>(u[h], inverse, packed[h]);
             } else {
                 it.values(held[h], h, u[0]);
-                high[h] = pack_most<N>(u[0], inverse, unlike[h]);
+                packed[h][0] = pack_most<N>(u[0], inverse, unlike[h]);
                 some |= any_unlike(unlike[h]);
             }
         }
@@ -87,14 +87,14 @@ __global__ void __launch_bounds__(THREADS_OF<LANES>, DIGITS == 1 && LANES == 256
             for (int h = 0; h < HELD; ++h) {
                 if (!any_unlike(unlike[h])) continue;
                 it.values(held[h], h, u[0]);
-                high[h] = pack_all<N>(u[0], inverse);
+                packed[h][0] = pack_all<N>(u[0], inverse);
             }
         }
     }
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
-        if (full) it.put(h, high[h], low[DIGITS == 2 ? h : 0]);
-        else if (column<N, LANES, ALIGNED>(h, lane, 0) < P.width) it.store(h, high[h], low[DIGITS == 2 ? h : 0]);
+        if (full) it.put(h, packed[h]);
+        else if (column<N, LANES, ALIGNED>(h, lane, 0) < P.width) it.store(h, packed[h]);
     }
     for (uint32_t h = HELD; h < pieces; ++h) it.write(load_values<T, LANES, ALIGNED>(row, h, lane, P.width), h, none, inverse);
 }
@@ -112,7 +112,7 @@ template <typename T, int DIGITS, int LANES, int HELD> void quantize_rows_with(C
 template <typename T, int DIGITS> void quantize_rows_typed(CudaDevice &dev, const RowParams &P)
 {
     const size_t apart = P.n == 1 ? 0 : P.ld * sizeof(T), codes_apart = P.n == 1 ? 0 : P.ld_codes; // (one row has no next one)
-    const bool aligned = (reinterpret_cast<uintptr_t>(P.x) | apart) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.codes) | codes_apart | reinterpret_cast<uintptr_t>(P.low)) % 8 == 0;
+    const bool aligned = (reinterpret_cast<uintptr_t>(P.x) | apart) % 16 == 0 && (reinterpret_cast<uintptr_t>(P.codes) | codes_apart | P.plane) % 8 == 0;
     const size_t pieces = (P.width + Piece<T>::N - 1) / Piece<T>::N;
     if (pieces <= 64) quantize_rows_with<T, DIGITS, 32, 2>(dev, P, aligned);
     else if (pieces <= 128) quantize_rows_with<T, DIGITS, 32, 4>(dev, P, aligned);
@@ -128,7 +128,7 @@ template <int DIGITS> void quantize_rows_any(CudaDevice &dev, const char *name, 
     KernelScope ks(dev, name);
     if (type == VALUE_F16) quantize_rows_typed<__half, DIGITS>(dev, P);
     else if (type == VALUE_BF16) quantize_rows_typed<__nv_bfloat16, DIGITS>(dev, P);
-    else if (DIGITS == 1) quantize_rows_typed<float, 1>(dev, P); // (two digits are 16-bit rows')
+    else if (DIGITS == 1) quantize_rows_typed<float, 1>(dev, P); // (three digits are 16-bit rows')
     dev.count_launch();
 }
 
@@ -164,15 +164,15 @@ __global__ void align_codes_kernel(const int8_t *codes, size_t n, size_t width, 
 void launch_quantize_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, int8_t *codes, size_t ld_codes, float *scales,
                           bool product_follows)
 {
-    RowParams P{x, n, ld, (uint32_t)width, codes, nullptr, ld_codes, scales, nullptr, nullptr, 0, product_follows};
+    RowParams P{x, n, ld, (uint32_t)width, codes, ld_codes, 0, scales, nullptr, nullptr, 0, product_follows};
     quantize_rows_any<1>(dev, "quantize_rows", P, type);
 }
 
 void launch_digit_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, const float *column_scales, size_t groups, const int64_t *offsets,
                        int8_t *digits, size_t ld_codes, float *scales)
 {
-    RowParams P{x, n, ld, (uint32_t)width, digits, digits + n * ld_codes, ld_codes, scales, column_scales, reinterpret_cast<const long long *>(offsets), (int)groups, true};
-    quantize_rows_any<2>(dev, "digit_rows", P, type);
+    RowParams P{x, n, ld, (uint32_t)width, digits, ld_codes, n * ld_codes, scales, column_scales, reinterpret_cast<const long long *>(offsets), (int)groups, true};
+    quantize_rows_any<3>(dev, "digit_rows", P, type);
 }
 
 void launch_turn_codes(CudaDevice &dev, const int8_t *codes, size_t groups, size_t rows, size_t width, int8_t *turned)

@@ -11,7 +11,7 @@
 namespace vqb {
 
 constexpr float MAGIC = 12582912.0f; // 1.5 2^23: adding it rounds to a whole number, whose two's complement is then in the low bits
-constexpr float LARGEST_8 = 127.0f, LARGEST_15 = 16256.0f; // 16256 = 127 * 128: the high digit stays within 127
+constexpr float LARGEST_8 = 127.0f, LARGEST_24 = 8323072.0f; // 127 * 65536: the first of three digits stays within 127 (127.5 would)
 
 template <typename T> struct Piece; // 16 bytes of a row
 template <> struct Piece<float> {
@@ -97,12 +97,12 @@ template <int N> struct Packed {
 
 // What a row's values are multiplied by: the f32 numbers on both sides of 1 / scale.
 struct Inverse {
-    float scale;
+    float scale, nearest;
     uint64_t up, down;
     __device__ __forceinline__ explicit Inverse(float s) : scale(s)
     {
-        const uint32_t nearest = __float_as_uint(__frcp_rn(s));
-        const float u = __uint_as_float(nearest + 1), d = __uint_as_float(nearest - 1);
+        nearest = __frcp_rn(s);
+        const float u = __uint_as_float(__float_as_uint(nearest) + 1), d = __uint_as_float(__float_as_uint(nearest) - 1);
         up = pair_of(u, u), down = pair_of(d, d);
     }
 };
@@ -168,22 +168,19 @@ template <int N> __device__ __forceinline__ Packed<N> pack_codes(const float (&v
     return __builtin_expect(any_unlike(unlike), 0) ? pack_all<N>(v, inverse) : out;
 }
 
-// The two digits of v = u / t, |v| <= 16256: the high one is the whole number nearest to v / 128.  With w = v + 64 in 16 bits they are w >> 7 and
-// (w & 127) - 64; two such words are taken at a time.
-template <int N> __device__ __forceinline__ void pack_digits(const float (&u)[N], const Inverse &inverse, Packed<N> &high, Packed<N> &low)
+// The three digits of the whole number v next to u / t, |v| <= 127 * 65536: v = 65536 d0 + 256 d1 + d2, each in -128 .. 127.  They are the bytes of
+// v + 0x808080, which is positive and below 2^24, less 128 each.  (v is off by at most half a step, and 2^-24 of v for the reciprocal and 2^-25 for the product.)
+template <int N> __device__ __forceinline__ void pack_digits(const float (&u)[N], const Inverse &inverse, Packed<N> (&digits)[3])
 {
-    const uint64_t magic = pair_of(MAGIC + 64.0f, MAGIC + 64.0f);
-    uint32_t w[N / 2];
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        float a, b;
-        halves_of(fma_pair(pair_of(u[i], u[i + 1]), inverse.up, magic), a, b);
-        w[i / 2] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410);
-    }
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-        high.w[i] = __byte_perm(w[2 * i] >> 7, w[2 * i + 1] >> 7, 0x6420); // (bits 7 .. 14 of each)
-        low.w[i] = __byte_perm((w[2 * i] & 0x007F007Fu) + 0x00C000C0u, (w[2 * i + 1] & 0x007F007Fu) + 0x00C000C0u, 0x6420);
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = (uint32_t)(__float2int_rn(__fmul_rn(u[4 * i + j], inverse.nearest)) + 0x808080);
+        const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140); // the last and the middle digits of two
+        digits[2].w[i] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+        digits[1].w[i] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
+        digits[0].w[i] = __byte_perm(__byte_perm(w[0], w[1], 0x0062), __byte_perm(w[2], w[3], 0x0062), 0x5410) ^ 0x80808080u;
     }
 }
 
@@ -206,10 +203,10 @@ struct RowParams {
     const void *x;
     size_t n, ld;
     uint32_t width;
-    int8_t *codes, *low; // low: the low digits' plane (two digits)
-    size_t ld_codes;
+    int8_t *codes;
+    size_t ld_codes, plane; // plane: bytes from a digit's rows to the next digit's (three digits)
     float *scales;
-    const float *column_scales; // groups x width (two digits)
+    const float *column_scales; // groups x width (three digits)
     const long long *offsets;
     int groups;
     bool product_follows; // the next kernel of the stream is a product of this call
@@ -225,12 +222,12 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
     bool columns4; // N neighbouring columns' scales are 16-byte aligned
     uint32_t most = 0;
 
-    __device__ __forceinline__ RowOf(const RowParams &p, size_t row, int l, const float *c) : P(p), r(row), lane(l), columns(c), columns4(DIGITS == 2 && ALIGNED && p.width % 4 == 0) {}
+    __device__ __forceinline__ RowOf(const RowParams &p, size_t row, int l, const float *c) : P(p), r(row), lane(l), columns(c), columns4(DIGITS == 3 && ALIGNED && p.width % 4 == 0) {}
 
     __device__ __forceinline__ void values(const Piece<T> &p, uint32_t piece, float (&v)[N]) const
     {
         float c[N];
-        if (DIGITS == 2) {
+        if (DIGITS == 3) {
             const uint32_t k = column<N, LANES, ALIGNED>(piece, lane, 0);
             if (columns4 && k + N <= P.width) {
 #pragma unroll
@@ -247,7 +244,7 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
             }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = DIGITS == 2 ? p.at(i) * c[i] : p.at(i);
+        for (int i = 0; i < N; ++i) v[i] = DIGITS == 3 ? p.at(i) * c[i] : p.at(i);
     }
     // the largest magnitude so far (two 16-bit ones at a time); its sign means nothing, NaN wins
     __device__ __forceinline__ void look(const Piece<T> &p, uint32_t piece)
@@ -281,39 +278,35 @@ template <typename T, int DIGITS, int LANES, bool ALIGNED> struct RowOf {
     static __device__ __forceinline__ float scale_of(uint32_t largest)
     {
         if (largest >= 0x7F800000u) return __int_as_float(0x7FC00000);
-        return largest == 0 ? 0.0f : fmaxf(__fdiv_rn(__uint_as_float(largest), DIGITS == 1 ? LARGEST_8 : LARGEST_15), 0x1p-126f);
+        return largest == 0 ? 0.0f : fmaxf(__fdiv_rn(__uint_as_float(largest), DIGITS == 1 ? LARGEST_8 : LARGEST_24), 0x1p-126f);
     }
-    __device__ __forceinline__ void pack(const Piece<T> &p, uint32_t piece, const Inverse &inverse, Packed<N> &high, Packed<N> &low) const
+    __device__ __forceinline__ void pack(const Piece<T> &p, uint32_t piece, const Inverse &inverse, Packed<N> (&digits)[DIGITS]) const
     {
         float v[N];
         values(p, piece, v);
-        pack(v, inverse, high, low);
-    }
-    __device__ __forceinline__ void pack(const float (&v)[N], const Inverse &inverse, Packed<N> &high, Packed<N> &low) const
-    {
-        if (DIGITS == 1) high = pack_codes<N>(v, inverse);
-        else pack_digits<N>(v, inverse, high, low);
+        if constexpr (DIGITS == 1) digits[0] = pack_codes<N>(v, inverse);
+        else pack_digits<N>(v, inverse, digits);
     }
     __device__ __forceinline__ void write(const Piece<T> &p, uint32_t piece, bool none, const Inverse &inverse) const
     {
-        Packed<N> high = {}, low = {};
-        if (!none) pack(p, piece, inverse, high, low);
-        store(piece, high, low);
+        Packed<N> digits[DIGITS] = {};
+        if (!none) pack(p, piece, inverse, digits);
+        store(piece, digits);
     }
     // a whole piece, aligned
-    __device__ __forceinline__ void put(uint32_t piece, const Packed<N> &high, const Packed<N> &low) const
+    __device__ __forceinline__ void put(uint32_t piece, const Packed<N> (&digits)[DIGITS]) const
     {
-        const size_t at = r * P.ld_codes + column<N, LANES, true>(piece, lane, 0);
-        if (N == 8) *reinterpret_cast<uint2 *>(P.codes + at) = make_uint2(high.w[0], high.w[N / 4 - 1]);
-        else *reinterpret_cast<uint32_t *>(P.codes + at) = high.w[0];
-        if (DIGITS == 1) return;
-        if (N == 8) *reinterpret_cast<uint2 *>(P.low + at) = make_uint2(low.w[0], low.w[N / 4 - 1]);
-        else *reinterpret_cast<uint32_t *>(P.low + at) = low.w[0];
+        int8_t *to = P.codes + r * P.ld_codes + column<N, LANES, true>(piece, lane, 0);
+#pragma unroll
+        for (int d = 0; d < DIGITS; ++d, to += P.plane) {
+            if (N == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(digits[d].w[0], digits[d].w[N / 4 - 1]);
+            else *reinterpret_cast<uint32_t *>(to) = digits[d].w[0];
+        }
     }
-    __device__ __forceinline__ void store(uint32_t piece, const Packed<N> &high, const Packed<N> &low) const
+    __device__ __forceinline__ void store(uint32_t piece, const Packed<N> (&digits)[DIGITS]) const
     {
-        store_codes<N, LANES, ALIGNED>(P.codes + r * P.ld_codes, piece, lane, P.width, high);
-        if (DIGITS == 2) store_codes<N, LANES, ALIGNED>(P.low + r * P.ld_codes, piece, lane, P.width, low);
+#pragma unroll
+        for (int d = 0; d < DIGITS; ++d) store_codes<N, LANES, ALIGNED>(P.codes + d * P.plane + r * P.ld_codes, piece, lane, P.width, digits[d]);
     }
 };
 
