@@ -804,6 +804,13 @@ def _beside(v, x: _Values, name: str, shape, what: str):
     return v, ptr
 
 
+def _record_nothing(**operands):
+    """Products are not part of torch's record of a computation: an operand that asks for a gradient would go without one."""
+    for what, v in operands.items():
+        if getattr(v, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
+            raise ValueError(f"{what} requires a gradient, which this call does not record: pass {what}.detach() (input_gradient gives the rows' gradient)")
+
+
 def _context_of(rows) -> Context:
     """The context of the device that the rows are on."""
     if _is_torch(rows) and rows.is_cuda:
@@ -857,7 +864,10 @@ class QuantizedMatrix:
     ``product`` takes rows of float32, float16 or bfloat16, quantizes each as RowQuantizer does and multiplies: the sums of products
     of codes are exact.  With `offsets` (groups + 1 ascending row numbers, int64; best where the rows are) group g's matrix takes the rows
     offsets[g] .. offsets[g + 1] - 1; rows of no group come out as 0 in a fresh result and stay as they are in the caller's `out`.  `gradient`:
-    keep the codes transposed too, for ``input_gradient``."""
+    keep the codes transposed too, for ``input_gradient``.
+
+    torch does not record these calls.  An operand that requires a gradient is refused while torch records; who trains what is in front of a matrix calls
+    ``product`` in the forward and ``input_gradient`` in the backward method of a torch.autograd.Function (where nothing is recorded)."""
 
     def __init__(self, handle, ctx: Context, grouped: bool):
         self._h, self._ctx, self._grouped = handle, ctx, grouped
@@ -940,6 +950,7 @@ class QuantizedMatrix:
     def product(self, rows, bias=None, *, offsets=None, dtype=None, out=None):
         """rows (n x inputs, or one vector) times the matrix: n x outputs of `dtype` (the rows' own by default), plus the bias (outputs, or
         groups x outputs; added in float32)."""
+        _record_nothing(rows=rows, bias=bias, out=out)
         x = _Values(rows, self._ctx, "rows")
         ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
         kb, bptr = self._bias(x, bias) if bias is not None else (None, None)
@@ -949,6 +960,7 @@ class QuantizedMatrix:
 
     def product_of_codes(self, codes, scales, bias=None, *, offsets=None, dtype=None, out=None):
         """The same for what RowQuantizer.quantize returned, so that several matrices can share it; `dtype` is float32 by default."""
+        _record_nothing(scales=scales, bias=bias, out=out)
         x = _Values(codes, self._ctx, "codes", integers=True)
         ks, sptr = _beside(scales, x, "float32", () if x.single else (x.n,), "scales")
         ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
@@ -961,6 +973,7 @@ class QuantizedMatrix:
         """The gradient of ``product`` with respect to its rows, given the one with respect to its result (n x outputs, float16 or bfloat16): n x inputs of
         the same type.  The rounding to codes counts as the identity.  Each dy * channel scale enters with 24 bits of the largest of its
         row, as a sum of them in float32 would hold it."""
+        _record_nothing(dy=dy, out=out)
         x = _Values(dy, self._ctx, "dy")
         ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
         y, yptr, kind, ld = _result(x, self._shape[2], x.keep.dtype if out is None else None, out)
