@@ -83,7 +83,8 @@ int set_err(vqb_ctx *ctx, int code, const std::string &msg)
     return code;
 }
 
-template <typename F> int guarded(vqb_ctx *ctx, F &&f)
+// sets_stream: the call does nothing on the stream that it finds, which the caller may have destroyed.
+template <typename F> int guarded(vqb_ctx *ctx, F &&f, bool sets_stream = false)
 {
     struct AtEnd {
         vqb_ctx *ctx;
@@ -93,7 +94,10 @@ template <typename F> int guarded(vqb_ctx *ctx, F &&f)
         }
     } at_end{ctx};
     try {
-        if (ctx) ctx->dev->make_current();
+        if (ctx) {
+            ctx->dev->make_current();
+            if (!sets_stream) ctx->dev->begin_call();
+        }
         f();
         return VQB_OK;
     } catch (const Error &e) {
@@ -108,11 +112,11 @@ template <typename F> int guarded(vqb_ctx *ctx, F &&f)
 }
 
 // One call of a context.
-template <typename F> int locked(vqb_ctx *ctx, F &&f)
+template <typename F> int locked(vqb_ctx *ctx, F &&f, bool sets_stream = false)
 {
     CallLock::Hold hold(ctx->lock);
     if (!hold) return set_err(ctx, VQB_ERR_CALLBACK, "a callback may not call the context that is calling it");
-    return guarded(ctx, f);
+    return guarded(ctx, f, sets_stream);
 }
 
 // What a destroy function frees.  Inside a callback (a garbage collector may run there) only that happens: what the fit in
@@ -493,13 +497,13 @@ const char *vqb_last_error(const vqb_ctx *ctx) { return ctx ? ctx->err.c_str() :
 int vqb_ctx_set_stream(vqb_ctx *ctx, void *cuda_stream)
 {
     if (!ctx) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "ctx is NULL");
-    return locked(ctx, [&] { ctx->dev->set_stream(static_cast<cudaStream_t>(cuda_stream)); });
+    return locked(ctx, [&] { ctx->dev->set_stream(static_cast<cudaStream_t>(cuda_stream)); }, true);
 }
 
 int vqb_ctx_reset_stream(vqb_ctx *ctx)
 {
     if (!ctx) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "ctx is NULL");
-    return locked(ctx, [&] { ctx->dev->reset_stream(); });
+    return locked(ctx, [&] { ctx->dev->reset_stream(); }, true);
 }
 
 int vqb_ctx_synchronize(vqb_ctx *ctx)

@@ -45,7 +45,8 @@ CudaDevice::CudaDevice(int device) : device_(device)
     smem_limit_ = prop.sharedMemPerBlockOptin;
     VQB_CUDA_CHECK(cudaStreamCreateWithFlags(&own_stream_, cudaStreamNonBlocking));
     stream_ = own_stream_;
-    VQB_CUDA_CHECK(cudaEventCreateWithFlags(&order_event_, cudaEventDisableTiming));
+    VQB_CUDA_CHECK(cudaEventCreateWithFlags(&order_.api.event, cudaEventDisableTiming));
+    order_.api.own = own_stream_;
     ++device_allocs_;
     if (cudaHostAlloc(reinterpret_cast<void **>(&stage_), STAGE_BYTES + UPLOAD_BYTES, cudaHostAllocMapped) != cudaSuccess) {
         stage_ = nullptr; // pinned memory is an optimisation only
@@ -89,7 +90,7 @@ CudaDevice::~CudaDevice()
             if (aux_[i]) cudaStreamDestroy(aux_[i]);
         if (stage_event_) cudaEventDestroy(stage_event_);
         if (upload_event_) cudaEventDestroy(upload_event_);
-        if (order_event_) cudaEventDestroy(order_event_);
+        if (order_.api.event) cudaEventDestroy(order_.api.event);
         for (cudaEvent_t e : arrival_done_) cudaEventDestroy(e);
         if (arrival_fence_) cudaEventDestroy(arrival_fence_);
         if (stage_) cudaFreeHost(stage_);
@@ -185,8 +186,7 @@ void allow_shared_memory(const CudaDevice &dev, const void *kernel)
     done.push_back(key);
 }
 
-// A stream that is being captured into a graph takes no part in the order of calls: an event from outside may not be waited for
-// there, and one from inside not outside.  (The query fails for the default stream while another one is being captured.)
+// (The query fails for the default stream while another one is being captured.)
 static bool captured(cudaStream_t s)
 {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
@@ -195,38 +195,36 @@ static bool captured(cudaStream_t s)
     return true;
 }
 
+bool CudaDevice::OrderEvent::lasting(cudaStream_t s) const { return s == own || s == nullptr || s == cudaStreamLegacy; }
+bool CudaDevice::OrderEvent::captured(cudaStream_t s) const { return vqb::captured(s); }
+void CudaDevice::OrderEvent::record(cudaStream_t s) { VQB_CUDA_CHECK(cudaEventRecord(event, s)); }
+void CudaDevice::OrderEvent::wait(cudaStream_t s) { VQB_CUDA_CHECK(cudaStreamWaitEvent(s, event, 0)); }
+
 // The scratch of the tensor-core kernels and the memory of a quantizer that is being destroyed are the context's, whatever stream a call
-// runs on.  The caller may destroy a stream of its own as soon as its work is done, so
-// such a stream gets the event while the call is still there (end_call); the context's own and the default stream get it here,
-// so that programs that never change streams pay nothing.
+// runs on (stream_order.hpp).
 void CudaDevice::set_stream(cudaStream_t s)
 {
     const cudaStream_t old = stream_;
-    if (s == old) return;
     stream_ = s;
-    if (!unfinished_) return;
-    if (lasting(old)) {
-        if (captured(old)) return;
-        VQB_CUDA_CHECK(cudaEventRecord(order_event_, old));
-    }
-    if (!captured(s)) VQB_CUDA_CHECK(cudaStreamWaitEvent(s, order_event_, 0)); // (otherwise the first call after the capture does)
+    order_.change(old, s);
 }
-
-bool CudaDevice::lasting(cudaStream_t s) const { return s == own_stream_ || s == nullptr || s == cudaStreamLegacy; }
 
 void CudaDevice::end_call()
 {
     release_dense();
     bop_fresh_ = dense_fresh_ = nullptr; // the next call's centroids may have the same address
     if (upload_at_) upload_at_ = UPLOAD_BYTES; // and its stream another one: its first upload waits for the last of this call
-    if (!later_.empty() && !captured(stream_)) {
-        for (void *p : later_) release(p);
-        later_.clear();
-        unfinished_ = true;
+    try {
+        if (!later_.empty() && !captured(stream_)) {
+            order_.settle(stream_);
+            for (void *p : later_) release(p);
+            later_.clear();
+            order_.launched();
+        }
+        order_.call_ends(stream_);
+    } catch (...) {
+        cudaGetLastError(); // (not the next launch's error)
     }
-    if (!unfinished_ || lasting(stream_)) return;
-    // (What was unfinished before a captured call still is, and has its event.)
-    if (!captured(stream_) && cudaEventRecord(order_event_, stream_) != cudaSuccess) cudaGetLastError(); // (not the next launch's error)
 }
 
 cudaStream_t CudaDevice::aux_stream(int i)
@@ -243,7 +241,7 @@ void CudaDevice::synchronize()
 {
     if (tc_error_) check_tc_error();
     else VQB_CUDA_CHECK(cudaStreamSynchronize(stream_));
-    unfinished_ = false;
+    order_.waited();
 }
 
 bool CudaDevice::is_device_pointer(const void *p) const
@@ -329,7 +327,7 @@ void CudaDevice::upload_queued(void *dst, const void *src, size_t bytes)
     VQB_CUDA_CHECK(cudaMemcpyAsync(dst, from, bytes, cudaMemcpyHostToDevice, stream_));
     VQB_CUDA_CHECK(cudaEventRecord(upload_event_, stream_)); // (a call has one stream)
     upload_at_ += room;
-    unfinished_ = true;
+    order_.launched();
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -422,7 +420,7 @@ void CudaDevice::download(void *dst, const void *src, size_t bytes, void *dst2, 
         wait_until([&] { return (q = cudaEventQuery(stage_event_)) != cudaErrorNotReady; },
                    [&] { return std::to_string(bytes + bytes2) + " bytes from the GPU, behind kernel " + last_kernel_; });
         VQB_CUDA_CHECK(q);
-        unfinished_ = false;
+        order_.waited();
         if (bytes) std::memcpy(dst, stage_ + 16, bytes);
         if (bytes2) std::memcpy(dst2, second, bytes2);
         if (tc_error_) {
@@ -437,7 +435,7 @@ void CudaDevice::download(void *dst, const void *src, size_t bytes, void *dst2, 
     if (bytes) VQB_CUDA_CHECK(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToHost, stream_));
     if (bytes2) VQB_CUDA_CHECK(cudaMemcpyAsync(dst2, src2, bytes2, cudaMemcpyDeviceToHost, stream_));
     VQB_CUDA_CHECK(cudaStreamSynchronize(stream_));
-    unfinished_ = false;
+    order_.waited();
     check_tc_error();
 }
 
@@ -457,7 +455,7 @@ void CudaDevice::ensure_tc_buffers()
     VQB_CUDA_CHECK(cudaMemsetAsync(tc_stats_, 0, 3 * sizeof(unsigned long long), stream_));
     VQB_CUDA_CHECK(cudaMalloc(&tc_error_, sizeof(int)));
     VQB_CUDA_CHECK(cudaMemsetAsync(tc_error_, 0, sizeof(int), stream_));
-    unfinished_ = true; // the first call may come on another stream
+    order_.launched(); // the first call may come on another stream
 }
 
 void *CudaDevice::try_alloc(size_t bytes)
@@ -665,14 +663,14 @@ void CudaDevice::copy(void *dst, const void *src, size_t bytes)
 {
     if (!bytes) return;
     VQB_CUDA_CHECK(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToDevice, stream_));
-    unfinished_ = true;
+    order_.launched();
 }
 
 void CudaDevice::zero(void *dst, size_t bytes)
 {
     if (!bytes) return;
     VQB_CUDA_CHECK(cudaMemsetAsync(dst, 0, bytes, stream_));
-    unfinished_ = true;
+    order_.launched();
 }
 
 static inline unsigned blocks_for(size_t items, int threads, size_t cap = 1u << 20)

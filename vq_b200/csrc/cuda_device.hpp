@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "backend.hpp"
+#include "stream_order.hpp"
 #include "dense_tc.hpp"
 #include "iter_status.cuh"
 #include "pq_tc.hpp"
@@ -108,10 +109,12 @@ class CudaDevice : public Device {
     int device() const { return device_; }
     int sm_count() const { return sm_count_; }
     size_t smem_limit() const { return smem_limit_; }
-    void end_call(); // at the end of every call of the C ABI
+    // at the start and the end of every call of the C ABI
+    void begin_call() { order_.settle(stream_); }
+    void end_call();
     int *error_word() const { return tc_error_; } // null with VQB_NO_TENSOR=1
     uint64_t launches() const { return launches_.load(); }
-    void count_launch(uint64_t n = 1) { launches_ += n, unfinished_ = true; }
+    void count_launch(uint64_t n = 1) { launches_ += n, order_.launched(); }
     // How often this context has asked CUDA for device or pinned memory (cudaMalloc, cudaMallocAsync, cudaHostAlloc).
     uint64_t device_allocs() const { return device_allocs_.load(); }
     void make_current() const;
@@ -133,12 +136,17 @@ class CudaDevice : public Device {
     int sm_count_ = 148;
     size_t smem_limit_ = 0;
     cudaStream_t own_stream_ = nullptr, stream_ = nullptr, aux_[2] = {nullptr, nullptr};
-    // A call may leave work behind on its stream that uses the context's scratch, and the next call may run on another one: set_stream
-    // puts that one behind order_event_.
-    bool unfinished_ = false; // nothing has waited for stream_ since the last launch or copy
-    cudaEvent_t order_event_ = nullptr;
+    struct OrderEvent {
+        using Stream = cudaStream_t;
+        cudaEvent_t event = nullptr;
+        cudaStream_t own = nullptr;
+        bool lasting(cudaStream_t s) const;
+        bool captured(cudaStream_t s) const;
+        void record(cudaStream_t s);
+        void wait(cudaStream_t s);
+    };
+    StreamOrder<OrderEvent> order_;
     std::vector<void *> later_; // release_later
-    bool lasting(cudaStream_t s) const;
     static constexpr size_t STAGE_BYTES = 1u << 20; // pinned staging for small downloads
     static constexpr size_t UPLOAD_BYTES = 1u << 20; // behind it, a ring for small uploads
     size_t upload_at_ = 0;
