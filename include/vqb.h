@@ -290,7 +290,9 @@ int vqb_bq_quantize(vqb_ctx *ctx, float threshold, uint8_t low, uint8_t high, co
  * 0 .. n, nothing outside the n rows is touched, but which results are written is not defined.
  *
  * A matrix is complete when the call that makes it returns (which therefore cannot be captured into a graph); a graph of a product reads the matrix
- * whenever it is replayed.  Products may be captured; but for one or two rows with one matrix they take memory of the call, which then is the graph's.
+ * whenever it is replayed.  Products and vqb_row_quantize may be captured, with all their operands in device memory (VQB_ERR_UNSUPPORTED otherwise: a graph would read and
+ * write the caller's host memory at every replay); but for one or two rows with one matrix they take memory of the call, which then is the graph's.  What a call is
+ * given in host memory, page-locked or not, it has read when it returns.
  *
  * Values are f32, f16 or bf16 (the same bits in and out as the caller's); ld: values from row to row (>= the row's width).  Outputs may not
  * overlap inputs.  No rows (n == 0) is no error.  Limits: width 131071 (VQB_ERR_UNSUPPORTED beyond: the sums are 32 bits), 1024 groups, 2^30 - 1 rows. */

@@ -862,7 +862,8 @@ class QuantizedMatrix:
     scale for each output channel, and its products with rows that are quantized too.
 
     ``product`` takes rows of float32, float16 or bfloat16, quantizes each as RowQuantizer does and multiplies: the sums of products
-    of codes are exact.  With `offsets` (groups + 1 ascending row numbers, int64; best where the rows are) group g's matrix takes the rows
+    of codes are exact.  With `offsets` (groups + 1 ascending row numbers, int64; best where the rows are, and in a captured call they and the
+    bias have to be there) group g's matrix takes the rows
     offsets[g] .. offsets[g + 1] - 1; rows of no group come out as 0 in a fresh result and stay as they are in the caller's `out`.  `gradient`:
     keep the codes transposed too, for ``input_gradient``.
 

@@ -195,18 +195,57 @@ struct RowsIn {
     RowsIn &operator=(const RowsIn &) = delete;
 };
 
+// Before anything of the call becomes part of the graph.
+void refuse_captured(CudaDevice &dev, const char *what)
+{
+    if (dev.capturing()) throw Error(VQB_ERR_UNSUPPORTED, std::string(what) + " is in host memory, which a graph would use again at every replay: a captured call takes device memory");
+}
+
+// An input of the calls on codes: what is in host memory has been read when the call returns, whatever kind of memory it is.
+struct CallIn {
+    CudaDevice &dev;
+    const void *d = nullptr;
+    void *owned = nullptr;
+    CallIn(CudaDevice &dv, const char *what, const void *p, size_t bytes) : dev(dv)
+    {
+        bool page_locked = false;
+        if (bytes == 0 || dev.is_device_pointer(p, &page_locked)) {
+            d = p;
+            return;
+        }
+        refuse_captured(dev, what);
+        bring(p, bytes, page_locked);
+    }
+    void bring(const void *p, size_t bytes, bool page_locked)
+    {
+        d = owned = dev.alloc(bytes);
+        try {
+            dev.upload_within_call(owned, p, bytes, page_locked);
+        } catch (...) {
+            dev.release(owned);
+            throw;
+        }
+    }
+    ~CallIn() { dev.release(owned); }
+    CallIn(const CallIn &) = delete;
+    CallIn &operator=(const CallIn &) = delete;
+    template <typename T> const T *as() const { return static_cast<const T *>(d); }
+};
+
 // An output that is produced on the device and, when the caller's pointer is host memory, copied back.
 struct Out {
     CudaDevice &dev;
     void *d = nullptr;
     void *host = nullptr;
     size_t bytes = 0;
-    Out(CudaDevice &dv, void *p, size_t b) : dev(dv), bytes(b)
+    // not_captured: what the caller calls it, where a captured call has to be refused
+    Out(CudaDevice &dv, void *p, size_t b, const char *not_captured = nullptr) : dev(dv), bytes(b)
     {
         if (!p) return;
         if (b == 0 || dev.is_device_pointer(p)) {
             d = p;
         } else {
+            if (not_captured) refuse_captured(dev, not_captured);
             host = p;
             d = dev.alloc(b);
         }
@@ -331,9 +370,9 @@ void check_row_count(size_t n)
 // Bytes from the first value of the first row to the last one of the last.
 size_t span(size_t n, size_t width, size_t ld, size_t bytes) { return n ? ((n - 1) * ld + width) * bytes : 0; }
 
-// The groups' offsets: on the device as they are, from the host once they have been looked at.
+// The groups' offsets: on the device as they are, from the host as they were when they were looked at.
 struct OffsetsIn {
-    std::unique_ptr<In> in;
+    std::unique_ptr<CallIn> in;
     OffsetsIn(CudaDevice &dev, const int64_t *offsets, size_t groups, size_t n)
     {
         if (!offsets) {
@@ -341,11 +380,16 @@ struct OffsetsIn {
             return;
         }
         check_words("offsets", offsets, sizeof(int64_t));
-        if (!dev.is_device_pointer(offsets))
+        std::vector<int64_t> seen;
+        if (!dev.is_device_pointer(offsets)) {
+            refuse_captured(dev, "offsets");
+            seen.assign(offsets, offsets + groups + 1);
             for (size_t g = 0; g <= groups; ++g)
-                if (offsets[g] < (g ? offsets[g - 1] : 0) || offsets[g] > (int64_t)n)
+                if (seen[g] < (g ? seen[g - 1] : 0) || seen[g] > (int64_t)n)
                     throw Error(VQB_ERR_INVALID_PARAMETER, "Invalid parameter: offsets must ascend from 0 or more to at most the number of rows");
-        in.reset(new In(dev, offsets, sizeof(int64_t) * (groups + 1)));
+            offsets = seen.data();
+        }
+        in.reset(new CallIn(dev, "offsets", offsets, sizeof(int64_t) * (groups + 1)));
     }
     const int64_t *get() const { return in ? in->as<int64_t>() : nullptr; }
 };
@@ -353,7 +397,7 @@ struct OffsetsIn {
 // A product's result.  Host memory that the product does not write all of is brought in first.
 struct RowsOut {
     Out out;
-    RowsOut(CudaDevice &dev, void *y, size_t n, size_t width, size_t ld, int type, bool all) : out(dev, y, span(n, width, ld, value_bytes(type)))
+    RowsOut(CudaDevice &dev, const char *what, void *y, size_t n, size_t width, size_t ld, int type, bool all) : out(dev, y, span(n, width, ld, value_bytes(type)), what)
     {
         if (out.host && (!all || ld != width)) VQB_CUDA_CHECK(cudaMemcpyAsync(out.d, out.host, out.bytes, cudaMemcpyHostToDevice, dev.stream()));
     }
@@ -1285,8 +1329,8 @@ int vqb_row_quantize(vqb_ctx *ctx, const void *x, int type, size_t n, size_t dim
         if (ld_codes < dim) throw Error(VQB_ERR_BAD_ARGUMENT, "codes: rows overlap");
         check_words("scales", scales, sizeof(float));
         CudaDevice &dev = *ctx->dev;
-        In ix(dev, x, span(n, dim, ld, value_bytes(type)));
-        Out oc(dev, codes, span(n, dim, ld_codes, 1)), os(dev, scales, sizeof(float) * n);
+        CallIn ix(dev, "x", x, span(n, dim, ld, value_bytes(type)));
+        Out oc(dev, codes, span(n, dim, ld_codes, 1), "codes"), os(dev, scales, sizeof(float) * n, "scales");
         if (oc.host && ld_codes != dim) VQB_CUDA_CHECK(cudaMemcpyAsync(oc.d, oc.host, oc.bytes, cudaMemcpyHostToDevice, dev.stream()));
         launch_quantize_rows(dev, ix.d, type, n, dim, ld, oc.as<int8_t>(), ld_codes, os.as<float>(), false);
         finish(oc, os);
@@ -1346,7 +1390,7 @@ int vqb_qmat_parts(const vqb_qmat *qm, int8_t *codes_out, float *scales_out)
         CudaDevice &dev = *ctx->dev;
         const Qmat &m = qm->mat;
         const size_t rows = m.groups * m.outputs;
-        Out oc(dev, codes_out, rows * m.inputs), os(dev, scales_out, sizeof(float) * rows);
+        Out oc(dev, codes_out, rows * m.inputs, "codes"), os(dev, scales_out, sizeof(float) * rows, "scales");
         if (oc.d) VQB_CUDA_CHECK(cudaMemcpy2DAsync(oc.d, m.inputs, m.codes, codes_ld(m.inputs), m.inputs, rows, cudaMemcpyDeviceToDevice, dev.stream()));
         if (os.d) dev.copy(os.d, m.scales, sizeof(float) * rows);
         finish(oc, os);
@@ -1365,8 +1409,8 @@ int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim
         OffsetsIn io(dev, offsets, m.groups, n);
         if (n == 0) return;
         check_values("x", x, type, dim, ld);
-        In ix(dev, x, span(n, dim, ld, value_bytes(type))), ib(dev, bias, bias ? sizeof(float) * m.groups * m.outputs : 0);
-        RowsOut oy(dev, y, n, m.outputs, y_ld, y_type, !offsets || (flags & VQB_ZERO_REST));
+        CallIn ix(dev, "x", x, span(n, dim, ld, value_bytes(type))), ib(dev, "bias", bias, bias ? sizeof(float) * m.groups * m.outputs : 0);
+        RowsOut oy(dev, "y", y, n, m.outputs, y_ld, y_type, !offsets || (flags & VQB_ZERO_REST));
         Product p = product_of(m);
         p.n = n, p.rows_ld = codes_ld(dim), p.offsets = io.get(), p.bias = ib.as<float>();
         p.y = oy.out.d, p.y_type = y_type, p.y_ld = y_ld, p.zero_rest = (flags & VQB_ZERO_REST) != 0;
@@ -1394,8 +1438,8 @@ int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, size_t ld_codes, c
         if (!codes || !scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
         check_words("scales", scales, sizeof(float));
         if (ld_codes < dim) throw Error(VQB_ERR_BAD_ARGUMENT, "codes: rows overlap");
-        In ic(dev, codes, span(n, dim, ld_codes, 1)), is(dev, scales, sizeof(float) * n), ib(dev, bias, bias ? sizeof(float) * m.groups * m.outputs : 0);
-        RowsOut oy(dev, y, n, m.outputs, y_ld, y_type, !offsets || (flags & VQB_ZERO_REST));
+        CallIn ic(dev, "codes", codes, span(n, dim, ld_codes, 1)), is(dev, "scales", scales, sizeof(float) * n), ib(dev, "bias", bias, bias ? sizeof(float) * m.groups * m.outputs : 0);
+        RowsOut oy(dev, "y", y, n, m.outputs, y_ld, y_type, !offsets || (flags & VQB_ZERO_REST));
         Product p = product_of(m);
         p.n = n, p.offsets = io.get(), p.bias = ib.as<float>(), p.row_scales = is.as<float>();
         p.y = oy.out.d, p.y_type = y_type, p.y_ld = y_ld, p.zero_rest = (flags & VQB_ZERO_REST) != 0;
@@ -1428,8 +1472,8 @@ int vqb_qmat_input_gradient(vqb_qmat *qm, const void *dy, int type, size_t n, si
         if (n == 0) return;
         check_values("dy", dy, type, dim, ld);
         check_values("dx", dx, type, m.inputs, dx_ld);
-        In iy(dev, dy, span(n, dim, ld, value_bytes(type)));
-        RowsOut ox(dev, dx, n, m.inputs, dx_ld, type, !offsets || (flags & VQB_ZERO_REST));
+        CallIn iy(dev, "dy", dy, span(n, dim, ld, value_bytes(type)));
+        RowsOut ox(dev, "dx", dx, n, m.inputs, dx_ld, type, !offsets || (flags & VQB_ZERO_REST));
         Product p;
         p.codes = m.turned, p.groups = m.groups, p.channels = m.inputs, p.width = m.outputs, p.digits = 3;
         p.n = n, p.rows_ld = codes_ld(dim), p.offsets = io.get();

@@ -214,6 +214,8 @@ void CudaDevice::end_call()
     release_dense();
     bop_fresh_ = dense_fresh_ = nullptr; // the next call's centroids may have the same address
     if (upload_at_) upload_at_ = UPLOAD_BYTES; // and its stream another one: its first upload waits for the last of this call
+    if (host_copies_) cudaStreamSynchronize(stream_);
+    host_copies_ = false;
     try {
         if (!later_.empty() && !captured(stream_)) {
             order_.settle(stream_);
@@ -244,7 +246,9 @@ void CudaDevice::synchronize()
     order_.waited();
 }
 
-bool CudaDevice::is_device_pointer(const void *p) const
+bool CudaDevice::capturing() const { return captured(stream_); }
+
+bool CudaDevice::is_device_pointer(const void *p, bool *page_locked) const
 {
     if (!p) return false;
     cudaPointerAttributes attr;
@@ -253,6 +257,7 @@ bool CudaDevice::is_device_pointer(const void *p) const
         cudaGetLastError();
         return false;
     }
+    if (page_locked) *page_locked = attr.type == cudaMemoryTypeHost;
     return attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeManaged;
 }
 
@@ -305,6 +310,20 @@ void CudaDevice::upload(void *dst, const void *src, size_t bytes)
     }
     VQB_CUDA_CHECK(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, stream_));
     VQB_CUDA_CHECK(cudaStreamSynchronize(stream_));
+}
+
+// A copy from pageable memory has been staged by the driver when cudaMemcpyAsync returns; from page-locked memory it reads when the stream gets there, by when the
+// caller may have filled it anew.  Small ones go through pageable memory, so that nobody waits; behind large ones the call waits.
+void CudaDevice::upload_within_call(void *dst, const void *src, size_t bytes, bool page_locked)
+{
+    if (page_locked && bytes <= STAGE_BYTES) {
+        const std::vector<unsigned char> copy(static_cast<const unsigned char *>(src), static_cast<const unsigned char *>(src) + bytes);
+        VQB_CUDA_CHECK(cudaMemcpyAsync(dst, copy.data(), bytes, cudaMemcpyHostToDevice, stream_));
+    } else {
+        VQB_CUDA_CHECK(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, stream_));
+        host_copies_ |= page_locked;
+    }
+    order_.launched();
 }
 
 // Small ones go through pinned memory, and nobody waits for them: a fit of 10,000 x 128 spent 75 of its 550 us in two copies from pageable

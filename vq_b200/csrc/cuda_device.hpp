@@ -128,8 +128,12 @@ class CudaDevice : public Device {
     std::string timing_report();
     // Diagnostic: raw tensor-core dot products (n x 256) and shortlist statistics {rows, candidates, full scans}.
     void dense_debug(const float *x, size_t n, size_t dim, const float *codebook, size_t k, float *dots, unsigned long long *stats3);
-    // True when p points to device memory usable by kernels on this GPU.
-    bool is_device_pointer(const void *p) const;
+    // True when p points to device memory usable by kernels on this GPU.  page_locked: set for host memory that copies read while the host goes on.
+    bool is_device_pointer(const void *p, bool *page_locked = nullptr) const;
+    // The stream is being captured into a graph.
+    bool capturing() const;
+    // From the caller's host memory, which has been read by the end of the call.
+    void upload_within_call(void *dst, const void *src, size_t bytes, bool page_locked);
 
   private:
     int device_;
@@ -147,6 +151,7 @@ class CudaDevice : public Device {
     };
     StreamOrder<OrderEvent> order_;
     std::vector<void *> later_; // release_later
+    bool host_copies_ = false;  // copies from the caller's page-locked memory may be under way: the call ends behind them
     static constexpr size_t STAGE_BYTES = 1u << 20; // pinned staging for small downloads
     static constexpr size_t UPLOAD_BYTES = 1u << 20; // behind it, a ring for small uploads
     size_t upload_at_ = 0;
