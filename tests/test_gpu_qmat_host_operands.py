@@ -107,3 +107,24 @@ def test_rows_and_results_in_host_memory_are_not_captured(ctx):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(z, want) and torch.equal(m.product(x), want)
+
+
+@pytest.mark.parametrize("pinned", [False, True])
+def test_a_matrix_of_weights_in_host_memory_is_refused_ahead_of_their_copy(pinned, ctx):
+    torch = torch_()
+    m, x = vq.QuantizedMatrix.fit(normal(1, OUTPUTS, INPUTS), ctx=ctx), normal(2, N, INPUTS)
+    want = m.product(x)
+    w, codes, scales = torch.zeros(64, 64), torch.zeros(64, 64, dtype=torch.int8), torch.zeros(64)
+    if pinned:
+        w, codes, scales = w.pin_memory(), codes.pin_memory(), scales.pin_memory()
+    there = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    graph, made = torch.cuda.CUDAGraph(), C.c_void_p()
+    with torch.cuda.graph(graph):
+        y = m.product(x)  # (the context is on the captured stream)
+        before = ctx.alloc_count()
+        assert ctx._L.vqb_qmat_fit(ctx.handle, there(w), 0, 1, 64, 64, 0, C.byref(made)) == 103 and not made
+        assert ctx._L.vqb_qmat_from_parts(ctx.handle, there(codes), there(scales), 1, 64, 64, 1, C.byref(made)) == 103 and not made
+        assert ctx.alloc_count() == before, "memory was asked for inside the capture"
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and torch.equal(m.product(x), want)

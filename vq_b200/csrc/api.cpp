@@ -403,6 +403,12 @@ struct RowsOut {
     }
 };
 
+// Ahead of anything that would become part of the graph.
+void check_not_captured(CudaDevice &dev)
+{
+    if (dev.capturing()) throw Error(VQB_ERR_UNSUPPORTED, "a matrix cannot be made while its stream is being captured");
+}
+
 void check_qmat_shape(size_t groups, size_t outputs, size_t inputs, int flags)
 {
     if (groups == 0 || outputs == 0 || inputs == 0) throw Error(VQB_ERR_EMPTY_INPUT, "Empty input: at least one vector is required.");
@@ -421,12 +427,6 @@ struct NewQmat {
     {
         Qmat &m = qm->mat;
         m.groups = groups, m.outputs = outputs, m.inputs = inputs;
-        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(dev.stream(), &capture) != cudaSuccess) { // (the default stream while another one is being captured)
-            cudaGetLastError();
-            capture = cudaStreamCaptureStatusActive;
-        }
-        if (capture != cudaStreamCaptureStatusNone) throw Error(VQB_ERR_UNSUPPORTED, "a matrix cannot be made while its stream is being captured");
         try {
             m.codes = static_cast<int8_t *>(dev.alloc(groups * outputs * codes_ld(inputs)));
             if (inputs % 16) dev.zero(m.codes, groups * outputs * codes_ld(inputs));
@@ -1346,6 +1346,7 @@ int vqb_qmat_fit(vqb_ctx *ctx, const void *weights, int type, size_t groups, siz
         check_qmat_shape(groups, outputs, inputs, flags);
         check_values("weights", weights, type, inputs, inputs);
         CudaDevice &dev = *ctx->dev;
+        check_not_captured(dev);
         In iw(dev, weights, groups * outputs * inputs * value_bytes(type));
         NewQmat made(ctx, groups, outputs, inputs, flags);
         Qmat &m = made.qm->mat;
@@ -1364,6 +1365,7 @@ int vqb_qmat_from_parts(vqb_ctx *ctx, const int8_t *codes, const float *scales, 
         if (!codes || !scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
         check_words("scales", scales, sizeof(float));
         CudaDevice &dev = *ctx->dev;
+        check_not_captured(dev);
         In ic(dev, codes, groups * outputs * inputs), is(dev, scales, sizeof(float) * groups * outputs);
         NewQmat made(ctx, groups, outputs, inputs, flags);
         Qmat &m = made.qm->mat;
