@@ -200,7 +200,7 @@ template <typename T, int EIGHTS, int PAIRS> __global__ void __launch_bounds__(T
             }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_relaxed(&empty[st]);
+        if (lane == 0) mbar_arrive(&empty[st]); // (a release: the reads of this place are before whatever the copy that waits for it writes there)
         if ((i + P.stages) / steps == part && i + P.stages < all) continue;
         // (the next stage has other channels)
 #pragma unroll

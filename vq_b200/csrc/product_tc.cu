@@ -109,7 +109,9 @@ __device__ __forceinline__ void tma_load_plane_counted(void *dst, const CUtensor
                  "r"(bar), "r"(c0), "r"(c1), "r"(c2)
                  : "memory");
 }
-// Without release ordering: what is handed back has been read, and a release would wait for the results' stores (1 us a tile).
+// Hands an accumulator back.  Nothing but tensor memory is handed over, and what orders that is the pair of tcgen05 fences around the barrier: PTX has tcgen05.ld of one thread before
+// tcgen05.mma of another as tcgen05.wait::ld, tcgen05.fence::before_thread_sync and a relaxed arrival, then the wait and tcgen05.fence::after_thread_sync.  (The other lanes' loads
+// and fences are before the arrival by __syncwarp.)  A release would wait for the results' stores, too, 1 us a tile.
 __device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void cluster_sync()
 {
