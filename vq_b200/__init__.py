@@ -720,8 +720,8 @@ class _Values:
                     raise ValueError(f"{what} must be int8")
                 self.type = None
             else:
-                if x.dtype.name not in ("float32", "float16"):
-                    x = x.astype(np.float32)
+                if x.dtype not in (np.float32, np.float16):  # (of this machine's byte order; the name says nothing about that)
+                    x = x.astype(np.float16 if x.dtype.name == "float16" else np.float32)
                 self.type = _VALUE_TYPES[x.dtype.name]
             x = np.ascontiguousarray(x)
             self.stream = None
@@ -773,7 +773,7 @@ def _result(x: _Values, width: int, dtype, out):
         strides = out.stride() if ok else ()
     else:
         given, out = out, out.numpy() if _is_torch(out) and not out.is_cuda and out.dtype in (sys.modules["torch"].float32, sys.modules["torch"].float16) else out
-        ok = isinstance(out, np.ndarray) and out.flags.writeable
+        ok = isinstance(out, np.ndarray) and out.flags.writeable and out.dtype.isnative
         strides = tuple(s // out.itemsize for s in out.strides) if ok and all(s % out.itemsize == 0 for s in out.strides) else ()
     ok = ok and kind is not None and tuple(out.shape) == shape and len(strides) == len(shape) and (width <= 1 or strides[-1] == 1)
     ld = strides[0] if ok and not x.single and x.n > 1 else width
