@@ -789,6 +789,8 @@ def _beside(v, x: _Values, name: str, shape, what: str):
             raise ValueError(f"{what} is on another device than the rows")
         want = getattr(sys.modules["torch"], name)
         if v.dtype is not want:
+            if name == "int64" and (v.dtype.is_floating_point or v.dtype.is_complex or v.dtype is sys.modules["torch"].bool):
+                raise ValueError(f"{what} must be whole numbers")
             v = v.detach().to(want)
         if not v.is_contiguous():
             v = v.contiguous()
@@ -797,7 +799,10 @@ def _beside(v, x: _Values, name: str, shape, what: str):
         if _is_torch(v):
             v = v.detach().cpu()
             v = (v.float() if str(v.dtype) == "torch.bfloat16" else v).numpy()
-        v = np.ascontiguousarray(v, dtype=name).reshape(np.shape(v))  # (a single scale stays one)
+        v = np.asarray(v)
+        if name == "int64" and v.dtype.kind not in "iu" and v.size:
+            raise ValueError(f"{what} must be whole numbers")
+        v = np.ascontiguousarray(v, dtype=name).reshape(v.shape)  # (a single scale stays one)
         found, ptr = v.shape, v.ctypes.data
     if found != shape:
         raise ValueError(f"{what} must have shape {shape}, not {tuple(found)}")
