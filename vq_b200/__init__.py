@@ -800,7 +800,7 @@ def _beside(v, x: _Values, name: str, shape, what: str):
             v = v.detach().cpu()
             v = (v.float() if str(v.dtype) == "torch.bfloat16" else v).numpy()
         v = np.asarray(v)
-        if name == "int64" and v.dtype.kind not in "iu" and v.size:
+        if name == "int64" and v.dtype.kind not in "iu" and v.shape == shape:
             raise ValueError(f"{what} must be whole numbers")
         v = np.ascontiguousarray(v, dtype=name).reshape(v.shape)  # (a single scale stays one)
         found, ptr = v.shape, v.ctypes.data
