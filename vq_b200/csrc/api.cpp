@@ -1394,6 +1394,7 @@ int vqb_qmat_parts(const vqb_qmat *qm, int8_t *codes_out, float *scales_out)
         const size_t rows = m.groups * m.outputs;
         Out oc(dev, codes_out, rows * m.inputs, "codes"), os(dev, scales_out, sizeof(float) * rows, "scales");
         if (oc.d) VQB_CUDA_CHECK(cudaMemcpy2DAsync(oc.d, m.inputs, m.codes, codes_ld(m.inputs), m.inputs, rows, cudaMemcpyDeviceToDevice, dev.stream()));
+        dev.count_launch(0); // (no kernel, but work that the next call on another stream comes behind)
         if (os.d) dev.copy(os.d, m.scales, sizeof(float) * rows);
         finish(oc, os);
     });
