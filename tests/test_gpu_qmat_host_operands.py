@@ -1,5 +1,6 @@
 """Operands in host memory beside rows on the GPU: read by the end of the call whatever kind of memory they are in, and refused while a graph is captured."""
 import ctypes as C
+import gc
 
 import numpy as np
 import pytest
@@ -9,6 +10,16 @@ from tests.test_gpu_qmat import normal, torch_
 
 pytestmark = pytest.mark.gpu
 N, INPUTS, OUTPUTS, GROUPS = 300, 256, 200, 3
+
+
+@pytest.fixture(autouse=True)
+def collected():
+    """A graph that the collector finds inside a capture would end the capture."""
+    gc.collect()
+    gc.disable()
+    yield
+    gc.enable()
+    gc.collect()
 
 
 def operands(pinned, first):
