@@ -284,7 +284,7 @@ int vqb_bq_quantize(vqb_ctx *ctx, float threshold, uint8_t low, uint8_t high, co
  *          s[i] = 0 for a row of zeros; s[i] = NaN for a row that holds an infinity or a NaN; the codes are 0 in both
  *   y[i][j] = (sum_k q[i][k] w[j][k]) s[i] t[j] + bias[j]         w, t: codes and scales of the matrix's rows (channels)
  *
- * The sum is exact; the steps behind it are f32.  A matrix may be one of `groups`: group g then has the rows offsets[g] .. offsets[g + 1] - 1
+ * The sum is exact; the steps behind it are f32, in that order (a sum times s[i] that leaves f32, from rows of 1e32 or more, is infinite).  A matrix may be one of `groups`: group g then has the rows offsets[g] .. offsets[g + 1] - 1
  * of the call, any number of them.  Rows of no group (in front of offsets[0], behind offsets[groups]) are not written, or become 0
  * with VQB_ZERO_REST.  Offsets in device memory are not looked at by the host: where they are not ascending, or leave
  * 0 .. n, nothing outside the n rows is touched, but which results are written is not defined.

@@ -82,3 +82,19 @@ def test_groups_of_any_rows(counts, front, dtype):
         want, lost = limits(dy[a:b], wq[g], ws[g])
         assert bool(((dx[a:b].double() - want).abs() <= torch.finfo(dx.dtype).eps / 2 * want.abs() * (1 + 2.0**-12) + lost + tiny).all()), g
     assert not dx[:front].any() and not dx[n - 5:].any()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_the_widest_sums_of_digits_stay_in_32_bits(dtype):
+    """131071 outputs of code -128, all but one with both last digits -128: 32640 = 65536 - 256 128 - 128 steps."""
+    torch = torch_()
+    outputs, part = 131071, 32640 / STEPS
+    codes = torch.full((outputs, 2), -128, dtype=torch.int8, device="cuda")
+    codes[:, 1] = 127
+    scales = torch.full((outputs,), part, device="cuda")
+    scales[77] = 1.0
+    m = vq.QuantizedMatrix.from_parts(codes, scales, gradient=True)
+    dx = m.input_gradient(torch.ones(3, outputs, device="cuda", dtype=getattr(torch, dtype)) / 1024)
+    total = (1.0 + (outputs - 1) * part) / 1024
+    want = torch.tensor([[-128.0 * total, 127.0 * total]] * 3, dtype=torch.float64, device="cuda")
+    assert bool(((dx.double() - want).abs() <= want.abs() * (torch.finfo(dx.dtype).eps / 2 + 2.0**-18)).all())

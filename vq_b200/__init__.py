@@ -767,6 +767,7 @@ def _result(x: _Values, width: int, dtype, out):
         return a, a.ctypes.data, _VALUE_TYPES[name], width
     if dtype is not None and _type_name(dtype) != _type_name(out.dtype):
         raise ValueError("out has another dtype than asked for")
+    _record_nothing("out", out)
     kind = _VALUE_TYPES.get(_type_name(out.dtype))
     if x.cuda:
         ok = _is_torch(out) and out.is_cuda and out.get_device() == x.keep.get_device()
@@ -809,11 +810,10 @@ def _beside(v, x: _Values, name: str, shape, what: str):
     return v, ptr
 
 
-def _record_nothing(**operands):
+def _record_nothing(what: str, v):
     """Products are not part of torch's record of a computation: an operand that asks for a gradient would go without one."""
-    for what, v in operands.items():
-        if getattr(v, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
-            raise ValueError(f"{what} requires a gradient, which this call does not record: pass {what}.detach() (input_gradient gives the rows' gradient)")
+    if getattr(v, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, which this call does not record: pass {what}.detach() (input_gradient gives the rows' gradient)")
 
 
 def _context_of(rows) -> Context:
@@ -829,7 +829,7 @@ class RowQuantizer:
 
     The scale is a 127th of the row's largest magnitude (0 for a row of zeros, NaN for one that holds an infinity or a NaN), the
     code the whole number nearest to ``x / scale``, halves to even.  Unlike ScalarQuantizer there is no range to choose, and the codes can be
-    multiplied as they are (QuantizedMatrix)."""
+    multiplied as they are (QuantizedMatrix).  torch records nothing of it; bfloat16 rows in host memory are taken as float32."""
 
     def __init__(self, ctx):
         self._ctx = ctx
@@ -941,6 +941,7 @@ class QuantizedMatrix:
         return _beside(offsets, x, "int64", (self._shape[0] + 1,), "offsets")
 
     def _bias(self, x, bias):
+        _record_nothing("bias", bias)
         g, o, _ = self._shape
         return _beside(bias, x, "float32", (g, o) if self._grouped else (o,), "bias")
 
@@ -954,9 +955,9 @@ class QuantizedMatrix:
                 _raise(rc, ctx.handle)
 
     def product(self, rows, bias=None, *, offsets=None, dtype=None, out=None):
-        """rows (n x inputs, or one vector) times the matrix: n x outputs of `dtype` (the rows' own by default), plus the bias (outputs, or
+        """rows (n x inputs, or one vector) times the matrix: n x outputs of `dtype` (the rows' own by default; float32 of bfloat16 rows in host memory), plus the bias (outputs, or
         groups x outputs; added in float32)."""
-        _record_nothing(rows=rows, bias=bias, out=out)
+        _record_nothing("rows", rows)
         x = _Values(rows, self._ctx, "rows")
         ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
         kb, bptr = self._bias(x, bias) if bias is not None else (None, None)
@@ -966,7 +967,7 @@ class QuantizedMatrix:
 
     def product_of_codes(self, codes, scales, bias=None, *, offsets=None, dtype=None, out=None):
         """The same for what RowQuantizer.quantize returned, so that several matrices can share it; `dtype` is float32 by default."""
-        _record_nothing(scales=scales, bias=bias, out=out)
+        _record_nothing("scales", scales)
         x = _Values(codes, self._ctx, "codes", integers=True)
         ks, sptr = _beside(scales, x, "float32", () if x.single else (x.n,), "scales")
         ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
@@ -976,10 +977,10 @@ class QuantizedMatrix:
         return y
 
     def input_gradient(self, dy, *, offsets=None, out=None):
-        """The gradient of ``product`` with respect to its rows, given the one with respect to its result (n x outputs, float16 or bfloat16): n x inputs of
+        """The gradient of ``product`` with respect to its rows, given the one with respect to its result (n x outputs, float16, or bfloat16 on the GPU): n x inputs of
         the same type.  The rounding to codes counts as the identity.  Each dy * channel scale enters with 24 bits of the largest of its
         row, as a sum of them in float32 would hold it."""
-        _record_nothing(dy=dy, out=out)
+        _record_nothing("dy", dy)
         x = _Values(dy, self._ctx, "dy")
         ko, optr = self._groups(x, offsets) if offsets is not None or self._grouped else (None, None)
         y, yptr, kind, ld = _result(x, self._shape[2], x.keep.dtype if out is None else None, out)

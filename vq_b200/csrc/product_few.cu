@@ -144,7 +144,7 @@ template <typename T, int EIGHTS, int PAIRS> __global__ void __launch_bounds__(T
         const T *row = static_cast<const T *>(P.rows.x) + t * P.rows.ld;
         RowOf<T, 1, 1, true> it(P.rows, t, 0, nullptr); // (piece i: 16 bytes at 16 i)
         const int last = (int)((P.rows.width + N - 1) / N);
-        const Piece<T> held = load_values<T, 1, true>(row, l, 0, P.rows.width); // (up to 512 pieces a row there are no others)
+        const Piece<T> held = load_values<T, 1, true>(row, l, 0, P.rows.width); // (up to `step` pieces a row, 640 or of two rows 320 each, there are no others)
         it.look(held, l);
 #pragma unroll 4
         for (int i = l + step; i < last; i += step) it.look(load_values<T, 1, true>(row, i, 0, P.rows.width), i);
@@ -241,7 +241,7 @@ template <typename T, int EIGHTS> void product_few_pairs(CudaDevice &dev, const 
 bool launch_product_few(CudaDevice &dev, const Product &p, const void *x, int type, size_t ld)
 {
     if (!dev.error_word() || p.offsets || p.digits != 1 || p.n > 16) return false;
-    // every block quantizes the rows: with more than 32 values a thread that takes longer than a kernel before this one
+    // every block quantizes the rows: with more than 25 values a thread (16384 over 20 warps) that takes longer than a kernel before this one
     if (x && (p.n > 2 || p.n * p.width > 16384 || (reinterpret_cast<uintptr_t>(x) | (p.n == 1 ? 0 : ld * value_bytes(type))) % 16)) return false;
     const size_t eights = (p.n + 7) / 8;
     FewParams P{};

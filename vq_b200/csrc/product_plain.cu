@@ -1,7 +1,7 @@
 // product_plain.cu -- the products of codes on the CUDA cores: what VQB_NO_TENSOR=1 runs, and what product_tc.cu is compared with.
 //
 // A block takes 64 channels x 64 rows; 64 bytes of both at a time go through shared memory, a thread keeps 4 x 4 sums and adds four
-// products an instruction (dp4a).  What bounds it is that instruction: 64 of them an SM and cycle.
+// products an instruction (dp4a).  What bounds it is that instruction, which runs at some ten lanes an SM and cycle here.
 #include <algorithm>
 
 #include "cuda_device.hpp"

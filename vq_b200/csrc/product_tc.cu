@@ -548,7 +548,7 @@ void launch_product(CudaDevice &dev, const Product &p)
     // The tile's rows, and among how many pairs its width is parted: whatever makes the rounds of all SM pairs last the shortest.  Measured, in units of one
     // column's time in one stage (1.15 ns): a stage takes as long as its columns, but 160 and an eighth of them at least (0.20 us at 64 or 128 columns,
     // 0.22 at 160, 0.30 at 256); a tile's change 400; its results leave at 10 a column, behind the next tile's stages or, at the end, behind
-    // nothing.  Joining parts takes 700 and 52 a column, shared by the pairs (us for 1, 2 and 4 parts: 128 rows of 8192 with 2048 channels 17.4, 13.4, 11.7; 100 of
+    // nothing.  (Three digits have three columns a row; the rule held there: within 10 % of the best height for ten of twelve sizes, 18 % for 192 to 5184 of 4057 rows.)  Joining parts takes 700 and 52 a column, shared by the pairs (us for 1, 2 and 4 parts: 128 rows of 8192 with 2048 channels 17.4, 13.4, 11.7; 100 of
     // 1024 with 1024 6.3, 7.2, 7.1).
     const size_t chunks = (p.width + KB - 1) / KB;
     size_t least = ~size_t(0);

@@ -49,7 +49,7 @@ struct Product {
     bool rows_follow = false; // the kernel directly before wrote `rows` and `row_scales`, and had itself waited for all that was before it
 };
 
-// codes[i][k] = x[i][k] / s[i] to the nearest whole number (halves to even, of the real quotient), s[i] = max_k |x[i][k]| / 127; s is 0 for
+// codes[i][k] = x[i][k] / s[i] to the nearest whole number (halves to even, of the real quotient), s[i] = max(max_k |x[i][k]| / 127, 2^-126); s is 0 for
 // a row of zeros and NaN for one with an infinity or a NaN, with codes 0.  Bytes behind the row's width stay as they are.
 // product_follows: the caller's next launch is launch_product or launch_product_few (which waits for these codes itself; other kernels that may start early take
 // what was written for invariant).
