@@ -17,7 +17,7 @@
 //
 // Three digits (gradients): the first CTA fetches the rows' first digits and the second one their middle digits, each half of the last ones; two instructions a step, the
 // first one's columns' halves are the first and the middle sums, the second one's the last sums.  A tile of 128 rows has 384 columns, for which there is room once: its sums
-// are joined in registers, and the next tile's begin, before they leave.  (Tiles of 64 rows, two at a time, read 1.9 GB of L2 for 4096 x 4096 x 4096 and take 170 us for that, not 81.)
+// are joined in registers, and the next tile's begin, before they leave.  (Tiles of 64 rows, two at a time, read 1.9 GB of L2 for 4096 x 4096 x 4096 and take 170 us for that, not 120.)
 #include <algorithm>
 #include <map>
 #include <mutex>
