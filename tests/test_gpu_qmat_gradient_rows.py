@@ -49,7 +49,7 @@ def test_softmax_rows_keep_their_small_entries(n, outputs, mean, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
-@pytest.mark.parametrize("n,inputs,outputs", [(1, 1, 1), (3, 129, 1000), (33, 65, 64), (40, 130, 4100), (65, 700, 129), (129, 128, 256), (300, 1001, 515), (1000, 257, 96), (5000, 40, 33), (700, 3000, 300)])
+@pytest.mark.parametrize("n,inputs,outputs", [(1, 1, 1), (3, 129, 1000), (33, 65, 64), (40, 130, 4100), (65, 700, 129), (129, 128, 256), (300, 1001, 515), (1000, 257, 96), (5000, 40, 33), (700, 3000, 300), (5, 64, 20_001)])
 def test_gradients_are_the_definitions_to_their_own_rounding(n, inputs, outputs, dtype):
     torch = torch_()
     dy = normal(n, n, outputs, dtype=dtype, scale=0.01)
@@ -82,6 +82,20 @@ def test_groups_of_any_rows(counts, front, dtype):
         want, lost = limits(dy[a:b], wq[g], ws[g])
         assert bool(((dx[a:b].double() - want).abs() <= torch.finfo(dx.dtype).eps / 2 * want.abs() * (1 + 2.0**-12) + lost + tiny).all()), g
     assert not dx[:front].any() and not dx[n - 5:].any()
+
+
+@pytest.mark.parametrize("groups", [492, 493, 494, 495])
+def test_as_many_groups_as_leave_room_for_five_stages_and_more(groups):
+    torch = torch_()
+    outputs, inputs = 700, 40  # (six stages' worth of width)
+    w = normal(5, groups, outputs, inputs)
+    wq, ws = codes64(w)
+    off = torch.arange(groups + 1, device="cuda") * 3
+    dy = softmax_rows(3 * groups, outputs, 1.0, "bfloat16")
+    dx = vq.QuantizedMatrix.fit(w, gradient=True).input_gradient(dy, offsets=off)
+    for g in range(0, groups, 41):
+        want, lost = limits(dy[3 * g:3 * g + 3], wq[g], ws[g])
+        assert bool(((dx[3 * g:3 * g + 3].double() - want).abs() <= 2.0**-8 * want.abs() * (1 + 2.0**-12) + lost).all()), g
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
