@@ -315,7 +315,7 @@ int vqb_qmat_product(vqb_qmat *qm, const void *x, int type, size_t n, size_t dim
 int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, size_t ld_codes, const float *scales, size_t n, size_t dim, const int64_t *offsets,
                            const float *bias, void *y, int y_type, size_t y_ld, int flags);
 /* dx[i][k] = sum_j dy[i][j] t[j] w[j][k]: the product's gradient with respect to the rows that were quantized (the rounding taken for the identity).
- * u = dy[i][j] t[j] (a f32 product) enters in 24 bits of the row's largest magnitude: as a whole number of steps, each a 8323072nd of it (2^-126 at least), off by at most
+ * u = dy[i][j] t[j] (a f32 product) enters in 24 bits of the row's largest magnitude: as a whole number of steps, 127 * 65536 of which make up that magnitude (each 2^-126 at least), off by at most
  * half a step and 2^-23 of u.  The sums of those are exact.  dy is n x outputs, dx n x inputs, both f16 or both bf16 (f32 is refused: it would promise more digits than that).
  * Needs VQB_QMAT_GRADIENT. */
 int vqb_qmat_input_gradient(vqb_qmat *qm, const void *dy, int type, size_t n, size_t dim, size_t ld, const int64_t *offsets, void *dx, size_t dx_ld, int flags);

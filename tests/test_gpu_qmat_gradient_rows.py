@@ -1,7 +1,7 @@
 """Input gradients of rows that have a few large entries among many small ones, as the gradient of a softmax has, against the same in 64 bits.
 
-Tolerances go by each row's result: half a step of its type, and what the arithmetic in front may lose.  u = dy t is a f32 product (2^-24 of it), comes to whole steps of a 8323072th
-of its row's largest by a reciprocal (2^-24) and a product (2^-25 at most, as 8323072 < 2^23), and half a step is lost there; three whole-number sums are joined and scaled in f32
+Tolerances go by each row's result: half a step of its type, and what the arithmetic in front may lose.  u = dy t is a f32 product (2^-24 of it), comes to whole steps, 127 2^16 of which are
+its row's largest, by a reciprocal (2^-24) and a product (2^-25 at most, as 127 2^16 < 2^23), and half a step is lost there; three whole-number sums are joined and scaled in f32
 (six roundings of 2^-24 relative to the sum of magnitudes)."""
 import pytest
 

@@ -54,7 +54,7 @@ struct Product {
 // product_follows: the caller's next launch is launch_product or launch_product_few (which waits for these codes itself; other kernels that may start early take
 // what was written for invariant).
 void launch_quantize_rows(CudaDevice &dev, const void *x, int type, size_t n, size_t width, size_t ld, int8_t *codes, size_t ld_codes, float *scales, bool product_follows);
-// u[i][j] = x[i][j] column_scales[g][j] of the row's group g as the whole number next to u / t, t = max(max |u| / 8323072, 2^-126), in three digits (Product).  24 bits of the row's
+// u[i][j] = x[i][j] column_scales[g][j] of the row's group g as the whole number next to u / t, t = max(max |u| / (127 * 65536), 2^-126), in three digits (Product).  24 bits of the row's
 // largest are what a sum of the u in f32 holds.  (With the 15 that two digits of 128 have, rows of one large entry and many small ones, as a softmax's gradient has, lose the small
 // ones: of 128,256 outputs 5 to 15 % of the result where a channel's weights have a mean of 0.1 to 0.3 of their spread.  The third digit takes half as long again on the tensor cores:
 // 4096 x 4096 x 4096 bf16 in 120 us, 81 before.)  digits: n x ld_codes of each.

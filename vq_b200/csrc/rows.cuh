@@ -11,7 +11,7 @@
 namespace vqb {
 
 constexpr float MAGIC = 12582912.0f; // 1.5 2^23: adding it rounds to a whole number, whose two's complement is then in the low bits
-constexpr float LARGEST_8 = 127.0f, LARGEST_24 = 8323072.0f; // 127 * 65536: the first of three digits stays within 127 (127.5 would)
+constexpr float LARGEST_8 = 127.0f, LARGEST_24 = 127.0f * 65536.0f; // the first of three digits stays within 127 (127.5 would)
 
 template <typename T> struct Piece; // 16 bytes of a row
 template <> struct Piece<float> {
