@@ -321,6 +321,47 @@ int vqb_qmat_product_codes(vqb_qmat *qm, const int8_t *codes, size_t ld_codes, c
 int vqb_qmat_input_gradient(vqb_qmat *qm, const void *dy, int type, size_t n, size_t dim, size_t ld, const int64_t *offsets, void *dx, size_t dx_ld, int flags);
 int vqb_qmat_destroy(vqb_qmat *qm);
 
+/* ---- keys and values of attention in 8 bits -----------------------------------------------------------------
+ * A cache holds keys and values of tokens as int8 codes, VQB_CACHE_PAGE tokens to a page, with one f32 scale for each page and head (of keys, and of
+ * values).  Which pages a sequence has is the caller's: `table` has a row of page numbers for each sequence, token j of which is token j % 64 of page
+ * table[b][j / 64].  No counterpart in the reference.
+ *
+ * Rows of a call belong to sequences: sequence b has rows offsets[b] .. offsets[b + 1] - 1 (n / sequences each where offsets is NULL), and they are its last
+ * tokens, lengths[b] counting them: the last row has position lengths[b] - 1.  Tokens at negative positions (a length below the number of rows, as of an empty
+ * place in a batch), of columns that the table does not have, and of pages outside 0 .. pages - 1 are not there: they are not written, nobody sees
+ * them, and they read as 0.  table, lengths (int32) and offsets (int64, as of the products) may be in device memory, where the host does not look at them.
+ *
+ *   write   s = max(s_old, max |x| / 127, 2^-126) over the page's new tokens, s_old = 0 when the page's first token is among them; new codes are x / s, codes of
+ *           the page's tokens before them code s_old / s, to the nearest whole number (halves to even).  A page with nothing but zeros has s = 0, one that got an infinity or a
+ *           NaN s = NaN, until its first token is written again.  What a page holds behind the last token that was written is not defined.
+ *           No page may be written to by two sequences of one call (nothing outside the cache's pages is touched if it is).
+ *   read    code s, rounded to the type
+ *   attend  y[i] = sum_j e^(S_ij - m_i) v_j / sum_j e^(S_ij - m_i),  S_ij = scale x_i . k_j,  m_i = max_j S_ij,  over the tokens that row i sees: those up to its own
+ *           position p_i that are there and, with window > 0, have j > p_i - window or j < sinks.  Query head h reads the cache's head h / (query_heads / heads).  A row that
+ *           sees nothing is 0.  Scores, maxima and sums are f32; the codes enter the products as they are, queries as f16 numbers of 11 bits and of the row's own scale (a
+ *           power of two), e^(S - m) s_v as f16 numbers relative to the row's largest.
+ *
+ * Queries and results are f16 or bf16 (VQB_ERR_UNSUPPORTED for f32: it would promise more digits than that).  ld and head_ld: values from row to row and from head to head.
+ * Rows of no sequence (in front of offsets[0], behind the last offset) are left as they are, or become 0 with VQB_ZERO_REST; vqb_cache_read, whose results are
+ * n x heads x width without gaps, makes them 0.  Limits (VQB_ERR_UNSUPPORTED beyond): width 256, 4096 heads, 65535 sequences.  A cache is made outside of captures; the calls
+ * on it may be captured with all operands in device memory, as products may. */
+#define VQB_CACHE_PAGE 64
+typedef struct vqb_cache vqb_cache;
+int vqb_cache_create(vqb_ctx *ctx, size_t pages, size_t heads, size_t width, vqb_cache **out); /* of zeros */
+/* codes: pages x heads x 64 x width, scales: pages x heads (a negative or infinite one counts as NaN) */
+int vqb_cache_from_parts(vqb_ctx *ctx, const int8_t *key_codes, const float *key_scales, const int8_t *value_codes, const float *value_scales, size_t pages,
+                         size_t heads, size_t width, vqb_cache **out);
+int vqb_cache_shape(const vqb_cache *cache, size_t *pages, size_t *heads, size_t *width);
+int vqb_cache_parts(const vqb_cache *cache, int8_t *key_codes_out, float *key_scales_out, int8_t *value_codes_out, float *value_scales_out); /* each may be NULL */
+int vqb_cache_write(vqb_cache *cache, const void *keys, size_t keys_ld, size_t keys_head_ld, const void *values, size_t values_ld, size_t values_head_ld, int type, size_t n,
+                    size_t heads, size_t dim, const int32_t *table, size_t sequences, size_t columns, size_t table_ld, const int32_t *lengths, const int64_t *offsets);
+int vqb_cache_read(vqb_cache *cache, void *keys, void *values, int type, size_t n, const int32_t *table, size_t sequences, size_t columns, size_t table_ld,
+                   const int32_t *lengths, const int64_t *offsets);
+int vqb_cache_attend(vqb_cache *cache, const void *queries, int type, size_t n, size_t query_heads, size_t dim, size_t ld, size_t head_ld, const int32_t *table,
+                     size_t sequences, size_t columns, size_t table_ld, const int32_t *lengths, const int64_t *offsets, float scale, size_t window, size_t sinks, void *y,
+                     size_t y_ld, size_t y_head_ld, int flags);
+int vqb_cache_destroy(vqb_cache *cache);
+
 /* ---- stand-in row sampler ----------------------------------------------- */
 /* For hosts without the reference's StdRng: one SplitMix64 stream per LBG call, seeded `seed + stream` (src/pq.rs:119).
  * vqb_seeder_sample draws the initial rows of `streams` sub-spaces (streams x k indices); the other three are a

@@ -998,6 +998,271 @@ class QuantizedMatrix:
             pass
 
 
+# ---- keys and values of attention in 8 bits ------------------------------------------------------
+class _Heads:
+    """The caller's rows of heads (n x heads x width) as they are: float32, float16 or bfloat16, any distance from row to row and from head to head."""
+
+    __slots__ = ("cuda", "keep", "n", "heads", "dim", "ptr", "type", "ld", "head_ld", "stream")
+
+    def __init__(self, x, ctx, what):
+        _record_nothing(what, x)
+        torch = sys.modules.get("torch")
+        self.cuda = torch is not None and isinstance(x, torch.Tensor) and x.is_cuda
+        if self.cuda:
+            device = ctx.device
+            if x.get_device() != device:
+                raise ValueError(f"{what} is on cuda:{x.get_device()}, the context on cuda:{device}")
+            self.type = (_TORCH_VALUES or _torch_values(torch)).get(x.dtype)
+            if self.type is None:
+                raise ValueError(f"{what} must be float32, float16 or bfloat16")
+            self.stream = torch._C._cuda_getCurrentRawStream(device)
+        else:
+            if _is_torch(x):
+                x = x.detach()
+                x = (x.float() if str(x.dtype) == "torch.bfloat16" else x).numpy()
+            x = np.asarray(x)
+            if x.dtype not in (np.float32, np.float16):
+                x = x.astype(np.float16 if x.dtype.name == "float16" else np.float32)
+            x = np.ascontiguousarray(x)
+            self.type, self.stream = _VALUE_TYPES[x.dtype.name], None
+        if len(x.shape) != 3:
+            raise ValueError(f"{what}: expected rows x heads x width")
+        self.n, self.heads, self.dim = n, heads, dim = x.shape
+        self.ld, self.head_ld = heads * dim, dim
+        if self.cuda:
+            ld, head_ld, step = x.stride()
+            if n <= 1:
+                ld = self.ld
+            if heads <= 1:
+                head_ld = dim
+            inside = head_ld >= dim and ld >= (heads - 1) * head_ld + dim if heads > 1 else ld >= dim
+            if (dim > 1 and step != 1) or not (inside or (ld >= dim and head_ld >= (n - 1) * ld + dim)):
+                x = x.detach().contiguous()
+            else:
+                self.ld, self.head_ld = ld, head_ld
+            self.ptr = x.data_ptr()
+        else:
+            self.ptr = x.ctypes.data
+        self.keep = x
+
+
+def _heads_result(x: _Heads, out):
+    """(array, pointer, values from row to row, from head to head) of an attention's result, of the queries' shape and type."""
+    if out is None:
+        if x.cuda:
+            a = sys.modules["torch"].empty((x.n, x.heads, x.dim), dtype=x.keep.dtype, device=x.keep.device)
+            return a, a.data_ptr(), x.heads * x.dim, x.dim
+        a = np.empty((x.n, x.heads, x.dim), x.keep.dtype)
+        return a, a.ctypes.data, x.heads * x.dim, x.dim
+    _record_nothing("out", out)
+    if x.cuda:
+        ok = _is_torch(out) and out.is_cuda and out.get_device() == x.keep.get_device() and out.dtype is x.keep.dtype
+        strides = out.stride() if ok else ()
+        a = out
+    else:
+        a = out.detach().numpy() if _is_torch(out) and not out.is_cuda and str(out.dtype) in ("torch.float16", "torch.float32") else out
+        ok = isinstance(a, np.ndarray) and a.flags.writeable and a.dtype == x.keep.dtype and a.dtype.isnative and all(v % a.itemsize == 0 for v in a.strides)
+        strides = tuple(v // a.itemsize for v in a.strides) if ok else ()
+    n, heads, dim = x.n, x.heads, x.dim
+    ok = ok and tuple(a.shape) == (n, heads, dim) and (dim <= 1 or strides[2] == 1)
+    if ok:
+        ld, head_ld = strides[0] if n > 1 else heads * max(strides[1], dim), strides[1] if heads > 1 else dim
+        ok = (head_ld >= dim and ld >= (heads - 1) * head_ld + dim) or (ld >= dim and head_ld >= (n - 1) * ld + dim)
+    if not ok:
+        raise ValueError(f"out must be an array of the queries' type and shape {(n, heads, dim)} on their side, neither rows nor heads overlapping")
+    return out, a.data_ptr() if x.cuda else a.ctypes.data, ld, head_ld
+
+
+def _numbers(v, x, what, axes):
+    """int32 numbers that go with the rows `x`: (to keep alive, pointer, shape, numbers from row to row)."""
+    if x.cuda and _is_torch(v) and v.is_cuda:
+        if v.get_device() != x.keep.get_device():
+            raise ValueError(f"{what} is on another device than the rows")
+        if v.dtype is not sys.modules["torch"].int32:
+            raise ValueError(f"{what} must be int32")
+        shape = v.shape
+        if len(shape) == axes:
+            steps = v.stride()
+            ld = steps[0] if shape[0] > 1 else shape[-1]
+            if steps[-1] != 1 and shape[-1] > 1 or axes == 2 and ld < shape[1]:
+                v = v.contiguous()
+                ld = shape[-1]
+            return v, v.data_ptr(), shape, ld
+    else:
+        a = np.asarray(v.detach().cpu().numpy() if _is_torch(v) else v)
+        if a.size and a.dtype.kind not in "iu":
+            raise ValueError(f"{what} must be whole numbers")
+        if a.size and (a.max() > 2**31 - 1 or a.min() < -(2**31)):
+            raise ValueError(f"{what} must be numbers of 32 bits")
+        shape = a.shape
+        if len(shape) == axes:
+            a = np.ascontiguousarray(a, np.int32)
+            return a, a.ctypes.data, shape, shape[-1]
+    raise ValueError("table must be sequences x columns" if axes == 2 else f"{what} must be one number a sequence")
+
+
+class QuantizedCache:
+    """Keys and values of attention as int8 codes: pages of 64 tokens, with a scale for each page and head of the keys, and one of the values.
+
+    Which pages a sequence has is the caller's business: `table` (sequences x columns of page numbers, int32) says that token j of sequence b is token j % 64 of
+    page ``table[b][j // 64]``, -1 that there is none.  The rows of a call are the last tokens of its sequences, which `lengths` (int32, one a sequence) counts: a step
+    writes its new keys and values and lets their queries attend, all three with the same `table`, `lengths` and `offsets`.  With `offsets` (sequences + 1
+    ascending row numbers, int64) sequence b has the rows offsets[b] .. offsets[b + 1] - 1, without it every sequence has equally many.  All three
+    are best where the rows are, and have to be there in a captured call; in GPU memory nobody looks at them on the host.
+
+    Tokens at negative positions (a length of 0: an empty place of a batch), of columns that the table does not have and of pages that the cache does not have are not
+    there: they are not written, nobody sees them, and they read as 0.
+
+    Serving only: torch does not record these calls, and an operand that requires a gradient is refused while torch records."""
+
+    PAGE = 64
+
+    def __init__(self, handle, ctx: Context):
+        self._h, self._ctx = handle, ctx
+        p, h, w = C.c_size_t(), C.c_size_t(), C.c_size_t()
+        _lib.load().vqb_cache_shape(handle, C.byref(p), C.byref(h), C.byref(w))
+        self._shape = int(p.value), int(h.value), int(w.value)
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, width: int, *, ctx: Context | None = None):
+        """A cache of zeros."""
+        if min(pages, heads, width) < 0:
+            raise ValueError("pages, heads and width must be positive")
+        ctx = ctx or default_context()
+        h = C.c_void_p()
+        ctx.call(None, _lib.load().vqb_cache_create, ctx.handle, pages, heads, width, C.byref(h))
+        return cls(h, ctx)
+
+    @classmethod
+    def from_parts(cls, key_codes, key_scales, value_codes, value_scales, *, ctx: Context | None = None):
+        """A cache of given codes (pages x heads x 64 x width, int8) and scales (pages x heads, float32; a negative or infinite one counts as NaN)."""
+        ctx = ctx or _context_of(key_codes)
+        shape = tuple(key_codes.shape)
+        if len(shape) != 4 or shape[2] != cls.PAGE or tuple(value_codes.shape) != shape:
+            raise ValueError("expected pages x heads x 64 x width codes of keys and of values")
+        pages, heads, _, width = shape
+        parts = []
+        for what, codes, scales in (("key_codes", key_codes, key_scales), ("value_codes", value_codes, value_scales)):
+            x = _Values(codes.reshape(pages * heads * cls.PAGE, width), ctx, what, integers=True)
+            if x.ld != x.dim:
+                x = _Values(x.keep.contiguous(), ctx, what, integers=True)
+            parts += [x, _beside(scales, x, "float32", (pages, heads), "scales")]
+        (k, (ks, ksptr), v, (vs, vsptr)), h = parts, C.c_void_p()
+        ctx.call(k if k.cuda else v, _lib.load().vqb_cache_from_parts, ctx.handle, k.ptr, ksptr, v.ptr, vsptr, pages, heads, width, C.byref(h))
+        return cls(h, ctx)
+
+    def shape(self):
+        """(pages, heads, width)"""
+        return self._shape
+
+    def _part(self, which):
+        p, h, w = self._shape
+        out = np.empty((p, h), np.float32) if which % 2 else np.empty((p, h, self.PAGE, w), np.int8)
+        self._ctx.call(None, _lib.load().vqb_cache_parts, self._h, *(out.ctypes.data if which == i else None for i in range(4)))
+        return out
+
+    @property
+    def key_codes(self) -> np.ndarray:
+        return self._part(0)
+
+    @property
+    def key_scales(self) -> np.ndarray:
+        return self._part(1)
+
+    @property
+    def value_codes(self) -> np.ndarray:
+        return self._part(2)
+
+    @property
+    def value_scales(self) -> np.ndarray:
+        return self._part(3)
+
+    def _sequences(self, x, table, lengths, offsets):
+        """(to keep alive, the library's arguments): `x` says where the rows are."""
+        t, tptr, shape, ld = _numbers(table, x, "table", 2)
+        n, nptr, many, _ = _numbers(lengths, x, "lengths", 1)
+        sequences, columns = shape
+        if many[0] != sequences:
+            raise ValueError(f"lengths must have shape {(sequences,)}, not {tuple(many)}")
+        o, optr = (None, None) if offsets is None else _beside(offsets, x, "int64", (sequences + 1,), "offsets")
+        return (t, n, o), (tptr, sequences, columns, ld, nptr, optr)
+
+    def _call(self, x, fn, *args):
+        ctx = self._ctx
+        with ctx._lock:
+            if x.stream != ctx._stream:
+                ctx._run_on(x.stream)
+            rc = fn(self._h, *args)
+            if rc:
+                _raise(rc, ctx.handle)
+
+    def write(self, keys, values, table, lengths, *, offsets=None):
+        """Writes the rows (n x heads x width each) into their pages, `lengths` counting them.
+
+        The codes are whole numbers of the page's and head's scale: a 127th of the largest magnitude that was written to it since its first token.  Where that grows, the codes
+        of the page's older tokens are rounded to the new scale.  An infinity or a NaN makes its page and head NaN until the page's first token is written again."""
+        k, v = _Heads(keys, self._ctx, "keys"), _Heads(values, self._ctx, "values")
+        if (v.n, v.heads, v.dim) != (k.n, k.heads, k.dim) or v.type != k.type or v.cuda != k.cuda:
+            raise ValueError("keys and values must have the same shape and type, on the same side")
+        keep, sequences = self._sequences(k, table, lengths, offsets)
+        self._call(k, self._ctx._L.vqb_cache_write, k.ptr, k.ld, k.head_ld, v.ptr, v.ld, v.head_ld, k.type, k.n, k.heads, k.dim, *sequences)
+
+    def read(self, table, lengths, rows: int, *, offsets=None, dtype=None):
+        """(keys, values) of the last tokens of every sequence, `rows` in all: rows x heads x width of `dtype` (float32 by default), on the table's side."""
+        rows = int(rows)
+        if rows < 0:
+            raise ValueError("rows must not be negative")
+        shape, torch = (rows,) + self._shape[1:], sys.modules.get("torch")
+        name = _type_name(dtype or np.float32)
+        cuda = torch is not None and isinstance(table, torch.Tensor) and table.is_cuda
+        if name not in _VALUE_TYPES or (name == "bfloat16" and not cuda):
+            raise ValueError(f"a result of {name} is not offered" + ("" if cuda else " for tables in host memory"))
+        x = _Side()
+        if cuda:
+            if table.get_device() != self._ctx.device:
+                raise ValueError(f"table is on cuda:{table.get_device()}, the context on cuda:{self._ctx.device}")
+            k = torch.empty(shape, dtype=getattr(torch, name), device=table.device)
+            v = torch.empty_like(k)
+            x.cuda, x.keep, x.stream, kptr, vptr = True, k, torch._C._cuda_getCurrentRawStream(self._ctx.device), k.data_ptr(), v.data_ptr()
+        else:
+            k, v = np.empty(shape, name), np.empty(shape, name)
+            x.cuda, x.keep, x.stream, kptr, vptr = False, k, None, k.ctypes.data, v.ctypes.data
+        keep, sequences = self._sequences(x, table, lengths, offsets)
+        self._call(x, self._ctx._L.vqb_cache_read, kptr, vptr, _VALUE_TYPES[name], rows, *sequences)
+        return k, v
+
+    def attend(self, queries, table, lengths, *, offsets=None, scale: float | None = None, window: int | None = None, sinks: int = 0, out=None):
+        """Causal attention of the rows (n x query heads x width, float16 or bfloat16) over their sequences' cached tokens: n x query heads x width of their type.
+
+        Query head h reads the cache's head ``h // (query heads // heads)``.  A row sees the tokens up to its own; with `window` only the last so many of
+        them, itself among these, and the first `sinks` ones.  `scale` multiplies the scores (width ** -0.5 by default).  A row that sees nothing
+        comes out as 0; rows of no sequence do in a fresh result and stay as they are in the caller's `out`."""
+        x = _Heads(queries, self._ctx, "queries")
+        if window is not None and window < 1:
+            raise ValueError("window must be positive, or None")
+        if sinks < 0:
+            raise ValueError("sinks must not be negative")
+        y, yptr, y_ld, y_head_ld = _heads_result(x, out)
+        keep, sequences = self._sequences(x, table, lengths, offsets)
+        self._call(x, self._ctx._L.vqb_cache_attend, x.ptr, x.type, x.n, x.heads, x.dim, x.ld, x.head_ld, *sequences, self._shape[2] ** -0.5 if scale is None else scale,
+                   window or 0, sinks, yptr, y_ld, y_head_ld, 1 if out is None else 0)
+        return y
+
+    def __del__(self):
+        try:
+            if self._h:
+                _lib.load().vqb_cache_destroy(self._h)
+                self._h = None
+        except Exception:
+            pass
+
+
+class _Side:
+    """Where a call's results are, for what goes with them."""
+
+    __slots__ = ("cuda", "keep", "stream")
+
+
 class TSVQ:
     """TSVQ (src/tsvq.rs:189-250): ``TSVQ(training_data, max_depth, distance)`` builds the tree, ``quantize`` returns the
     leaf centroid as f16.  ``tree()`` gives (centroids, left, right) with nodes numbered breadth-first."""

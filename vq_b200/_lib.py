@@ -88,6 +88,14 @@ SIGNATURES = {
     "vqb_qmat_product_codes": (C.c_int, [_P, _P, _SZ, _P, _SZ, _SZ, _P, _P, _P, C.c_int, _SZ, C.c_int]),
     "vqb_qmat_input_gradient": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, _P, _P, _SZ, C.c_int]),
     "vqb_qmat_destroy": (C.c_int, [_P]),
+    "vqb_cache_create": (C.c_int, [_P, _SZ, _SZ, _SZ, C.POINTER(_P)]),
+    "vqb_cache_from_parts": (C.c_int, [_P, _P, _P, _P, _P, _SZ, _SZ, _SZ, C.POINTER(_P)]),
+    "vqb_cache_shape": (C.c_int, [_P, C.POINTER(_SZ), C.POINTER(_SZ), C.POINTER(_SZ)]),
+    "vqb_cache_parts": (C.c_int, [_P, _P, _P, _P, _P]),
+    "vqb_cache_write": (C.c_int, [_P, _P, _SZ, _SZ, _P, _SZ, _SZ, C.c_int, _SZ, _SZ, _SZ, _P, _SZ, _SZ, _SZ, _P, _P]),
+    "vqb_cache_read": (C.c_int, [_P, _P, _P, C.c_int, _SZ, _P, _SZ, _SZ, _SZ, _P, _P]),
+    "vqb_cache_attend": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, _SZ, _SZ, _P, _SZ, _SZ, _SZ, _P, _P, C.c_float, _SZ, _SZ, _P, _SZ, _SZ, C.c_int]),
+    "vqb_cache_destroy": (C.c_int, [_P]),
     "vqb_seeder_create": (C.c_int, [C.c_uint64, C.POINTER(_P)]),
     "vqb_seeder_destroy": (C.c_int, [_P]),
     "vqb_seeder_sample": (C.c_int, [_P, _SZ, C.c_uint64, _SZ, _P]),

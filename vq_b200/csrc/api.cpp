@@ -4,6 +4,7 @@
 // src/rvq.rs:96-98; src/sq.rs:51-68; src/bq.rs:47-54; src/exceptions.rs).  Host pointers are staged
 // through device buffers; device pointers are used in place.
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <new>
@@ -11,6 +12,7 @@
 #include <vector>
 
 #include "../../include/vqb.h"
+#include "cache.hpp"
 #include "call_lock.hpp"
 #include "cuda_device.hpp"
 #include "opq_parts.hpp"
@@ -59,6 +61,11 @@ struct vqb_tsvq {
 struct vqb_qmat {
     vqb_ctx *ctx;
     Qmat mat;
+};
+
+struct vqb_cache {
+    vqb_ctx *ctx;
+    Cache cache;
 };
 
 struct vqb_opq {
@@ -404,9 +411,9 @@ struct RowsOut {
 };
 
 // Ahead of anything that would become part of the graph.
-void check_not_captured(CudaDevice &dev)
+void check_not_captured(CudaDevice &dev, const char *what = "a matrix")
 {
-    if (dev.capturing()) throw Error(VQB_ERR_UNSUPPORTED, "a matrix cannot be made while its stream is being captured");
+    if (dev.capturing()) throw Error(VQB_ERR_UNSUPPORTED, std::string(what) + " cannot be made while its stream is being captured");
 }
 
 void check_qmat_shape(size_t groups, size_t outputs, size_t inputs, int flags)
@@ -470,6 +477,100 @@ void check_product(const Qmat &m, size_t n, size_t dim, const float *bias, void 
     if (n) check_values("y", y, y_type, m.outputs, y_ld);
     check_words("bias", bias, sizeof(float));
 }
+
+void check_cache_shape(size_t pages, size_t heads, size_t width)
+{
+    if (pages == 0 || heads == 0 || width == 0) throw Error(VQB_ERR_EMPTY_INPUT, "Empty input: at least one vector is required.");
+    if (width > CACHE_MOST_WIDTH) throw Error(VQB_ERR_UNSUPPORTED, "heads of more than 256 values");
+    if (heads > CACHE_MOST_HEADS) throw Error(VQB_ERR_UNSUPPORTED, "more than 4096 heads");
+    if (pages > CACHE_MOST_PAGES / heads) throw Error(VQB_ERR_UNSUPPORTED, "more than 2^31 - 1 pages of all heads");
+}
+
+// A cache of zeros; what is left of it when something fails is released.
+struct NewCache {
+    CudaDevice &dev;
+    std::unique_ptr<vqb_cache> made;
+    NewCache(vqb_ctx *ctx, size_t pages, size_t heads, size_t width) : dev(*ctx->dev), made(new vqb_cache{ctx, Cache{}})
+    {
+        Cache &c = made->cache;
+        c.pages = pages, c.heads = heads, c.width = width, c.padded = (width + 31) / 32 * 32;
+        try {
+            c.codes = static_cast<uint8_t *>(dev.alloc(c.code_bytes()));
+            c.scales = static_cast<float *>(dev.alloc(c.scale_bytes()));
+            dev.zero(c.codes, c.code_bytes());
+            dev.zero(c.scales, c.scale_bytes());
+        } catch (...) {
+            drop();
+            throw;
+        }
+    }
+    void drop()
+    {
+        if (!made) return;
+        dev.release(made->cache.codes), dev.release(made->cache.scales);
+        made.reset();
+    }
+    vqb_cache *done()
+    {
+        dev.synchronize();
+        return made.release();
+    }
+    ~NewCache() { drop(); }
+};
+
+// Rows of heads: neither rows nor heads overlap, whichever of the two is the outer one.
+void check_heads(const char *what, const void *p, int type, size_t n, size_t heads, size_t width, size_t ld, size_t head_ld)
+{
+    check_values(what, p, type, 1, 1);
+    constexpr size_t FAR = size_t(1) << 40; // (values; no product below leaves 64 bits)
+    if ((n > 1 && ld > FAR) || (heads > 1 && head_ld > FAR / 4096)) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + ": rows are too far apart");
+    const bool heads_inside = (heads == 1 || head_ld >= width) && (n == 1 || ld >= (heads - 1) * head_ld + width);
+    const bool rows_inside = (n == 1 || ld >= width) && (heads == 1 || (head_ld >= width && (head_ld - width) / std::max<size_t>(ld, 1) >= n - 1));
+    if (!heads_inside && !rows_inside) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + ": rows or heads overlap");
+}
+size_t heads_span(int type, size_t n, size_t heads, size_t width, size_t ld, size_t head_ld)
+{
+    return n ? ((n - 1) * ld + (heads - 1) * head_ld + width) * value_bytes(type) : 0;
+}
+
+// The arguments that say which tokens a call's rows are, in device memory for as long as the call lasts.
+struct SequencesIn {
+    Sequences s;
+    CallIn table, lengths;
+    OffsetsIn offsets;
+    SequencesIn(CudaDevice &dev, const int32_t *table_, size_t sequences, size_t columns, size_t table_ld, const int32_t *lengths_, const int64_t *offsets_, size_t n)
+        : table(dev, "table", checked(table_, sequences, columns, table_ld, lengths_, offsets_, n), columns ? span(sequences, columns, table_ld, sizeof(int32_t)) : 0),
+          lengths(dev, "lengths", lengths_, sequences * sizeof(int32_t)), offsets(dev, offsets_, offsets_ ? sequences : 1, n)
+    {
+        s.table = table.as<int32_t>(), s.table_ld = table_ld, s.sequences = (int)sequences, s.columns = (int)columns;
+        s.lengths = lengths.as<int32_t>(), s.offsets = reinterpret_cast<const long long *>(offsets.get()), s.n = (int)n;
+    }
+    static const int32_t *checked(const int32_t *table, size_t sequences, size_t columns, size_t table_ld, const int32_t *lengths, const int64_t *offsets, size_t n)
+    {
+        check_row_count(n);
+        if (sequences == 0) throw Error(VQB_ERR_EMPTY_INPUT, "Empty input: at least one vector is required.");
+        if (sequences > CACHE_MOST_SEQUENCES) throw Error(VQB_ERR_UNSUPPORTED, "more than 65535 sequences");
+        if (columns > CACHE_MOST_COLUMNS) throw Error(VQB_ERR_UNSUPPORTED, "more than 2^25 - 1 columns of pages");
+        if ((columns && !table) || !lengths) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
+        if (sequences > 1 && table_ld < columns) throw Error(VQB_ERR_BAD_ARGUMENT, "table: rows overlap");
+        if (sequences > 1 && table_ld > (size_t(1) << 40)) throw Error(VQB_ERR_BAD_ARGUMENT, "table: rows are too far apart");
+        check_words("table", table, sizeof(int32_t));
+        check_words("lengths", lengths, sizeof(int32_t));
+        if (!offsets && n % sequences) throw Error(VQB_ERR_INVALID_PARAMETER, "Invalid parameter: the rows are not the same number for each sequence: offsets are needed");
+        return table;
+    }
+};
+
+// Rows of heads that a call fills.  Host memory that it does not write all of is brought in first.
+struct HeadsOut {
+    Out out;
+    HeadsOut(CudaDevice &dev, const char *what, void *y, int type, size_t n, size_t heads, size_t width, size_t ld, size_t head_ld, bool all)
+        : out(dev, y, heads_span(type, n, heads, width, ld, head_ld), what)
+    {
+        if (out.host && (!all || n * heads * width * value_bytes(type) != out.bytes))
+            VQB_CUDA_CHECK(cudaMemcpyAsync(out.d, out.host, out.bytes, cudaMemcpyHostToDevice, dev.stream()));
+    }
+};
 
 void check_minkowski(int metric, double p)
 {
@@ -1500,6 +1601,153 @@ int vqb_qmat_destroy(vqb_qmat *qm)
         ctx->dev->release_later(qm->mat.turned);
     });
     delete qm;
+    return VQB_OK;
+}
+
+int vqb_cache_create(vqb_ctx *ctx, size_t pages, size_t heads, size_t width, vqb_cache **out)
+{
+    if (!ctx) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "ctx is NULL");
+    return locked(ctx, [&] {
+        if (!out) throw Error(VQB_ERR_BAD_ARGUMENT, "out is NULL");
+        *out = nullptr;
+        check_cache_shape(pages, heads, width);
+        check_not_captured(*ctx->dev, "a cache");
+        *out = NewCache(ctx, pages, heads, width).done();
+    });
+}
+
+int vqb_cache_from_parts(vqb_ctx *ctx, const int8_t *key_codes, const float *key_scales, const int8_t *value_codes, const float *value_scales, size_t pages,
+                         size_t heads, size_t width, vqb_cache **out)
+{
+    if (!ctx) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "ctx is NULL");
+    return locked(ctx, [&] {
+        if (!out) throw Error(VQB_ERR_BAD_ARGUMENT, "out is NULL");
+        *out = nullptr;
+        check_cache_shape(pages, heads, width);
+        if (!key_codes || !key_scales || !value_codes || !value_scales) throw Error(VQB_ERR_BAD_ARGUMENT, "NULL data pointer");
+        check_words("key scales", key_scales, sizeof(float));
+        check_words("value scales", value_scales, sizeof(float));
+        CudaDevice &dev = *ctx->dev;
+        check_not_captured(dev, "a cache");
+        NewCache made(ctx, pages, heads, width);
+        const int8_t *codes[2] = {key_codes, value_codes};
+        const float *scales[2] = {key_scales, value_scales};
+        for (int which = 0; which < 2; ++which) {
+            In ic(dev, codes[which], pages * heads * CACHE_PAGE * width), is(dev, scales[which], sizeof(float) * pages * heads);
+            launch_cache_pages_in(dev, made.made->cache, which, ic.as<int8_t>(), is.as<float>());
+        }
+        *out = made.done();
+    });
+}
+
+int vqb_cache_shape(const vqb_cache *cache, size_t *pages, size_t *heads, size_t *width)
+{
+    if (!cache) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "cache is NULL");
+    if (pages) *pages = cache->cache.pages;
+    if (heads) *heads = cache->cache.heads;
+    if (width) *width = cache->cache.width;
+    return VQB_OK;
+}
+
+int vqb_cache_parts(const vqb_cache *cache, int8_t *key_codes_out, float *key_scales_out, int8_t *value_codes_out, float *value_scales_out)
+{
+    if (!cache) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "cache is NULL");
+    vqb_ctx *ctx = cache->ctx;
+    return locked(ctx, [&] {
+        CudaDevice &dev = *ctx->dev;
+        const Cache &c = cache->cache;
+        int8_t *codes[2] = {key_codes_out, value_codes_out};
+        float *scales[2] = {key_scales_out, value_scales_out};
+        check_words("key scales", key_scales_out, sizeof(float));
+        check_words("value scales", value_scales_out, sizeof(float));
+        for (int which = 0; which < 2; ++which) {
+            if (!codes[which] && !scales[which]) continue;
+            Out oc(dev, codes[which], c.pages * c.heads * CACHE_PAGE * c.width, "codes"), os(dev, scales[which], sizeof(float) * c.pages * c.heads, "scales");
+            launch_cache_pages_out(dev, c, which, oc.as<int8_t>(), os.as<float>());
+            finish(oc, os);
+        }
+    });
+}
+
+int vqb_cache_write(vqb_cache *cache, const void *keys, size_t keys_ld, size_t keys_head_ld, const void *values, size_t values_ld, size_t values_head_ld, int type, size_t n,
+                    size_t heads, size_t dim, const int32_t *table, size_t sequences, size_t columns, size_t table_ld, const int32_t *lengths, const int64_t *offsets)
+{
+    if (!cache) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "cache is NULL");
+    vqb_ctx *ctx = cache->ctx;
+    return locked(ctx, [&] {
+        const Cache &c = cache->cache;
+        CudaDevice &dev = *ctx->dev;
+        if (heads != c.heads) throw Error(VQB_ERR_DIMENSION_MISMATCH, dim_mismatch(c.heads, heads));
+        if (dim != c.width) throw Error(VQB_ERR_DIMENSION_MISMATCH, dim_mismatch(c.width, dim));
+        SequencesIn in(dev, table, sequences, columns, table_ld, lengths, offsets, n);
+        if (n == 0) return;
+        check_heads("keys", keys, type, n, heads, dim, keys_ld, keys_head_ld);
+        check_heads("values", values, type, n, heads, dim, values_ld, values_head_ld);
+        CallIn ik(dev, "keys", keys, heads_span(type, n, heads, dim, keys_ld, keys_head_ld)), iv(dev, "values", values, heads_span(type, n, heads, dim, values_ld, values_head_ld));
+        launch_cache_write(dev, c, in.s, HeadRows{const_cast<void *>(ik.d), type, keys_ld, keys_head_ld}, HeadRows{const_cast<void *>(iv.d), type, values_ld, values_head_ld});
+    });
+}
+
+int vqb_cache_read(vqb_cache *cache, void *keys, void *values, int type, size_t n, const int32_t *table, size_t sequences, size_t columns, size_t table_ld,
+                   const int32_t *lengths, const int64_t *offsets)
+{
+    if (!cache) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "cache is NULL");
+    vqb_ctx *ctx = cache->ctx;
+    return locked(ctx, [&] {
+        const Cache &c = cache->cache;
+        CudaDevice &dev = *ctx->dev;
+        SequencesIn in(dev, table, sequences, columns, table_ld, lengths, offsets, n);
+        if (n == 0) return;
+        const size_t ld = c.heads * c.width;
+        check_heads("keys", keys, type, n, c.heads, c.width, ld, c.width);
+        check_heads("values", values, type, n, c.heads, c.width, ld, c.width);
+        HeadsOut ok(dev, "keys", keys, type, n, c.heads, c.width, ld, c.width, true), ov(dev, "values", values, type, n, c.heads, c.width, ld, c.width, true);
+        launch_cache_read(dev, c, in.s, HeadRows{ok.out.d, type, ld, c.width}, HeadRows{ov.out.d, type, ld, c.width});
+        finish(ok.out, ov.out);
+    });
+}
+
+int vqb_cache_attend(vqb_cache *cache, const void *queries, int type, size_t n, size_t query_heads, size_t dim, size_t ld, size_t head_ld, const int32_t *table,
+                     size_t sequences, size_t columns, size_t table_ld, const int32_t *lengths, const int64_t *offsets, float scale, size_t window, size_t sinks, void *y,
+                     size_t y_ld, size_t y_head_ld, int flags)
+{
+    if (!cache) return set_err(nullptr, VQB_ERR_BAD_ARGUMENT, "cache is NULL");
+    vqb_ctx *ctx = cache->ctx;
+    return locked(ctx, [&] {
+        const Cache &c = cache->cache;
+        CudaDevice &dev = *ctx->dev;
+        if (dim != c.width) throw Error(VQB_ERR_DIMENSION_MISMATCH, dim_mismatch(c.width, dim));
+        if (query_heads == 0 || query_heads % c.heads) throw Error(VQB_ERR_INVALID_PARAMETER, "Invalid parameter: the query heads must be a multiple of the cache's heads");
+        if (query_heads > CACHE_MOST_HEADS) throw Error(VQB_ERR_UNSUPPORTED, "more than 4096 query heads");
+        if (type == VQB_F32) throw Error(VQB_ERR_UNSUPPORTED, "queries are f16 or bf16");
+        if (!std::isfinite(scale)) throw Error(VQB_ERR_INVALID_PARAMETER, "Invalid parameter: the scores' scale must be finite");
+        if (flags & ~VQB_ZERO_REST) throw Error(VQB_ERR_BAD_ARGUMENT, "unknown flag");
+        SequencesIn in(dev, table, sequences, columns, table_ld, lengths, offsets, n);
+        if (n == 0) return;
+        if (n > CACHE_MOST_PAGES / query_heads) throw Error(VQB_ERR_UNSUPPORTED, "more than 2^31 - 1 rows of all query heads");
+        check_heads("queries", queries, type, n, query_heads, dim, ld, head_ld);
+        check_heads("y", y, type, n, query_heads, dim, y_ld, y_head_ld);
+        CallIn iq(dev, "queries", queries, heads_span(type, n, query_heads, dim, ld, head_ld));
+        HeadsOut oy(dev, "y", y, type, n, query_heads, dim, y_ld, y_head_ld, !offsets || (flags & VQB_ZERO_REST));
+        Attend a;
+        a.cache = c, a.seq = in.s, a.group = (int)(query_heads / c.heads), a.scale = scale;
+        a.queries = HeadRows{const_cast<void *>(iq.d), type, ld, head_ld}, a.y = HeadRows{oy.out.d, type, y_ld, y_head_ld};
+        a.window = (int)std::min<size_t>(window, (size_t(1) << 31) - 1), a.sinks = (int)std::min<size_t>(sinks, (size_t(1) << 31) - 1);
+        a.zero_rest = (flags & VQB_ZERO_REST) != 0;
+        launch_attend(dev, a);
+        oy.out.finish();
+    });
+}
+
+int vqb_cache_destroy(vqb_cache *cache)
+{
+    if (!cache) return VQB_OK;
+    vqb_ctx *ctx = cache->ctx;
+    destroyed(ctx, [&] {
+        ctx->dev->release_later(cache->cache.codes);
+        ctx->dev->release_later(cache->cache.scales);
+    });
+    delete cache;
     return VQB_OK;
 }
 

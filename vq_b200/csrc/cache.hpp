@@ -1,0 +1,66 @@
+// cache.hpp -- keys and values of attention as 8-bit codes: pages of 64 tokens, one scale for each page and head.
+//
+// cache.cu writes tokens into pages, reads them back and lays pages out; attend.cu computes attention over them.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+#include "qmat.hpp"
+
+namespace vqb {
+
+constexpr int CACHE_PAGE = 64;
+constexpr size_t CACHE_MOST_WIDTH = 256;
+constexpr size_t CACHE_MOST_HEADS = 4096, CACHE_MOST_SEQUENCES = 65535;
+constexpr size_t CACHE_MOST_PAGES = (size_t(1) << 31) - 1;
+constexpr size_t CACHE_MOST_COLUMNS = (size_t(1) << 25) - 1; // (positions of tokens are 32-bit numbers)
+
+// Of page p and head h: 64 rows of `padded` bytes, a token's key each, and behind them `padded` rows of 64 bytes, a dimension's value in each token.  (Both as
+// the tensor cores' operands want them: what is summed over lies side by side.)  Keys' and values' bytes of the dimensions behind `width` are 0.
+struct Cache {
+    size_t pages = 0, heads = 0, width = 0;
+    size_t padded = 0;         // width to the next multiple of 32
+    uint8_t *codes = nullptr;  // pages x heads x 2 x 64 x padded
+    float *scales = nullptr;   // pages x heads x 2
+    size_t code_bytes() const { return pages * heads * 2 * CACHE_PAGE * padded; }
+    size_t scale_bytes() const { return pages * heads * 2 * sizeof(float); }
+};
+
+// Which tokens of which pages the rows of a call are.  Sequence b has rows offsets[b] .. offsets[b + 1] - 1 of the n (n / sequences each where offsets is null), and they
+// are its last tokens: the last one has position lengths[b] - 1.  Position j is token j % 64 of page table[b][j / 64].  Tokens at negative positions, of columns that the table does
+// not have, or of pages that the cache does not have are not there.
+struct Sequences {
+    const int32_t *table = nullptr; // sequences x table_ld
+    size_t table_ld = 0;
+    int sequences = 0, columns = 0;
+    const int32_t *lengths = nullptr;
+    const long long *offsets = nullptr;
+    int n = 0;
+};
+
+// Values of n rows x heads x width, each head's next to each other.
+struct HeadRows {
+    void *x = nullptr;
+    int type = VALUE_F32;
+    size_t ld = 0, head_ld = 0; // values from row to row, from head to head
+};
+
+void launch_cache_write(CudaDevice &dev, const Cache &c, const Sequences &s, const HeadRows &keys, const HeadRows &values);
+void launch_cache_read(CudaDevice &dev, const Cache &c, const Sequences &s, const HeadRows &keys, const HeadRows &values);
+// natural: pages x heads x 64 x width, of keys (which = 0) or values (1); scales: pages x heads
+void launch_cache_pages_in(CudaDevice &dev, const Cache &c, int which, const int8_t *natural, const float *scales);
+void launch_cache_pages_out(CudaDevice &dev, const Cache &c, int which, int8_t *natural, float *scales);
+
+struct Attend {
+    Cache cache;
+    Sequences seq;
+    HeadRows queries, y;
+    int group = 1;      // query heads to a key head
+    float scale = 1.0f; // of the scores
+    int window = 0;     // 0: none
+    int sinks = 0;
+    bool zero_rest = false; // rows of no sequence become 0
+};
+void launch_attend(CudaDevice &dev, const Attend &a);
+
+} // namespace vqb
