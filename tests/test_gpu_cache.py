@@ -2,8 +2,8 @@
 
 Tolerances.  Codes, scales and what is read back are the definition's, bit for bit.  Attention: a score is a sum of `width` products in f32, off by at most
 (width + 8) 2^-23 of the products' magnitudes (tensor cores may cut off where others round), and that much of itself is what e^score is off, with 2^-21 for the exponential and 2^-22 of
-the scores' distance from the largest for its argument; e^(S - m) s_v is an f16 number, 2^-12 off, or 2^-25 of the largest; sums over n tokens are off by (n + 64) 2^-23 of
-their magnitudes.  The result's own rounding is half a step of its type."""
+the scores' distance from the largest for its argument; e^(S - m) s_v is an f16 number of the row's largest, which is between 1/2 and 1: its eleven bits are off by half a step, eps / 2 =
+2^-11 of it, or, below 2^-14, by half of 2^-24, which is 2^-24 of the largest; sums over n tokens are off by (n + 64) 2^-23 of their magnitudes.  The result's own rounding is half a step of its type."""
 import math
 import threading
 
@@ -147,8 +147,8 @@ def attend64(parts, queries, table, lengths, offsets, scale=None, window=None, s
             vh = torch.where(seen.any(0)[:, None], v[:, h], 0.0)
             z = p @ vh
             far = torch.where(mask, (S - m).abs(), 0.0)
-            eps = p * (2.0**-12 + 2.0**-21 + (width + 8) * 2.0**-23 * A + 2.0**-22 * far + (keys + 64) * 2.0**-23)
-            small = (p * sv[:, h].abs()).amax(-1, keepdim=True) * 2.0**-25 * 128 * keys  # weights of 2^-25 of the largest times codes
+            eps = p * (2.0**-11 + 2.0**-21 + (width + 8) * 2.0**-23 * A + 2.0**-22 * far + (keys + 64) * 2.0**-23)
+            small = (p * sv[:, h].abs()).amax(-1, keepdim=True) * 2.0**-24 * 128 * keys  # weights off by 2^-24 of the largest, times codes
             y[r0:r1, h * group : (h + 1) * group] = z
             limit[r0:r1, h * group : (h + 1) * group] = eps @ vh.abs() + z.abs() * eps.sum(-1, keepdim=True) + small
     return y, limit

@@ -497,7 +497,7 @@ struct NewCache {
         try {
             c.codes = static_cast<uint8_t *>(dev.alloc(c.code_bytes()));
             c.scales = static_cast<float *>(dev.alloc(c.scale_bytes()));
-            dev.zero(c.codes, c.code_bytes());
+            VQB_CUDA_CHECK(cudaMemsetAsync(c.codes, Cache::ZERO, c.code_bytes(), dev.stream()));
             dev.zero(c.scales, c.scale_bytes());
         } catch (...) {
             drop();

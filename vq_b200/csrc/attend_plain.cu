@@ -1,8 +1,8 @@
-// attend.cu -- attention over a cache of 8-bit codes.
+// attend_plain.cu -- attention over a cache of 8-bit codes on the CUDA cores, which VQB_NO_TENSOR=1 selects.
 //
 //   y_i = sum_j e^(S_ij - m_i) s_v v_j / sum_j e^(S_ij - m_i),  S_ij = scale (x_i . k_j) s_k,  over the tokens j that row i sees
 //
-// A warp for each row and query head.
+// A warp for each row and query head.  s_v enters with its exponent in the power: values of pages whose scales are far apart keep their weights.
 #include <algorithm>
 
 #include "cache.cuh"
@@ -14,7 +14,7 @@ namespace {
 
 constexpr int THREADS = 256;
 
-__global__ void __launch_bounds__(THREADS) attend_kernel(const Attend P)
+__global__ void __launch_bounds__(THREADS) attend_plain_kernel(const Attend P)
 {
     cache_is_there();
     const Cache &c = P.cache;
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const Attend P)
             for (int d = lane; d < width; d += 32) put_value(P.y, yo + d, 0.0f);
         return;
     }
-    const int position = span.first + r - span.row, last = min(position, span.keys - 1), begin = P.window ? max(position - P.window + 1, 0) : 0;
+    const int position = span.first + r - span.row, last = min(position, span.keys - 1), begin = P.window ? max(max(position, 0) - P.window + 1, 0) : 0;
     float x[8], y[8] = {};
 #pragma unroll
     for (int d = 0; d < 8; ++d) x[d] = lane + 32 * d < width ? value_at(P.queries, xo + lane + 32 * d) : 0.0f;
@@ -43,13 +43,13 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const Attend P)
         const int p = page_of(P.seq, c.pages, i, j / CACHE_PAGE);
         if (p < 0) continue;
         const size_t part = (size_t)p * c.heads + h;
-        const int8_t *codes = reinterpret_cast<const int8_t *>(c.codes) + part * 2 * CACHE_PAGE * padded, *k = codes + (j % CACHE_PAGE) * padded;
-        const int8_t *v = codes + CACHE_PAGE * padded + j % CACHE_PAGE;
+        const uint8_t *codes = c.codes + part * 2 * CACHE_PAGE * padded, *v = codes + CACHE_PAGE * padded + j % CACHE_PAGE;
+        const int t = j % CACHE_PAGE;
         const float ks = c.scales[2 * part], vs = c.scales[2 * part + 1];
         float s = 0.0f;
 #pragma unroll
         for (int d = 0; d < 8; ++d)
-            if (32 * d < padded) s = fmaf(x[d], (float)k[lane + 32 * d], s);
+            if (32 * d < padded) s = fmaf(x[d], (float)((int)codes[key_at(padded, t, lane + 32 * d)] - 128), s);
 #pragma unroll
         for (int o = 16; o; o /= 2) s += __shfl_xor_sync(~0u, s, o);
         s *= ks * P.scale;
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const Attend P)
         top = higher;
 #pragma unroll
         for (int d = 0; d < 8; ++d)
-            if (32 * d < padded) y[d] = fmaf(w, (float)v[(lane + 32 * d) * CACHE_PAGE], y[d] * old);
+            if (32 * d < padded) y[d] = fmaf(w, (float)((int)v[(lane + 32 * d) * CACHE_PAGE] - 128), y[d] * old);
     }
 #pragma unroll
     for (int d = 0; d < 8; ++d)
@@ -71,11 +71,11 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const Attend P)
 
 } // namespace
 
-void launch_attend(CudaDevice &dev, const Attend &a)
+void launch_attend_plain(CudaDevice &dev, const Attend &a)
 {
     const size_t warps = (size_t)a.seq.n * a.cache.heads * a.group;
-    KernelScope ks(dev, "attend");
-    launch_following(attend_kernel, dim3((unsigned)((warps + THREADS / 32 - 1) / (THREADS / 32))), dim3(THREADS), 0, dev.stream(), a);
+    KernelScope ks(dev, "attend_plain");
+    launch_following(attend_plain_kernel, dim3((unsigned)((warps + THREADS / 32 - 1) / (THREADS / 32))), dim3(THREADS), 0, dev.stream(), a);
     dev.count_launch();
 }
 

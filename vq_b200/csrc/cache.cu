@@ -46,14 +46,16 @@ __device__ __forceinline__ float *scale_of(const Cache &c, int page, int head, i
 // blocks that are enough for the pages of n rows of so many sequences (sequence_of)
 inline unsigned parts_of(const Sequences &s) { return (unsigned)(s.n / CACHE_PAGE + 2 * s.sequences); }
 
-// Four codes of scale `old` in the new one; the quotient's nearest whole number in 64 bits is the real quotient's (|code old / scale - (k + 1/2)| is 0 or more than 2^-31).
+constexpr uint32_t ZEROS = 0x01010101u * Cache::ZERO; // four bytes that stand for 0; a byte is the code with its first bit turned
+
+// Four codes' bytes of scale `old` in the new one; the quotient's nearest whole number in 64 bits is the real quotient's (|code old / scale - (k + 1/2)| is 0 or more than 2^-31).
 __device__ __forceinline__ uint32_t codes_again(uint32_t four, float old, float scale)
 {
     uint32_t out = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int q = (int8_t)(four >> (8 * i));
-        out |= ((uint32_t)__double2int_rn((double)q * old / scale) & 255u) << (8 * i);
+        const int q = (int)(four >> (8 * i) & 255u) - 128;
+        out |= (uint32_t)(__double2int_rn((double)q * old / scale) + 128) << (8 * i);
     }
     return out;
 }
@@ -97,28 +99,28 @@ template <typename T> __global__ void __launch_bounds__(THREADS) cache_write_ker
     if (which == 0) { // a token's key: words of four dimensions
         for (int i = threadIdx.x; i < (grown ? b : count) * words; i += THREADS) {
             const int k = i / words, d = 4 * (i - k * words), t = (grown ? 0 : a) + k;
-            uint32_t w = 0;
+            uint32_t w = ZEROS, *to = codes + key_at(padded, t, d) / 4;
             if (t < a) {
-                w = codes_again(codes[t * words + d / 4], old, scale);
+                w = codes_again(*to, old, scale);
             } else if (!none) {
                 float v[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = d + j < width ? to_float(x[(t - a) * in.ld + d + j]) : 0.0f;
-                w = pack_codes<4>(v, inverse).w[0];
+                w = pack_codes<4>(v, inverse).w[0] ^ ZEROS;
             }
-            codes[t * words + d / 4] = w;
+            *to = w;
         }
         return;
     }
     // values: turned in shared memory, a dimension's words of four tokens
     for (int i = threadIdx.x; i < count * words; i += THREADS) {
         const int k = i / words, d = 4 * (i - k * words);
-        uint32_t w = 0;
+        uint32_t w = ZEROS;
         if (!none) {
             float v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = d + j < width ? to_float(x[k * in.ld + d + j]) : 0.0f;
-            w = pack_codes<4>(v, inverse).w[0];
+            w = pack_codes<4>(v, inverse).w[0] ^ ZEROS;
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) reinterpret_cast<uint8_t *>(tile)[(d + j) * PITCH + a + k] = (uint8_t)(w >> (8 * j));
@@ -172,10 +174,10 @@ template <typename T> __global__ void __launch_bounds__(THREADS) cache_read_kern
     }
     for (int i = threadIdx.x; i < count * words; i += THREADS) {
         const int k = i / words, d = 4 * (i - k * words);
-        const uint32_t w = which ? 0 : codes[(a + k) * words + d / 4];
+        const uint32_t w = which ? 0 : codes[key_at((int)c.padded, a + k, d) / 4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int q = which ? reinterpret_cast<const int8_t *>(tile)[(d + j) * PITCH + a + k] : (int8_t)(w >> (8 * j));
+            const int q = (which ? reinterpret_cast<const uint8_t *>(tile)[(d + j) * PITCH + a + k] : (int)(w >> (8 * j) & 255u)) - 128;
             if (d + j < width) y[k * out.ld + d + j] = from_float<T>((float)q * scale);
         }
     }
@@ -194,11 +196,12 @@ template <bool IN> __global__ void __launch_bounds__(THREADS) cache_pages_kernel
     }
     if (!natural) return;
     natural += at * CACHE_PAGE * width;
-    int8_t *codes = reinterpret_cast<int8_t *>(codes_of(c, page, head, which));
+    uint8_t *codes = codes_of(c, page, head, which);
     for (int i = threadIdx.x; i < CACHE_PAGE * padded; i += THREADS) {
         const int t = which ? i % CACHE_PAGE : i / padded, d = which ? i / CACHE_PAGE : i % padded;
-        if (IN) codes[i] = d < width ? natural[t * width + d] : 0;
-        else if (d < width) natural[t * width + d] = codes[i];
+        uint8_t *code = codes + (which ? i : key_at(padded, t, d));
+        if (IN) *code = (uint8_t)((d < width ? natural[t * width + d] : 0) ^ Cache::ZERO);
+        else if (d < width) natural[t * width + d] = (int8_t)(*code ^ Cache::ZERO);
     }
 }
 

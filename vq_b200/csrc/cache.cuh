@@ -55,6 +55,9 @@ __device__ __forceinline__ int page_of(const Sequences &s, size_t pages, int b, 
     return p < 0 || (size_t)p >= pages ? -1 : p;
 }
 
+// Where byte d of token t's key is in its page's keys.
+__device__ __forceinline__ int key_at(int padded, int t, int d) { return t * padded + (padded % 128 == 0 ? d ^ ((t & 1) * 64) : d); }
+
 __device__ __forceinline__ float value_at(const HeadRows &r, size_t at)
 {
     if (r.type == VALUE_F32) return static_cast<const float *>(r.x)[at];

@@ -16,12 +16,15 @@ constexpr size_t CACHE_MOST_PAGES = (size_t(1) << 31) - 1;
 constexpr size_t CACHE_MOST_COLUMNS = (size_t(1) << 25) - 1; // (positions of tokens are 32-bit numbers)
 
 // Of page p and head h: 64 rows of `padded` bytes, a token's key each, and behind them `padded` rows of 64 bytes, a dimension's value in each token.  (Both as
-// the tensor cores' operands want them: what is summed over lies side by side.)  Keys' and values' bytes of the dimensions behind `width` are 0.
+// the tensor cores' operands want them: what is summed over lies side by side.)  A byte is the code + 128 (three instructions make two f16 numbers of two such bytes, four
+// of two codes); those of the dimensions behind `width` stand for 0.  Where a key's row is a multiple of 128 bytes, the halves of each 128 of an odd token's change places, so that
+// lanes that read the same 64 bytes of two neighbouring tokens find them in different banks.
 struct Cache {
     size_t pages = 0, heads = 0, width = 0;
     size_t padded = 0;         // width to the next multiple of 32
     uint8_t *codes = nullptr;  // pages x heads x 2 x 64 x padded
     float *scales = nullptr;   // pages x heads x 2
+    static constexpr int ZERO = 0x80; // a byte that stands for 0
     size_t code_bytes() const { return pages * heads * 2 * CACHE_PAGE * padded; }
     size_t scale_bytes() const { return pages * heads * 2 * sizeof(float); }
 };
@@ -61,6 +64,12 @@ struct Attend {
     int sinks = 0;
     bool zero_rest = false; // rows of no sequence become 0
 };
+// Rows of a sequence are taken together where they have the same cached head: `group` query heads of one token, then those of the next.  A sequence of up to ATTEND_FEW of
+// them is taken sixteen at a time, by tensor-core instructions of a warp on pages that the warp fetches for itself; nothing counts there but the cache's bytes.
+constexpr int ATTEND_FEW = 64;
 void launch_attend(CudaDevice &dev, const Attend &a);
+// Sequences of up to ATTEND_FEW rows (all if `all`); zero_rest of `a` holds.
+void launch_attend_few(CudaDevice &dev, const Attend &a, bool all);
+void launch_attend_plain(CudaDevice &dev, const Attend &a); // CUDA cores
 
 } // namespace vqb
