@@ -104,4 +104,201 @@ __device__ __forceinline__ bool seen(int token, int position, int keys, int wind
     return token <= position && token < keys && (!window || token > position - window || token < sinks);
 }
 
+// What a kernel that shares tiles out is given.
+struct ShareParams {
+    Attend a;
+    int least, most; // rows (counting query heads) of the sequences that it takes: above least, at most `most`
+    int slots;       // numbers of tiles (slots_of)
+    int blocks;      // that share the pages
+    int unit;        // pages that are not shared out
+    float *parts;    // 2 x blocks parts
+    int *error;
+};
+
+// A part of a tile: ROWS x padded sums, and ROWS each of m, M and the sum below the line.
+template <int ROWS> __host__ __device__ constexpr size_t part_floats(int padded) { return (size_t)ROWS * (padded + 3); }
+
+// A row's result from the sums of its values' weights times codes, by the figures that these are relative to.  0 for a row that saw nothing (or only values of 0).
+struct RowEnd {
+    float first, second; // (in two steps: 2^(top - m) may leave f32 where the result does not)
+    __device__ __forceinline__ RowEnd(float m, float top, float l)
+    {
+        second = exp2f(0.5f * (top - m)), first = second / l;
+        if (l == 0.0f || (top == -INFINITY && l == l)) first = second = 0.0f;
+    }
+    __device__ __forceinline__ float of(float sum) const { return sum * first * second; }
+};
+
+// Tiles that there may be of all sequences, whatever their rows: sequence b's are numbered from offsets[b] group / ROWS + b on.
+template <int ROWS> inline size_t slots_of(const Attend &a)
+{
+    const size_t rows = (size_t)a.seq.n * a.group, sequences = a.seq.sequences;
+    return a.seq.offsets ? rows / ROWS + sequences : sequences * ((rows / sequences + ROWS - 1) / ROWS);
+}
+
+// One tile of one head.
+template <int ROWS> struct Tile {
+    int b, head, first_row; // first_row: of the sequence's rows, counting query heads
+    int units;              // numbered for it
+    long long begin;        // number of its first unit
+};
+
+// Units of all tiles and heads in a row; every block has an equal share of them.  Block barriers: THREADS threads.
+template <int ROWS, int THREADS> struct Plan {
+    static constexpr int MOST_GROUPS = 1024, WARPS = THREADS / 32;
+    struct Room {
+        long long before[MOST_GROUPS + 1]; // of a group of `per` slots
+        long long sums[WARPS];
+    };
+    const ShareParams &P;
+    long long *before;
+    int per, groups;
+    long long total, share;
+
+    // units of a slot's tile, 0 where it has none
+    __device__ __forceinline__ int of_slot(int u, int &b, int &first_row) const
+    {
+        const Attend &a = P.a;
+        if (!a.seq.offsets) {
+            const int each = P.slots / a.seq.sequences;
+            b = u / each, first_row = (u - b * each) * ROWS;
+        } else {
+            int lo = 0, hi = a.seq.sequences - 1; // the last one that begins at or before u
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if ((int)((long long)offset_of(a.seq, mid) * a.group / ROWS) + mid <= u) lo = mid;
+                else hi = mid - 1;
+            }
+            b = lo;
+            const int r = u - (int)((long long)offset_of(a.seq, b) * a.group / ROWS) - b;
+            if (r < 0) return 0;
+            first_row = r * ROWS;
+        }
+        const Span span(a.seq, b);
+        const long long rows = (long long)span.count * a.group;
+        if (first_row >= rows || rows <= P.least || rows > P.most) return 0;
+        const int last_row = (int)min((long long)first_row + ROWS, rows) - 1;
+        const Pages pages(span.first + first_row / a.group, span.first + last_row / a.group, span.keys, a.window, a.sinks);
+        return max((pages.count + P.unit - 1) / P.unit, 1); // (at least one: somebody writes its rows)
+    }
+    // by all threads; ends with a block barrier
+    __device__ __forceinline__ Plan(const ShareParams &params, Room &room) : P(params), before(room.before)
+    {
+        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+        per = (P.slots + MOST_GROUPS - 1) / MOST_GROUPS, groups = (P.slots + per - 1) / per;
+        long long base = 0;
+        for (int g0 = 0; g0 < groups; g0 += THREADS) {
+            long long mine = 0;
+            for (int u = (g0 + (int)threadIdx.x) * per; u < min((g0 + (int)threadIdx.x + 1) * per, P.slots); ++u) {
+                int b, row;
+                mine += of_slot(u, b, row);
+            }
+            long long up = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const long long other = __shfl_up_sync(~0u, up, d);
+                if (lane >= d) up += other;
+            }
+            if (lane == 31) room.sums[warp] = up;
+            __syncthreads();
+            long long all = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                if (w < warp) up += room.sums[w];
+                all += room.sums[w];
+            }
+            if (g0 + (int)threadIdx.x < groups) before[g0 + threadIdx.x + 1] = (base + up) * (long long)P.a.cache.heads;
+            base += all;
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) before[0] = 0;
+        __syncthreads();
+        total = before[groups];
+        share = max((total + P.blocks - 1) / P.blocks, 1ll);
+    }
+    // By a whole warp: the tile that unit x (below total) is of.
+    __device__ __forceinline__ bool find(long long x, Tile<ROWS> &tile) const
+    {
+        const int lane = threadIdx.x % 32, heads = (int)P.a.cache.heads;
+        int lo = 0, hi = groups - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (before[mid] <= x) lo = mid;
+            else hi = mid - 1;
+        }
+        long long rest = x - before[lo];
+        for (int u = lo * per, end = min(u + per, P.slots); u < end; u += 32) {
+            int b = 0, row = 0;
+            const int units = u + lane < end ? of_slot(u + lane, b, row) : 0;
+            const long long mine = (long long)units * heads;
+            long long up = mine;
+            if (per > 1) {
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const long long other = __shfl_up_sync(~0u, up, d);
+                    if (lane >= d) up += other;
+                }
+            }
+            const unsigned behind = __ballot_sync(~0u, up > rest);
+            if (behind) {
+                const int k = __ffs(behind) - 1;
+                rest -= __shfl_sync(~0u, up - mine, k);
+                tile.units = __shfl_sync(~0u, units, k), tile.b = __shfl_sync(~0u, b, k), tile.first_row = __shfl_sync(~0u, row, k);
+                const int i = (int)(rest / tile.units);
+                tile.head = i, tile.begin = x - rest + (long long)i * tile.units;
+                return true;
+            }
+            rest -= __shfl_sync(~0u, up, 31);
+        }
+        return false;
+    }
+    // The part that a block's share of a tile leaves: what begins with the share is its first one.
+    __device__ __forceinline__ float *part(long long block, bool begins_share, int padded) const { return P.parts + (2 * (size_t)block + !begins_share) * part_floats<ROWS>(padded); }
+};
+
+// The parts of tiles that more than one block had a share of: a warp for each row.
+template <int PADDED, int ROWS> __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ ShareParams P)
+{
+    using JoinPlan = Plan<ROWS, 128>;
+    __shared__ typename JoinPlan::Room room;
+    const Attend &a = P.a;
+    const int lane = threadIdx.x % 32;
+    const JoinPlan plan(P, room); // (from what was there before the kernel in front began)
+    cache_is_there();
+    // a warp for each row of the tile that a share's end cuts, if it is the tile's first such end
+    for (long long at = (long long)blockIdx.x * 4 + threadIdx.x / 32;; at += (long long)gridDim.x * 4) {
+        const long long x = (at / ROWS + 1) * plan.share;
+        const int r = (int)(at % ROWS);
+        Tile<ROWS> tile;
+        if (x >= plan.total || !plan.find(x, tile)) return;
+        if (tile.begin >= x || tile.begin < x - plan.share) continue;
+        const Span span(a.seq, tile.b);
+        if (r >= span.count * a.group - tile.first_row) continue;
+        const long long first = tile.begin / plan.share, last = (tile.begin + tile.units - 1) / plan.share;
+        const auto part_of = [&](long long block) { return plan.part(block, tile.begin <= block * plan.share, PADDED); };
+        float m = -INFINITY, top = -INFINITY, l = 0.0f;
+        for (long long s = first + lane; s <= last; s += 32) {
+            const float *f = part_of(s) + ROWS * PADDED + r;
+            m = fmaxf(m, f[0]), top = fmaxf(top, f[ROWS]);
+        }
+#pragma unroll
+        for (int o = 16; o; o /= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, o)), top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        float y[PADDED / 32] = {};
+#pragma unroll 4
+        for (long long s = first; s <= last; ++s) {
+            const float *part = part_of(s), *f = part + ROWS * PADDED + r;
+            l += f[2 * ROWS] * relative(f[0], m);
+            const float by = relative(f[ROWS], top);
+#pragma unroll
+            for (int d = 0; d < PADDED / 32; ++d) y[d] += part[r * PADDED + 32 * d + lane] * by;
+        }
+        const RowEnd row_end(m, top, l);
+        const int row = tile.first_row + r;
+        const size_t to = (size_t)(span.row + row / a.group) * a.y.ld + (size_t)(tile.head * a.group + row % a.group) * a.y.head_ld;
+#pragma unroll
+        for (int d = 0; d < PADDED / 32; ++d)
+            if (32 * d + lane < (int)a.cache.width) put_value(a.y, to + 32 * d + lane, row_end.of(y[d]));
+    }
+}
+
 } // namespace vqb

@@ -19,139 +19,9 @@ namespace vqb {
 namespace {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS, ROWS = 16, STAGES = 3;
-constexpr int MOST_GROUPS = 1024; // of sequences, whose pages are numbered in shared memory
 
-struct FewParams {
-    Attend a;
-    bool all;      // every sequence, whatever its rows
-    int blocks;    // that share the pages
-    int unit;      // pages that are not shared out
-    float *parts;  // 2 x blocks parts
-    int *error;
-};
-
-// A row's result from the sums of its values' weights times codes and the figures that these are relative to.  0 for a row that saw nothing (or only values of 0).
-__device__ __forceinline__ float finish_row(float y, float m, float top, float l)
-{
-    if (l == 0.0f || (top == -INFINITY && l == l)) return 0.0f;
-    const float root = exp2f(0.5f * (top - m)); // (in two steps: 2^(top - m) may leave f32 where the result does not)
-    return y / l * root * root;
-}
-
-// A part of a tile: ROWS x padded sums, and ROWS each of m, M and the sum below the line.
-__host__ __device__ constexpr size_t part_floats(int padded) { return (size_t)ROWS * (padded + 3); }
-
-// Units of all tiles in a row: sequence by sequence, tile by tile, head by head, the same number for each of a sequence's.
-struct Plan {
-    long long *before; // of a group of `per` sequences; groups + 1
-    int per, groups;
-    long long total, share;
-
-    // units of one tile and head (at least one: somebody writes its rows), tiles of the sequence; 0 tiles: not this kernel's
-    static __device__ __forceinline__ void of_sequence(const FewParams &P, int b, int &units, int &tiles)
-    {
-        const Span span(P.a.seq, b);
-        const int rows = span.count * P.a.group;
-        tiles = (rows + ROWS - 1) / ROWS, units = 1;
-        if (!P.all && rows > ATTEND_FEW) tiles = 0;
-        if (tiles == 0) return;
-        const int last = min(span.first + span.count - 1, span.keys - 1);
-        if (last < 0) return;
-        long long most = (last >> 6) + 1;
-        if (P.a.window) most = min(most, (((long long)P.a.sinks + 63) >> 6) + ((long long)P.a.window + ROWS + 62) / CACHE_PAGE + 1);
-        units = ((int)most + P.unit - 1) / P.unit;
-    }
-    // by all threads; ends with a block barrier.  sums: WARPS
-    __device__ __forceinline__ void make(const FewParams &P, long long *before_, long long *sums)
-    {
-        before = before_;
-        const int sequences = P.a.seq.sequences, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-        per = (sequences + MOST_GROUPS - 1) / MOST_GROUPS, groups = (sequences + per - 1) / per;
-        long long base = 0;
-        for (int g0 = 0; g0 < groups; g0 += THREADS) {
-            long long mine = 0;
-            for (int b = (g0 + (int)threadIdx.x) * per; b < min((g0 + (int)threadIdx.x + 1) * per, sequences); ++b) {
-                int units, tiles;
-                of_sequence(P, b, units, tiles);
-                mine += (long long)units * tiles;
-            }
-            long long up = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const long long other = __shfl_up_sync(~0u, up, d);
-                if (lane >= d) up += other;
-            }
-            if (lane == 31) sums[warp] = up;
-            __syncthreads();
-            long long all = 0;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                if (w < warp) up += sums[w];
-                all += sums[w];
-            }
-            if (g0 + (int)threadIdx.x < groups) before[g0 + threadIdx.x + 1] = (base + up) * (long long)P.a.cache.heads;
-            base += all;
-            __syncthreads();
-        }
-        if (threadIdx.x == 0) before[0] = 0;
-        __syncthreads();
-        total = before[groups];
-        share = max((total + P.blocks - 1) / P.blocks, 1ll);
-    }
-    // By a whole warp: the sequence that unit x is of, units of its tiles, and x less what is before it.
-    __device__ __forceinline__ int find(const FewParams &P, long long x, int &units, long long &rest) const
-    {
-        int lo = 0, hi = groups - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (before[mid] <= x) lo = mid;
-            else hi = mid - 1;
-        }
-        rest = x - before[lo];
-        int b = lo * per;
-        const int end = min(b + per, P.a.seq.sequences), lane = threadIdx.x % 32;
-        for (; b < end; b += 32) {
-            int p = 1, t = 0;
-            if (b + lane < end) of_sequence(P, b + lane, p, t);
-            const long long mine = (long long)p * t * (long long)P.a.cache.heads;
-            long long up = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const long long other = __shfl_up_sync(~0u, up, d);
-                if (lane >= d) up += other;
-            }
-            const unsigned behind = __ballot_sync(~0u, up > rest);
-            const int k = behind ? __ffs(behind) - 1 : 31;
-            const long long skipped = __shfl_sync(~0u, up - mine, k), whole = __shfl_sync(~0u, up, 31);
-            if (behind) {
-                units = __shfl_sync(~0u, p, k), rest -= skipped;
-                return b + k;
-            }
-            rest -= whole;
-        }
-        units = 1;
-        return -1; // (x is not below total)
-    }
-};
-
-// One tile of one head.
-struct Tile {
-    int b, head, first_row; // first_row: of the sequence's rows, counting query heads
-    int rows;               // of the tile
-    int units;              // numbered for it
-    long long begin;        // number of its first unit
-    // by a whole warp
-    __device__ __forceinline__ bool find(const FewParams &P, const Plan &plan, long long x)
-    {
-        long long rest;
-        b = plan.find(P, x, units, rest);
-        if (b < 0) return false;
-        const int heads = (int)P.a.cache.heads, i = (int)(rest / units);
-        begin = x - rest + (long long)i * units;
-        head = i % heads, first_row = i / heads * ROWS;
-        return true;
-    }
-};
+using FewPlan = Plan<ROWS, THREADS>;
+using FewTile = Tile<ROWS>;
 
 __device__ __forceinline__ void mma_f16(float (&sums)[4], const uint4 &a, uint32_t b0, uint32_t b1)
 {
@@ -300,11 +170,11 @@ __device__ __forceinline__ void weigh(float (&s)[8][4], const float (&factor)[2]
 
 // A tile's queries as operand fragments, and each row's factor of scores: lane 4 g + t of step i of chunk c has dimensions d .. d + 3, d = (4 c + t) PIECE + 4 i, of
 // rows g and g + 8.  By the block: eight threads a row.
-template <int PADDED> __device__ __forceinline__ void bring_queries(const Attend &a, const Span &span, const Tile &tile, uint32_t *queries, float *down)
+template <int PADDED> __device__ __forceinline__ void bring_queries(const Attend &a, const Span &span, const FewTile &tile, int rows, uint32_t *queries, float *down)
 {
     using Shape = FewShape<PADDED>;
     const int r = threadIdx.x / 8, part = threadIdx.x % 8, at = tile.first_row + r, width = (int)a.cache.width;
-    const bool there = r < tile.rows;
+    const bool there = r < rows;
     const size_t from = there ? (size_t)(span.row + at / a.group) * a.queries.ld + (size_t)(tile.head * a.group + at % a.group) * a.queries.head_ld : 0;
     const uint16_t *x = static_cast<const uint16_t *>(a.queries.x) + from;
     const bool f16 = a.queries.type == VALUE_F16, aligned = (reinterpret_cast<uintptr_t>(x) & 7) == 0;
@@ -344,11 +214,11 @@ template <int PADDED> __device__ __forceinline__ void bring_queries(const Attend
     }
 }
 
-template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ? 2 : 1) attend_few_kernel(const FewParams P)
+template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ? 2 : 1) attend_few_kernel(const __grid_constant__ ShareParams P)
 {
     using Shape = FewShape<PADDED>;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ long long before[MOST_GROUPS + 1], sums[WARPS];
+    __shared__ FewPlan::Room room;
     __shared__ unsigned long long full[WARPS][STAGES];
     __shared__ float down[ROWS], figures[WARPS][3][ROWS], final_figures[3][ROWS];
     __shared__ int abort_word;
@@ -372,17 +242,16 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
             put_value(a.y, (r < (size_t)front ? r : r - front + behind) * a.y.ld + rest / width * a.y.head_ld + rest % width, 0.0f);
         }
     }
-    Plan plan;
-    plan.make(P, before, sums);
+    const FewPlan plan(P, room);
     const long long start = plan.share * blockIdx.x, end = min(start + plan.share, plan.total);
     int st = 0;          // of the ring, and how often it went round
     uint32_t parity = 0;
     for (long long x = start; x < end;) {
-        Tile tile;
-        if (!tile.find(P, plan, x)) break;
+        FewTile tile;
+        if (!plan.find(x, tile)) break;
         const Span span(a.seq, tile.b);
-        tile.rows = min(span.count * a.group - tile.first_row, ROWS);
-        const int p0 = span.first + tile.first_row / a.group, p1 = span.first + (tile.first_row + tile.rows - 1) / a.group;
+        const int rows = min(span.count * a.group - tile.first_row, ROWS);
+        const int p0 = span.first + tile.first_row / a.group, p1 = span.first + (tile.first_row + rows - 1) / a.group;
         const Pages pages(p0, p1, span.keys, a.window, a.sinks);
         const int first = (int)(x - tile.begin), behind = (int)(min(end, tile.begin + tile.units) - tile.begin); // units
         const int from = first * P.unit, last = (int)min((long long)behind * P.unit, (long long)pages.count);
@@ -415,14 +284,14 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
             fetch(k, stage, 0);
             if (++stage == STAGES) stage = 0;
         }
-        bring_queries<PADDED>(a, span, tile, queries, down);
+        bring_queries<PADDED>(a, span, tile, rows, queries, down);
         __syncthreads();
         Running<PADDED> run;
 #pragma unroll
         for (int d = 0; d < PADDED / 8; ++d) run.y[d][0] = run.y[d][1] = run.y[d][2] = run.y[d][3] = 0.0f;
         run.m[0] = run.m[1] = run.top[0] = run.top[1] = -INFINITY, run.l[0] = run.l[1] = 0.0f;
         const float mine[2] = {down[g], down[g + 8]};
-        const int position[2] = {span.first + (tile.first_row + min(g, tile.rows - 1)) / a.group, span.first + (tile.first_row + min(g + 8, tile.rows - 1)) / a.group};
+        const int position[2] = {span.first + (tile.first_row + min(g, rows - 1)) / a.group, span.first + (tile.first_row + min(g + 8, rows - 1)) / a.group};
         for (int i = 0; i < many; ++i) {
             const int page = __shfl_sync(~0u, page_now, i % 32);
             const float2 both = make_float2(__shfl_sync(~0u, scales_now.x, i % 32), __shfl_sync(~0u, scales_now.y, i % 32));
@@ -488,9 +357,9 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
         }
         __syncthreads();
         const bool whole = first == 0 && behind == tile.units;
-        float *part = whole ? nullptr : P.parts + (2 * (size_t)blockIdx.x + (x > start)) * part_floats(PADDED);
+        float *part = whole ? nullptr : plan.part(blockIdx.x, x == start, PADDED);
         if (!whole && threadIdx.x < 3 * ROWS) part[ROWS * PADDED + threadIdx.x] = (&final_figures[0][0])[threadIdx.x];
-        for (int i = threadIdx.x; i < tile.rows * PADDED; i += THREADS) {
+        for (int i = threadIdx.x; i < rows * PADDED; i += THREADS) {
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) v += reinterpret_cast<const float *>(smem + (size_t)w * STAGES * Shape::HALF)[i];
@@ -498,7 +367,7 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
             if (!whole) part[i] = v;
             else if (d < (int)c.width)
                 put_value(a.y, (size_t)(span.row + at / a.group) * a.y.ld + (size_t)(tile.head * a.group + at % a.group) * a.y.head_ld + d,
-                          finish_row(v, final_figures[0][r], final_figures[1][r], final_figures[2][r]));
+                          RowEnd(final_figures[0][r], final_figures[1][r], final_figures[2][r]).of(v));
         }
         x = tile.begin + behind;
         if (*(volatile int *)&abort_word) break; // (set before the barriers above if at all)
@@ -511,53 +380,7 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
         for (int w = 0; w < 1000; ++w) __nanosleep(1000);
 }
 
-// The parts of tiles that more than one block had a share of: a warp for each row.
-template <int PADDED> __global__ void __launch_bounds__(THREADS) attend_join_kernel(const FewParams P)
-{
-    __shared__ long long before[MOST_GROUPS + 1], sums[WARPS];
-    const Attend &a = P.a;
-    const int lane = threadIdx.x % 32;
-    Plan plan;
-    plan.make(P, before, sums); // (from what was there before the kernel in front began)
-    cache_is_there();
-    // boundaries between shares; the tile that one cuts is joined by whoever has its first boundary
-    for (long long at = (long long)blockIdx.x * WARPS + threadIdx.x / 32;; at += (long long)gridDim.x * WARPS) {
-        const long long cut = at / ROWS + 1, x = cut * plan.share;
-        const int r = (int)(at % ROWS);
-        if (x >= plan.total) return;
-        Tile tile;
-        if (!tile.find(P, plan, x)) return;
-        if (tile.begin >= x || tile.begin < x - plan.share) continue; // (not cut, or not here first)
-        const Span span(a.seq, tile.b);
-        tile.rows = min(span.count * a.group - tile.first_row, ROWS);
-        if (r >= tile.rows) continue;
-        const long long first = tile.begin / plan.share, last = (tile.begin + tile.units - 1) / plan.share; // shares
-        const auto part_of = [&](long long share) { return P.parts + (2 * (size_t)share + (tile.begin > share * plan.share)) * part_floats(PADDED); };
-        float m = -INFINITY, top = -INFINITY, l = 0.0f;
-        for (long long s = first + lane; s <= last; s += 32) {
-            const float *f = part_of(s) + ROWS * PADDED + r;
-            m = fmaxf(m, f[0]), top = fmaxf(top, f[ROWS]);
-        }
-#pragma unroll
-        for (int o = 16; o; o /= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, o)), top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        float y[PADDED / 32] = {};
-#pragma unroll 4
-        for (long long s = first; s <= last; ++s) {
-            const float *part = part_of(s), *f = part + ROWS * PADDED + r;
-            l += f[2 * ROWS] * relative(f[0], m);
-            const float by = relative(f[ROWS], top);
-#pragma unroll
-            for (int d = 0; d < PADDED / 32; ++d) y[d] += part[r * PADDED + 32 * d + lane] * by;
-        }
-        const int row = tile.first_row + r;
-        const size_t to = (size_t)(span.row + row / a.group) * a.y.ld + (size_t)(tile.head * a.group + row % a.group) * a.y.head_ld;
-#pragma unroll
-        for (int d = 0; d < PADDED / 32; ++d)
-            if (32 * d + lane < (int)a.cache.width) put_value(a.y, to + 32 * d + lane, finish_row(y[d], m, top, l));
-    }
-}
-
-template <int PADDED> void attend_few_with(CudaDevice &dev, FewParams &P, bool join)
+template <int PADDED> void attend_few_with(CudaDevice &dev, const ShareParams &P, bool join)
 {
     const size_t smem = FewShape<PADDED>::SMEM + 128;
     allow_shared_memory(dev, attend_few_kernel<PADDED>);
@@ -568,34 +391,31 @@ template <int PADDED> void attend_few_with(CudaDevice &dev, FewParams &P, bool j
     }
     if (!join) return;
     KernelScope ks(dev, "attend_join");
-    launch_following(attend_join_kernel<PADDED>, dim3((unsigned)std::min(P.blocks * ROWS / WARPS, 4 * dev.sm_count())), dim3(THREADS), 0, dev.stream(), P);
+    launch_following(attend_join_kernel<PADDED, ROWS>, dim3((unsigned)std::min(P.blocks * ROWS / 4, 4 * dev.sm_count())), dim3(128), 0, dev.stream(), P);
     dev.count_launch();
 }
 
 } // namespace
 
-void launch_attend_few(CudaDevice &dev, const Attend &a, bool all)
+void launch_attend_few(CudaDevice &dev, const Attend &a)
 {
-    FewParams P{};
-    P.a = a, P.all = all, P.error = dev.error_word();
-    const size_t padded = a.cache.padded, sequences = a.seq.sequences;
-    // what the host knows: tiles at most, pages of each at most
-    const size_t rows = (size_t)a.seq.n * a.group;
-    const size_t tiles = (a.seq.offsets ? rows / ROWS + std::min(sequences, (size_t)a.seq.n) : sequences * ((rows / sequences + ROWS - 1) / ROWS)) * a.cache.heads;
-    size_t pages = std::max(a.seq.columns, 1);
+    ShareParams P{};
+    P.a = a, P.error = dev.error_word();
+    P.least = 0, P.most = ATTEND_FEW, P.slots = (int)slots_of<ROWS>(a);
+    const size_t padded = a.cache.padded;
+    size_t pages = std::max(a.seq.columns, 1); // of a tile at most
     if (a.window) pages = std::min(pages, ((size_t)a.sinks + 63) / 64 + ((size_t)a.window + ROWS + 62) / CACHE_PAGE + 1);
     const size_t rounds = (pages + WARPS - 1) / WARPS;
     const bool join = rounds > 4;
     P.unit = (int)(join ? WARPS : rounds * WARPS);
-    const size_t units = tiles * (join ? rounds : 1), places = (size_t)dev.sm_count() * (padded <= 128 ? 2 : 1);
+    const size_t units = (size_t)P.slots * a.cache.heads * (join ? rounds : 1), places = (size_t)dev.sm_count() * (padded <= 128 ? 2 : 1);
     P.blocks = (int)std::min(units, places);
-    float *parts = nullptr;
-    if (join) P.parts = parts = static_cast<float *>(dev.alloc(2 * (size_t)P.blocks * part_floats((int)padded) * sizeof(float)));
-    struct Release {
+    struct Parts {
         CudaDevice &dev;
         void *p;
-        ~Release() { dev.release(p); }
-    } release{dev, parts};
+        ~Parts() { dev.release(p); }
+    } parts{dev, join ? dev.alloc(2 * (size_t)P.blocks * part_floats<ROWS>((int)padded) * sizeof(float)) : nullptr};
+    P.parts = static_cast<float *>(parts.p);
     switch (padded / 32) {
     case 1: return attend_few_with<32>(dev, P, join);
     case 2: return attend_few_with<64>(dev, P, join);
@@ -611,7 +431,11 @@ void launch_attend_few(CudaDevice &dev, const Attend &a, bool all)
 void launch_attend(CudaDevice &dev, const Attend &a)
 {
     if (!dev.error_word()) return launch_attend_plain(dev, a);
-    launch_attend_few(dev, a, true);
+    // sequences of many rows, if there can be any, go to the one kernel, the others to the other
+    const size_t rows = (size_t)a.seq.n * a.group, most = a.seq.offsets ? rows : rows / a.seq.sequences;
+    const bool few = a.seq.offsets || most <= ATTEND_FEW, many = most > ATTEND_FEW;
+    if (few) launch_attend_few(dev, a);
+    if (many) launch_attend_many(dev, a);
 }
 
 } // namespace vqb

@@ -66,10 +66,11 @@ struct Attend {
 };
 // Rows of a sequence are taken together where they have the same cached head: `group` query heads of one token, then those of the next.  A sequence of up to ATTEND_FEW of
 // them is taken sixteen at a time, by tensor-core instructions of a warp on pages that the warp fetches for itself; nothing counts there but the cache's bytes.
+// Others are taken 256 or 128 at a time by tcgen05 instructions.
 constexpr int ATTEND_FEW = 64;
 void launch_attend(CudaDevice &dev, const Attend &a);
-// Sequences of up to ATTEND_FEW rows (all if `all`); zero_rest of `a` holds.
-void launch_attend_few(CudaDevice &dev, const Attend &a, bool all);
+void launch_attend_few(CudaDevice &dev, const Attend &a);  // sequences of up to ATTEND_FEW rows, and rows of no sequence
+void launch_attend_many(CudaDevice &dev, const Attend &a); // the other sequences
 void launch_attend_plain(CudaDevice &dev, const Attend &a); // CUDA cores
 
 } // namespace vqb
