@@ -8,6 +8,7 @@
 // below 2^-28 of the row's largest, which are off by at most 2^-39 of it.
 #pragma once
 #include "cache.cuh"
+#include "cuda_device.hpp"
 
 namespace vqb {
 
@@ -111,8 +112,19 @@ struct ShareParams {
     int slots;       // numbers of tiles (slots_of)
     int blocks;      // that share the pages
     int unit;        // pages that are not shared out
-    float *parts;    // 2 x blocks parts
+    int extra;       // units that a tile counts for beside its pages
+    float *parts;    // 2 x blocks parts; null where no share's end cuts a tile
+    struct Cut *cuts; // what each block's begin cuts
     int *error;
+};
+
+// A tile that the end of a share, in front of a block, cuts, if it is the first such end: the tile has parts in blocks first .. last.
+struct Cut {
+    int row, rows;       // first row of the sequence, rows of the tile (0: nothing is cut here first)
+    int first_row, head; // as of Tile
+    int first, last;
+    int begins; // the tile begins with the first block's share
+    int unused;
 };
 
 // A part of a tile: ROWS x padded sums, and ROWS each of m, M and the sum below the line.
@@ -145,7 +157,7 @@ template <int ROWS> struct Tile {
 
 // Units of all tiles and heads in a row; every block has an equal share of them.  Block barriers: THREADS threads.
 template <int ROWS, int THREADS> struct Plan {
-    static constexpr int MOST_GROUPS = 1024, WARPS = THREADS / 32;
+    static constexpr int MOST_GROUPS = 512, WARPS = THREADS / 32;
     struct Room {
         long long before[MOST_GROUPS + 1]; // of a group of `per` slots
         long long sums[WARPS];
@@ -179,7 +191,7 @@ template <int ROWS, int THREADS> struct Plan {
         if (first_row >= rows || rows <= P.least || rows > P.most) return 0;
         const int last_row = (int)min((long long)first_row + ROWS, rows) - 1;
         const Pages pages(span.first + first_row / a.group, span.first + last_row / a.group, span.keys, a.window, a.sinks);
-        return max((pages.count + P.unit - 1) / P.unit, 1); // (at least one: somebody writes its rows)
+        return max((pages.count + P.unit - 1) / P.unit, 1) + P.extra; // (at least one: somebody writes its rows)
     }
     // by all threads; ends with a block barrier
     __device__ __forceinline__ Plan(const ShareParams &params, Room &room) : P(params), before(room.before)
@@ -253,52 +265,85 @@ template <int ROWS, int THREADS> struct Plan {
         return false;
     }
     // The part that a block's share of a tile leaves: what begins with the share is its first one.
-    __device__ __forceinline__ float *part(long long block, bool begins_share, int padded) const { return P.parts + (2 * (size_t)block + !begins_share) * part_floats<ROWS>(padded); }
+    __device__ __forceinline__ float *part(int block, bool begins_share, int padded) const { return P.parts + (2 * (size_t)block + !begins_share) * part_floats<ROWS>(padded); }
+    // The first tile that this block has some of; null: it has none.  By one thread.
+    __device__ __forceinline__ void tell(const Tile<ROWS> *tile, int row, int rows) const
+    {
+        if (!P.parts) return;
+        Cut cut = {};
+        const long long start = share * blockIdx.x;
+        if (tile && tile->begin < start && tile->begin >= start - share)
+            cut = Cut{row, rows, tile->first_row, tile->head, (int)blockIdx.x - 1, (int)((tile->begin + tile->units - 1) / share), tile->begin == start - share, 0};
+        P.cuts[blockIdx.x] = cut;
+    }
 };
 
 // The parts of tiles that more than one block had a share of: a warp for each row.
 template <int PADDED, int ROWS> __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ ShareParams P)
 {
-    using JoinPlan = Plan<ROWS, 128>;
-    __shared__ typename JoinPlan::Room room;
-    const Attend &a = P.a;
-    const int lane = threadIdx.x % 32;
-    const JoinPlan plan(P, room); // (from what was there before the kernel in front began)
     cache_is_there();
-    // a warp for each row of the tile that a share's end cuts, if it is the tile's first such end
-    for (long long at = (long long)blockIdx.x * 4 + threadIdx.x / 32;; at += (long long)gridDim.x * 4) {
-        const long long x = (at / ROWS + 1) * plan.share;
-        const int r = (int)(at % ROWS);
-        Tile<ROWS> tile;
-        if (x >= plan.total || !plan.find(x, tile)) return;
-        if (tile.begin >= x || tile.begin < x - plan.share) continue;
-        const Span span(a.seq, tile.b);
-        if (r >= span.count * a.group - tile.first_row) continue;
-        const long long first = tile.begin / plan.share, last = (tile.begin + tile.units - 1) / plan.share;
-        const auto part_of = [&](long long block) { return plan.part(block, tile.begin <= block * plan.share, PADDED); };
-        float m = -INFINITY, top = -INFINITY, l = 0.0f;
-        for (long long s = first + lane; s <= last; s += 32) {
-            const float *f = part_of(s) + ROWS * PADDED + r;
-            m = fmaxf(m, f[0]), top = fmaxf(top, f[ROWS]);
+    const Attend &a = P.a;
+    const int lane = threadIdx.x % 32, at = blockIdx.x * 4 + threadIdx.x / 32, r = at % ROWS;
+    if (at / ROWS + 1 >= P.blocks) return;
+    const Cut cut = P.cuts[at / ROWS + 1];
+    if (r >= cut.rows) return;
+    const auto part_of = [&](int block) { return P.parts + (2 * (size_t)block + (block == cut.first && !cut.begins)) * part_floats<ROWS>(PADDED); };
+    float m = -INFINITY, top = -INFINITY, l = 0.0f;
+    float y[PADDED / 32] = {};
+    for (int s0 = cut.first; s0 <= cut.last; s0 += 32) { // (usually once)
+        const int s = s0 + lane, many = min(cut.last - s0 + 1, 32);
+        const float *f = part_of(min(s, cut.last)) + ROWS * PADDED + r;
+        const float part_m = s <= cut.last ? f[0] : -INFINITY, part_top = s <= cut.last ? f[ROWS] : -INFINITY, part_l = s <= cut.last ? f[2 * ROWS] : 0.0f;
+        float new_m = fmaxf(m, part_m), new_top = fmaxf(top, part_top);
+#pragma unroll
+        for (int o = 16; o; o /= 2) new_m = fmaxf(new_m, __shfl_xor_sync(~0u, new_m, o)), new_top = fmaxf(new_top, __shfl_xor_sync(~0u, new_top, o));
+        float sum = part_l * relative(part_m, new_m);
+        const float by = relative(part_top, new_top);
+#pragma unroll
+        for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
+        l = l * relative(m, new_m) + sum;
+        const float old = relative(top, new_top);
+#pragma unroll
+        for (int d = 0; d < PADDED / 32; ++d) y[d] *= old;
+        m = new_m, top = new_top;
+#pragma unroll 8
+        for (int k = 0; k < many; ++k) {
+            const float *part = part_of(s0 + k) + r * PADDED + lane;
+            const float w = __shfl_sync(~0u, by, k);
+#pragma unroll
+            for (int d = 0; d < PADDED / 32; ++d)
+                if (w != 0.0f) y[d] += part[32 * d] * w; // (a part that saw nothing may have no sums)
         }
-#pragma unroll
-        for (int o = 16; o; o /= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, o)), top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        float y[PADDED / 32] = {};
-#pragma unroll 4
-        for (long long s = first; s <= last; ++s) {
-            const float *part = part_of(s), *f = part + ROWS * PADDED + r;
-            l += f[2 * ROWS] * relative(f[0], m);
-            const float by = relative(f[ROWS], top);
-#pragma unroll
-            for (int d = 0; d < PADDED / 32; ++d) y[d] += part[r * PADDED + 32 * d + lane] * by;
-        }
-        const RowEnd row_end(m, top, l);
-        const int row = tile.first_row + r;
-        const size_t to = (size_t)(span.row + row / a.group) * a.y.ld + (size_t)(tile.head * a.group + row % a.group) * a.y.head_ld;
-#pragma unroll
-        for (int d = 0; d < PADDED / 32; ++d)
-            if (32 * d + lane < (int)a.cache.width) put_value(a.y, to + 32 * d + lane, row_end.of(y[d]));
     }
+    const RowEnd row_end(m, top, l);
+    const int row = cut.first_row + r;
+    const size_t to = (size_t)(cut.row + row / a.group) * a.y.ld + (size_t)(cut.head * a.group + row % a.group) * a.y.head_ld;
+#pragma unroll
+    for (int d = 0; d < PADDED / 32; ++d)
+        if (32 * d + lane < (int)a.cache.width) put_value(a.y, to + 32 * d + lane, row_end.of(y[d]));
+}
+
+// Memory for what is left to join, for the time of a call.
+struct Parts {
+    CudaDevice &dev;
+    unsigned char *p = nullptr;
+    template <int ROWS> static size_t cuts_at(const ShareParams &P, int padded) { return 2 * (size_t)P.blocks * part_floats<ROWS>(padded) * sizeof(float); }
+    explicit Parts(CudaDevice &d) : dev(d) {}
+    template <int ROWS> void make(ShareParams &P, int padded)
+    {
+        p = static_cast<unsigned char *>(dev.alloc(cuts_at<ROWS>(P, padded) + P.blocks * sizeof(Cut)));
+        P.parts = reinterpret_cast<float *>(p), P.cuts = reinterpret_cast<Cut *>(p + cuts_at<ROWS>(P, padded));
+    }
+    ~Parts() { dev.release(p); }
+    Parts(const Parts &) = delete;
+    Parts &operator=(const Parts &) = delete;
+};
+template <int PADDED, int ROWS> void launch_join(CudaDevice &dev, const ShareParams &P)
+{
+    if (!P.parts || P.blocks < 2) return;
+    KernelScope ks(dev, "attend_join");
+    launch_following(attend_join_kernel<PADDED, ROWS>, dim3((unsigned)(((size_t)(P.blocks - 1) * ROWS + 3) / 4)), dim3(128), 0, dev.stream(), P);
+    dev.count_launch();
 }
 
 } // namespace vqb

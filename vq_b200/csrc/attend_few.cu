@@ -1,10 +1,11 @@
 // attend_few.cu -- attention of a few rows of each sequence (single tokens above all) over a cache of 8-bit codes.
 //
-// Sixteen rows that share a cached head (query heads of a token, then those of the next one) are a tile.  What bounds it is the cache's bytes, read once for a tile: 2 x 64 x
-// width of them a page and head.  Every warp fetches pages for itself (one bulk copy for a page's keys, one for its values) into a ring of its own, some 90 KB of an SM's on their
-// way at any time, turns the codes to f16 numbers in registers and multiplies (mma.sync m16n8k16: with sixteen rows the tensor cores' larger instructions would
-// be seven eighths empty).  Scores never leave registers: columns of a page's score tile stand for tokens in such an order that a lane's scores are
-// the operand of the product with the values, whose tokens lie side by side.
+// Eight or sixteen rows that share a cached head (query heads of a token, then those of the next one) are a tile.  What bounds it is the cache's bytes, read once for a tile:
+// 2 x 64 x width of them a page and head.  Every warp fetches pages for itself (one bulk copy for a page's keys, one for its values) into a ring of its own,
+// turns the codes to f16 numbers in registers and multiplies: mma.sync m16n8k16 with sixteen tokens by eight rows, then sixteen dimensions by eight rows.  (The tensor
+// cores' larger instructions have 128 rows where there are eight.)  A lane's 16 bytes of a key serve four instructions: which of its dimensions go into
+// which is free as long as the queries have the same.  So is which tokens are a score tile's rows; they are chosen so that the tile, transposed (movmatrix), is the operand
+// of the product with the values, of which a lane has four tokens side by side.
 //
 // All tiles' pages are numbered in a row, and each block takes an equal share of that, whatever the sequences' lengths are (nobody on the host knows them).  What
 // a share's end cuts off a tile leaves as a part (its largest scores, sum, and sums of values), and a second kernel joins parts, in the order of their pages.
@@ -18,16 +19,21 @@ namespace vqb {
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = 32 * WARPS, ROWS = 16, STAGES = 3;
+constexpr int WARPS = 4, THREADS = 32 * WARPS, STAGES = 2;
+constexpr float LATE = 8.0f; // a row's largest score is followed when it is 2^LATE times as large
 
-using FewPlan = Plan<ROWS, THREADS>;
-using FewTile = Tile<ROWS>;
-
-__device__ __forceinline__ void mma_f16(float (&sums)[4], const uint4 &a, uint32_t b0, uint32_t b1)
+__device__ __forceinline__ void mma_f16(float (&sums)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(sums[0]), "+f"(sums[1]), "+f"(sums[2]), "+f"(sums[3])
-                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+// 8 x 8 16-bit values, two of a row a lane, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t v)
+{
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
 }
 
 template <int BYTES> struct Words;
@@ -41,191 +47,229 @@ template <> struct Words<8> {
 };
 template <int BYTES> __device__ __forceinline__ Words<BYTES> words_at(const uint8_t *p) { return *reinterpret_cast<const Words<BYTES> *>(p); }
 
-template <int PADDED> struct FewShape {
-    static constexpr int PIECE = PADDED % 64 == 0 ? 16 : 8;     // bytes of a key that a lane reads at once
+// EIGHTS: of rows a tile has
+template <int PADDED, int EIGHTS> struct FewShape {
+    static constexpr int ROWS = 8 * EIGHTS;
+    static constexpr int PIECE = PADDED % 64 == 0 ? 16 : 8;                // bytes of a key that a lane reads at once
     static constexpr int CHUNKS = PADDED / (4 * PIECE), STEPS = PIECE / 4; // a chunk: four lanes' pieces, STEPS instructions
-    static constexpr uint32_t HALF = CACHE_PAGE * PADDED;       // a page's keys, or its values
-    static constexpr size_t QUERIES = (size_t)ROWS * PADDED * 2; // operand fragments
-    static constexpr size_t SMEM = WARPS * STAGES * HALF + QUERIES;
+    static constexpr uint32_t HALF = CACHE_PAGE * PADDED;                  // a page's keys, or its values
+    static constexpr size_t QUERIES = (size_t)ROWS * PADDED * 2;           // operand fragments
+    static constexpr bool HELD = PADDED * EIGHTS <= 256;                   // in registers
+    static constexpr size_t RING = WARPS * STAGES * HALF;
+    static_assert(ROWS * PADDED * 4 <= STAGES * HALF, "the ring takes the warps' sums");
+    static constexpr size_t SMEM = RING + QUERIES;
+    static constexpr int BLOCKS = PADDED <= 128 ? EIGHTS == 1 ? 3 : 2 : PADDED <= 192 ? 2 : 1; // an SM's
+    using Sharing = Plan<ROWS, THREADS>;
 };
 
-// the rows' largest scores, the sum below the line and the sums of values, of one warp's pages
-template <int PADDED> struct Running {
-    float y[PADDED / 8][4]; // rows g, g, g + 8, g + 8; dimensions 2 t, 2 t + 1 of each eight (lane = 4 g + t)
-    float m[2], top[2], l[2];
+// Lane 4 g + t: sums of values of dimensions 16 i + g (first two) and 16 i + 8 + g, for rows 2 t and 2 t + 1 (of each eight); these rows' figures.
+template <int PADDED, int EIGHTS> struct Running {
+    float y[EIGHTS][PADDED / 16][4];
+    float m[EIGHTS][2], top[EIGHTS][2], l[EIGHTS][2];
 };
 
-// products of the rows with a page's keys
-template <int PADDED> __device__ __forceinline__ void take_keys(const uint8_t *keys, const uint4 *queries, float (&s)[8][4])
+// Products of a page's keys with the rows.  Tile i: row g of it is token 16 (g / 2) + 4 i + g % 2, row 8 + g the token two behind that.
+template <int PADDED, int EIGHTS> __device__ __forceinline__ void take_keys(const uint8_t *keys, const uint2 *queries, const uint2 (&held)[EIGHTS][PADDED / 16], float (&s)[EIGHTS][4][4])
 {
-    using Shape = FewShape<PADDED>;
+    using Shape = FewShape<PADDED, EIGHTS>;
     const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-    const uint8_t *mine = keys + (16 * (g >> 1) + (g & 1)) * PADDED; // tile j's column g is token 16 (g / 2) + 2 j + g % 2
+    for (int e = 0; e < EIGHTS; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[e][i][0] = s[e][i][1] = s[e][i][2] = s[e][i][3] = 0.0f;
+    const uint8_t *mine = keys + (16 * (g >> 1) + (g & 1)) * PADDED;
     const int turned = PADDED % 128 == 0 ? 64 * (g & 1) : 0;
 #pragma unroll
     for (int c = 0; c < Shape::CHUNKS; ++c) {
-        uint4 a[Shape::STEPS];
+        uint2 b[EIGHTS][Shape::STEPS];
 #pragma unroll
-        for (int i = 0; i < Shape::STEPS; ++i) a[i] = queries[(c * Shape::STEPS + i) * 32 + lane];
+        for (int e = 0; e < EIGHTS; ++e)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const Words<Shape::PIECE> w = words_at<Shape::PIECE>(mine + 2 * j * PADDED + ((c * 4 * Shape::PIECE + t * Shape::PIECE) ^ turned));
+            for (int k = 0; k < Shape::STEPS; ++k) b[e][k] = Shape::HELD ? held[e][c * Shape::STEPS + k] : queries[(e * PADDED / 16 + c * Shape::STEPS + k) * 32 + lane];
+        const int at = (c * 4 * Shape::PIECE + t * Shape::PIECE) ^ turned;
 #pragma unroll
-            for (int i = 0; i < Shape::STEPS; ++i) {
-                uint32_t b0, b1;
-                codes_to_halves(w[i], b0, b1);
-                mma_f16(s[j], a[i], b0, b1);
+        for (int i = 0; i < 4; ++i) {
+            const Words<Shape::PIECE> w0 = words_at<Shape::PIECE>(mine + 4 * i * PADDED + at), w1 = words_at<Shape::PIECE>(mine + (4 * i + 2) * PADDED + at);
+#pragma unroll
+            for (int k = 0; k < Shape::STEPS; ++k) {
+                uint32_t a0, a1, a2, a3;
+                codes_to_halves(w0[k], a0, a2);
+                codes_to_halves(w1[k], a1, a3);
+#pragma unroll
+                for (int e = 0; e < EIGHTS; ++e) mma_f16(s[e][i], a0, a1, a2, a3, b[e][k]);
             }
         }
     }
 }
 
-template <int PADDED> __device__ __forceinline__ void take_values(const uint8_t *values, const uint4 (&weights)[4], float (&y)[PADDED / 8][4])
+template <int PADDED, int EIGHTS> __device__ __forceinline__ void take_values(const uint8_t *values, const uint2 (&weights)[EIGHTS][4], float (&y)[EIGHTS][PADDED / 16][4])
 {
     const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const uint8_t *mine = values + g * CACHE_PAGE + 16 * t;
 #pragma unroll
-    for (int d = 0; d < PADDED / 8; ++d) {
-        const Words<16> w = words_at<16>(mine + 8 * d * CACHE_PAGE);
+    for (int d = 0; d < PADDED / 16; ++d) {
+        const Words<16> w0 = words_at<16>(mine + 16 * d * CACHE_PAGE), w1 = words_at<16>(mine + (16 * d + 8) * CACHE_PAGE);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t b0, b1;
-            codes_to_halves(w[i], b0, b1);
-            mma_f16(y[d], weights[i], b0, b1);
+        for (int k = 0; k < 4; ++k) {
+            uint32_t a0, a1, a2, a3;
+            codes_to_halves(w0[k], a0, a2);
+            codes_to_halves(w1[k], a1, a3);
+#pragma unroll
+            for (int e = 0; e < EIGHTS; ++e) mma_f16(y[e][d], a0, a1, a2, a3, weights[e][k]);
         }
     }
 }
 
-// The scores of a page to weights of its values; the running figures go along.  hidden: bit 2 j + e for what row h (0, 1) does not see.
-template <int PADDED, bool MASKED>
-__device__ __forceinline__ void weigh(float (&s)[8][4], const float (&factor)[2], const PageScales &page, const uint32_t (&hidden)[2], Running<PADDED> &run, uint4 (&weights)[4])
+// A page's scores to weights of its values; the running figures go along.  hidden[e][h]: bit 2 i + j for token j of tile i (the lane's two) where row 2 t + h does not see it.
+template <int PADDED, int EIGHTS, bool MASKED>
+__device__ __forceinline__ void weigh(float (&s)[EIGHTS][4][4], const float (&down)[EIGHTS][2], float scale_k, float scale_v, const uint32_t (&hidden)[EIGHTS][2],
+                                      Running<PADDED, EIGHTS> &run, uint2 (&weights)[EIGHTS][4])
 {
-    float largest[2] = {-INFINITY, -INFINITY};
+    const bool none = scale_v == 0.0f, is_nan = scale_v != scale_v;
+    const float log_v = log2f(scale_v);
+    float factor[EIGHTS][2], higher[EIGHTS][2];
+    bool rise = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int e = 0; e < EIGHTS; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int h = i / 2;
-            s[j][i] *= factor[h];
-            if (MASKED && (hidden[h] >> (2 * j + i % 2) & 1u)) s[j][i] = -INFINITY;
-            largest[h] = fmaxf(largest[h], s[j][i]);
+        for (int h = 0; h < 2; ++h) {
+            if (MASKED) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (hidden[e][h] >> (2 * i + j) & 1u) s[e][i][2 * j + h] = -INFINITY;
+            }
+            factor[e][h] = score_factor(down[e][h], scale_k);
+            float most = fmaxf(s[e][0][h], s[e][0][2 + h]);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) most = fmaxf(fmaxf(most, s[e][i][h]), s[e][i][2 + h]);
+            higher[e][h] = most == -INFINITY ? most : most * factor[e][h];
+            rise |= higher[e][h] > run.m[e][h] + LATE || (!none && higher[e][h] + (is_nan ? 0.0f : log_v) > run.top[e][h] + LATE);
         }
-    float base[2], shift[2], old[2];
-    bool far = false;
+    if (__any_sync(~0u, rise)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        largest[h] = fmaxf(largest[h], __shfl_xor_sync(~0u, largest[h], 1));
-        largest[h] = fmaxf(largest[h], __shfl_xor_sync(~0u, largest[h], 2));
-        const float m = fmaxf(run.m[h], largest[h]), top = page.f == 0.0f ? run.top[h] : fmaxf(run.top[h], largest[h] + page.e);
-        run.l[h] *= relative(run.m[h], m);
-        old[h] = relative(run.top[h], top);
-        run.m[h] = m, run.top[h] = top;
-        base[h] = m == -INFINITY ? 0.0f : m;
-        const float from = top == -INFINITY ? 0.0f : top;
-        shift[h] = page.f == 0.0f ? -1e30f : base[h] + page.e - from; // weights: 2^(s - base) 2^shift f
-        far |= shift[h] > 60.0f;
-    }
-    if (__any_sync(~0u, old[0] != 1.0f || old[1] != 1.0f)) {
+        for (int e = 0; e < EIGHTS; ++e) {
+            float old[2];
 #pragma unroll
-        for (int d = 0; d < PADDED / 8; ++d) run.y[d][0] *= old[0], run.y[d][1] *= old[0], run.y[d][2] *= old[1], run.y[d][3] *= old[1];
-    }
-    float w[8][4];
-    if (__any_sync(~0u, far)) { // 2^(s - base) may be 0 where the weight is not
+            for (int h = 0; h < 2; ++h) {
+                float m = higher[e][h];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int h = i / 2;
-                run.l[h] += power_of_two(s[j][i] - base[h]);
-                w[j][i] = power_of_two(s[j][i] - (base[h] - shift[h])) * page.f;
+                for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, o)); // (NaN is passed over)
+                const float top = none ? -INFINITY : m + (is_nan ? 0.0f : log_v), new_m = fmaxf(run.m[e][h], m), new_top = fmaxf(run.top[e][h], top);
+                run.l[e][h] *= relative(run.m[e][h], new_m);
+                old[h] = relative(run.top[e][h], new_top);
+                run.m[e][h] = new_m, run.top[e][h] = new_top;
             }
-    } else {
-        float scale[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) scale[h] = exp2f(shift[h]) * page.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int h = i / 2;
-                const float p = power_of_two(s[j][i] - base[h]);
-                run.l[h] += p;
-                w[j][i] = p * scale[h];
-            }
+            for (int d = 0; d < PADDED / 16; ++d) run.y[e][d][0] *= old[0], run.y[e][d][1] *= old[1], run.y[e][d][2] *= old[0], run.y[e][d][3] *= old[1];
+        }
     }
-    if (MASKED) { // (0 times NaN)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+    for (int e = 0; e < EIGHTS; ++e) {
+        float shift[2], plus[2], from[2];
+        bool far = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            from[h] = run.m[e][h] == -INFINITY ? 0.0f : run.m[e][h];
+            const float from_top = run.top[e][h] == -INFINITY ? 0.0f : run.top[e][h], lv = none ? from_top - from[h] : log_v;
+            shift[h] = lv + from[h] - from_top; // a weight is 2^(s - m) 2^shift
+            plus[h] = lv - from_top;
+            far |= fabsf(shift[h]) > 60.0f;
+        }
+        far = __any_sync(~0u, far);
+        float w[4][4], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int h = j % 2;
+                w[i][j] = power_of_two(fmaf(s[e][i][j], factor[e][h], plus[h]));
+                if (MASKED && (hidden[e][h] >> (2 * i + j / 2) & 1u)) w[i][j] = 0.0f; // (NaN where a factor is 0 or NaN)
+                sum[h] += w[i][j];
+            }
+        if (far) { // either of 2^(s - m) and the weight may be 0 where the other is not
+            sum[0] = sum[1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (hidden[i / 2] >> (2 * j + i % 2) & 1u) w[j][i] = 0.0f;
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        weights[i] = make_uint4(halves_of_floats(w[2 * i][0], w[2 * i][1]), halves_of_floats(w[2 * i][2], w[2 * i][3]), halves_of_floats(w[2 * i + 1][0], w[2 * i + 1][1]),
-                                halves_of_floats(w[2 * i + 1][2], w[2 * i + 1][3]));
-}
-
-// A tile's queries as operand fragments, and each row's factor of scores: lane 4 g + t of step i of chunk c has dimensions d .. d + 3, d = (4 c + t) PIECE + 4 i, of
-// rows g and g + 8.  By the block: eight threads a row.
-template <int PADDED> __device__ __forceinline__ void bring_queries(const Attend &a, const Span &span, const FewTile &tile, int rows, uint32_t *queries, float *down)
-{
-    using Shape = FewShape<PADDED>;
-    const int r = threadIdx.x / 8, part = threadIdx.x % 8, at = tile.first_row + r, width = (int)a.cache.width;
-    const bool there = r < rows;
-    const size_t from = there ? (size_t)(span.row + at / a.group) * a.queries.ld + (size_t)(tile.head * a.group + at % a.group) * a.queries.head_ld : 0;
-    const uint16_t *x = static_cast<const uint16_t *>(a.queries.x) + from;
-    const bool f16 = a.queries.type == VALUE_F16, aligned = (reinterpret_cast<uintptr_t>(x) & 7) == 0;
-    constexpr int FOURS = PADDED / 32; // four dimensions at a time: 4 (8 i + part)
-    float v[FOURS][4];
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < FOURS; ++i) {
-        const int d = 4 * (8 * i + part);
-        uint32_t w[2] = {0, 0};
-        if (there && aligned && d + 4 <= width) {
-            const uint2 q = *reinterpret_cast<const uint2 *>(x + d);
-            w[0] = q.x, w[1] = q.y;
-        } else if (there) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (d + j < width) w[j / 2] |= (uint32_t)x[d + j] << (16 * (j % 2));
+                for (int j = 0; j < 4; ++j) {
+                    const int h = j % 2;
+                    const float p = power_of_two(fmaf(s[e][i][j], factor[e][h], -from[h]));
+                    sum[h] += MASKED && (hidden[e][h] >> (2 * i + j / 2) & 1u) ? 0.0f : p;
+                }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t half = j % 2 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu;
-            v[i][j] = f16 ? __half2float(__ushort_as_half((unsigned short)half)) : __uint_as_float(half << 16);
-            most = max(most, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
-        }
-    }
+        for (int h = 0; h < 2; ++h)
+            if (sum[h] != 0.0f) run.l[e][h] += far ? sum[h] : sum[h] * exp2f(-shift[h]);
 #pragma unroll
-    for (int o = 4; o; o /= 2) most = max(most, __shfl_xor_sync(~0u, most, o));
-    const QueryScale scale(most, a.scale);
-    if (part == 0) down[r] = scale.down;
-#pragma unroll
-    for (int i = 0; i < FOURS; ++i) {
-        const int d = 4 * (8 * i + part), c = d / (4 * Shape::PIECE), t = d / Shape::PIECE % 4, step = d % Shape::PIECE / 4;
-        uint32_t *to = queries + (((c * Shape::STEPS + step) * 32 + 4 * (r % 8) + t) * 4 + r / 8);
-        const bool none = scale.up == 0.0f; // (an infinity or a NaN: 0 times that is none)
-        to[0] = none ? 0u : halves_of_floats(v[i][0] * scale.up, v[i][1] * scale.up);
-        to[2] = none ? 0u : halves_of_floats(v[i][2] * scale.up, v[i][3] * scale.up);
+        for (int i = 0; i < 4; ++i) weights[e][i] = make_uint2(transposed(halves_of_floats(w[i][0], w[i][1])), transposed(halves_of_floats(w[i][2], w[i][3])));
     }
 }
 
-template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ? 2 : 1) attend_few_kernel(const __grid_constant__ ShareParams P)
+// A tile's queries as operand fragments, and each row's factor of scores: lane 4 g + t of step k of chunk c has dimensions d .. d + 3, d = (4 c + t) PIECE + 4 k, of row g of
+// each eight.  By the block: eight threads a row.  A negative scale turns the queries' signs: factors are not negative, and the largest product is the largest score.
+template <int PADDED, int EIGHTS>
+__device__ __forceinline__ void bring_queries(const Attend &a, const Span &span, const Tile<8 * EIGHTS> &tile, int rows, uint2 *queries, float *down)
 {
-    using Shape = FewShape<PADDED>;
+    using Shape = FewShape<PADDED, EIGHTS>;
+    const int part = threadIdx.x % 8, width = (int)a.cache.width;
+    for (int r = threadIdx.x / 8; r < Shape::ROWS; r += THREADS / 8) {
+        const int at = tile.first_row + r;
+        const bool there = r < rows;
+        const size_t from = there ? (size_t)(span.row + at / a.group) * a.queries.ld + (size_t)(tile.head * a.group + at % a.group) * a.queries.head_ld : 0;
+        const uint16_t *x = static_cast<const uint16_t *>(a.queries.x) + from;
+        const bool f16 = a.queries.type == VALUE_F16, aligned = (reinterpret_cast<uintptr_t>(x) & 7) == 0;
+        constexpr int FOURS = PADDED / 32; // four dimensions at a time: 4 (8 i + part)
+        float v[FOURS][4];
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < FOURS; ++i) {
+            const int d = 4 * (8 * i + part);
+            uint32_t w[2] = {0, 0};
+            if (there && aligned && d + 4 <= width) {
+                const uint2 q = *reinterpret_cast<const uint2 *>(x + d);
+                w[0] = q.x, w[1] = q.y;
+            } else if (there) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (d + j < width) w[j / 2] |= (uint32_t)x[d + j] << (16 * (j % 2));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t half = j % 2 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu;
+                v[i][j] = f16 ? __half2float(__ushort_as_half((unsigned short)half)) : __uint_as_float(half << 16);
+                most = max(most, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+            }
+        }
+#pragma unroll
+        for (int o = 4; o; o /= 2) most = max(most, __shfl_xor_sync(~0u, most, o));
+        const QueryScale scale(most, fabsf(a.scale));
+        const float up = a.scale < 0.0f ? -scale.up : scale.up;
+        if (part == 0) down[r] = scale.down;
+#pragma unroll
+        for (int i = 0; i < FOURS; ++i) {
+            const int d = 4 * (8 * i + part), c = d / (4 * Shape::PIECE), t = d / Shape::PIECE % 4, step = d % Shape::PIECE / 4;
+            const bool none = scale.up == 0.0f; // (an infinity or a NaN: 0 times that is none)
+            queries[(r / 8 * PADDED / 16 + c * Shape::STEPS + step) * 32 + 4 * (r % 8) + t] =
+                none ? make_uint2(0, 0) : make_uint2(halves_of_floats(v[i][0] * up, v[i][1] * up), halves_of_floats(v[i][2] * up, v[i][3] * up));
+        }
+    }
+}
+
+template <int PADDED, int EIGHTS> __global__ void __launch_bounds__(THREADS, FewShape<PADDED, EIGHTS>::BLOCKS) attend_few_kernel(const __grid_constant__ ShareParams P)
+{
+    using Shape = FewShape<PADDED, EIGHTS>;
+    constexpr int ROWS = Shape::ROWS;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ FewPlan::Room room;
+    __shared__ typename Shape::Sharing::Room room;
     __shared__ unsigned long long full[WARPS][STAGES];
     __shared__ float down[ROWS], figures[WARPS][3][ROWS], final_figures[3][ROWS];
     __shared__ int abort_word;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     uint8_t *ring = smem + (size_t)warp * STAGES * Shape::HALF;
-    uint32_t *queries = reinterpret_cast<uint32_t *>(smem + (size_t)WARPS * STAGES * Shape::HALF);
+    uint2 *queries = reinterpret_cast<uint2 *>(smem + Shape::RING);
     if (threadIdx.x == 0) abort_word = 0;
     if (lane < STAGES) mbar_init(&full[warp][lane], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -242,15 +286,17 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
             put_value(a.y, (r < (size_t)front ? r : r - front + behind) * a.y.ld + rest / width * a.y.head_ld + rest % width, 0.0f);
         }
     }
-    const FewPlan plan(P, room);
+    const typename Shape::Sharing plan(P, room);
     const long long start = plan.share * blockIdx.x, end = min(start + plan.share, plan.total);
-    int st = 0;          // of the ring, and how often it went round
+    if (start >= end && threadIdx.x == 0) plan.tell(nullptr, 0, 0);
+    int st = 0; // of the ring, and how often it went round
     uint32_t parity = 0;
     for (long long x = start; x < end;) {
-        FewTile tile;
+        Tile<ROWS> tile;
         if (!plan.find(x, tile)) break;
         const Span span(a.seq, tile.b);
         const int rows = min(span.count * a.group - tile.first_row, ROWS);
+        if (x == start && threadIdx.x == 0) plan.tell(&tile, span.row, rows);
         const int p0 = span.first + tile.first_row / a.group, p1 = span.first + (tile.first_row + rows - 1) / a.group;
         const Pages pages(p0, p1, span.keys, a.window, a.sinks);
         const int first = (int)(x - tile.begin), behind = (int)(min(end, tile.begin + tile.units) - tile.begin); // units
@@ -258,18 +304,17 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
         const int many = last > from + warp ? (last - from - warp + WARPS - 1) / WARPS : 0; // pages of this warp: from + warp + WARPS i
 
         // where the next 32 pages are, a lane each, and the 32 behind them
-        int page_now, page_next;
-        float2 scales_now, scales_next;
+        int page_now, page_next = -1;
+        float2 scales_now, scales_next = make_float2(0.0f, 0.0f);
         auto look = [&](int i0, int &page, float2 &scales) {
             const int i = i0 + lane;
             page = i < many ? page_of(a.seq, c.pages, tile.b, pages.column(from + warp + WARPS * i)) : -1;
             scales = page >= 0 ? *reinterpret_cast<const float2 *>(c.scales + ((size_t)page * c.heads + tile.head) * 2) : make_float2(0.0f, 0.0f);
         };
         look(0, page_now, scales_now);
-        page_next = -1, scales_next = scales_now;
         if (many > 32) look(32, page_next, scales_next);
-        // half 2 i: keys of page i, 2 i + 1: its values
-        auto fetch = [&](int half, int stage, int block) { // block: i / 32 of page_now
+        // half 2 i: keys of page i, 2 i + 1: its values; block: i / 32 of page_now
+        auto fetch = [&](int half, int stage, int block) {
             const int i = half / 2, page = __shfl_sync(~0u, i / 32 == block ? page_now : page_next, i % 32);
             if (lane == 0 && i < many) {
                 if (page >= 0) {
@@ -284,42 +329,55 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
             fetch(k, stage, 0);
             if (++stage == STAGES) stage = 0;
         }
-        bring_queries<PADDED>(a, span, tile, rows, queries, down);
+        bring_queries<PADDED, EIGHTS>(a, span, tile, rows, queries, down);
         __syncthreads();
-        Running<PADDED> run;
+        Running<PADDED, EIGHTS> run;
+        float mine[EIGHTS][2];
+        int position[EIGHTS][2];
+        uint2 held[EIGHTS][PADDED / 16];
 #pragma unroll
-        for (int d = 0; d < PADDED / 8; ++d) run.y[d][0] = run.y[d][1] = run.y[d][2] = run.y[d][3] = 0.0f;
-        run.m[0] = run.m[1] = run.top[0] = run.top[1] = -INFINITY, run.l[0] = run.l[1] = 0.0f;
-        const float mine[2] = {down[g], down[g + 8]};
-        const int position[2] = {span.first + (tile.first_row + min(g, rows - 1)) / a.group, span.first + (tile.first_row + min(g + 8, rows - 1)) / a.group};
+        for (int e = 0; e < EIGHTS; ++e) {
+#pragma unroll
+            for (int d = 0; d < PADDED / 16; ++d) run.y[e][d][0] = run.y[e][d][1] = run.y[e][d][2] = run.y[e][d][3] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 8 * e + 2 * t + h;
+                run.m[e][h] = run.top[e][h] = -INFINITY, run.l[e][h] = 0.0f;
+                mine[e][h] = down[r], position[e][h] = span.first + (tile.first_row + min(r, rows - 1)) / a.group;
+            }
+            if (Shape::HELD) {
+#pragma unroll
+                for (int k = 0; k < PADDED / 16; ++k) held[e][k] = queries[(e * PADDED / 16 + k) * 32 + lane];
+            }
+        }
         for (int i = 0; i < many; ++i) {
             const int page = __shfl_sync(~0u, page_now, i % 32);
-            const float2 both = make_float2(__shfl_sync(~0u, scales_now.x, i % 32), __shfl_sync(~0u, scales_now.y, i % 32));
-            uint4 weights[4];
+            const float scale_k = __shfl_sync(~0u, scales_now.x, i % 32), scale_v = __shfl_sync(~0u, scales_now.y, i % 32);
+            uint2 weights[EIGHTS][4];
             if (!__all_sync(~0u, mbar_wait(&full[warp][st], parity, &abort_word, P.error, 91))) break;
-            if (page >= 0) {
-                float s[8][4];
-                take_keys<PADDED>(ring + st * Shape::HALF, reinterpret_cast<const uint4 *>(queries), s);
-                const PageScales scales(both);
-                const float factor[2] = {score_factor(mine[0], scales.k), score_factor(mine[1], scales.k)};
-                const int column = pages.column(from + warp + WARPS * i);
-                uint32_t hidden[2] = {0, 0};
-                if (all_seen(column, p0, p1, span.keys, a.window, a.sinks)) {
-                    weigh<PADDED, false>(s, factor, scales, hidden, run, weights);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            if (!seen(column * CACHE_PAGE + 16 * t + j, position[h], span.keys, a.window, a.sinks)) hidden[h] |= 1u << j;
-                    weigh<PADDED, true>(s, factor, scales, hidden, run, weights);
-                }
-            }
+            float s[EIGHTS][4][4];
+            if (page >= 0) take_keys<PADDED, EIGHTS>(ring + st * Shape::HALF, queries, held, s);
             __syncwarp();
             fetch(2 * i + STAGES, st, i / 32);
             if (++st == STAGES) st = 0, parity ^= 1u;
+            if (page >= 0) {
+                const int column = pages.column(from + warp + WARPS * i);
+                uint32_t hidden[EIGHTS][2] = {};
+                if (all_seen(column, p0, p1, span.keys, a.window, a.sinks)) {
+                    weigh<PADDED, EIGHTS, false>(s, mine, scale_k, scale_v, hidden, run, weights);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < EIGHTS; ++e)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (!seen(column * CACHE_PAGE + 16 * (g >> 1) + (g & 1) + 2 * j, position[e][h], span.keys, a.window, a.sinks)) hidden[e][h] |= 1u << j;
+                    weigh<PADDED, EIGHTS, true>(s, mine, scale_k, scale_v, hidden, run, weights);
+                }
+            }
             if (!__all_sync(~0u, mbar_wait(&full[warp][st], parity, &abort_word, P.error, 92))) break;
-            if (page >= 0) take_values<PADDED>(ring + st * Shape::HALF, weights, run.y);
+            if (page >= 0) take_values<PADDED, EIGHTS>(ring + st * Shape::HALF, weights, run.y);
             __syncwarp();
             fetch(2 * i + 1 + STAGES, st, i / 32);
             if (++st == STAGES) st = 0, parity ^= 1u;
@@ -330,23 +388,28 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
         }
         // the warps' figures together, in the place of the ring (all that was asked for has come)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            run.l[h] += __shfl_xor_sync(~0u, run.l[h], 1);
-            run.l[h] += __shfl_xor_sync(~0u, run.l[h], 2);
-            if (t == 0) figures[warp][0][g + 8 * h] = run.m[h], figures[warp][1][g + 8 * h] = run.top[h], figures[warp][2][g + 8 * h] = run.l[h];
-        }
+        for (int e = 0; e < EIGHTS; ++e)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int o = 4; o < 32; o *= 2) run.l[e][h] += __shfl_xor_sync(~0u, run.l[e][h], o);
+                const int r = 8 * e + 2 * t + h;
+                if (g == 0) figures[warp][0][r] = run.m[e][h], figures[warp][1][r] = run.top[e][h], figures[warp][2][r] = run.l[e][h];
+            }
         __syncthreads();
-        float *sum = reinterpret_cast<float *>(ring); // ROWS x PADDED, of this warp: as many bytes as a stage
+        float *sum = reinterpret_cast<float *>(ring); // ROWS x PADDED, of this warp
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float top = -INFINITY;
+        for (int e = 0; e < EIGHTS; ++e)
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, figures[w][1][g + 8 * h]);
-            const float by = relative(run.top[h], top);
+            for (int h = 0; h < 2; ++h) {
+                const int r = 8 * e + 2 * t + h;
+                float top = -INFINITY;
 #pragma unroll
-            for (int d = 0; d < PADDED / 8; ++d)
-                *reinterpret_cast<float2 *>(sum + (g + 8 * h) * PADDED + 8 * d + 2 * t) = make_float2(run.y[d][2 * h] * by, run.y[d][2 * h + 1] * by);
-        }
+                for (int w = 0; w < WARPS; ++w) top = fmaxf(top, figures[w][1][r]);
+                const float by = relative(run.top[e][h], top);
+#pragma unroll
+                for (int d = 0; d < PADDED / 16; ++d) sum[r * PADDED + 16 * d + g] = run.y[e][d][h] * by, sum[r * PADDED + 16 * d + 8 + g] = run.y[e][d][2 + h] * by;
+            }
         if (threadIdx.x < ROWS) {
             float m = -INFINITY, top = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -380,19 +443,35 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, PADDED <= 128 ?
         for (int w = 0; w < 1000; ++w) __nanosleep(1000);
 }
 
-template <int PADDED> void attend_few_with(CudaDevice &dev, const ShareParams &P, bool join)
+template <int PADDED, int EIGHTS> void attend_few_with(CudaDevice &dev, ShareParams &P)
 {
-    const size_t smem = FewShape<PADDED>::SMEM + 128;
-    allow_shared_memory(dev, attend_few_kernel<PADDED>);
+    using Shape = FewShape<PADDED, EIGHTS>;
+    constexpr int ROWS = Shape::ROWS;
+    const Attend &a = P.a;
+    P.slots = (int)slots_of<ROWS>(a);
+    size_t pages = std::max(a.seq.columns, 1); // of a tile at most
+    if (a.window) pages = std::min(pages, ((size_t)a.sinks + 63) / 64 + ((size_t)a.window + ROWS + 62) / CACHE_PAGE + 1);
+    const size_t rounds = (pages + WARPS - 1) / WARPS;
+    const bool join = rounds > 4;
+    P.unit = (int)(join ? WARPS : rounds * WARPS);
+    const size_t units = (size_t)P.slots * a.cache.heads * (join ? rounds : 1), places = (size_t)dev.sm_count() * Shape::BLOCKS;
+    P.blocks = (int)std::min(units, places);
+    Parts parts(dev);
+    if (join) parts.make<ROWS>(P, PADDED);
+    allow_shared_memory(dev, attend_few_kernel<PADDED, EIGHTS>);
     {
         KernelScope ks(dev, "attend_few");
-        launch_following(attend_few_kernel<PADDED>, dim3((unsigned)P.blocks), dim3(THREADS), smem, dev.stream(), P);
+        launch_following(attend_few_kernel<PADDED, EIGHTS>, dim3((unsigned)P.blocks), dim3(THREADS), Shape::SMEM + 128, dev.stream(), P);
         dev.count_launch();
     }
-    if (!join) return;
-    KernelScope ks(dev, "attend_join");
-    launch_following(attend_join_kernel<PADDED, ROWS>, dim3((unsigned)std::min(P.blocks * ROWS / 4, 4 * dev.sm_count())), dim3(128), 0, dev.stream(), P);
-    dev.count_launch();
+    launch_join<PADDED, ROWS>(dev, P);
+}
+
+template <int PADDED> void attend_few_width(CudaDevice &dev, ShareParams &P)
+{
+    const size_t rows = (size_t)P.a.seq.n * P.a.group;
+    if (!P.a.seq.offsets && rows / P.a.seq.sequences <= 8) attend_few_with<PADDED, 1>(dev, P);
+    else attend_few_with<PADDED, 2>(dev, P);
 }
 
 } // namespace
@@ -400,31 +479,16 @@ template <int PADDED> void attend_few_with(CudaDevice &dev, const ShareParams &P
 void launch_attend_few(CudaDevice &dev, const Attend &a)
 {
     ShareParams P{};
-    P.a = a, P.error = dev.error_word();
-    P.least = 0, P.most = ATTEND_FEW, P.slots = (int)slots_of<ROWS>(a);
-    const size_t padded = a.cache.padded;
-    size_t pages = std::max(a.seq.columns, 1); // of a tile at most
-    if (a.window) pages = std::min(pages, ((size_t)a.sinks + 63) / 64 + ((size_t)a.window + ROWS + 62) / CACHE_PAGE + 1);
-    const size_t rounds = (pages + WARPS - 1) / WARPS;
-    const bool join = rounds > 4;
-    P.unit = (int)(join ? WARPS : rounds * WARPS);
-    const size_t units = (size_t)P.slots * a.cache.heads * (join ? rounds : 1), places = (size_t)dev.sm_count() * (padded <= 128 ? 2 : 1);
-    P.blocks = (int)std::min(units, places);
-    struct Parts {
-        CudaDevice &dev;
-        void *p;
-        ~Parts() { dev.release(p); }
-    } parts{dev, join ? dev.alloc(2 * (size_t)P.blocks * part_floats<ROWS>((int)padded) * sizeof(float)) : nullptr};
-    P.parts = static_cast<float *>(parts.p);
-    switch (padded / 32) {
-    case 1: return attend_few_with<32>(dev, P, join);
-    case 2: return attend_few_with<64>(dev, P, join);
-    case 3: return attend_few_with<96>(dev, P, join);
-    case 4: return attend_few_with<128>(dev, P, join);
-    case 5: return attend_few_with<160>(dev, P, join);
-    case 6: return attend_few_with<192>(dev, P, join);
-    case 7: return attend_few_with<224>(dev, P, join);
-    default: return attend_few_with<256>(dev, P, join);
+    P.a = a, P.error = dev.error_word(), P.least = 0, P.most = ATTEND_FEW;
+    switch (a.cache.padded / 32) {
+    case 1: return attend_few_width<32>(dev, P);
+    case 2: return attend_few_width<64>(dev, P);
+    case 3: return attend_few_width<96>(dev, P);
+    case 4: return attend_few_width<128>(dev, P);
+    case 5: return attend_few_width<160>(dev, P);
+    case 6: return attend_few_width<192>(dev, P);
+    case 7: return attend_few_width<224>(dev, P);
+    default: return attend_few_width<256>(dev, P);
     }
 }
 
