@@ -1,19 +1,20 @@
 // attend_many.cu -- attention of many rows of a sequence (prompts) over a cache of 8-bit codes, on the tensor cores (tcgen05, kind::f16).
 //
-// Rows that share a cached head (query heads of a token, then those of the next one) are taken 256 at a time (128 for heads of more than 128 values), over 128 tokens, two pages,
+// Rows that share a cached head (query heads of a token, then those of the next one) are taken 256 at a time (128 for heads of more than 128 values), over one page of 64 tokens
 // a step.  The codes become f16 numbers on their way into shared memory; scores and sums of values are in tensor memory, and so are the weights between the two products.
 //
+//   warp 0          issues the products: for each half of the rows weights times values of a step, then queries times keys of the step after the next one, so that the next
+//                   scores are there when a half's weights are done.  (With 128 tokens a step and room for one step's scores, each half waited for its products after every
+//                   step: 8192 tokens x 32 heads x 128 took 1.05 ms.)
 //   warp 1          finds what the block takes next, and tells the others ahead of time
-//   warp 0          issues the products: for each half of the rows weights times values of a step, then the next step's queries times keys, so that one half's
-//                   products run while the other half's scores become weights
-//   warps 4 .. 7    codes of a step's keys, then of its values, to operand tiles (128-byte rows, 128-byte swizzle); the next ones are on their way from memory meanwhile
+//   warps 2 .. 7    codes of a page's keys, or values, to operand tiles (128-byte rows, 128-byte swizzle); the next ones are on their way from memory meanwhile
 //   warps 8 .. 15   four for each half of the rows, a row a thread: scores to weights, largest score and sum; queries in, results out.  They take most of the registers
-//                   (setmaxnreg: 56 + 88 + 2 x 184 a thread of each four warps, of 4 x 128): a row's 128 scores are read from tensor memory once
+//                   (setmaxnreg: 2 x 96 + 2 x 160 a thread of each four warps, of 4 x 128)
 //
 // What bounds it is the tensor cores' rate (4 x width operations for each row and token) and, as much, the exponentials: 16 an SM and cycle.
 //
-// The largest score that weights are relative to stays as it is until a row has one 2^8 times as large; then the row's sums in tensor memory, which nobody
-// is adding to at that time, are brought down.  Weights are up to 2^8 until then, and f16 numbers all the same.
+// The largest score that weights are relative to stays as it is until a row has one 2^8 times as large; then the row's sums in tensor memory are brought down, once the product
+// that adds to them is done.  Weights are up to 2^8 until then, and f16 numbers all the same.
 //
 // Blocks share out all tiles' steps as those of attend_few.cu do their pages.
 #include <algorithm>
@@ -28,21 +29,22 @@ namespace vqb {
 
 namespace {
 
-constexpr int THREADS = 512, STEP = 2 * CACHE_PAGE; // tokens of a step
-constexpr float LATE = 8.0f;                        // a row's largest is followed when it is 2^LATE times as large
+constexpr int THREADS = 512, STEP = CACHE_PAGE; // tokens of a step
+constexpr float LATE = 8.0f;                    // a row's largest is followed when it is 2^LATE times as large
+constexpr int CONVERTERS = 6;                   // warps
 
 template <int PADDED> struct ManyShape {
     static constexpr int HALVES = PADDED <= 128 ? 2 : 1, ROWS = 128 * HALVES;
-    static constexpr int BLOCKS = (PADDED + 63) / 64;             // of 64 dimensions: a swizzled row of an operand tile
-    static constexpr uint32_t QUERIES = BLOCKS * 128 * 128;       // bytes of one half's queries
-    static constexpr uint32_t STAGE = BLOCKS * 128 * 128;         // of a step's keys; of its values (2 x PADDED rows of 128 bytes) as much or less
-    static constexpr int STAGES = PADDED <= 128 ? 4 : 2;
+    static constexpr int BLOCKS = (PADDED + 63) / 64;       // of 64 dimensions: a swizzled row of an operand tile
+    static constexpr uint32_t QUERIES = BLOCKS * 128 * 128; // bytes of one half's queries
+    static constexpr uint32_t STAGE = BLOCKS * STEP * 128;  // of a page's keys; of its values (PADDED rows of 128 bytes) as much or less
+    static constexpr int STAGES = PADDED <= 128 ? 8 : 4;
     static constexpr size_t SMEM = HALVES * QUERIES + STAGES * STAGE + 1024;
-    static constexpr uint32_t SCORES = 128, SUMS = 256; // columns of tensor memory: half h's scores from 128 h, sums from 256 + 128 h
+    static constexpr uint32_t SUMS = 256; // columns of tensor memory: half h's scores of step i from 128 h + 64 (i % 2), sums from 256 + 128 h
 };
 
 struct alignas(8) ManyBarriers {
-    unsigned long long full[4], empty[4], queries[2], scores[2], weights[2], sums[2], told[2], heard[2];
+    unsigned long long full[8], empty[8], queries[2], scores[2][2], weights[2][2], added[2], sums[2], told[2], heard[2];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -143,7 +145,7 @@ __device__ __forceinline__ void tell_parts(const ShareParams &P, const Plan<Many
             // the first P.extra units stand for what a tile takes beside its steps
             const int first = (int)(x - tile.begin), behind = (int)(min(end, tile.begin + tile.units) - tile.begin);
             work.from = 2 * max(first - P.extra, 0);
-            work.steps = (max(min(2 * max(behind - P.extra, 0), pages.count) - work.from, 0) + 1) / 2;
+            work.steps = max(min(2 * max(behind - P.extra, 0), pages.count) - work.from, 0);
             work.begins = x == start, work.whole = first == 0 && behind == tile.units;
             if (x == start && lane == 0) plan.tell(&tile, span.row, work.rows);
             x = tile.begin + behind;
@@ -227,53 +229,72 @@ __device__ __forceinline__ void issue_products(const ShareParams &P, ManyBarrier
     volatile int *abort_flag = &bars.abort_flag;
     const bool leader = elect_one(); // the one lane that knows the following
     int st = 0;
-    uint32_t parity = 0, weights_parity[2] = {0, 0}, queries_parity[2] = {0, 0}; // parity: of the ring's round
+    uint32_t parity = 0, weights_parity[2] = {0, 0}, queries_parity[2] = {0, 0}; // parity: of the ring's round; bit b of weights_parity[h]: of the next weights in buffer b
     bool ok = true;
     Listener listener{room, bars, P.error};
     for (Work work; listener.next(work);) {
         if (work.steps == 0) continue;
         const int halves = work.rows > 128 ? 2 : 1;
         if (leader) {
-            auto keys_times = [&](int h) {
-                const uint64_t q = smem_desc_sw128(smem_u32(queries + h * Shape::QUERIES)), k = smem_desc_sw128(smem_u32(ring + st * Shape::STAGE));
-#pragma unroll
-                for (int i = 0; i < PADDED / 16; ++i)
-                    umma_smem<idesc_f16(STEP)>(tmem + Shape::SCORES * h, q + (i / 4) * 1024 + (i % 4) * 2, k + (i / 4) * 1024 + (i % 4) * 2, i > 0);
-                umma_commit(&bars.scores[h]);
-            };
             auto next_stage = [&] {
                 if (++st == STAGES) st = 0, parity ^= 1u;
             };
-            ok = mbar_wait(&bars.full[st], parity, abort_flag, P.error, 101);
-            for (int h = 0; ok && h < halves; ++h) {
-                ok = mbar_wait(&bars.queries[h], queries_parity[h], abort_flag, P.error, 102);
-                queries_parity[h] ^= 1u;
-                tmem_after();
-                if (ok) keys_times(h);
-            }
-            if (ok) umma_commit(&bars.empty[st]);
-            next_stage();
-            for (int i = 0; ok && i < work.steps; ++i) {
-                const bool more = i + 1 < work.steps;
-                const int values_at = st;
-                ok = mbar_wait(&bars.full[st], parity, abort_flag, P.error, 103);
-                next_stage();
-                if (ok && more) ok = mbar_wait(&bars.full[st], parity, abort_flag, P.error, 104);
-                for (int h = 0; ok && h < halves; ++h) {
-                    ok = mbar_wait(&bars.weights[h], weights_parity[h], abort_flag, P.error, 105);
-                    if (!ok) break;
-                    weights_parity[h] ^= 1u;
-                    tmem_after();
-                    const uint64_t v = smem_desc_sw128(smem_u32(ring + values_at * Shape::STAGE));
+            auto stage_there = [&] { return mbar_wait(&bars.full[st], parity, abort_flag, P.error, 101); };
+            auto keys_times = [&](int h, int buffer) {
+                const uint64_t q = smem_desc_sw128(smem_u32(queries + h * Shape::QUERIES)), k = smem_desc_sw128(smem_u32(ring + st * Shape::STAGE));
+                const uint32_t to = tmem + 128 * h + 64 * buffer;
 #pragma unroll
-                    for (int k = 0; k < STEP / 16; ++k)
-                        umma_tmem<idesc_f16(PADDED)>(tmem + Shape::SUMS + 128 * h, tmem + Shape::SCORES * h + 8 * k, v + (k / 4) * (PADDED * 128 / 16) + (k % 4) * 2, i + k > 0);
-                    // (instructions of one thread run in the order they were issued: the next scores do not overtake the weights that they take the place of)
-                    if (more) keys_times(h);
-                    else umma_commit(&bars.sums[h]);
+                for (int i = 0; i < PADDED / 16; ++i) umma_smem<idesc_f16(STEP)>(to, q + (i / 4) * 1024 + (i % 4) * 2, k + (i / 4) * (STEP * 128 / 16) + (i % 4) * 2, i > 0);
+                umma_commit(&bars.scores[h][buffer]);
+            };
+            auto values_times = [&](int h, int buffer, bool add) {
+                const uint64_t v = smem_desc_sw128(smem_u32(ring + st * Shape::STAGE));
+                const uint32_t from = tmem + 128 * h + 64 * buffer;
+#pragma unroll
+                for (int k = 0; k < STEP / 16; ++k) umma_tmem<idesc_f16(PADDED)>(tmem + Shape::SUMS + 128 * h, from + 8 * k, v + k * 2, add || k > 0);
+                umma_commit(&bars.added[h]);
+            };
+            // the first two steps' scores
+            for (int i = 0; ok && i < min(work.steps, 2); ++i) {
+                ok = stage_there();
+                for (int h = 0; ok && h < halves; ++h) {
+                    if (i == 0) {
+                        ok = mbar_wait(&bars.queries[h], queries_parity[h], abort_flag, P.error, 102);
+                        queries_parity[h] ^= 1u;
+                        if (!ok) break;
+                    }
+                    tmem_after();
+                    keys_times(h, i);
+                }
+                if (ok) umma_commit(&bars.empty[st]);
+                next_stage();
+            }
+            for (int i = 0; ok && i < work.steps; ++i) {
+                const int buffer = i & 1, values_at = st;
+                const bool more = i + 2 < work.steps;
+                ok = stage_there();
+                if (ok && more) { // (the keys are behind the values in the ring)
+                    next_stage();
+                    ok = stage_there();
+                    if (--st < 0) st = STAGES - 1, parity ^= 1u;
+                }
+                for (int h = 0; ok && h < halves; ++h) {
+                    ok = mbar_wait(&bars.weights[h][buffer], weights_parity[h] >> buffer & 1u, abort_flag, P.error, 103);
+                    if (!ok) break;
+                    weights_parity[h] ^= 1u << buffer;
+                    tmem_after();
+                    values_times(h, buffer, i > 0);
+                    if (i + 1 == work.steps) umma_commit(&bars.sums[h]);
+                    // (instructions of one thread run in the order they were issued: the scores do not overtake the weights that they take the place of)
+                    if (more) {
+                        next_stage();
+                        keys_times(h, buffer);
+                        if (--st < 0) st = STAGES - 1, parity ^= 1u;
+                    }
                 }
                 if (!ok) break;
                 umma_commit(&bars.empty[values_at]);
+                next_stage();
                 if (more) {
                     umma_commit(&bars.empty[st]);
                     next_stage();
@@ -296,74 +317,82 @@ __device__ __forceinline__ void bring_codes(const ShareParams &P, ManyBarriers &
     volatile int *abort_flag = &bars.abort_flag;
     const Attend &a = P.a;
     [[maybe_unused]] const Cache &c = a.cache;
-    // codes to operand tiles
-    const int t = threadIdx.x - 128; // of 128
-    constexpr int PIECES = STEP * PADDED / 16 / 128, PER_ROW = PADDED / 16; // of 16 codes; a thread's, and those of a token's key
+    const int t = threadIdx.x - 64; // of the converters' threads
+    constexpr int THREADS_HERE = 32 * CONVERTERS, ALL = STEP * PADDED / 16, PIECES = (ALL + THREADS_HERE - 1) / THREADS_HERE; // pieces of 16 codes of a page, and a thread's
+    constexpr int PER_ROW = PADDED / 16;                                                                                     // of a token's key
     int st = 0;
     uint32_t parity = 0;
     bool ok = true;
-    constexpr int DEPTH = PADDED <= 64 ? 2 : 1; // half steps whose codes are on their way
-    uint4 piece[DEPTH][PIECES];
+    uint4 piece[2][PIECES]; // keys, values that come next
     const uint4 zeros = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
     Listener listener{room, bars, P.error};
     for (Work work; ok && listener.next(work);) {
         if (work.steps == 0) continue;
-        int look_now = work.page(a, lane), look_next = work.steps > 16 ? work.page(a, 32 + lane) : -1; // the next 32 pages, and the 32 behind them, a lane each
-        auto load = [&](uint4 (&to)[PIECES], int step, int which, bool behind) {
-            const int from = behind ? look_next : look_now, first = __shfl_sync(~0u, from, 2 * step % 32), second = __shfl_sync(~0u, from, 2 * step % 32 + 1);
-            const uint8_t *start[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) start[k] = c.codes + (((size_t)max(k ? second : first, 0) * c.heads + work.head) * 2 + which) * CACHE_PAGE * PADDED;
+        int look_now = work.page(a, lane), look_next = work.steps > 32 ? work.page(a, 32 + lane) : -1; // the pages of 32 steps, and the 32 behind them, a lane each
+        int looked = 0;                                                                                // look_now's first step
+        auto load = [&](int step, int which) {
+            const int page = __shfl_sync(~0u, step - looked >= 32 ? look_next : look_now, step % 32);
+            const uint8_t *from = c.codes + (((size_t)max(page, 0) * c.heads + work.head) * 2 + which) * CACHE_PAGE * PADDED;
 #pragma unroll
             for (int k = 0; k < PIECES; ++k) {
-                const int at = t + 128 * k, half = at / (STEP * PADDED / 32); // (pieces of a page: 64 PADDED / 16)
-                to[k] = (half ? second : first) < 0 ? zeros : *reinterpret_cast<const uint4 *>((half ? start[1] : start[0]) + (at - half * (STEP * PADDED / 32)) * 16);
+                const int at = t + THREADS_HERE * k;
+                if (ALL % THREADS_HERE && at >= ALL) continue;
+                piece[which][k] = page < 0 ? zeros : *reinterpret_cast<const uint4 *>(from + at * 16);
             }
         };
-        load(piece[0], 0, 0, false);
-        if (DEPTH == 2) load(piece[DEPTH - 1], 0, 1, false);
-        for (int i = 0; ok && i < work.steps; ++i) {
+        auto convert = [&](int which) {
+            if (!__all_sync(~0u, mbar_wait(&bars.empty[st], parity ^ 1u, abort_flag, P.error, 106))) return false;
+            uint8_t *to = ring + st * Shape::STAGE;
 #pragma unroll
-            for (int which = 0; which < 2; ++which) { // keys, values
-                if (!__all_sync(~0u, mbar_wait(&bars.empty[st], parity ^ 1u, abort_flag, P.error, 106))) {
-                    ok = false;
-                    break;
+            for (int k = 0; k < PIECES; ++k) {
+                const int at = t + THREADS_HERE * k;
+                if (ALL % THREADS_HERE && at >= ALL) continue;
+                int row, chunk; // of 128 bytes; the first of two pieces of 16 bytes
+                uint8_t *part = to;
+                bool turned = false; // second piece first: lanes that write at once find different banks
+                if (which == 0) {
+                    row = at / PER_ROW; // token
+                    int p = at % PER_ROW;
+                    if (PADDED % 128 == 0) p ^= (row & 1) * 4;
+                    part += p / 4 * (STEP * 128), chunk = 2 * (p % 4), turned = p / 4 % 2;
+                } else {
+                    row = at / 4, chunk = 2 * (at % 4); // dimension
                 }
-                uint4(&mine)[PIECES] = piece[which % DEPTH];
-                uint8_t *to = ring + st * Shape::STAGE;
-#pragma unroll
-                for (int k = 0; k < PIECES; ++k) {
-                    const int at = t + 128 * k;
-                    int row, chunk; // of 128 bytes; the first of two pieces of 16 bytes
-                    uint8_t *part = to;
-                    bool turned = false; // second piece first: lanes that write at once find different banks
-                    if (which == 0) {
-                        row = at / PER_ROW; // token of the step
-                        int p = at % PER_ROW;
-                        if (PADDED % 128 == 0) p ^= (row & 1) * 4;
-                        part += p / 4 * 16384, chunk = 2 * (p % 4), turned = p / 4 % 2;
-                    } else {
-                        row = at / 4, chunk = 2 * (at % 4); // dimension; the second page's behind the first one's
-                    }
-                    uint4 first, second;
-                    codes_to_halves(mine[k].x, first.x, first.y);
-                    codes_to_halves(mine[k].y, first.z, first.w);
-                    codes_to_halves(mine[k].z, second.x, second.y);
-                    codes_to_halves(mine[k].w, second.z, second.w);
-                    uint8_t *at_row = part + row * 128;
-                    *reinterpret_cast<uint4 *>(at_row + ((chunk + turned) ^ (row & 7)) * 16) = turned ? second : first;
-                    *reinterpret_cast<uint4 *>(at_row + ((chunk + !turned) ^ (row & 7)) * 16) = turned ? first : second;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.full[st]);
-                if (++st == STAGES) st = 0, parity ^= 1u;
-                if (DEPTH == 1 && which == 0) load(mine, i, 1, false);
-                else if (i + 1 < work.steps) load(mine, i + 1, DEPTH == 2 ? which : 0, i % 16 == 15);
+                const uint4 w = piece[which][k];
+                uint4 first, second;
+                codes_to_halves(w.x, first.x, first.y);
+                codes_to_halves(w.y, first.z, first.w);
+                codes_to_halves(w.z, second.x, second.y);
+                codes_to_halves(w.w, second.z, second.w);
+                uint8_t *at_row = part + row * 128;
+                *reinterpret_cast<uint4 *>(at_row + ((chunk + turned) ^ (row & 7)) * 16) = turned ? second : first;
+                *reinterpret_cast<uint4 *>(at_row + ((chunk + !turned) ^ (row & 7)) * 16) = turned ? first : second;
             }
-            if (i % 16 == 15) {
-                look_now = look_next;
-                look_next = work.page(a, 2 * i + 34 + lane);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.full[st]);
+            if (++st == STAGES) st = 0, parity ^= 1u;
+            return true;
+        };
+        // keys 0, keys 1, values 0, keys 2, values 1, ..: the order in which they are multiplied
+        load(0, 0);
+        load(0, 1);
+        ok = convert(0);
+        if (ok && work.steps > 1) {
+            load(1, 0);
+            ok = convert(0);
+        }
+        if (work.steps > 2) load(2, 0);
+        for (int i = 0; ok && i < work.steps; ++i) {
+            ok = convert(1);
+            if (i + 1 < work.steps) load(i + 1, 1);
+            if (ok && i + 2 < work.steps) {
+                ok = convert(0);
+                if (i + 3 < work.steps) load(i + 3, 0);
+            }
+            if (i - looked == 30) { // (the next one to be asked for is looked + 32)
+                looked += 32, look_now = look_next;
+                look_next = work.page(a, looked + 32 + lane);
             }
         }
     }
@@ -379,8 +408,8 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
     const Attend &a = P.a;
     [[maybe_unused]] const Cache &c = a.cache;
     const int h = (warp - 8) / 4, r = (warp % 4) * 32 + lane; // half, row of it
-    const uint32_t lanes = (uint32_t)(warp % 4) << 21, scores = tmem + lanes + Shape::SCORES * h, sums = tmem + lanes + Shape::SUMS + 128 * h; // (lane 32 q: bits 16 ..)
-    uint32_t step_parity = 0, sums_parity = 0;
+    const uint32_t lanes = (uint32_t)(warp % 4) << 21, sums = tmem + lanes + Shape::SUMS + 128 * h; // (lane 32 q: bits 16 ..)
+    uint32_t scores_parity = 0, added_parity = 0, sums_parity = 0; // scores_parity: bit b of the next scores in buffer b; added_parity: of this step's product
     if (h >= HALVES) return;
     bool ok = true;
     Listener listener{room, bars, P.error};
@@ -391,7 +420,7 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
         float m = -INFINITY, top = -INFINITY, l = 0.0f;
         const bool taken = work.steps > 0 && 128 * h < work.rows;
         if (taken) {
-            // where the next 32 pages are, with s_k and log2(s_v) (-infinity: values of 0), a lane each
+            // the pages of 32 steps with s_k and log2(s_v) (-infinity: values of 0), a lane each, and the 32 behind them
             auto look = [&](int i, int &page, float2 &scale) {
                 page = work.page(a, i + lane);
                 scale = page >= 0 ? *reinterpret_cast<const float2 *>(c.scales + ((size_t)page * c.heads + work.head) * 2) : make_float2(0.0f, 0.0f);
@@ -400,7 +429,7 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
             int page_now, page_next = -1;
             float2 scale_now, scale_next = make_float2(0.0f, 0.0f);
             look(0, page_now, scale_now);
-            if (work.steps > 16) look(32, page_next, scale_next);
+            if (work.steps > 32) look(32, page_next, scale_next);
             bring_rows<PADDED>(a, work, 128 * h + warp % 4 * 32, queries + h * Shape::QUERIES, warp % 4 * 32, down_room + 128 * h);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tmem_before(); // (the last tile's sums have been read)
@@ -408,69 +437,56 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
             if (lane == 0) mbar_arrive(&bars.queries[h]);
             const float down = down_room[in_tile];
             for (int i = 0; i < work.steps; ++i) {
-                uint64_t bits[2];
-                bool masked = false;
-                float factor[2], log_v[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int column = work.column(2 * i + k);
-                    const bool is_there = __shfl_sync(~0u, page_now, 2 * i % 32 + k) >= 0;
-                    bits[k] = is_there ? ~0ull : 0;
-                    if (is_there && !all_seen(column, work.p0, work.p1, work.keys, a.window, a.sinks)) bits[k] = seen_bits(column, position, work.keys, a.window, a.sinks);
-                    masked |= bits[k] != ~0ull;
-                    factor[k] = score_factor(down, __shfl_sync(~0u, scale_now.x, 2 * i % 32 + k));
-                    log_v[k] = __shfl_sync(~0u, scale_now.y, 2 * i % 32 + k);
-                }
-                if (i % 16 == 15) {
+                const uint32_t buffer = i & 1, scores = tmem + lanes + 128 * h + 64 * buffer;
+                const int column = work.column(i);
+                const bool is_there = __shfl_sync(~0u, page_now, i % 32) >= 0;
+                const float factor = score_factor(down, __shfl_sync(~0u, scale_now.x, i % 32));
+                float log_v = __shfl_sync(~0u, scale_now.y, i % 32);
+                uint64_t bits = is_there ? ~0ull : 0;
+                if (is_there && !all_seen(column, work.p0, work.p1, work.keys, a.window, a.sinks)) bits = seen_bits(column, position, work.keys, a.window, a.sinks);
+                const bool masked = __any_sync(~0u, bits != ~0ull);
+                if (i % 32 == 31) {
                     page_now = page_next, scale_now = scale_next;
-                    look(2 * i + 34, page_next, scale_next);
+                    look(i + 33, page_next, scale_next);
                 }
-                masked = __any_sync(~0u, masked);
-                if (!__all_sync(~0u, mbar_wait(&bars.scores[h], step_parity, abort_flag, P.error, 107))) {
+                if (!__all_sync(~0u, mbar_wait(&bars.scores[h][buffer], scores_parity >> buffer & 1u, abort_flag, P.error, 107))) {
                     ok = false;
                     break;
                 }
-                step_parity ^= 1u;
+                scores_parity ^= 1u << buffer;
                 tmem_after();
-                uint32_t v[4][32];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_ld32_issue(scores + 32 * q, v[q]);
+                uint32_t v[2][32];
+                tmem_ld32_issue(scores, v[0]);
+                tmem_ld32_issue(scores + 32, v[1]);
                 tmem_wait();
                 if (masked) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t some = (uint32_t)(bits[q / 2] >> (32 * (q % 2)));
+                    for (int q = 0; q < 2; ++q)
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            if (!(some >> j & 1u)) v[q][j] = 0xFF800000u;
-                    }
+                            if (!((uint32_t)(bits >> (32 * q)) >> j & 1u)) v[q][j] = 0xFF800000u;
                 }
-                // the largest score
-                float higher_m = -INFINITY, higher_top = -INFINITY;
+                float most[4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float most[4];
+                for (int e = 0; e < 4; ++e) most[e] = fmaxf(__uint_as_float(v[e / 2][e % 2 * 16]), __uint_as_float(v[e / 2][e % 2 * 16 + 1]));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) most[e] = __uint_as_float(v[2 * k + e / 2][e % 2 * 16]);
+                for (int j = 2; j < 16; j += 2)
 #pragma unroll
-                    for (int j = 1; j < 15; j += 2)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t *two = &v[2 * k + e / 2][e % 2 * 16 + j];
-                            most[e] = max3f(most[e], __uint_as_float(two[0]), __uint_as_float(two[1]));
-                        }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) most[e] = fmaxf(most[e], __uint_as_float(v[2 * k + e / 2][e % 2 * 16 + 15]));
-                    const float raw = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), s = raw == -INFINITY ? raw : raw * factor[k];
-                    higher_m = fmaxf(higher_m, s);
-                    higher_top = fmaxf(higher_top, s + (log_v[k] == log_v[k] ? log_v[k] : 0.0f));
-                }
-                if (higher_m > m + LATE) l *= relative(m, higher_m), m = higher_m;
+                    for (int e = 0; e < 4; ++e) most[e] = max3f(most[e], __uint_as_float(v[e / 2][e % 2 * 16 + j]), __uint_as_float(v[e / 2][e % 2 * 16 + j + 1]));
+                const float raw = fmaxf(max3f(most[0], most[1], most[2]), most[3]), higher_m = raw == -INFINITY ? raw : raw * factor;
+                const float higher_top = higher_m + (log_v == log_v ? log_v : 0.0f);
                 const bool rise = higher_top > top + LATE;
-                if (__any_sync(~0u, rise)) {
+                if (__any_sync(~0u, rise || higher_m > m + LATE)) {
+                    if (higher_m > m + LATE) l *= relative(m, higher_m), m = higher_m;
                     const float by = rise ? relative(top, higher_top) : 1.0f;
                     if (rise) top = higher_top;
-                    if (i > 0) { // (the products that add to the sums are done: this step's scores came behind them)
+                    if (i > 0) {
+                        // the last step's product; the one before it is done (these scores came behind it), so that its turn is not taken for this one
+                        if (!__all_sync(~0u, mbar_wait(&bars.added[h], added_parity ^ 1u, abort_flag, P.error, 104))) {
+                            ok = false;
+                            break;
+                        }
+                        tmem_after();
 #pragma unroll 1
                         for (int d = 0; d < PADDED; d += 16) {
                             uint32_t y[16];
@@ -482,25 +498,17 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
                         }
                     }
                 }
+                added_parity ^= 1u;
                 const float from_m = m == -INFINITY ? 0.0f : m, from_top = top == -INFINITY ? 0.0f : top;
-                float shift[2], plus[2];
-                bool far = false;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    if (log_v[k] == -INFINITY) log_v[k] = from_top - from_m;
-                    shift[k] = log_v[k] + from_m - from_top; // a weight is 2^(s - m) 2^shift
-                    plus[k] = log_v[k] - from_top;
-                    far |= fabsf(shift[k]) > 60.0f;
-                }
+                if (log_v == -INFINITY) log_v = from_top - from_m;
+                const float shift = log_v + from_m - from_top, plus = log_v - from_top; // a weight is 2^(s - m) 2^shift
                 // (a factor of 0 or NaN, or NaN for s_v, would make NaN of what is hidden)
-                far |= masked && !(factor[0] > 0.0f && factor[1] > 0.0f && shift[0] == shift[0] && shift[1] == shift[1]);
-                if (__any_sync(~0u, far)) {
+                if (__any_sync(~0u, fabsf(shift) > 60.0f || (masked && !(factor > 0.0f && shift == shift)))) {
 #pragma unroll 1
-                    for (int q = 0; q < 4; ++q) {
+                    for (int q = 0; q < 2; ++q) {
                         tmem_ld32_issue(scores + 32 * q, v[0]);
                         tmem_wait();
-                        const float by = q / 2 ? factor[1] : factor[0], and_plus = q / 2 ? plus[1] : plus[0];
-                        const uint32_t some = (uint32_t)((q / 2 ? bits[1] : bits[0]) >> (32 * (q % 2)));
+                        const uint32_t some = (uint32_t)(bits >> (32 * q));
                         uint32_t out[16];
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
@@ -509,40 +517,37 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
                             for (int e = 0; e < 2; ++e) {
                                 const float s = __uint_as_float(v[0][j + e]);
                                 const bool shown = some >> (j + e) & 1u;
-                                w[e] = shown ? power_of_two(fmaf(s, by, and_plus)) : 0.0f;
-                                l += shown ? power_of_two(fmaf(s, by, -from_m)) : 0.0f; // (either may be 0 where the other is not)
+                                w[e] = shown ? power_of_two(fmaf(s, factor, plus)) : 0.0f;
+                                l += shown ? power_of_two(fmaf(s, factor, -from_m)) : 0.0f; // (either may be 0 where the other is not)
                             }
                             out[j / 2] = halves_of_floats(w[0], w[1]);
                         }
                         tmem_st16(scores + 16 * q, out);
                     }
                 } else {
+                    const uint64_t by = pair_of(factor, factor), and_plus = pair_of(plus, plus);
+                    uint64_t sum[2] = {0, 0};
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint64_t by = pair_of(factor[k], factor[k]), and_plus = pair_of(plus[k], plus[k]);
-                        uint64_t sum[2] = {0, 0};
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t out[16];
 #pragma unroll
-                        for (int q = 2 * k; q < 2 * k + 2; ++q) {
-                            uint32_t out[16];
-#pragma unroll
-                            for (int j = 0; j < 32; j += 2) {
-                                float x0, x1;
-                                halves_of(fma_pair(pair_of(__uint_as_float(v[q][j]), __uint_as_float(v[q][j + 1])), by, and_plus), x0, x1);
-                                x0 = power_of_two(x0), x1 = power_of_two(x1);
-                                sum[j / 2 % 2] = add_pair(sum[j / 2 % 2], pair_of(x0, x1));
-                                out[j / 2] = halves_of_floats(x0, x1);
-                            }
-                            tmem_st16(scores + 16 * q, out);
+                        for (int j = 0; j < 32; j += 2) {
+                            float w0, w1;
+                            halves_of(fma_pair(pair_of(__uint_as_float(v[q][j]), __uint_as_float(v[q][j + 1])), by, and_plus), w0, w1);
+                            w0 = power_of_two(w0), w1 = power_of_two(w1);
+                            sum[j / 2 % 2] = add_pair(sum[j / 2 % 2], pair_of(w0, w1));
+                            out[j / 2] = halves_of_floats(w0, w1);
                         }
-                        float a0, a1;
-                        halves_of(add_pair(sum[0], sum[1]), a0, a1);
-                        l += (a0 + a1) * exp2f(-shift[k]);
+                        tmem_st16(scores + 16 * q, out);
                     }
+                    float a0, a1;
+                    halves_of(add_pair(sum[0], sum[1]), a0, a1);
+                    l += (a0 + a1) * exp2f(-shift);
                 }
                 tmem_stored();
                 tmem_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.weights[h]);
+                if (lane == 0) mbar_arrive(&bars.weights[h][buffer]);
             }
             if (!ok) break;
             if (!__all_sync(~0u, mbar_wait(&bars.sums[h], sums_parity, abort_flag, P.error, 108))) {
@@ -629,9 +634,12 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, 1) attend_many_
     volatile int *abort_flag = &bars.abort_flag;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4; ++i) mbar_init(&bars.full[i], 4), mbar_init(&bars.empty[i], 1);
-        for (int h = 0; h < 2; ++h) mbar_init(&bars.queries[h], 4), mbar_init(&bars.scores[h], 1), mbar_init(&bars.weights[h], 4), mbar_init(&bars.sums[h], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&bars.told[i], 1), mbar_init(&bars.heard[i], 1 + 4 + 4 * HALVES);
+        for (int i = 0; i < 8; ++i) mbar_init(&bars.full[i], CONVERTERS), mbar_init(&bars.empty[i], 1);
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(&bars.queries[h], 4), mbar_init(&bars.added[h], 1), mbar_init(&bars.sums[h], 1);
+            for (int i = 0; i < 2; ++i) mbar_init(&bars.scores[h][i], 1), mbar_init(&bars.weights[h][i], 4);
+        }
+        for (int i = 0; i < 2; ++i) mbar_init(&bars.told[i], 1), mbar_init(&bars.heard[i], 1 + CONVERTERS + 4 * HALVES);
         bars.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -651,15 +659,13 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, 1) attend_many_
     if (start >= end && threadIdx.x == 0) plan.tell(nullptr, 0, 0);
 
     // (each in its role's own branch: the compiler counts a role's registers from there)
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (warp == 0) issue_products<PADDED>(P, bars, work_room, queries, ring, tmem);
-        if (warp == 1) tell_parts<PADDED>(P, plan, bars, work_room, start, end);
-    } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        bring_codes<PADDED>(P, bars, work_room, ring);
+        else if (warp == 1) tell_parts<PADDED>(P, plan, bars, work_room, start, end);
+        else bring_codes<PADDED>(P, bars, work_room, ring);
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         weigh_rows<PADDED>(P, bars, work_room, queries, down_room, tmem);
     }
     tmem_before();
