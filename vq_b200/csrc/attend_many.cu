@@ -6,8 +6,9 @@
 //   warp 0          issues the products: for each half of the rows weights times values of a step, then queries times keys of the step after the next one, so that the next
 //                   scores are there when a half's weights are done.  (With 128 tokens a step and room for one step's scores, each half waited for its products after every
 //                   step: 8192 tokens x 32 heads x 128 took 1.05 ms.)
-//   warp 1          finds what the block takes next, and tells the others ahead of time
-//   warps 2 .. 7    codes of a page's keys, or values, to operand tiles (128-byte rows, 128-byte swizzle); the next ones are on their way from memory meanwhile
+//   warp 1          finds what the block takes next, tells the others ahead of time, and fetches its pages' codes (bulk copies)
+//   warps 2 .. 7    codes of a page's keys, or values, to operand tiles (128-byte rows, 128-byte swizzle).  (With the codes on their way to registers instead, the fence between
+//                   these stores and the products waited for them, a memory's latency every half step.)
 //   warps 8 .. 15   four for each half of the rows, a row a thread: scores to weights, largest score and sum; queries in, results out.  They take most of the registers
 //                   (setmaxnreg: 2 x 96 + 2 x 160 a thread of each four warps, of 4 x 128)
 //
@@ -38,15 +39,18 @@ template <int PADDED> struct ManyShape {
     static constexpr int BLOCKS = (PADDED + 63) / 64;       // of 64 dimensions: a swizzled row of an operand tile
     static constexpr uint32_t QUERIES = BLOCKS * 128 * 128; // bytes of one half's queries
     static constexpr uint32_t STAGE = BLOCKS * STEP * 128;  // of a page's keys; of its values (PADDED rows of 128 bytes) as much or less
-    static constexpr int STAGES = PADDED <= 128 ? 8 : 4;
-    static constexpr size_t SMEM = HALVES * QUERIES + STAGES * STAGE + 1024;
+    static constexpr int STAGES = PADDED <= 128 ? 6 : 3;
+    static constexpr uint32_t CODES = STEP * PADDED; // bytes of a page's keys, or values
+    static constexpr int CODE_STAGES = PADDED <= 128 ? 4 : 2;
+    static constexpr size_t SMEM = HALVES * QUERIES + STAGES * STAGE + CODE_STAGES * CODES + 1024;
     static constexpr uint32_t SUMS = 256; // columns of tensor memory: half h's scores of step i from 128 h + 64 (i % 2), sums from 256 + 128 h
 };
 
 struct alignas(8) ManyBarriers {
-    unsigned long long full[8], empty[8], queries[2], scores[2][2], weights[2][2], added[2], sums[2], told[2], heard[2];
+    unsigned long long full[6], empty[6], codes_full[4], codes_empty[4], queries[2], scores[2][2], weights[2][2], added[2], sums[2], told[2], heard[2];
     uint32_t tmem_base;
     int abort_flag;
+    int missing[4]; // codes that are not there
 };
 
 // kind::f16, binary16 operands, f32 sums, both K-major, M = 128, N = n
@@ -124,12 +128,15 @@ struct Listener {
 };
 
 template <int PADDED>
-__device__ __forceinline__ void tell_parts(const ShareParams &P, const Plan<ManyShape<PADDED>::ROWS, THREADS> &plan, ManyBarriers &bars, WorkRoom &room, long long start, long long end)
+__device__ __forceinline__ void tell_parts(const ShareParams &P, const Plan<ManyShape<PADDED>::ROWS, THREADS> &plan, ManyBarriers &bars, WorkRoom &room, uint8_t *codes, long long start, long long end)
 {
-    constexpr int ROWS = ManyShape<PADDED>::ROWS;
+    using Shape = ManyShape<PADDED>;
+    constexpr int ROWS = Shape::ROWS;
     const int lane = threadIdx.x % 32;
     const Attend &a = P.a;
     long long x = start;
+    int slot = 0;
+    uint32_t parity = 0; // of the codes' places
     for (uint32_t number = 0;; ++number) {
         const uint32_t at = number & 1u;
         Work work = {};
@@ -156,6 +163,34 @@ __device__ __forceinline__ void tell_parts(const ShareParams &P, const Plan<Many
             mbar_arrive(&bars.told[at]);
         }
         if (work.steps < 0) return;
+        // the pages of 32 steps, and the 32 behind them, a lane each
+        int look_now = work.page(a, lane), look_next = work.steps > 32 ? work.page(a, 32 + lane) : -1, looked = 0;
+        auto fetch = [&](int step, int which) {
+            const int page = __shfl_sync(~0u, step - looked >= 32 ? look_next : look_now, step % 32);
+            if (!__all_sync(~0u, mbar_wait(&bars.codes_empty[slot], parity ^ 1u, &bars.abort_flag, P.error, 112))) return false;
+            if (lane == 0) {
+                bars.missing[slot] = page < 0;
+                if (page >= 0) {
+                    mbar_expect_tx(&bars.codes_full[slot], Shape::CODES);
+                    bulk_load_1d(codes + slot * Shape::CODES, a.cache.codes + (((size_t)page * a.cache.heads + work.head) * 2 + which) * Shape::CODES, Shape::CODES, &bars.codes_full[slot]);
+                } else {
+                    mbar_arrive(&bars.codes_full[slot]);
+                }
+            }
+            if (++slot == Shape::CODE_STAGES) slot = 0, parity ^= 1u;
+            return true;
+        };
+        // keys 0, keys 1, values 0, keys 2, values 1, ..: the order in which they are multiplied
+        if (work.steps > 0 && !fetch(0, 0)) return;
+        if (work.steps > 1 && !fetch(1, 0)) return;
+        for (int i = 0; i < work.steps; ++i) {
+            if (!fetch(i, 1)) return;
+            if (i + 2 < work.steps && !fetch(i + 2, 0)) return;
+            if (i - looked == 30) { // (the next one to be asked for is looked + 32)
+                looked += 32, look_now = look_next;
+                look_next = work.page(a, looked + 32 + lane);
+            }
+        }
     }
 }
 
@@ -309,7 +344,7 @@ __device__ __forceinline__ void issue_products(const ShareParams &P, ManyBarrier
 }
 
 template <int PADDED>
-__device__ __forceinline__ void bring_codes(const ShareParams &P, ManyBarriers &bars, const WorkRoom &room, uint8_t *ring)
+__device__ __forceinline__ void convert_codes(const ShareParams &P, ManyBarriers &bars, const WorkRoom &room, const uint8_t *codes, uint8_t *ring)
 {
     using Shape = ManyShape<PADDED>;
     [[maybe_unused]] constexpr int ROWS = Shape::ROWS, HALVES = Shape::HALVES, STAGES = Shape::STAGES;
@@ -320,27 +355,22 @@ __device__ __forceinline__ void bring_codes(const ShareParams &P, ManyBarriers &
     const int t = threadIdx.x - 64; // of the converters' threads
     constexpr int THREADS_HERE = 32 * CONVERTERS, ALL = STEP * PADDED / 16, PIECES = (ALL + THREADS_HERE - 1) / THREADS_HERE; // pieces of 16 codes of a page, and a thread's
     constexpr int PER_ROW = PADDED / 16;                                                                                     // of a token's key
-    int st = 0;
-    uint32_t parity = 0;
+    int st = 0, slot = 0;
+    uint32_t parity = 0, codes_parity = 0;
     bool ok = true;
-    uint4 piece[2][PIECES]; // keys, values that come next
-    const uint4 zeros = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
     Listener listener{room, bars, P.error};
     for (Work work; ok && listener.next(work);) {
-        if (work.steps == 0) continue;
-        int look_now = work.page(a, lane), look_next = work.steps > 32 ? work.page(a, 32 + lane) : -1; // the pages of 32 steps, and the 32 behind them, a lane each
-        int looked = 0;                                                                                // look_now's first step
-        auto load = [&](int step, int which) {
-            const int page = __shfl_sync(~0u, step - looked >= 32 ? look_next : look_now, step % 32);
-            const uint8_t *from = c.codes + (((size_t)max(page, 0) * c.heads + work.head) * 2 + which) * CACHE_PAGE * PADDED;
-#pragma unroll
-            for (int k = 0; k < PIECES; ++k) {
-                const int at = t + THREADS_HERE * k;
-                if (ALL % THREADS_HERE && at >= ALL) continue;
-                piece[which][k] = page < 0 ? zeros : *reinterpret_cast<const uint4 *>(from + at * 16);
-            }
-        };
         auto convert = [&](int which) {
+            if (!__all_sync(~0u, mbar_wait(&bars.codes_full[slot], codes_parity, abort_flag, P.error, 105))) return false;
+            uint4 piece[PIECES];
+            if (bars.missing[slot]) {
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) piece[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            } else {
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k)
+                    if (ALL % THREADS_HERE == 0 || t + THREADS_HERE * k < ALL) piece[k] = reinterpret_cast<const uint4 *>(codes + slot * Shape::CODES)[t + THREADS_HERE * k];
+            }
             if (!__all_sync(~0u, mbar_wait(&bars.empty[st], parity ^ 1u, abort_flag, P.error, 106))) return false;
             uint8_t *to = ring + st * Shape::STAGE;
 #pragma unroll
@@ -358,42 +388,30 @@ __device__ __forceinline__ void bring_codes(const ShareParams &P, ManyBarriers &
                 } else {
                     row = at / 4, chunk = 2 * (at % 4); // dimension
                 }
-                const uint4 w = piece[which][k];
                 uint4 first, second;
-                codes_to_halves(w.x, first.x, first.y);
-                codes_to_halves(w.y, first.z, first.w);
-                codes_to_halves(w.z, second.x, second.y);
-                codes_to_halves(w.w, second.z, second.w);
+                codes_to_halves(piece[k].x, first.x, first.y);
+                codes_to_halves(piece[k].y, first.z, first.w);
+                codes_to_halves(piece[k].z, second.x, second.y);
+                codes_to_halves(piece[k].w, second.z, second.w);
                 uint8_t *at_row = part + row * 128;
                 *reinterpret_cast<uint4 *>(at_row + ((chunk + turned) ^ (row & 7)) * 16) = turned ? second : first;
                 *reinterpret_cast<uint4 *>(at_row + ((chunk + !turned) ^ (row & 7)) * 16) = turned ? first : second;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.full[st]);
+            if (lane == 0) {
+                mbar_arrive(&bars.full[st]);
+                mbar_arrive(&bars.codes_empty[slot]);
+            }
             if (++st == STAGES) st = 0, parity ^= 1u;
+            if (++slot == Shape::CODE_STAGES) slot = 0, codes_parity ^= 1u;
             return true;
         };
-        // keys 0, keys 1, values 0, keys 2, values 1, ..: the order in which they are multiplied
-        load(0, 0);
-        load(0, 1);
-        ok = convert(0);
-        if (ok && work.steps > 1) {
-            load(1, 0);
-            ok = convert(0);
-        }
-        if (work.steps > 2) load(2, 0);
+        ok = work.steps == 0 || convert(0);
+        if (ok && work.steps > 1) ok = convert(0);
         for (int i = 0; ok && i < work.steps; ++i) {
             ok = convert(1);
-            if (i + 1 < work.steps) load(i + 1, 1);
-            if (ok && i + 2 < work.steps) {
-                ok = convert(0);
-                if (i + 3 < work.steps) load(i + 3, 0);
-            }
-            if (i - looked == 30) { // (the next one to be asked for is looked + 32)
-                looked += 32, look_now = look_next;
-                look_next = work.page(a, looked + 32 + lane);
-            }
+            if (ok && i + 2 < work.steps) ok = convert(0);
         }
     }
 }
@@ -629,12 +647,13 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, 1) attend_many_
     __shared__ WorkRoom work_room;
     __shared__ float down_room[ROWS];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *queries = base, *ring = base + HALVES * Shape::QUERIES;
+    uint8_t *queries = base, *ring = base + HALVES * Shape::QUERIES, *codes = ring + Shape::STAGES * Shape::STAGE;
     const int warp = threadIdx.x / 32;
     volatile int *abort_flag = &bars.abort_flag;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 8; ++i) mbar_init(&bars.full[i], CONVERTERS), mbar_init(&bars.empty[i], 1);
+        for (int i = 0; i < 6; ++i) mbar_init(&bars.full[i], CONVERTERS), mbar_init(&bars.empty[i], 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&bars.codes_full[i], 1), mbar_init(&bars.codes_empty[i], CONVERTERS);
         for (int h = 0; h < 2; ++h) {
             mbar_init(&bars.queries[h], 4), mbar_init(&bars.added[h], 1), mbar_init(&bars.sums[h], 1);
             for (int i = 0; i < 2; ++i) mbar_init(&bars.scores[h][i], 1), mbar_init(&bars.weights[h][i], 4);
@@ -662,8 +681,8 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, 1) attend_many_
     if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (warp == 0) issue_products<PADDED>(P, bars, work_room, queries, ring, tmem);
-        else if (warp == 1) tell_parts<PADDED>(P, plan, bars, work_room, start, end);
-        else bring_codes<PADDED>(P, bars, work_room, ring);
+        else if (warp == 1) tell_parts<PADDED>(P, plan, bars, work_room, codes, start, end);
+        else convert_codes<PADDED>(P, bars, work_room, codes, ring);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         weigh_rows<PADDED>(P, bars, work_room, queries, down_room, tmem);
