@@ -543,7 +543,7 @@ struct SequencesIn {
           lengths(dev, "lengths", lengths_, sequences * sizeof(int32_t)), offsets(dev, offsets_, offsets_ ? sequences : 1, n)
     {
         s.table = table.as<int32_t>(), s.table_ld = table_ld, s.sequences = (int)sequences, s.columns = (int)columns;
-        s.lengths = lengths.as<int32_t>(), s.offsets = reinterpret_cast<const long long *>(offsets.get()), s.n = (int)n;
+        s.lengths = lengths.as<int32_t>(), s.offsets = reinterpret_cast<const long long *>(offsets.get()), s.n = (int)n, s.each = (int)(n / sequences);
     }
     static const int32_t *checked(const int32_t *table, size_t sequences, size_t columns, size_t table_ld, const int32_t *lengths, const int64_t *offsets, size_t n)
     {

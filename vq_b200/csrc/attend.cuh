@@ -47,7 +47,7 @@ struct QueryScale {
         const int exponent = (int)(largest >> 23) - 127, k = min(14 - exponent, 126); // (f32 numbers below 2^-112 stay below 2^14: 2^126 is enough for bf16's smallest)
         const float factor = scale * LOG2_E;
         up = __int_as_float((k + 127) << 23);
-        down = k <= 126 - 1 && k >= -126 ? factor * __int_as_float((127 - k) << 23) : ldexpf(factor, -k);
+        down = factor * __int_as_float((127 - k) << 23); // (-113 <= k <= 126)
         if (largest == 0) up = 1.0f, down = factor;
         if (largest >= 0x7F800000u) up = 0.0f, down = __int_as_float(0x7FC00000);
     }
@@ -176,6 +176,7 @@ template <int ROWS, int THREADS> struct Plan {
             b = u / each, first_row = (u - b * each) * ROWS;
         } else {
             int lo = 0, hi = a.seq.sequences - 1; // the last one that begins at or before u
+#pragma unroll 1
             while (lo < hi) {
                 const int mid = (lo + hi + 1) / 2;
                 if ((int)((long long)offset_of(a.seq, mid) * a.group / ROWS) + mid <= u) lo = mid;
@@ -199,8 +200,10 @@ template <int ROWS, int THREADS> struct Plan {
         const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
         per = (P.slots + MOST_GROUPS - 1) / MOST_GROUPS, groups = (P.slots + per - 1) / per;
         long long base = 0;
+#pragma unroll 1
         for (int g0 = 0; g0 < groups; g0 += THREADS) {
             long long mine = 0;
+#pragma unroll 1
             for (int u = (g0 + (int)threadIdx.x) * per; u < min((g0 + (int)threadIdx.x + 1) * per, P.slots); ++u) {
                 int b, row;
                 mine += of_slot(u, b, row);
@@ -233,12 +236,14 @@ template <int ROWS, int THREADS> struct Plan {
     {
         const int lane = threadIdx.x % 32, heads = (int)P.a.cache.heads;
         int lo = 0, hi = groups - 1;
+#pragma unroll 1
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
             if (before[mid] <= x) lo = mid;
             else hi = mid - 1;
         }
         long long rest = x - before[lo];
+#pragma unroll 1
         for (int u = lo * per, end = min(u + per, P.slots); u < end; u += 32) {
             int b = 0, row = 0;
             const int units = u + lane < end ? of_slot(u + lane, b, row) : 0;

@@ -214,27 +214,29 @@ __device__ __forceinline__ void bring_queries(const Attend &a, const Span &span,
 {
     using Shape = FewShape<PADDED, EIGHTS>;
     const int part = threadIdx.x % 8, width = (int)a.cache.width;
+    const bool f16 = a.queries.type == VALUE_F16;
+    const bool aligned = width % 4 == 0 && a.queries.ld % 4 == 0 && a.queries.head_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.queries.x) & 7) == 0;
     for (int r = threadIdx.x / 8; r < Shape::ROWS; r += THREADS / 8) {
-        const int at = tile.first_row + r;
-        const bool there = r < rows;
-        const size_t from = there ? (size_t)(span.row + at / a.group) * a.queries.ld + (size_t)(tile.head * a.group + at % a.group) * a.queries.head_ld : 0;
-        const uint16_t *x = static_cast<const uint16_t *>(a.queries.x) + from;
-        const bool f16 = a.queries.type == VALUE_F16, aligned = (reinterpret_cast<uintptr_t>(x) & 7) == 0;
+        const int at = tile.first_row + min(r, rows - 1); // (rows behind the tile's: its last one)
+        const uint16_t *x = static_cast<const uint16_t *>(a.queries.x) + (size_t)(span.row + at / a.group) * a.queries.ld + (size_t)(tile.head * a.group + at % a.group) * a.queries.head_ld;
         constexpr int FOURS = PADDED / 32; // four dimensions at a time: 4 (8 i + part)
+        uint2 four[FOURS];
         float v[FOURS][4];
         uint32_t most = 0;
+        if (aligned) { // (no branch for each load, at whose end it would be waited for)
+#pragma unroll
+            for (int i = 0; i < FOURS; ++i) four[i] = *reinterpret_cast<const uint2 *>(x + min(4 * (8 * i + part), width - 4));
+        } else {
+#pragma unroll
+            for (int i = 0; i < FOURS; ++i) {
+                const int d = 4 * (8 * i + part);
+                four[i] = make_uint2(x[min(d, width - 1)] | (uint32_t)x[min(d + 1, width - 1)] << 16, x[min(d + 2, width - 1)] | (uint32_t)x[min(d + 3, width - 1)] << 16);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < FOURS; ++i) {
             const int d = 4 * (8 * i + part);
-            uint32_t w[2] = {0, 0};
-            if (there && aligned && d + 4 <= width) {
-                const uint2 q = *reinterpret_cast<const uint2 *>(x + d);
-                w[0] = q.x, w[1] = q.y;
-            } else if (there) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (d + j < width) w[j / 2] |= (uint32_t)x[d + j] << (16 * (j % 2));
-            }
+            const uint32_t w[2] = {four[i].x & ((d < width ? 0xFFFFu : 0u) | (d + 1 < width ? 0xFFFF0000u : 0u)), four[i].y & ((d + 2 < width ? 0xFFFFu : 0u) | (d + 3 < width ? 0xFFFF0000u : 0u))};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t half = j % 2 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu;

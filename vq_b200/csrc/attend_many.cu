@@ -6,8 +6,9 @@
 //   warp 0          issues the products: for each half of the rows weights times values of a step, then queries times keys of the step after the next one, so that the next
 //                   scores are there when a half's weights are done.  (With 128 tokens a step and room for one step's scores, each half waited for its products after every
 //                   step: 8192 tokens x 32 heads x 128 took 1.05 ms.)
-//   warp 1          finds what the block takes next, tells the others ahead of time, and fetches its pages' codes (bulk copies)
-//   warps 2 .. 7    codes of a page's keys, or values, to operand tiles (128-byte rows, 128-byte swizzle).  (With the codes on their way to registers instead, the fence between
+//   warp 1          finds what the block takes next, and tells the others ahead of time
+//   warp 2          fetches pages' codes (bulk copies)
+//   warps 4 .. 7    codes of a page's keys, or values, to operand tiles (128-byte rows, 128-byte swizzle).  (With the codes on their way to registers instead, the fence between
 //                   these stores and the products waited for them, a memory's latency every half step.)
 //   warps 8 .. 15   four for each half of the rows, a row a thread: scores to weights, largest score and sum; queries in, results out.  They take most of the registers
 //                   (setmaxnreg: 2 x 96 + 2 x 160 a thread of each four warps, of 4 x 128)
@@ -32,7 +33,7 @@ namespace {
 
 constexpr int THREADS = 512, STEP = CACHE_PAGE; // tokens of a step
 constexpr float LATE = 8.0f;                    // a row's largest is followed when it is 2^LATE times as large
-constexpr int CONVERTERS = 6;                   // warps
+constexpr int CONVERTERS = 4;                   // warps
 
 template <int PADDED> struct ManyShape {
     static constexpr int HALVES = PADDED <= 128 ? 2 : 1, ROWS = 128 * HALVES;
@@ -72,6 +73,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
 __device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16])
@@ -127,16 +133,23 @@ struct Listener {
     }
 };
 
+// The order in which a part's codes are multiplied: keys 0, keys 1, values 0, keys 2, values 1, .. values steps - 1; the n-th one of 2 x steps.
+struct HalfStep {
+    int step, which; // 0: keys, 1: values
+    __device__ __forceinline__ HalfStep(int n, int steps)
+    {
+        which = n > 0 && (n % 2 == 0 || n == 2 * steps - 1);
+        step = n == 0 ? 0 : which == 0 ? (n + 1) / 2 : n == 2 * steps - 1 ? steps - 1 : n / 2 - 1;
+    }
+};
+
 template <int PADDED>
-__device__ __forceinline__ void tell_parts(const ShareParams &P, const Plan<ManyShape<PADDED>::ROWS, THREADS> &plan, ManyBarriers &bars, WorkRoom &room, uint8_t *codes, long long start, long long end)
+__device__ __forceinline__ void tell_parts(const ShareParams &P, const Plan<ManyShape<PADDED>::ROWS, THREADS> &plan, ManyBarriers &bars, WorkRoom &room, long long start, long long end)
 {
-    using Shape = ManyShape<PADDED>;
-    constexpr int ROWS = Shape::ROWS;
+    constexpr int ROWS = ManyShape<PADDED>::ROWS;
     const int lane = threadIdx.x % 32;
     const Attend &a = P.a;
     long long x = start;
-    int slot = 0;
-    uint32_t parity = 0; // of the codes' places
     for (uint32_t number = 0;; ++number) {
         const uint32_t at = number & 1u;
         Work work = {};
@@ -163,88 +176,125 @@ __device__ __forceinline__ void tell_parts(const ShareParams &P, const Plan<Many
             mbar_arrive(&bars.told[at]);
         }
         if (work.steps < 0) return;
+    }
+}
+
+template <int PADDED> __device__ __forceinline__ void fetch_codes(const ShareParams &P, ManyBarriers &bars, const WorkRoom &room, uint8_t *codes)
+{
+    using Shape = ManyShape<PADDED>;
+    const int lane = threadIdx.x % 32;
+    const Attend &a = P.a;
+    int slot = 0;
+    uint32_t parity = 0;
+    Listener listener{room, bars, P.error};
+    for (Work work; listener.next(work);) {
         // the pages of 32 steps, and the 32 behind them, a lane each
         int look_now = work.page(a, lane), look_next = work.steps > 32 ? work.page(a, 32 + lane) : -1, looked = 0;
-        auto fetch = [&](int step, int which) {
-            const int page = __shfl_sync(~0u, step - looked >= 32 ? look_next : look_now, step % 32);
-            if (!__all_sync(~0u, mbar_wait(&bars.codes_empty[slot], parity ^ 1u, &bars.abort_flag, P.error, 112))) return false;
+#pragma unroll 1
+        for (int n = 0; n < 2 * work.steps; ++n) {
+            const HalfStep half(n, work.steps);
+            if (half.which == 1 && half.step - looked == 32) { // (everything before has been asked for)
+                looked += 32, look_now = look_next;
+                look_next = work.page(a, looked + 32 + lane);
+            }
+            const int page = __shfl_sync(~0u, half.step - looked >= 32 ? look_next : look_now, half.step % 32);
+            if (!__all_sync(~0u, mbar_wait(&bars.codes_empty[slot], parity ^ 1u, &bars.abort_flag, P.error, 112))) return;
             if (lane == 0) {
                 bars.missing[slot] = page < 0;
                 if (page >= 0) {
                     mbar_expect_tx(&bars.codes_full[slot], Shape::CODES);
-                    bulk_load_1d(codes + slot * Shape::CODES, a.cache.codes + (((size_t)page * a.cache.heads + work.head) * 2 + which) * Shape::CODES, Shape::CODES, &bars.codes_full[slot]);
+                    bulk_load_1d(codes + slot * Shape::CODES, a.cache.codes + (((size_t)page * a.cache.heads + work.head) * 2 + half.which) * Shape::CODES, Shape::CODES, &bars.codes_full[slot]);
                 } else {
                     mbar_arrive(&bars.codes_full[slot]);
                 }
             }
             if (++slot == Shape::CODE_STAGES) slot = 0, parity ^= 1u;
-            return true;
-        };
-        // keys 0, keys 1, values 0, keys 2, values 1, ..: the order in which they are multiplied
-        if (work.steps > 0 && !fetch(0, 0)) return;
-        if (work.steps > 1 && !fetch(1, 0)) return;
-        for (int i = 0; i < work.steps; ++i) {
-            if (!fetch(i, 1)) return;
-            if (i + 2 < work.steps && !fetch(i + 2, 0)) return;
-            if (i - looked == 30) { // (the next one to be asked for is looked + 32)
-                looked += 32, look_now = look_next;
-                look_next = work.page(a, looked + 32 + lane);
-            }
         }
     }
 }
 
 template <int N> __host__ __device__ constexpr int power_above() { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : 32; }
 
-// The 32 rows of queries of a warp to their places in the operand tile, 0 behind their width and behind the tile's rows; their factors of scores to `down`.  Lanes next to
+// The 32 rows of queries of a warp to their places in the operand tile, 0 behind their width; their factors of scores to `down`.  Lanes next to
 // each other have eight values of a row each.  Factors are not negative: the largest product is the largest score.
-template <int PADDED> __device__ __forceinline__ void bring_rows(const Attend &a, const Work &work, int r0, uint8_t *tile, int tile_row, float *down)
-{
-    constexpr int LANES = power_above<PADDED / 8>(), ROWS_AT_ONCE = 32 / LANES, BATCH = LANES < 8 ? LANES : 8; // (32 rows: LANES times)
-    const int lane = threadIdx.x % 32, piece = lane % LANES, width = (int)a.cache.width, d = 8 * piece;
-    const bool f16 = a.queries.type == VALUE_F16;
-#pragma unroll 1
-    for (int i0 = 0; i0 < LANES; i0 += BATCH) {
-        uint4 w[BATCH];
+template <int PADDED> struct Bringer {
+    static constexpr int LANES = power_above<PADDED / 8>(), ROWS_AT_ONCE = 32 / LANES; // lanes of a row
+    const Attend &a;
+    const Work &work;
+    const int r0, tile_row; // first of the warp's rows, of the tile and of its half
+    uint8_t *tile;
+    float *down;
+    const int token0, head0; // of the tile's first row
+    const float inverse;     // 1 / group: numbers of rows are small enough for that
+    const int lane, piece, d, width;
+    const bool f16;
+    __device__ __forceinline__ Bringer(const Attend &a_, const Work &work_, int r0_, uint8_t *tile_, int tile_row_, float *down_)
+        : a(a_), work(work_), r0(r0_), tile_row(tile_row_), tile(tile_), down(down_), token0(work_.first_row / a_.group), head0(work_.first_row % a_.group), inverse(1.0f / (float)a_.group),
+          lane(threadIdx.x % 32), piece(lane % LANES), d(8 * piece), width((int)a_.cache.width), f16(a_.queries.type == VALUE_F16)
+    {
+    }
+    __device__ __forceinline__ const uint16_t *row_at(int i) const // (of rows behind the tile's: its last one)
+    {
+        const int x = head0 + min(r0 + i * ROWS_AT_ONCE + lane / LANES, work.rows - 1), t = (int)(((float)x + 0.5f) * inverse);
+        return static_cast<const uint16_t *>(a.queries.x) + (size_t)(work.row + token0 + t) * a.queries.ld + (size_t)(work.head * a.group + x - t * a.group) * a.queries.head_ld;
+    }
+    // Rows i0 .. of the warp's turns.  All rows' steps next to each other: one row's take a thousand cycles.
+    template <int N> __device__ __forceinline__ void convert(int i0, uint4 (&w)[N]) const
+    {
+        uint32_t most[N]; // magnitudes' order is that of their bits in either type
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int r = r0 + (i0 + i) * ROWS_AT_ONCE + lane / LANES, at = work.first_row + r;
-            w[i] = make_uint4(0, 0, 0, 0);
-            if (r >= work.rows || d >= width) continue;
-            const uint16_t *x = static_cast<const uint16_t *>(a.queries.x) + (size_t)(work.row + at / a.group) * a.queries.ld + (size_t)(work.head * a.group + at % a.group) * a.queries.head_ld + d;
-            if ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && d + 8 <= width) {
-                w[i] = *reinterpret_cast<const uint4 *>(x);
-            } else {
+        for (int i = 0; i < N; ++i) {
+            if (d + 8 > width) { // 0 behind the width
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (d + j < width) (&w[i].x)[j / 2] |= (uint32_t)x[j] << (16 * (j % 2));
+                for (int j = 0; j < 4; ++j) (&w[i].x)[j] &= (d + 2 * j < width ? 0xFFFFu : 0u) | (d + 2 * j + 1 < width ? 0xFFFF0000u : 0u);
             }
+            most[i] = __vmaxu2(__vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu));
         }
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
+        for (int o = LANES / 2; o; o /= 2)
+#pragma unroll
+            for (int i = 0; i < N; ++i) most[i] = __vmaxu2(most[i], __shfl_xor_sync(~0u, most[i], o));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
             const int r = (i0 + i) * ROWS_AT_ONCE + lane / LANES; // of the warp's
-            auto value = [&](int j) {
-                const uint32_t half = j % 2 ? (&w[i].x)[j / 2] >> 16 : (&w[i].x)[j / 2] & 0xFFFFu;
-                return f16 ? __half2float(__ushort_as_half((unsigned short)half)) : __uint_as_float(half << 16);
-            };
-            uint32_t most = 0; // magnitudes' order is that of their bits in either type
-#pragma unroll
-            for (int j = 0; j < 4; ++j) most = __vmaxu2(most, (&w[i].x)[j] & 0x7FFF7FFFu);
-#pragma unroll
-            for (int o = LANES / 2; o; o /= 2) most = __vmaxu2(most, __shfl_xor_sync(~0u, most, o));
-            const uint32_t half = max(most & 0xFFFFu, most >> 16);
+            const uint32_t half = max(most[i] & 0xFFFFu, most[i] >> 16);
             const QueryScale scale(f16 ? __float_as_uint(__half2float(__ushort_as_half((unsigned short)half))) : half << 16, fabsf(a.scale));
             const float up = a.scale < 0.0f ? -scale.up : scale.up;
-            uint4 h = make_uint4(0, 0, 0, 0);
-            if (scale.up != 0.0f) {
+            uint4 h;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) (&h.x)[j] = halves_of_floats(value(2 * j) * up, value(2 * j + 1) * up);
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t two = (&w[i].x)[j];
+                const float low = f16 ? __half2float(__ushort_as_half((unsigned short)(two & 0xFFFFu))) : __uint_as_float(two << 16);
+                const float high = f16 ? __half2float(__ushort_as_half((unsigned short)(two >> 16))) : __uint_as_float(two & 0xFFFF0000u);
+                (&h.x)[j] = scale.up == 0.0f ? 0u : halves_of_floats(low * up, high * up); // (an infinity or a NaN: 0 times that is none)
             }
             if (d < PADDED) *reinterpret_cast<uint4 *>(tile + d / 64 * 16384 + (tile_row + r) * 128 + ((piece % 8) ^ (r & 7)) * 16) = h;
             if (piece == 0) down[tile_row + r] = scale.down;
         }
     }
-}
+    __device__ __forceinline__ void all() const
+    {
+        if (width % 8 == 0 && a.queries.ld % 8 == 0 && a.queries.head_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(a.queries.x) & 15) == 0) {
+            constexpr int N = 4;
+#pragma unroll 1
+            for (int i = 0; i < LANES; i += N) {
+                uint4 w[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) w[k] = *reinterpret_cast<const uint4 *>(row_at(i + k) + min(d, width - 8));
+                convert<N>(i, w);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < LANES; ++i) {
+                const uint16_t *x = row_at(i);
+                uint4 w[1] = {make_uint4(0, 0, 0, 0)};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) (&w[0].x)[j / 2] |= (uint32_t)x[min(d + j, width - 1)] << (16 * (j % 2));
+                convert<1>(i, w);
+            }
+        }
+    }
+};
 
 // Bits of a page's tokens that a row sees.
 __device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
@@ -290,8 +340,10 @@ __device__ __forceinline__ void issue_products(const ShareParams &P, ManyBarrier
                 umma_commit(&bars.added[h]);
             };
             // the first two steps' scores
+#pragma unroll 1
             for (int i = 0; ok && i < min(work.steps, 2); ++i) {
                 ok = stage_there();
+#pragma unroll 1
                 for (int h = 0; ok && h < halves; ++h) {
                     if (i == 0) {
                         ok = mbar_wait(&bars.queries[h], queries_parity[h], abort_flag, P.error, 102);
@@ -304,6 +356,7 @@ __device__ __forceinline__ void issue_products(const ShareParams &P, ManyBarrier
                 if (ok) umma_commit(&bars.empty[st]);
                 next_stage();
             }
+#pragma unroll 1
             for (int i = 0; ok && i < work.steps; ++i) {
                 const int buffer = i & 1, values_at = st;
                 const bool more = i + 2 < work.steps;
@@ -313,6 +366,7 @@ __device__ __forceinline__ void issue_products(const ShareParams &P, ManyBarrier
                     ok = stage_there();
                     if (--st < 0) st = STAGES - 1, parity ^= 1u;
                 }
+#pragma unroll 1
                 for (int h = 0; ok && h < halves; ++h) {
                     ok = mbar_wait(&bars.weights[h][buffer], weights_parity[h] >> buffer & 1u, abort_flag, P.error, 103);
                     if (!ok) break;
@@ -352,7 +406,7 @@ __device__ __forceinline__ void convert_codes(const ShareParams &P, ManyBarriers
     volatile int *abort_flag = &bars.abort_flag;
     const Attend &a = P.a;
     [[maybe_unused]] const Cache &c = a.cache;
-    const int t = threadIdx.x - 64; // of the converters' threads
+    const int t = threadIdx.x - 128; // of the converters' threads
     constexpr int THREADS_HERE = 32 * CONVERTERS, ALL = STEP * PADDED / 16, PIECES = (ALL + THREADS_HERE - 1) / THREADS_HERE; // pieces of 16 codes of a page, and a thread's
     constexpr int PER_ROW = PADDED / 16;                                                                                     // of a token's key
     int st = 0, slot = 0;
@@ -360,8 +414,10 @@ __device__ __forceinline__ void convert_codes(const ShareParams &P, ManyBarriers
     bool ok = true;
     Listener listener{room, bars, P.error};
     for (Work work; ok && listener.next(work);) {
-        auto convert = [&](int which) {
-            if (!__all_sync(~0u, mbar_wait(&bars.codes_full[slot], codes_parity, abort_flag, P.error, 105))) return false;
+#pragma unroll 1
+        for (int n = 0; n < 2 * work.steps; ++n) {
+            const int which = HalfStep(n, work.steps).which;
+            if (!(ok = __all_sync(~0u, mbar_wait(&bars.codes_full[slot], codes_parity, abort_flag, P.error, 105)))) break;
             uint4 piece[PIECES];
             if (bars.missing[slot]) {
 #pragma unroll
@@ -371,7 +427,7 @@ __device__ __forceinline__ void convert_codes(const ShareParams &P, ManyBarriers
                 for (int k = 0; k < PIECES; ++k)
                     if (ALL % THREADS_HERE == 0 || t + THREADS_HERE * k < ALL) piece[k] = reinterpret_cast<const uint4 *>(codes + slot * Shape::CODES)[t + THREADS_HERE * k];
             }
-            if (!__all_sync(~0u, mbar_wait(&bars.empty[st], parity ^ 1u, abort_flag, P.error, 106))) return false;
+            if (!(ok = __all_sync(~0u, mbar_wait(&bars.empty[st], parity ^ 1u, abort_flag, P.error, 106)))) break;
             uint8_t *to = ring + st * Shape::STAGE;
 #pragma unroll
             for (int k = 0; k < PIECES; ++k) {
@@ -405,13 +461,6 @@ __device__ __forceinline__ void convert_codes(const ShareParams &P, ManyBarriers
             }
             if (++st == STAGES) st = 0, parity ^= 1u;
             if (++slot == Shape::CODE_STAGES) slot = 0, codes_parity ^= 1u;
-            return true;
-        };
-        ok = work.steps == 0 || convert(0);
-        if (ok && work.steps > 1) ok = convert(0);
-        for (int i = 0; ok && i < work.steps; ++i) {
-            ok = convert(1);
-            if (ok && i + 2 < work.steps) ok = convert(0);
         }
     }
 }
@@ -448,14 +497,26 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
             float2 scale_now, scale_next = make_float2(0.0f, 0.0f);
             look(0, page_now, scale_now);
             if (work.steps > 32) look(32, page_next, scale_next);
-            bring_rows<PADDED>(a, work, 128 * h + warp % 4 * 32, queries + h * Shape::QUERIES, warp % 4 * 32, down_room + 128 * h);
+            Bringer<PADDED>(a, work, 128 * h + warp % 4 * 32, queries + h * Shape::QUERIES, warp % 4 * 32, down_room + 128 * h).all();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tmem_before(); // (the last tile's sums have been read)
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.queries[h]);
             const float down = down_room[in_tile];
+            uint32_t v[2][32]; // a step's scores; the next ones are on their way to where weights have been made of these
+            auto scores_there = [&](int i) {
+                const uint32_t buffer = i & 1;
+                ok = __all_sync(~0u, mbar_wait(&bars.scores[h][buffer], scores_parity >> buffer & 1u, abort_flag, P.error, 107));
+                scores_parity ^= 1u << buffer;
+                tmem_after();
+                return ok;
+            };
+            if (!scores_there(0)) break;
+            tmem_ld32_issue(tmem + lanes + 128 * h, v[0]);
+            tmem_ld32_issue(tmem + lanes + 128 * h + 32, v[1]);
             for (int i = 0; i < work.steps; ++i) {
-                const uint32_t buffer = i & 1, scores = tmem + lanes + 128 * h + 64 * buffer;
+                const uint32_t buffer = i & 1, scores = tmem + lanes + 128 * h + 64 * buffer, scores_next = tmem + lanes + 128 * h + 64 * (buffer ^ 1);
+                const bool more = i + 1 < work.steps;
                 const int column = work.column(i);
                 const bool is_there = __shfl_sync(~0u, page_now, i % 32) >= 0;
                 const float factor = score_factor(down, __shfl_sync(~0u, scale_now.x, i % 32));
@@ -467,15 +528,6 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
                     page_now = page_next, scale_now = scale_next;
                     look(i + 33, page_next, scale_next);
                 }
-                if (!__all_sync(~0u, mbar_wait(&bars.scores[h][buffer], scores_parity >> buffer & 1u, abort_flag, P.error, 107))) {
-                    ok = false;
-                    break;
-                }
-                scores_parity ^= 1u << buffer;
-                tmem_after();
-                uint32_t v[2][32];
-                tmem_ld32_issue(scores, v[0]);
-                tmem_ld32_issue(scores + 32, v[1]);
                 tmem_wait();
                 if (masked) {
 #pragma unroll
@@ -523,24 +575,28 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
                 // (a factor of 0 or NaN, or NaN for s_v, would make NaN of what is hidden)
                 if (__any_sync(~0u, fabsf(shift) > 60.0f || (masked && !(factor > 0.0f && shift == shift)))) {
 #pragma unroll 1
-                    for (int q = 0; q < 2; ++q) {
-                        tmem_ld32_issue(scores + 32 * q, v[0]);
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t some[16], out[8];
+                        tmem_ld16_issue(scores + 16 * q, some);
                         tmem_wait();
-                        const uint32_t some = (uint32_t)(bits >> (32 * q));
-                        uint32_t out[16];
+                        const uint32_t shown = (uint32_t)(bits >> (16 * q));
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
+                        for (int j = 0; j < 16; j += 2) {
                             float w[2];
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const float s = __uint_as_float(v[0][j + e]);
-                                const bool shown = some >> (j + e) & 1u;
-                                w[e] = shown ? power_of_two(fmaf(s, factor, plus)) : 0.0f;
-                                l += shown ? power_of_two(fmaf(s, factor, -from_m)) : 0.0f; // (either may be 0 where the other is not)
+                                const float s = __uint_as_float(some[j + e]);
+                                w[e] = shown >> (j + e) & 1u ? power_of_two(fmaf(s, factor, plus)) : 0.0f;
+                                l += shown >> (j + e) & 1u ? power_of_two(fmaf(s, factor, -from_m)) : 0.0f; // (either may be 0 where the other is not)
                             }
                             out[j / 2] = halves_of_floats(w[0], w[1]);
                         }
-                        tmem_st16(scores + 16 * q, out);
+                        tmem_st8(scores + 8 * q, out);
+                    }
+                    if (more) {
+                        if (!scores_there(i + 1)) break;
+                        tmem_ld32_issue(scores_next, v[0]);
+                        tmem_ld32_issue(scores_next + 32, v[1]);
                     }
                 } else {
                     const uint64_t by = pair_of(factor, factor), and_plus = pair_of(plus, plus);
@@ -557,7 +613,12 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
                             out[j / 2] = halves_of_floats(w0, w1);
                         }
                         tmem_st16(scores + 16 * q, out);
+                        if (more) {
+                            if (q == 0 && !scores_there(i + 1)) break;
+                            tmem_ld32_issue(scores_next + 32 * q, v[q]);
+                        }
                     }
+                    if (!ok) break;
                     float a0, a1;
                     halves_of(add_pair(sum[0], sum[1]), a0, a1);
                     l += (a0 + a1) * exp2f(-shift);
@@ -585,53 +646,38 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
         const size_t to = (size_t)(work.row + token) * a.y.ld + (size_t)(work.head * a.group + at % a.group) * a.y.head_ld;
         const RowEnd row_end(m, top, l);
         const bool wide = !part && (reinterpret_cast<uintptr_t>(static_cast<uint16_t *>(a.y.x) + to) & 15) == 0;
-        constexpr int AT_ONCE = PADDED < 128 ? PADDED / 32 : PADDED % 128 == 0 ? 4 : PADDED % 96 == 0 ? 3 : 1; // times 32 dimensions
 #pragma unroll 1
-        for (int d0 = 0; d0 < PADDED; d0 += 32 * AT_ONCE) {
-            uint32_t v[AT_ONCE][32];
+        for (int d = 0; d < PADDED; d += 16) {
+            uint32_t v[16];
             __syncwarp();
             if (taken) {
-#pragma unroll
-                for (int q = 0; q < AT_ONCE; ++q) tmem_ld32_issue(sums + d0 + 32 * q, v[q]);
+                tmem_ld16_issue(sums + d, v);
                 tmem_wait();
             } else {
 #pragma unroll
-                for (int q = 0; q < AT_ONCE; ++q)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[q][j] = 0;
+                for (int j = 0; j < 16; ++j) v[j] = 0;
             }
             if (!there) continue;
+            if (part) {
 #pragma unroll
-            for (int q = 0; q < AT_ONCE; ++q) {
-                const int d = d0 + 32 * q;
-                if (part) {
+                for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4 *>(part + (size_t)in_tile * PADDED + d + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                continue;
+            }
+            uint32_t o[8];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4 *>(part + (size_t)in_tile * PADDED + d + j) = make_uint4(v[q][j], v[q][j + 1], v[q][j + 2], v[q][j + 3]);
-                    continue;
-                }
+            for (int j = 0; j < 8; ++j) {
+                const float y0 = row_end.of(__uint_as_float(v[2 * j])), y1 = row_end.of(__uint_as_float(v[2 * j + 1]));
+                const __nv_bfloat162 b = __floats2bfloat162_rn(y0, y1);
+                o[j] = a.y.type == VALUE_F16 ? halves_of_floats(y0, y1) : *reinterpret_cast<const uint32_t *>(&b);
+            }
+            uint16_t *y = static_cast<uint16_t *>(a.y.x) + to + d;
+            if (wide && d + 16 <= (int)c.width) {
+                *reinterpret_cast<uint4 *>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4 *>(y + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+            } else {
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = row_end.of(__uint_as_float(v[q][j + e]));
-                    if (wide && d + j + 8 <= (int)c.width) {
-                        uint4 o;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (a.y.type == VALUE_F16) {
-                                (&o.x)[e] = halves_of_floats(y[2 * e], y[2 * e + 1]);
-                            } else {
-                                const __nv_bfloat162 b = __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]);
-                                (&o.x)[e] = *reinterpret_cast<const uint32_t *>(&b);
-                            }
-                        }
-                        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.y.x) + to + d + j) = o;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (d + j + e < (int)c.width) put_value(a.y, to + d + j + e, y[e]);
-                    }
-                }
+                for (int j = 0; j < 16; ++j)
+                    if (d + j < (int)c.width) y[j] = (uint16_t)(o[j / 2] >> (16 * (j % 2)));
             }
         }
     }
@@ -658,7 +704,7 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, 1) attend_many_
             mbar_init(&bars.queries[h], 4), mbar_init(&bars.added[h], 1), mbar_init(&bars.sums[h], 1);
             for (int i = 0; i < 2; ++i) mbar_init(&bars.scores[h][i], 1), mbar_init(&bars.weights[h][i], 4);
         }
-        for (int i = 0; i < 2; ++i) mbar_init(&bars.told[i], 1), mbar_init(&bars.heard[i], 1 + CONVERTERS + 4 * HALVES);
+        for (int i = 0; i < 2; ++i) mbar_init(&bars.told[i], 1), mbar_init(&bars.heard[i], 2 + CONVERTERS + 4 * HALVES);
         bars.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -681,8 +727,9 @@ template <int PADDED> __global__ void __launch_bounds__(THREADS, 1) attend_many_
     if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (warp == 0) issue_products<PADDED>(P, bars, work_room, queries, ring, tmem);
-        else if (warp == 1) tell_parts<PADDED>(P, plan, bars, work_room, codes, start, end);
-        else convert_codes<PADDED>(P, bars, work_room, codes, ring);
+        else if (warp == 1) tell_parts<PADDED>(P, plan, bars, work_room, start, end);
+        else if (warp == 2) fetch_codes<PADDED>(P, bars, work_room, codes);
+        else if (warp >= 4) convert_codes<PADDED>(P, bars, work_room, codes, ring);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         weigh_rows<PADDED>(P, bars, work_room, queries, down_room, tmem);

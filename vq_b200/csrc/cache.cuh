@@ -10,7 +10,7 @@ __device__ __forceinline__ void cache_is_there() { asm volatile("griddepcontrol.
 
 __device__ __forceinline__ int offset_of(const Sequences &s, int b)
 {
-    if (!s.offsets) return (int)((long long)s.n * b / s.sequences); // (n is a multiple)
+    if (!s.offsets) return s.each * b;
     const long long o = s.offsets[b];
     return (int)(o < 0 ? 0 : o > s.n ? s.n : o);
 }

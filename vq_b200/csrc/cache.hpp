@@ -38,7 +38,7 @@ struct Sequences {
     int sequences = 0, columns = 0;
     const int32_t *lengths = nullptr;
     const long long *offsets = nullptr;
-    int n = 0;
+    int n = 0, each = 0; // each: n / sequences, where offsets is null
 };
 
 // Values of n rows x heads x width, each head's next to each other.
