@@ -60,6 +60,14 @@ __device__ __forceinline__ uint32_t codes_again(uint32_t four, float old, float 
     return out;
 }
 
+// Numbers below 64 x 256 in rows of `length`: division by multiplication with the reciprocal, half a step up (exact: i / length + 1 / (2 length) is 2^-9 or more from the next whole number).
+struct Rows {
+    int length;
+    float inverse;
+    __device__ __forceinline__ explicit Rows(int l) : length(l), inverse(1.0f / (float)l) {}
+    __device__ __forceinline__ int of(int i) const { return (int)(((float)i + 0.5f) * inverse); }
+};
+
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float(float v) { return v; }
 template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
@@ -79,10 +87,25 @@ template <typename T> __global__ void __launch_bounds__(THREADS) cache_write_ker
     const T *x = static_cast<const T *>(in.x) + (size_t)part.row * in.ld + (size_t)head * in.head_ld;
     const int a = part.a, b = part.b, count = b - a;
     if (threadIdx.x == 0) old_scale = a == 0 ? 0.0f : *scale_of(c, part.page, head, which); // (a page that begins anew)
+    // eight or four values at a time where rows begin at multiples of 16 bytes; the second time they come from L1
+    constexpr int N = Piece<T>::N;
+    const bool aligned = width % N == 0 && in.ld % N == 0 && in.head_ld % N == 0 && (reinterpret_cast<uintptr_t>(in.x) & 15) == 0;
+    const Rows rows(aligned ? width / N : width);
     uint32_t most = 0;
-    for (int i = threadIdx.x; i < count * width; i += THREADS) {
-        const int t = i / width;
-        most = max(most, __float_as_uint(to_float(x[t * in.ld + (i - t * width)])) & 0x7FFFFFFFu);
+    if (aligned) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < count * rows.length; i += THREADS) {
+            const int t = rows.of(i);
+            Piece<T> piece;
+            piece.w = *reinterpret_cast<const uint4 *>(x + t * in.ld + (i - t * rows.length) * N);
+#pragma unroll
+            for (int j = 0; j < N; ++j) most = max(most, __float_as_uint(piece.at(j)) & 0x7FFFFFFFu);
+        }
+    } else {
+        for (int i = threadIdx.x; i < count * width; i += THREADS) {
+            const int t = rows.of(i);
+            most = max(most, __float_as_uint(to_float(x[t * in.ld + (i - t * width)])) & 0x7FFFFFFFu);
+        }
     }
     most = __reduce_max_sync(~0u, most);
     if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = most;
@@ -96,39 +119,64 @@ template <typename T> __global__ void __launch_bounds__(THREADS) cache_write_ker
     if (threadIdx.x == 0) *scale_of(c, part.page, head, which) = scale;
     uint32_t *codes = reinterpret_cast<uint32_t *>(codes_of(c, part.page, head, which));
     const int words = padded / 4;
-    if (which == 0) { // a token's key: words of four dimensions
-        for (int i = threadIdx.x; i < (grown ? b : count) * words; i += THREADS) {
-            const int k = i / words, d = 4 * (i - k * words), t = (grown ? 0 : a) + k;
-            uint32_t w = ZEROS, *to = codes + key_at(padded, t, d) / 4;
-            if (t < a) {
-                w = codes_again(*to, old, scale);
-            } else if (!none) {
+    if (which == 0 && grown)
+        for (int i = threadIdx.x; i < a * words; i += THREADS) codes[i] = codes_again(codes[i], old, scale);
+    // keys to their places, values (turned) to shared memory
+    uint8_t *bytes = reinterpret_cast<uint8_t *>(tile);
+    if (aligned) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < count * rows.length; i += THREADS) {
+            const int t = rows.of(i), d = (i - t * rows.length) * N;
+            Piece<T> piece;
+            piece.w = *reinterpret_cast<const uint4 *>(x + t * in.ld + d);
+            Packed<N> four = {};
+            if (!none) {
+                float v[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] = piece.at(j);
+                four = pack_codes<N>(v, inverse);
+            }
+            if (which == 0) {
+                uint32_t *to = codes + key_at(padded, a + t, d) / 4;
+                if (N == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(four.w[0] ^ ZEROS, four.w[N / 4 - 1] ^ ZEROS);
+                else *to = four.w[0] ^ ZEROS;
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) bytes[(d + j) * PITCH + a + t] = (uint8_t)((four.w[j / 4] ^ ZEROS) >> (8 * (j % 4)));
+            }
+        }
+    } else {
+        const Rows fours((width + 3) / 4);
+        for (int i = threadIdx.x; i < count * fours.length; i += THREADS) {
+            const int t = fours.of(i), d = 4 * (i - t * fours.length);
+            uint32_t w = ZEROS;
+            if (!none) {
                 float v[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = d + j < width ? to_float(x[(t - a) * in.ld + d + j]) : 0.0f;
+                for (int j = 0; j < 4; ++j) v[j] = d + j < width ? to_float(x[t * in.ld + d + j]) : 0.0f;
                 w = pack_codes<4>(v, inverse).w[0] ^ ZEROS;
             }
-            *to = w;
+            if (which == 0) {
+                codes[key_at(padded, a + t, d) / 4] = w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) bytes[(d + j) * PITCH + a + t] = (uint8_t)(w >> (8 * j));
+            }
+        }
+    }
+    if (which == 0) return;
+    __syncthreads();
+    if (count == CACHE_PAGE) {
+        for (int i = threadIdx.x; i < 4 * width; i += THREADS) {
+            const uint32_t *from = tile + i / 4 * (PITCH / 4) + i % 4 * 4;
+            reinterpret_cast<uint4 *>(codes)[i] = make_uint4(from[0], from[1], from[2], from[3]);
         }
         return;
     }
-    // values: turned in shared memory, a dimension's words of four tokens
-    for (int i = threadIdx.x; i < count * words; i += THREADS) {
-        const int k = i / words, d = 4 * (i - k * words);
-        uint32_t w = ZEROS;
-        if (!none) {
-            float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = d + j < width ? to_float(x[k * in.ld + d + j]) : 0.0f;
-            w = pack_codes<4>(v, inverse).w[0] ^ ZEROS;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) reinterpret_cast<uint8_t *>(tile)[(d + j) * PITCH + a + k] = (uint8_t)(w >> (8 * j));
-    }
-    __syncthreads();
-    const int first = grown ? 0 : a / 4, many = (b + 3) / 4 - first; // words of a dimension
-    for (int i = threadIdx.x; i < many * padded; i += THREADS) {
-        const int d = i / many, at = first + i - d * many, t = 4 * at;
+    const int first = grown ? 0 : a / 4; // words of a dimension
+    const Rows dims((b + 3) / 4 - first);
+    for (int i = threadIdx.x; i < dims.length * width; i += THREADS) {
+        const int d = dims.of(i), at = first + i - d * dims.length, t = 4 * at;
         uint32_t *to = codes + d * (CACHE_PAGE / 4) + at, w = tile[d * (PITCH / 4) + at];
         if (t < a || t + 4 > b) { // bytes of tokens a .. b - 1 among others
             uint32_t others = *to;
@@ -147,7 +195,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) cache_read_kern
     __shared__ uint32_t tile[CACHE_MOST_WIDTH * PITCH / 4];
     cache_is_there();
     const Cache &c = P.c;
-    const int head = blockIdx.y, which = blockIdx.z, width = (int)c.width, words = (int)c.padded / 4;
+    const int head = blockIdx.y, which = blockIdx.z, width = (int)c.width;
     const HeadRows &out = P.x[which];
     T *y = static_cast<T *>(out.x) + (size_t)head * out.head_ld;
     if (blockIdx.x >= blocks) { // rows of no sequence
@@ -168,17 +216,51 @@ template <typename T> __global__ void __launch_bounds__(THREADS) cache_read_kern
     }
     const uint32_t *codes = reinterpret_cast<const uint32_t *>(codes_of(c, part.page, head, which));
     const float scale = *scale_of(c, part.page, head, which);
+    const uint8_t *bytes = reinterpret_cast<const uint8_t *>(tile);
     if (which) {
-        for (int i = threadIdx.x; i < (int)c.padded * (CACHE_PAGE / 4); i += THREADS) tile[i / (CACHE_PAGE / 4) * (PITCH / 4) + i % (CACHE_PAGE / 4)] = codes[i];
+#pragma unroll 4
+        for (int i = threadIdx.x; i < 4 * width; i += THREADS) {
+            const uint4 w = reinterpret_cast<const uint4 *>(codes)[i];
+            uint32_t *to = tile + i / 4 * (PITCH / 4) + i % 4 * 4;
+            to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+        }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < count * words; i += THREADS) {
-        const int k = i / words, d = 4 * (i - k * words);
-        const uint32_t w = which ? 0 : codes[key_at((int)c.padded, a + k, d) / 4];
+    // eight values at a time where rows begin at multiples of 16 bytes
+    const bool aligned = width % 8 == 0 && out.ld % 8 == 0 && out.head_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(out.x) & 15) == 0;
+    const Rows rows(aligned ? width / 8 : (width + 3) / 4);
+    if (aligned) {
+#pragma unroll 2
+        for (int i = threadIdx.x; i < count * rows.length; i += THREADS) {
+            const int t = rows.of(i), d = 8 * (i - t * rows.length);
+            uint2 w = make_uint2(0, 0);
+            if (!which) w = *reinterpret_cast<const uint2 *>(codes + key_at((int)c.padded, a + t, d) / 4);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = (float)((which ? (int)bytes[(d + j) * PITCH + a + t] : (int)((&w.x)[j / 4] >> (8 * (j % 4)) & 255u)) - 128) * scale;
+            T *to = y + t * out.ld + d;
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4 *>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                uint4 o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    T two[2] = {from_float<T>(v[2 * j]), from_float<T>(v[2 * j + 1])};
+                    (&o.x)[j] = *reinterpret_cast<const uint32_t *>(two);
+                }
+                *reinterpret_cast<uint4 *>(to) = o;
+            }
+        }
+        return;
+    }
+    for (int i = threadIdx.x; i < count * rows.length; i += THREADS) {
+        const int t = rows.of(i), d = 4 * (i - t * rows.length);
+        const uint32_t w = which ? 0 : codes[key_at((int)c.padded, a + t, d) / 4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int q = (which ? reinterpret_cast<const uint8_t *>(tile)[(d + j) * PITCH + a + k] : (int)(w >> (8 * j) & 255u)) - 128;
-            if (d + j < width) y[k * out.ld + d + j] = from_float<T>((float)q * scale);
+            const int q = (which ? (int)bytes[(d + j) * PITCH + a + t] : (int)(w >> (8 * j) & 255u)) - 128;
+            if (d + j < width) y[t * out.ld + d + j] = from_float<T>((float)q * scale);
         }
     }
 }
