@@ -1122,6 +1122,7 @@ class QuantizedCache:
         p, h, w = C.c_size_t(), C.c_size_t(), C.c_size_t()
         _lib.load().vqb_cache_shape(handle, C.byref(p), C.byref(h), C.byref(w))
         self._shape = int(p.value), int(h.value), int(w.value)
+        self._scale = self._shape[2] ** -0.5
 
     @classmethod
     def empty(cls, pages: int, heads: int, width: int, *, ctx: Context | None = None):
@@ -1196,6 +1197,14 @@ class QuantizedCache:
             if rc:
                 _raise(rc, ctx.handle)
 
+    def _plain(self, torch, x, table, lengths):
+        """Whether rows (a tensor), table and lengths are what a server has: contiguous on the cache's GPU, of types that are taken as they are.  (For one token of one request a
+        call lasts as long as its host code does.)"""
+        device, Tensor = self._ctx.device, torch.Tensor
+        return (type(table) is Tensor and type(lengths) is Tensor and x.is_cuda and table.is_cuda and lengths.is_cuda and x.is_contiguous() and table.is_contiguous()
+                and lengths.is_contiguous() and table.dtype is torch.int32 and lengths.dtype is torch.int32 and x.dim() == 3 and table.dim() == 2 and lengths.dim() == 1
+                and x.get_device() == device and table.get_device() == device and lengths.get_device() == device and not x.requires_grad)
+
     def write(self, keys, values, table, lengths, *, offsets=None):
         """Writes the rows (n x heads x width each) into their pages, `lengths` counting them.
 
@@ -1237,14 +1246,30 @@ class QuantizedCache:
         Query head h reads the cache's head ``h // (query heads // heads)``.  A row sees the tokens up to its own; with `window` only the last so many of
         them, itself among these, and the first `sinks` ones.  `scale` multiplies the scores (width ** -0.5 by default).  A row that sees nothing
         comes out as 0; rows of no sequence do in a fresh result and stay as they are in the caller's `out`."""
-        x = _Heads(queries, self._ctx, "queries")
         if window is not None and window < 1:
             raise ValueError("window must be positive, or None")
         if sinks < 0:
             raise ValueError("sinks must not be negative")
+        torch = sys.modules.get("torch")
+        if out is None and offsets is None and torch is not None and type(queries) is torch.Tensor and self._plain(torch, queries, table, lengths):
+            kind = (_TORCH_VALUES or _torch_values(torch)).get(queries.dtype)
+            n, heads, dim = queries.shape
+            sequences, columns = table.shape
+            if kind is not None and lengths.shape[0] == sequences:
+                ctx, y, ld = self._ctx, torch.empty_like(queries), heads * dim
+                stream = torch._C._cuda_getCurrentRawStream(ctx.device)
+                with ctx._lock:
+                    if stream != ctx._stream:
+                        ctx._run_on(stream)
+                    rc = ctx._L.vqb_cache_attend(self._h, queries.data_ptr(), kind, n, heads, dim, ld, dim, table.data_ptr(), sequences, columns, columns, lengths.data_ptr(), None,
+                                                 self._scale if scale is None else scale, window or 0, sinks, y.data_ptr(), ld, dim, 1)
+                    if rc:
+                        _raise(rc, ctx.handle)
+                return y
+        x = _Heads(queries, self._ctx, "queries")
         y, yptr, y_ld, y_head_ld = _heads_result(x, out)
         keep, sequences = self._sequences(x, table, lengths, offsets)
-        self._call(x, self._ctx._L.vqb_cache_attend, x.ptr, x.type, x.n, x.heads, x.dim, x.ld, x.head_ld, *sequences, self._shape[2] ** -0.5 if scale is None else scale,
+        self._call(x, self._ctx._L.vqb_cache_attend, x.ptr, x.type, x.n, x.heads, x.dim, x.ld, x.head_ld, *sequences, self._scale if scale is None else scale,
                    window or 0, sinks, yptr, y_ld, y_head_ld, 1 if out is None else 0)
         return y
 

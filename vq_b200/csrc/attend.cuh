@@ -316,8 +316,10 @@ template <int PADDED, int ROWS> __global__ void __launch_bounds__(128) attend_jo
             const float *part = part_of(s0 + k) + r * PADDED + lane;
             const float w = __shfl_sync(~0u, by, k);
 #pragma unroll
-            for (int d = 0; d < PADDED / 32; ++d)
-                if (w != 0.0f) y[d] += part[32 * d] * w; // (a part that saw nothing may have no sums)
+            for (int d = 0; d < PADDED / 32; ++d) {
+                const float v = part[32 * d];
+                y[d] += w != 0.0f ? v * w : 0.0f; // (a part that saw nothing may have no sums)
+            }
         }
     }
     const RowEnd row_end(m, top, l);

@@ -19,7 +19,7 @@ namespace vqb {
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = 32 * WARPS, STAGES = 2;
+constexpr int STAGES = 2;
 constexpr float LATE = 8.0f; // a row's largest score is followed when it is 2^LATE times as large
 
 __device__ __forceinline__ void mma_f16(float (&sums)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b)
@@ -47,9 +47,9 @@ template <> struct Words<8> {
 };
 template <int BYTES> __device__ __forceinline__ Words<BYTES> words_at(const uint8_t *p) { return *reinterpret_cast<const Words<BYTES> *>(p); }
 
-// EIGHTS: of rows a tile has
-template <int PADDED, int EIGHTS> struct FewShape {
-    static constexpr int ROWS = 8 * EIGHTS;
+// EIGHTS: of rows a tile has; WARPS: of a block
+template <int PADDED, int EIGHTS, int WARPS> struct FewShape {
+    static constexpr int ROWS = 8 * EIGHTS, THREADS = 32 * WARPS;
     static constexpr int PIECE = PADDED % 64 == 0 ? 16 : 8;                // bytes of a key that a lane reads at once
     static constexpr int CHUNKS = PADDED / (4 * PIECE), STEPS = PIECE / 4; // a chunk: four lanes' pieces, STEPS instructions
     static constexpr uint32_t HALF = CACHE_PAGE * PADDED;                  // a page's keys, or its values
@@ -58,7 +58,7 @@ template <int PADDED, int EIGHTS> struct FewShape {
     static constexpr size_t RING = WARPS * STAGES * HALF;
     static_assert(ROWS * PADDED * 4 <= STAGES * HALF, "the ring takes the warps' sums");
     static constexpr size_t SMEM = RING + QUERIES;
-    static constexpr int BLOCKS = PADDED <= 128 ? EIGHTS == 1 ? 3 : 2 : PADDED <= 192 ? 2 : 1; // an SM's
+    static constexpr int BLOCKS = WARPS == 8 ? 1 : PADDED <= 128 ? EIGHTS == 1 ? 3 : 2 : PADDED <= 192 ? 2 : 1; // an SM's
     using Sharing = Plan<ROWS, THREADS>;
 };
 
@@ -69,9 +69,9 @@ template <int PADDED, int EIGHTS> struct Running {
 };
 
 // Products of a page's keys with the rows.  Tile i: row g of it is token 16 (g / 2) + 4 i + g % 2, row 8 + g the token two behind that.
-template <int PADDED, int EIGHTS> __device__ __forceinline__ void take_keys(const uint8_t *keys, const uint2 *queries, const uint2 (&held)[EIGHTS][PADDED / 16], float (&s)[EIGHTS][4][4])
+template <int PADDED, int EIGHTS, int WARPS> __device__ __forceinline__ void take_keys(const uint8_t *keys, const uint2 *queries, const uint2 (&held)[EIGHTS][PADDED / 16], float (&s)[EIGHTS][4][4])
 {
-    using Shape = FewShape<PADDED, EIGHTS>;
+    using Shape = FewShape<PADDED, EIGHTS, WARPS>;
     const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
 #pragma unroll
     for (int e = 0; e < EIGHTS; ++e)
@@ -209,14 +209,14 @@ __device__ __forceinline__ void weigh(float (&s)[EIGHTS][4][4], const float (&do
 
 // A tile's queries as operand fragments, and each row's factor of scores: lane 4 g + t of step k of chunk c has dimensions d .. d + 3, d = (4 c + t) PIECE + 4 k, of row g of
 // each eight.  By the block: eight threads a row.  A negative scale turns the queries' signs: factors are not negative, and the largest product is the largest score.
-template <int PADDED, int EIGHTS>
+template <int PADDED, int EIGHTS, int WARPS>
 __device__ __forceinline__ void bring_queries(const Attend &a, const Span &span, const Tile<8 * EIGHTS> &tile, int rows, uint2 *queries, float *down)
 {
-    using Shape = FewShape<PADDED, EIGHTS>;
+    using Shape = FewShape<PADDED, EIGHTS, WARPS>;
     const int part = threadIdx.x % 8, width = (int)a.cache.width;
     const bool f16 = a.queries.type == VALUE_F16;
     const bool aligned = width % 4 == 0 && a.queries.ld % 4 == 0 && a.queries.head_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.queries.x) & 7) == 0;
-    for (int r = threadIdx.x / 8; r < Shape::ROWS; r += THREADS / 8) {
+    for (int r = threadIdx.x / 8; r < Shape::ROWS; r += Shape::THREADS / 8) {
         const int at = tile.first_row + min(r, rows - 1); // (rows behind the tile's: its last one)
         const uint16_t *x = static_cast<const uint16_t *>(a.queries.x) + (size_t)(span.row + at / a.group) * a.queries.ld + (size_t)(tile.head * a.group + at % a.group) * a.queries.head_ld;
         constexpr int FOURS = PADDED / 32; // four dimensions at a time: 4 (8 i + part)
@@ -259,10 +259,11 @@ __device__ __forceinline__ void bring_queries(const Attend &a, const Span &span,
     }
 }
 
-template <int PADDED, int EIGHTS> __global__ void __launch_bounds__(THREADS, FewShape<PADDED, EIGHTS>::BLOCKS) attend_few_kernel(const __grid_constant__ ShareParams P)
+template <int PADDED, int EIGHTS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, FewShape<PADDED, EIGHTS, WARPS>::BLOCKS) attend_few_kernel(const __grid_constant__ ShareParams P)
 {
-    using Shape = FewShape<PADDED, EIGHTS>;
-    constexpr int ROWS = Shape::ROWS;
+    using Shape = FewShape<PADDED, EIGHTS, WARPS>;
+    constexpr int ROWS = Shape::ROWS, THREADS = Shape::THREADS;
     extern __shared__ unsigned char smem_raw[];
     __shared__ typename Shape::Sharing::Room room;
     __shared__ unsigned long long full[WARPS][STAGES];
@@ -331,7 +332,7 @@ template <int PADDED, int EIGHTS> __global__ void __launch_bounds__(THREADS, Few
             fetch(k, stage, 0);
             if (++stage == STAGES) stage = 0;
         }
-        bring_queries<PADDED, EIGHTS>(a, span, tile, rows, queries, down);
+        bring_queries<PADDED, EIGHTS, WARPS>(a, span, tile, rows, queries, down);
         __syncthreads();
         Running<PADDED, EIGHTS> run;
         float mine[EIGHTS][2];
@@ -358,7 +359,7 @@ template <int PADDED, int EIGHTS> __global__ void __launch_bounds__(THREADS, Few
             uint2 weights[EIGHTS][4];
             if (!__all_sync(~0u, mbar_wait(&full[warp][st], parity, &abort_word, P.error, 91))) break;
             float s[EIGHTS][4][4];
-            if (page >= 0) take_keys<PADDED, EIGHTS>(ring + st * Shape::HALF, queries, held, s);
+            if (page >= 0) take_keys<PADDED, EIGHTS, WARPS>(ring + st * Shape::HALF, queries, held, s);
             __syncwarp();
             fetch(2 * i + STAGES, st, i / 32);
             if (++st == STAGES) st = 0, parity ^= 1u;
@@ -445,35 +446,50 @@ template <int PADDED, int EIGHTS> __global__ void __launch_bounds__(THREADS, Few
         for (int w = 0; w < 1000; ++w) __nanosleep(1000);
 }
 
-template <int PADDED, int EIGHTS> void attend_few_with(CudaDevice &dev, ShareParams &P)
+// Pages of a tile at most, as far as the host knows.
+template <int ROWS> size_t most_pages(const Attend &a)
 {
-    using Shape = FewShape<PADDED, EIGHTS>;
+    const size_t pages = std::max(a.seq.columns, 1);
+    return a.window ? std::min(pages, ((size_t)a.sinks + 63) / 64 + ((size_t)a.window + ROWS + 62) / CACHE_PAGE + 1) : pages;
+}
+
+template <int PADDED, int EIGHTS, int WARPS> void attend_few_with(CudaDevice &dev, ShareParams &P)
+{
+    using Shape = FewShape<PADDED, EIGHTS, WARPS>;
     constexpr int ROWS = Shape::ROWS;
-    const Attend &a = P.a;
-    P.slots = (int)slots_of<ROWS>(a);
-    size_t pages = std::max(a.seq.columns, 1); // of a tile at most
-    if (a.window) pages = std::min(pages, ((size_t)a.sinks + 63) / 64 + ((size_t)a.window + ROWS + 62) / CACHE_PAGE + 1);
-    const size_t rounds = (pages + WARPS - 1) / WARPS;
-    const bool join = rounds > 4;
+    P.slots = (int)slots_of<ROWS>(P.a);
+    const size_t rounds = (most_pages<ROWS>(P.a) + WARPS - 1) / WARPS;
+    const bool join = rounds > 16 / WARPS; // (up to sixteen pages are not shared out: one token behind 1000 in 14 us, 12 and another launch where they are)
     P.unit = (int)(join ? WARPS : rounds * WARPS);
-    const size_t units = (size_t)P.slots * a.cache.heads * (join ? rounds : 1), places = (size_t)dev.sm_count() * Shape::BLOCKS;
+    const size_t units = (size_t)P.slots * P.a.cache.heads * (join ? rounds : 1), places = (size_t)dev.sm_count() * Shape::BLOCKS;
     P.blocks = (int)std::min(units, places);
     Parts parts(dev);
     if (join) parts.make<ROWS>(P, PADDED);
-    allow_shared_memory(dev, attend_few_kernel<PADDED, EIGHTS>);
+    allow_shared_memory(dev, attend_few_kernel<PADDED, EIGHTS, WARPS>);
     {
         KernelScope ks(dev, "attend_few");
-        launch_following(attend_few_kernel<PADDED, EIGHTS>, dim3((unsigned)P.blocks), dim3(THREADS), Shape::SMEM + 128, dev.stream(), P);
+        launch_following(attend_few_kernel<PADDED, EIGHTS, WARPS>, dim3((unsigned)P.blocks), dim3(Shape::THREADS), Shape::SMEM + 128, dev.stream(), P);
         dev.count_launch();
     }
     launch_join<PADDED, ROWS>(dev, P);
 }
 
+// Eight warps a block where every tile has an SM to itself and as few pages as are not shared out: one token behind 1000 in 11.7 us instead of 14.2.  (Elsewhere four are better
+// used: 64 sequences of up to 8192 tokens take 101 us and not 118.)
+template <int PADDED, int EIGHTS> void attend_few_rows(CudaDevice &dev, ShareParams &P)
+{
+    if constexpr (PADDED <= 160) {
+        const size_t pages = most_pages<8 * EIGHTS>(P.a);
+        if (pages > 4 && pages <= 16 && slots_of<8 * EIGHTS>(P.a) * P.a.cache.heads <= (size_t)dev.sm_count()) return attend_few_with<PADDED, EIGHTS, 8>(dev, P);
+    }
+    attend_few_with<PADDED, EIGHTS, 4>(dev, P);
+}
+
 template <int PADDED> void attend_few_width(CudaDevice &dev, ShareParams &P)
 {
     const size_t rows = (size_t)P.a.seq.n * P.a.group;
-    if (!P.a.seq.offsets && rows / P.a.seq.sequences <= 8) attend_few_with<PADDED, 1>(dev, P);
-    else attend_few_with<PADDED, 2>(dev, P);
+    if (!P.a.seq.offsets && rows / P.a.seq.sequences <= 8) attend_few_rows<PADDED, 1>(dev, P);
+    else attend_few_rows<PADDED, 2>(dev, P);
 }
 
 } // namespace

@@ -1,6 +1,6 @@
 // cache.hpp -- keys and values of attention as 8-bit codes: pages of 64 tokens, one scale for each page and head.
 //
-// cache.cu writes tokens into pages, reads them back and lays pages out; attend.cu computes attention over them.
+// cache.cu writes tokens into pages, reads them back and lays pages out; attend_few.cu, attend_many.cu and attend_plain.cu compute attention over them.
 #pragma once
 #include <cstddef>
 #include <cstdint>
@@ -66,8 +66,9 @@ struct Attend {
 };
 // Rows of a sequence are taken together where they have the same cached head: `group` query heads of one token, then those of the next.  A sequence of up to ATTEND_FEW of
 // them is taken sixteen at a time, by tensor-core instructions of a warp on pages that the warp fetches for itself; nothing counts there but the cache's bytes.
-// Others are taken 256 or 128 at a time by tcgen05 instructions.
-constexpr int ATTEND_FEW = 64;
+// Others are taken 256 or 128 at a time by tcgen05 instructions.  (us by the one and by the other: 16 sequences of up to 8192 tokens with 32 rows each 107 and 167, with 64 rows 203 and 167; 64 of
+// up to 1000 with 64 rows 167 and 134.)
+constexpr int ATTEND_FEW = 32;
 void launch_attend(CudaDevice &dev, const Attend &a);
 void launch_attend_few(CudaDevice &dev, const Attend &a);  // sequences of up to ATTEND_FEW rows, and rows of no sequence
 void launch_attend_many(CudaDevice &dev, const Attend &a); // the other sequences
