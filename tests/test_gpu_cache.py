@@ -532,6 +532,31 @@ def test_many_sequences():
     attend_case(35, lengths, counts, 1, 2, 64)
 
 
+@pytest.mark.parametrize("heads,group,tokens", [(2, 1, 100), (4, 2, 128), (3, 1, 64), (8, 2, 33)])
+def test_many_short_prompts(heads, group, tokens):
+    """More tiles than SMs, none of which has more than two pages."""
+    torch = torch_()
+    lengths = np.random.RandomState(tokens).randint(tokens, 129, 150)
+    attend_case(36, lengths, [tokens] * 150, heads, group, 64)
+    counts = np.random.RandomState(7).randint(0, tokens + 1, 150)
+    attend_case(37, lengths, counts, heads, group, 128, rest=(1, 1))
+
+
+def test_without_tensor_cores():
+    """VQB_NO_TENSOR=1, in a process of its own: the same results, by other sums."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import numpy as np, torch
+from tests import test_gpu_cache as t
+t.attend_case(41, [300, 0, 64], [1, 1, 1], 2, 4, 72)
+t.attend_case(42, [300, 5, 200], [120, 5, 33], 1, 3, 128, "float16", rest=(2, 1), window=50, sinks=3)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, env={**os.environ, "VQB_NO_TENSOR": "1"}, timeout=120)
+
+
 # ---- together --------------------------------------------------------------------------------------------------
 def run_together(step_of, tokens=70, seed=40):
     """A prompt, then single tokens, each of which writes and attends: (results, what they should be, limits)."""

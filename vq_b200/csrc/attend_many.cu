@@ -302,7 +302,7 @@ __device__ __forceinline__ uint64_t seen_bits(int column, int position, int keys
 {
     const int first = column * CACHE_PAGE;
     uint64_t bits = bits_below(min(position + 1, keys) - first);
-    if (window) bits &= ~(bits_below(max(position - window + 1, 0) - first) & ~bits_below(min(sinks, keys) - first));
+    if (window) bits &= ~(bits_below(max(max(position, 0) - window + 1, 0) - first) & ~bits_below(min(sinks, keys) - first));
     return position < 0 ? 0 : bits;
 }
 
@@ -753,7 +753,7 @@ template <int PADDED> void attend_many_with(CudaDevice &dev, ShareParams &P, con
     const size_t steps = (pages + 1) / 2;
     const bool join = steps > 1;
     const size_t places = dev.sm_count(), tiles = (size_t)P.slots * a.cache.heads;
-    P.unit = 2, P.extra = tiles > places ? 4 : 0; // (what a tile takes beside its steps, in steps)
+    P.unit = 2, P.extra = join && tiles > places ? 4 : 0; // (what a tile takes beside its steps, in units; where nothing is joined a tile is one unit, which no share's end cuts)
     P.blocks = (int)std::min(tiles * (steps + P.extra), places);
     Parts parts(dev);
     if (join) parts.make<ROWS>(P, PADDED);
