@@ -343,7 +343,7 @@ int vqb_qmat_destroy(vqb_qmat *qm);
  *
  * Queries and results are f16 or bf16 (VQB_ERR_UNSUPPORTED for f32: it would promise more digits than that).  ld and head_ld: values from row to row and from head to head.
  * Rows of no sequence (in front of offsets[0], behind the last offset) are left as they are, or become 0 with VQB_ZERO_REST; vqb_cache_read, whose results are
- * n x heads x width without gaps, makes them 0.  Limits (VQB_ERR_UNSUPPORTED beyond): width 256, 4096 heads, 65535 sequences.  A cache is made outside of captures; the calls
+ * n x heads x width without gaps, makes them 0.  Outputs may not overlap inputs.  Limits (VQB_ERR_UNSUPPORTED beyond): width 256, 4096 heads, 65535 sequences.  A cache is made outside of captures; the calls
  * on it may be captured with all operands in device memory, as products may. */
 #define VQB_CACHE_PAGE 64
 typedef struct vqb_cache vqb_cache;
