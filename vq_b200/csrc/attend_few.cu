@@ -172,9 +172,9 @@ __device__ __forceinline__ void weigh(float (&s)[EIGHTS][4][4], const float (&do
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             from[h] = run.m[e][h] == -INFINITY ? 0.0f : run.m[e][h];
-            const float from_top = run.top[e][h] == -INFINITY ? 0.0f : run.top[e][h], lv = none ? from_top - from[h] : log_v;
-            shift[h] = lv + from[h] - from_top; // a weight is 2^(s - m) 2^shift
-            plus[h] = lv - from_top;
+            const float from_top = run.top[e][h] == -INFINITY ? 0.0f : run.top[e][h];
+            shift[h] = log_v + from[h] - from_top; // a weight is 2^(s - m) 2^shift (values of 0: shift is -infinity, weights are 0)
+            plus[h] = log_v - from_top;
             far |= fabsf(shift[h]) > 60.0f;
         }
         far = __any_sync(~0u, far);

@@ -520,7 +520,7 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
                 const int column = work.column(i);
                 const bool is_there = __shfl_sync(~0u, page_now, i % 32) >= 0;
                 const float factor = score_factor(down, __shfl_sync(~0u, scale_now.x, i % 32));
-                float log_v = __shfl_sync(~0u, scale_now.y, i % 32);
+                const float log_v = __shfl_sync(~0u, scale_now.y, i % 32);
                 uint64_t bits = is_there ? ~0ull : 0;
                 if (is_there && !all_seen(column, work.p0, work.p1, work.keys, a.window, a.sinks)) bits = seen_bits(column, position, work.keys, a.window, a.sinks);
                 const bool masked = __any_sync(~0u, bits != ~0ull);
@@ -570,8 +570,7 @@ __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &b
                 }
                 added_parity ^= 1u;
                 const float from_m = m == -INFINITY ? 0.0f : m, from_top = top == -INFINITY ? 0.0f : top;
-                if (log_v == -INFINITY) log_v = from_top - from_m;
-                const float shift = log_v + from_m - from_top, plus = log_v - from_top; // a weight is 2^(s - m) 2^shift
+                const float shift = log_v + from_m - from_top, plus = log_v - from_top; // a weight is 2^(s - m) 2^shift (values of 0: shift is -infinity, weights are 0)
                 // (a factor of 0 or NaN, or NaN for s_v, would make NaN of what is hidden)
                 if (__any_sync(~0u, fabsf(shift) > 60.0f || (masked && !(factor > 0.0f && shift == shift)))) {
 #pragma unroll 1
