@@ -1,0 +1,33 @@
+"""Distances of rows and heads that the calls on a cache take: by the library's own rule, compiled and run without a GPU, and at the C ABI."""
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import vq_b200 as vq
+from vq_b200 import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_rules(tmp_path):
+    exe = os.path.join(str(tmp_path), "test_spans")
+    subprocess.check_call(["/usr/bin/g++", "-std=c++17", "-O1", "-Wall", "-o", exe, os.path.join(ROOT, "tests", "cpp", "test_spans.cpp")])
+    res = subprocess.run([exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=60)
+    assert res.returncode == 0, res.stdout.decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,ld", [(2**23 + 1, 2**40), (2**24 + 1, 2**40), (2, 2**63)])
+def test_rows_too_far_apart_are_refused_before_anything_is_read(n, ld):
+    """Host memory, as anything else would be the caller's own lie: none of it is touched."""
+    lib, cache = _lib.load(), vq.QuantizedCache.empty(1, 1, 4)
+    x, y = np.zeros(4, np.float16), np.full(4, 7, np.float16)
+    table, lengths = np.zeros((1, 1), np.int32), np.ones(1, np.int32)
+    sequences = table.ctypes.data, 1, 1, 1, lengths.ctypes.data, None
+    assert lib.vqb_cache_write(cache._h, x.ctypes.data, ld, 4, x.ctypes.data, 4, 4, 1, n, 1, 4, *sequences) == 90
+    assert lib.vqb_cache_write(cache._h, x.ctypes.data, 4, 4, x.ctypes.data, ld, 4, 1, n, 1, 4, *sequences) == 90
+    assert lib.vqb_cache_attend(cache._h, x.ctypes.data, 1, n, 1, 4, ld, 4, *sequences, 1.0, 0, 0, y.ctypes.data, 4, 4, 0) == 90
+    assert lib.vqb_cache_attend(cache._h, x.ctypes.data, 1, n, 1, 4, 4, 4, *sequences, 1.0, 0, 0, y.ctypes.data, ld, 4, 0) == 90
+    assert (y == 7).all()

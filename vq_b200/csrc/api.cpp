@@ -17,6 +17,7 @@
 #include "cuda_device.hpp"
 #include "opq_parts.hpp"
 #include "qmat.hpp"
+#include "spans.hpp"
 #include "tsvq.hpp"
 
 namespace vqb {
@@ -518,20 +519,12 @@ struct NewCache {
     ~NewCache() { drop(); }
 };
 
-// Rows of heads: neither rows nor heads overlap, whichever of the two is the outer one.
 void check_heads(const char *what, const void *p, int type, size_t n, size_t heads, size_t width, size_t ld, size_t head_ld)
 {
     check_values(what, p, type, 1, 1);
-    constexpr size_t FAR = size_t(1) << 40; // (values; no product below leaves 64 bits)
-    if ((n > 1 && ld > FAR) || (heads > 1 && head_ld > FAR / 4096)) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + ": rows are too far apart");
-    const bool heads_inside = (heads == 1 || head_ld >= width) && (n == 1 || ld >= (heads - 1) * head_ld + width);
-    const bool rows_inside = (n == 1 || ld >= width) && (heads == 1 || (head_ld >= width && (head_ld - width) / std::max<size_t>(ld, 1) >= n - 1));
-    if (!heads_inside && !rows_inside) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + ": rows or heads overlap");
+    if (const char *fault = heads_fault(n, heads, width, ld, head_ld)) throw Error(VQB_ERR_BAD_ARGUMENT, std::string(what) + ": " + fault);
 }
-size_t heads_span(int type, size_t n, size_t heads, size_t width, size_t ld, size_t head_ld)
-{
-    return n ? ((n - 1) * ld + (heads - 1) * head_ld + width) * value_bytes(type) : 0;
-}
+size_t heads_span(int type, size_t n, size_t heads, size_t width, size_t ld, size_t head_ld) { return heads_values(n, heads, width, ld, head_ld) * value_bytes(type); }
 
 // The arguments that say which tokens a call's rows are, in device memory for as long as the call lasts.
 struct SequencesIn {
