@@ -40,6 +40,11 @@ int main()
     expect(heads_fault((one << 23) + 1, 1, 4, one << 40, 4), "8388609 rows 2^40 values apart", 0, 0, 0, 0, 0);
     expect(heads_fault((one << 24) + 1, 1, 4, one << 40, 4), "16777217 rows 2^40 values apart", 0, 0, 0, 0, 0);
     expect(heads_fault(2, 1, 4, one << 63, 4), "2 rows 2^63 values apart", 0, 0, 0, 0, 0);
+    // heads as far apart as many rows of one make it
+    expect(!heads_fault((one << 21) + 1, 2, 128, 128, (one << 28) + 128), "2^21 + 1 rows of 128 values, head behind head", 0, 0, 0, 0, 0);
+    expect(!heads_fault(3, 4096, 64, 64, one << 40), "4096 heads 2^40 values apart", 0, 0, 0, 0, 0);
+    expect(heads_fault(3, 3, 64, 64, one << 58), "3 heads 2^58 values apart", 0, 0, 0, 0, 0);
+    expect(heads_fault(3, 4096, 64, 64, ~size_t(0)), "heads 2^64 - 1 values apart", 0, 0, 0, 0, 0);
     // distances that do not count
     expect(!heads_fault(1, 1, 4, ~size_t(0), ~size_t(0)), "one row of one head", 0, 0, 0, 0, 0);
     std::printf("%d taken, %d failed\n", taken, failed);

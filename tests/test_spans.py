@@ -31,3 +31,26 @@ def test_rows_too_far_apart_are_refused_before_anything_is_read(n, ld):
     assert lib.vqb_cache_attend(cache._h, x.ctypes.data, 1, n, 1, 4, ld, 4, *sequences, 1.0, 0, 0, y.ctypes.data, 4, 4, 0) == 90
     assert lib.vqb_cache_attend(cache._h, x.ctypes.data, 1, n, 1, 4, 4, 4, *sequences, 1.0, 0, 0, y.ctypes.data, ld, 4, 0) == 90
     assert (y == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 40])
+def test_heads_far_apart_are_taken(count):
+    """More than 2^28 values from head to head: what a head behind a head of 2^21 rows of 128 values has."""
+    import torch
+    from tests.test_gpu_cache import attend64, check, device, normal, some_cache
+    lengths = np.array([200])
+    cache, parts, table = some_cache(90, lengths, 2, 128)
+    apart = 2**28 + 128
+    room = torch.zeros(apart + count * 128, dtype=torch.float16, device="cuda")
+    far = torch.as_strided(room, (count, 2, 128), (128, apart, 1))
+    x = normal(91, count, 2, 128, dtype="float16")
+    far.copy_(x)
+    n, t = device(lengths.astype(np.int32)), device(table)
+    out = torch.as_strided(torch.zeros_like(room), (count, 2, 128), (128, apart, 1))
+    check(cache.attend(far, t, n, out=out), *attend64(parts, x, table, lengths, [0, count]))
+    same = vq.QuantizedCache.from_parts(*parts)
+    cache.write(far, far, t, n)
+    same.write(x, x, t, n)
+    for a, b in zip(cache.read(t, n, 200), same.read(t, n, 200)):
+        assert torch.equal(a, b)

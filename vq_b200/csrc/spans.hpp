@@ -1,6 +1,5 @@
 // spans.hpp -- how far the caller's rows reach in memory, from the distances that it gives.
 #pragma once
-#include <algorithm>
 #include <cstddef>
 
 namespace vqb {
@@ -14,9 +13,9 @@ constexpr bool too_far(size_t many, size_t step) { return many > 1 && step > MOS
 // What is wrong with the distances of n rows of heads, null where nothing is: neither rows nor heads overlap, whichever of the two is the outer one.
 inline const char *heads_fault(size_t n, size_t heads, size_t width, size_t ld, size_t head_ld)
 {
-    if (too_far(n, ld) || (heads > 1 && head_ld > (size_t(1) << 28))) return "rows are too far apart";
+    if (too_far(n, ld) || too_far(heads, head_ld)) return "rows are too far apart";
     const bool heads_inside = (heads == 1 || head_ld >= width) && (n == 1 || ld >= (heads - 1) * head_ld + width);
-    const bool rows_inside = (n == 1 || ld >= width) && (heads == 1 || (head_ld >= width && (head_ld - width) / std::max<size_t>(ld, 1) >= n - 1));
+    const bool rows_inside = (n == 1 || ld >= width) && (heads == 1 || head_ld >= (n - 1) * ld + width);
     return heads_inside || rows_inside ? nullptr : "rows or heads overlap";
 }
 
