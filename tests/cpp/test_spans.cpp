@@ -36,6 +36,8 @@ int main()
                         expect(heads_inside || rows_inside, "rows that overlap are taken", n, heads, width, ld, head_ld);
                     }
     expect(taken > 500, "hardly anything is taken", taken, 0, 0, 0, 0);
+    for (size_t n : rows)
+        for (size_t ld : steps) expect(too_far(n, ld) == ((wide)(n - 1) * ld > MOST_SPAN), "rows alone", n, 1, 0, ld, 0);
     // the bytes of these came out as 8, 0 and 0
     expect(heads_fault((one << 23) + 1, 1, 4, one << 40, 4), "8388609 rows 2^40 values apart", 0, 0, 0, 0, 0);
     expect(heads_fault((one << 24) + 1, 1, 4, one << 40, 4), "16777217 rows 2^40 values apart", 0, 0, 0, 0, 0);

@@ -1,4 +1,4 @@
-"""Distances of rows and heads that the calls on a cache take: by the library's own rule, compiled and run without a GPU, and at the C ABI."""
+"""Distances of rows and heads that the calls on 8-bit codes and on a cache take: by the library's own rule, compiled and run without a GPU, and at the C ABI."""
 import os
 import subprocess
 
@@ -31,6 +31,26 @@ def test_rows_too_far_apart_are_refused_before_anything_is_read(n, ld):
     assert lib.vqb_cache_attend(cache._h, x.ctypes.data, 1, n, 1, 4, ld, 4, *sequences, 1.0, 0, 0, y.ctypes.data, 4, 4, 0) == 90
     assert lib.vqb_cache_attend(cache._h, x.ctypes.data, 1, n, 1, 4, 4, 4, *sequences, 1.0, 0, 0, y.ctypes.data, ld, 4, 0) == 90
     assert (y == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ld", [2**63, 2**59, 2**64 - 4])
+def test_rows_of_products_too_far_apart_are_refused(ld):
+    """Two rows in host memory: what they span would have come out as a few bytes."""
+    lib, m = _lib.load(), vq.QuantizedMatrix.fit(np.ones((4, 4), np.float32), gradient=True)
+    x, codes, scales, y = np.zeros((2, 4), np.float16), np.zeros((2, 4), np.int8), np.ones(2, np.float32), np.full((2, 4), 7, np.float16)
+    at = [v.ctypes.data for v in (x, codes, scales, y)]
+    ctx = m._ctx.handle
+    assert lib.vqb_row_quantize(ctx, at[0], 1, 2, 4, ld, at[1], 4, at[2]) == 90
+    assert lib.vqb_row_quantize(ctx, at[0], 1, 2, 4, 4, at[1], ld, at[2]) == 90
+    assert lib.vqb_qmat_product(m._h, at[0], 1, 2, 4, ld, None, None, at[3], 1, 4, 0) == 90
+    assert lib.vqb_qmat_product(m._h, at[0], 1, 2, 4, 4, None, None, at[3], 1, ld, 0) == 90
+    assert lib.vqb_qmat_product_codes(m._h, at[1], ld, at[2], 2, 4, None, None, at[3], 1, 4, 0) == 90
+    assert lib.vqb_qmat_product_codes(m._h, at[1], 4, at[2], 2, 4, None, None, at[3], 1, ld, 0) == 90
+    assert lib.vqb_qmat_input_gradient(m._h, at[0], 1, 2, 4, ld, None, at[3], 4, 0) == 90
+    assert lib.vqb_qmat_input_gradient(m._h, at[0], 1, 2, 4, 4, None, at[3], ld, 0) == 90
+    assert (y == 7).all()
+    assert lib.vqb_qmat_product(m._h, at[0], 1, 1, 4, ld, None, None, at[3], 1, ld, 0) == 0 and (y[0] == 0).all()  # (one row: no distance)
 
 
 @pytest.mark.gpu

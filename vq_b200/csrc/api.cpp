@@ -376,7 +376,11 @@ void check_row_count(size_t n)
 }
 
 // Bytes from the first value of the first row to the last one of the last.
-size_t span(size_t n, size_t width, size_t ld, size_t bytes) { return n ? ((n - 1) * ld + width) * bytes : 0; }
+size_t span(size_t n, size_t width, size_t ld, size_t bytes)
+{
+    if (too_far(n, ld)) throw Error(VQB_ERR_BAD_ARGUMENT, "rows are too far apart");
+    return n ? ((n - 1) * ld + width) * bytes : 0;
+}
 
 // The groups' offsets: on the device as they are, from the host as they were when they were looked at.
 struct OffsetsIn {
