@@ -810,10 +810,18 @@ def _beside(v, x: _Values, name: str, shape, what: str):
     return v, ptr
 
 
+def _forward_mode() -> bool:
+    """Whether tensors may carry tangents (torch.autograd.forward_ad, torch.func.jvp)."""
+    forward = sys.modules.get("torch.autograd.forward_ad")
+    return forward is not None and getattr(forward, "_current_level", 0) >= 0
+
+
 def _record_nothing(what: str, v):
-    """Products are not part of torch's record of a computation: an operand that asks for a gradient would go without one."""
+    """Products are not part of torch's record of a computation: an operand that asks for a gradient, or carries a tangent, would go without one."""
     if getattr(v, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
         raise ValueError(f"{what} requires a gradient, which this call does not record: pass {what}.detach() (input_gradient gives the rows' gradient)")
+    if _forward_mode() and _is_torch(v) and sys.modules["torch.autograd.forward_ad"].unpack_dual(v).tangent is not None:
+        raise ValueError(f"{what} carries a tangent, which this call drops: pass {what}.detach()")
 
 
 def _context_of(rows) -> Context:
@@ -872,7 +880,7 @@ class QuantizedMatrix:
     offsets[g] .. offsets[g + 1] - 1; rows of no group come out as 0 in a fresh result and stay as they are in the caller's `out`.  `gradient`:
     keep the codes transposed too, for ``input_gradient``.
 
-    torch does not record these calls.  An operand that requires a gradient is refused while torch records; who trains what is in front of a matrix calls
+    torch does not record these calls.  An operand that requires a gradient is refused while torch records, one that carries a tangent always; who trains what is in front of a matrix calls
     ``product`` in the forward and ``input_gradient`` in the backward method of a torch.autograd.Function (where nothing is recorded)."""
 
     def __init__(self, handle, ctx: Context, grouped: bool):
@@ -1113,7 +1121,7 @@ class QuantizedCache:
     Tokens at negative positions (a length of 0: an empty place of a batch), of columns that the table does not have and of pages that the cache does not have are not
     there: they are not written, nobody sees them, and they read as 0.
 
-    Serving only: torch does not record these calls, and an operand that requires a gradient is refused while torch records."""
+    Serving only: torch does not record these calls.  An operand that requires a gradient is refused while torch records, one that carries a tangent always."""
 
     PAGE = 64
 
@@ -1203,7 +1211,8 @@ class QuantizedCache:
         device, Tensor = self._ctx.device, torch.Tensor
         return (type(table) is Tensor and type(lengths) is Tensor and x.is_cuda and table.is_cuda and lengths.is_cuda and x.is_contiguous() and table.is_contiguous()
                 and lengths.is_contiguous() and table.dtype is torch.int32 and lengths.dtype is torch.int32 and x.dim() == 3 and table.dim() == 2 and lengths.dim() == 1
-                and x.get_device() == device and table.get_device() == device and lengths.get_device() == device and not x.requires_grad)
+                and x.get_device() == device and table.get_device() == device and lengths.get_device() == device and not x.requires_grad
+                and not _forward_mode())
 
     def write(self, keys, values, table, lengths, *, offsets=None):
         """Writes the rows (n x heads x width each) into their pages, `lengths` counting them.
