@@ -338,12 +338,13 @@ int vqb_qmat_destroy(vqb_qmat *qm);
  *   read    code s, rounded to the type
  *   attend  y[i] = sum_j e^(S_ij - m_i) v_j / sum_j e^(S_ij - m_i),  S_ij = scale x_i . k_j,  m_i = max_j S_ij,  over the tokens that row i sees: those up to its own
  *           position p_i that are there and, with window > 0, have j > p_i - window or j < sinks.  Query head h reads the cache's head h / (query_heads / heads).  A row that
- *           sees nothing is 0.  Scores, maxima and sums are f32; the codes enter the products as they are, queries as f16 numbers of 11 bits and of the row's own scale (a
+ *           sees nothing is 0, and so are values of a page whose scale of values is 0, whatever their codes (its tokens count below the line).  Scores, maxima and sums are f32; the codes enter the products as they are, queries as f16 numbers of 11 bits and of the row's own scale (a
  *           power of two), e^(S - m) s_v as f16 numbers relative to the row's largest.
  *
  * Queries and results are f16 or bf16 (VQB_ERR_UNSUPPORTED for f32: it would promise more digits than that).  ld and head_ld: values from row to row and from head to head.
  * Rows of no sequence (in front of offsets[0], behind the last offset) are left as they are, or become 0 with VQB_ZERO_REST; vqb_cache_read, whose results are
- * n x heads x width without gaps, makes them 0.  Outputs may not overlap inputs.  Limits (VQB_ERR_UNSUPPORTED beyond): width 256, 4096 heads, 65535 sequences.  A cache is made outside of captures; the calls
+ * n x heads x width without gaps, makes them 0.  Outputs may not overlap inputs.  Rows or heads that
+ * reach further than 2^58 values are refused.  Limits (VQB_ERR_UNSUPPORTED beyond): width 256, 4096 heads, 65535 sequences.  A cache is made outside of captures; the calls
  * on it may be captured with all operands in device memory, as products may. */
 #define VQB_CACHE_PAGE 64
 typedef struct vqb_cache vqb_cache;

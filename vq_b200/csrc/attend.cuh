@@ -1,8 +1,9 @@
 // attend.cuh -- what the attention kernels on tensor cores share.
 //
-// Scores are in powers of two: s = S log2(e).  The weights of the values are e^(S - m) s_v; with s_v = f 2^e, 1/2 <= f < 1, they are held as 2^(s + e - M) f, M the
-// largest s + e of the row so far (not of s: pages whose s_v are far apart would lose the weights that count), which are at most 1 and f16 numbers for the product with the
-// codes.  The sum below the line is 2^(s - m) with the row's largest s, in f32.  y = (sum of weights times codes) / (sum) 2^(M - m).
+// Scores are in powers of two: s = S log2(e).  The weights of the values are e^(S - m) s_v; they are held as 2^(s + log2(s_v) - M), M the largest s + log2(s_v) of the
+// row so far (not of s: pages whose s_v are far apart would lose the weights that count), f16 numbers for the product with the codes.  M is followed when it is left behind by
+// 2^8: weights are up to 2^8 until then.  Values of scale 0 have weights of 0, whatever their codes.  The sum below the line is 2^(s - m) with the row's largest s (followed
+// likewise), in f32.  y = (sum of weights times codes) / (sum) 2^(M - m).
 //
 // Queries are f16 numbers: each row times the power of two that brings its largest magnitude to 2^14 .. 2^15.  f16 and bf16 values are those numbers exactly, but for those
 // below 2^-28 of the row's largest, which are off by at most 2^-39 of it.
@@ -53,27 +54,6 @@ struct QueryScale {
     }
 };
 
-// s_k and s_v of a page and head as the kernels take them
-struct PageScales {
-    float k;
-    float f; // s_v = f 2^e; 0 and NaN have e = 0
-    float e;
-    __device__ __forceinline__ PageScales(float2 s)
-    {
-        k = s.x;
-        const uint32_t bits = __float_as_uint(s.y);
-        const int exponent = (int)(bits >> 23);
-        if (exponent == 0 || exponent == 255) { // (subnormal ones exactly: 2^24 times that, and back)
-            const float big = s.y * 16777216.0f;
-            const bool small = exponent == 0 && big > 0.0f;
-            f = small ? __uint_as_float((__float_as_uint(big) & 0x7FFFFFu) | 0x3F000000u) : s.y;
-            e = small ? (float)((int)(__float_as_uint(big) >> 23) - 126 - 24) : 0.0f;
-        } else {
-            f = __uint_as_float((bits & 0x7FFFFFu) | 0x3F000000u);
-            e = (float)(exponent - 126);
-        }
-    }
-};
 // down s_k: what a row's products with a page's codes are multiplied by.  (Infinite only where any score but 0 is: 0 times that is to stay 0.)
 __device__ __forceinline__ float score_factor(float down, float k)
 {
@@ -124,7 +104,6 @@ struct Cut {
     int first_row, head; // as of Tile
     int first, last;
     int begins; // the tile begins with the first block's share
-    int unused;
 };
 
 // A part of a tile: ROWS x padded sums, and ROWS each of m, M and the sum below the line.
@@ -278,7 +257,7 @@ template <int ROWS, int THREADS> struct Plan {
         Cut cut = {};
         const long long start = share * blockIdx.x;
         if (tile && tile->begin < start && tile->begin >= start - share)
-            cut = Cut{row, rows, tile->first_row, tile->head, (int)blockIdx.x - 1, (int)((tile->begin + tile->units - 1) / share), tile->begin == start - share, 0};
+            cut = Cut{row, rows, tile->first_row, tile->head, (int)blockIdx.x - 1, (int)((tile->begin + tile->units - 1) / share), tile->begin == start - share};
         P.cuts[blockIdx.x] = cut;
     }
 };

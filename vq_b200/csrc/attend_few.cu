@@ -1,7 +1,8 @@
 // attend_few.cu -- attention of a few rows of each sequence (single tokens above all) over a cache of 8-bit codes.
 //
-// Eight or sixteen rows that share a cached head (query heads of a token, then those of the next one) are a tile.  What bounds it is the cache's bytes, read once for a tile:
-// 2 x 64 x width of them a page and head.  Every warp fetches pages for itself (one bulk copy for a page's keys, one for its values) into a ring of its own,
+// Eight or sixteen rows that share a cached head (query heads of a token, then those of the next one) are a tile.  The floor is the cache's bytes, 2 x 64 x width of them a page and head, read
+// once for a tile: of a sequence with 17 to 32 rows twice, by different blocks (16 sequences of up to 8192 tokens, 8 heads x 128: 47 us for one token of eight query heads a cached one, 61 for two, 98 for four;
+// the bytes once are 26).  What bounds it is less the bytes (76 % of the copy rate for 64 sequences, 59 % for two of 131,072) than fixed latencies with three warps a scheduler.  Every warp fetches pages for itself (one bulk copy for a page's keys, one for its values) into a ring of its own,
 // turns the codes to f16 numbers in registers and multiplies: mma.sync m16n8k16 with sixteen tokens by eight rows, then sixteen dimensions by eight rows.  (The tensor
 // cores' larger instructions have 128 rows where there are eight.)  A lane's 16 bytes of a key serve four instructions: which of its dimensions go into
 // which is free as long as the queries have the same.  So is which tokens are a score tile's rows; they are chosen so that the tile, transposed (movmatrix), is the operand
@@ -474,7 +475,8 @@ template <int PADDED, int EIGHTS, int WARPS> void attend_few_with(CudaDevice &de
     launch_join<PADDED, ROWS>(dev, P);
 }
 
-// Eight warps a block where every tile has an SM to itself and as few pages as are not shared out: one token behind 1000 in 11.7 us instead of 14.2.  (Elsewhere four are better
+// Eight warps a block where every tile has an SM to itself and as few pages as are not shared out: one token behind 1000 in 11.8 us instead of 14.  (The table's columns say how many pages there may
+// be, for the lengths are not known here: in a table of more than 16 columns the same token takes 14 us, whatever its length.)  (Elsewhere four are better
 // used: 64 sequences of up to 8192 tokens take 101 us and not 118.)
 template <int PADDED, int EIGHTS> void attend_few_rows(CudaDevice &dev, ShareParams &P)
 {

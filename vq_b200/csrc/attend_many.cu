@@ -13,7 +13,10 @@
 //   warps 8 .. 15   four for each half of the rows, a row a thread: scores to weights, largest score and sum; queries in, results out.  They take most of the registers
 //                   (setmaxnreg: 2 x 96 + 2 x 160 a thread of each four warps, of 4 x 128)
 //
-// What bounds it is the tensor cores' rate (4 x width operations for each row and token) and, as much, the exponentials: 16 an SM and cycle.
+// The floor is the tensor cores' rate (4 x width operations for each row and token); the exponentials, 16 an SM and cycle, take nearly as long.  What bounds it is neither: a step of 256 rows
+// of 128 takes some 2600 cycles, the tensor core 1280 of them (alone) and the exponentials 1024.  Two warps a scheduler make weights, each of them a chain of waits, loads, exponentials
+// and stores (2048 tokens behind 6144, 32 heads on 8: issue slots 54 %, tensor cores 35 to 44 %, the exponentials' unit 36 %).
+// Widths above 128 have one half, whose products and weights cannot take turns: 8192 tokens, 16 heads on 4 of 128 values in 400 us, of 160 in 831, of 256 in 1016 (687, 414 and 541 TFLOP/s).
 //
 // The largest score that weights are relative to stays as it is until a row has one 2^8 times as large; then the row's sums in tensor memory are brought down, once the product
 // that adds to them is done.  Weights are up to 2^8 until then, and f16 numbers all the same.
@@ -98,14 +101,14 @@ __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.s
 __device__ __forceinline__ void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// A part of a tile that the block takes, as one warp tells the others ahead of time.
-struct Work {
+// A part of a tile that the block takes, as one warp tells the others ahead of time.  (Aligned to be copied 16 bytes at a time: a prompt of 16,384 tokens through a window of 1024 takes 455 us,
+// and 463 without.)
+struct alignas(16) Work {
     int row, rows, p0, p1, keys;    // first row of the sequence, rows, positions of the first and last, tokens
     int first_row, head, b;         // as of Tile
     int sink_pages, begin, pages;   // as of Pages
     int from, steps;                // first page (of the tile's list), steps; -1: there are no more parts
     int begins, whole;              // the share begins here; the tile is all here
-    int unused;
     // page i of this part, -1 where there is none
     __device__ __forceinline__ int column(int i) const { return from + i < sink_pages ? from + i : begin + from + i - sink_pages; }
     __device__ __forceinline__ int page(const Attend &a, int i) const { return from + i < pages ? page_of(a.seq, a.cache.pages, b, column(i)) : -1; }
@@ -310,7 +313,7 @@ template <int PADDED>
 __device__ __forceinline__ void issue_products(const ShareParams &P, ManyBarriers &bars, const WorkRoom &room, uint8_t *queries, uint8_t *ring, uint32_t tmem)
 {
     using Shape = ManyShape<PADDED>;
-    [[maybe_unused]] constexpr int ROWS = Shape::ROWS, HALVES = Shape::HALVES, STAGES = Shape::STAGES;
+    constexpr int STAGES = Shape::STAGES;
     volatile int *abort_flag = &bars.abort_flag;
     const bool leader = elect_one(); // the one lane that knows the following
     int st = 0;
@@ -401,11 +404,9 @@ template <int PADDED>
 __device__ __forceinline__ void convert_codes(const ShareParams &P, ManyBarriers &bars, const WorkRoom &room, const uint8_t *codes, uint8_t *ring)
 {
     using Shape = ManyShape<PADDED>;
-    [[maybe_unused]] constexpr int ROWS = Shape::ROWS, HALVES = Shape::HALVES, STAGES = Shape::STAGES;
+    constexpr int STAGES = Shape::STAGES;
     const int lane = threadIdx.x % 32;
     volatile int *abort_flag = &bars.abort_flag;
-    const Attend &a = P.a;
-    [[maybe_unused]] const Cache &c = a.cache;
     const int t = threadIdx.x - 128; // of the converters' threads
     constexpr int THREADS_HERE = 32 * CONVERTERS, ALL = STEP * PADDED / 16, PIECES = (ALL + THREADS_HERE - 1) / THREADS_HERE; // pieces of 16 codes of a page, and a thread's
     constexpr int PER_ROW = PADDED / 16;                                                                                     // of a token's key
@@ -469,11 +470,11 @@ template <int PADDED>
 __device__ __forceinline__ void weigh_rows(const ShareParams &P, ManyBarriers &bars, const WorkRoom &room, uint8_t *queries, float *down_room, uint32_t tmem)
 {
     using Shape = ManyShape<PADDED>;
-    [[maybe_unused]] constexpr int ROWS = Shape::ROWS, HALVES = Shape::HALVES, STAGES = Shape::STAGES;
+    constexpr int ROWS = Shape::ROWS, HALVES = Shape::HALVES;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     volatile int *abort_flag = &bars.abort_flag;
     const Attend &a = P.a;
-    [[maybe_unused]] const Cache &c = a.cache;
+    const Cache &c = a.cache;
     const int h = (warp - 8) / 4, r = (warp % 4) * 32 + lane; // half, row of it
     const uint32_t lanes = (uint32_t)(warp % 4) << 21, sums = tmem + lanes + Shape::SUMS + 128 * h; // (lane 32 q: bits 16 ..)
     uint32_t scores_parity = 0, added_parity = 0, sums_parity = 0; // scores_parity: bit b of the next scores in buffer b; added_parity: of this step's product

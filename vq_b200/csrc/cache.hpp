@@ -65,7 +65,7 @@ struct Attend {
     bool zero_rest = false; // rows of no sequence become 0
 };
 // Rows of a sequence are taken together where they have the same cached head: `group` query heads of one token, then those of the next.  A sequence of up to ATTEND_FEW of
-// them is taken eight or sixteen at a time, by tensor-core instructions of a warp on pages that the warp fetches for itself; nothing counts there but the cache's bytes.
+// them is taken eight or sixteen at a time, by tensor-core instructions of a warp on pages that the warp fetches for itself (from 17 rows on, every page twice).
 // Others are taken 256 or 128 at a time by tcgen05 instructions.  (us by the one and by the other: 16 sequences of up to 8192 tokens with 32 rows each 107 and 167, with 64 rows 203 and 167; 64 of
 // up to 1000 with 64 rows 167 and 134.)
 constexpr int ATTEND_FEW = 32;
